@@ -356,6 +356,168 @@ int32_t cev_gather_rows(int32_t dtype, int32_t out_dtype, int64_t n, int64_t wid
                         const int32_t* ids, void* out, int64_t ld_out, cev_stream stream);
 
 /* ------------------------------------------------------------------ */
+/* Serving over a paged K/V cache.
+ *
+ * The caches of one layer are (n_pages, page_size, hkv, d) arrays of any
+ * strides; request r's key j lies in page block_table[r][j / page_size] at
+ * offset j % page_size.  A step is cev_paged_tables (once), cev_paged_plan
+ * (once for each window that the layers use), then for each layer cev_rope
+ * (or cev_qknorm_rope_kv with the same slots, where the cache's slots lie
+ * evenly spaced) and cev_paged_attention.  All lengths stay on the device:
+ * nothing of a step waits for the host, so a captured step can be replayed
+ * while the lengths grow.
+ *
+ * cev_paged_tables: the step's bookkeeping.  Request r (of n_requests <=
+ * 4096) holds lengths[r] cached tokens in the first ceil(lengths[r] /
+ * page_size) entries of its row of block_table (row stride bt_stride,
+ * max_pages entries) and brings new_len[r] >= 0 new ones; new_len[r] = -1
+ * ends it.  Pages that the new tokens need are taken from the free ring in
+ * request order and entered in block_table; an ended request's pages go back
+ * to the ring's end in request order (for later calls: none of them is
+ * taken by this one) and its length becomes 0.  The ring is free_pages
+ * (n_pages entries) with ring = {head, count, status, counter}: the free
+ * pages are free_pages[(head + i) % n_pages], i < count.  Written:
+ *   lengths_out (n_requests)  the lengths with the new tokens
+ *   ring_out (4)              head, count and status after the call
+ *   cu (n_requests + 1)       first packed row of each request, and their sum
+ *   pos, slots (max_tokens)   position and cache slot (page * page_size +
+ *                             offset) of each packed row; rows behind the
+ *                             last get position 0 and slot -1
+ * Status 0, or a sum of: 1 more than max_tokens new tokens, 2 a request
+ * longer than max_pages pages, 4 too few free pages, 8 a length or the ring
+ * out of its bounds.  Then nothing is taken, given back or counted (cu is
+ * all 0, slots all -1), so what the step launches next finds no rows.  An
+ * entry outside [0, n_pages) gives slots of -1.  lengths_out may be lengths
+ * and ring_out ring; ring_out[3] must be 0 before the first call (calls
+ * leave it 0).  free_pages NULL: block_table holds the new tokens' pages
+ * already, and ended requests' pages are the caller's. */
+int32_t cev_paged_tables(int32_t n_requests, int32_t page_size, int32_t n_pages, int32_t max_pages, int32_t max_tokens,
+                         const int32_t* lengths, const int32_t* new_len, int32_t* block_table, int64_t bt_stride, int32_t* free_pages,
+                         const int32_t* ring, int32_t* lengths_out, int32_t* ring_out, int32_t* cu, int32_t* pos, int32_t* slots,
+                         cev_stream stream);
+
+/* Rotary angles.  Pair i of rotary_dim / 2 turns by inv_i radians a position,
+ * inv_i = theta^(-2i / rotary_dim), scaled for contexts longer than the
+ * `original` one of the training:
+ *   CEV_ROPE_LINEAR      inv_i / factor
+ *   CEV_ROPE_YARN        inv_i (1 - r_i + r_i / factor), r_i the ramp from 0 to
+ *                        1 between the pairs (rounded outwards) that turn
+ *                        `high` and `low` times in the original context;
+ *                        cos and sin times attention_factor (0: 0.1 ln(factor) + 1)
+ *   CEV_ROPE_WAVELENGTH  the same sum, r_i = 1 - clamp((original inv_i / 2 pi -
+ *                        low) / (high - low), 0, 1)
+ * steps (rotary_dim / 2, host memory) receives the turns a position as
+ * fractions of 2^64: position times step modulo 2^64 is the angle's fraction of
+ * a turn, within 2^-34 at any 32-bit position.  *factor receives the factor on cos
+ * and sin.  Host only. */
+enum { CEV_ROPE_PLAIN = 0, CEV_ROPE_LINEAR = 1, CEV_ROPE_YARN = 2, CEV_ROPE_WAVELENGTH = 3 };
+typedef struct {
+  int32_t kind;       /* CEV_ROPE_* */
+  int32_t rotary_dim; /* even */
+  double theta;
+  double factor;           /* >= 1; unused by CEV_ROPE_PLAIN */
+  double original;         /* CEV_ROPE_YARN, CEV_ROPE_WAVELENGTH */
+  double low, high;        /* turns in the original context: all stretched below, none above */
+  double attention_factor; /* 0: the kind's own */
+} cev_rope_scaling;
+int32_t cev_rope_angles(const cev_rope_scaling* s, uint64_t* steps, float* factor);
+
+/* Rotary positions without a norm (cev_qknorm_rope is the fused form with
+ * one): the first rotary_dim values of each q and k row, taken as pairs
+ * (i, i + rotary_dim / 2) or, interleaved, (2i, 2i + 1), are turned by
+ * pos[token] * angle_i and scaled by factor; the others are copied.  Angles
+ * are exact (see above), products and sums f32, one rounding to the dtype.
+ * transposed: the transposed map, i.e. the gradient of the call's inputs from
+ * that of its outputs.
+ *   q_in (t, hq, d), k_in and v_in (t, hkv, d); q_out (t, hq, d)
+ *   slots NULL: k_out and v_out are (t, hkv, d) (strides *_stride_t, *_stride_h)
+ *   slots (t): token i's k and v rows go to slot slots[i] of (n_slots /
+ *   page_size, page_size, hkv, d) caches (strides *_stride_p, *_stride_t,
+ *   *_stride_h); a slot outside [0, n_slots) stores neither.  No two tokens
+ *   may have the same slot.
+ * v_in / v_out NULL: no v.  hq or hkv may be 0.  An output may be its own
+ * input with the same strides.  head_dim and rotary_dim are multiples of 16,
+ * head_dim <= 256; rows 16-byte aligned.  steps: device copy of
+ * cev_rope_angles' output. */
+typedef struct {
+  int32_t dtype;
+  int32_t n_q_heads, n_kv_heads, head_dim;
+  int32_t t;
+  int32_t rotary_dim;
+  int32_t interleaved;
+  int32_t transposed;
+  float factor;
+  int32_t page_size; /* a power of two; 0 without slots */
+  int32_t n_slots;
+  int32_t reserved;
+  int64_t qi_stride_t, qi_stride_h;
+  int64_t ki_stride_t, ki_stride_h;
+  int64_t vi_stride_t, vi_stride_h;
+  int64_t qo_stride_t, qo_stride_h;
+  int64_t ko_stride_p, ko_stride_t, ko_stride_h;
+  int64_t vo_stride_p, vo_stride_t, vo_stride_h;
+} cev_rope_desc;
+
+/* Fills d with dense strides (token-major rows; with page_size > 0 the
+ * outputs of k and v as (n_slots / page_size, page_size, hkv, d) caches). */
+int32_t cev_rope_desc_init(cev_rope_desc* d, int32_t dtype, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t t,
+                           int32_t rotary_dim, int32_t page_size, int32_t n_slots);
+int32_t cev_rope(const cev_rope_desc* d, const void* q_in, const void* k_in, const void* v_in, const int32_t* pos, const uint64_t* steps,
+                 const int32_t* slots, void* q_out, void* k_out, void* v_out, cev_stream stream);
+
+/* Attention of each request's new tokens over its pages.  Request r's new
+ * tokens are the packed rows [cu[r], cu[r + 1]) of q and out, its last
+ * positions: row i of them has position p = lengths[r] - (cu[r + 1] - cu[r])
+ * + i and sees key j when j <= p and (window == 0 or j > p - window or j <
+ * sinks).  lengths include the new tokens, whose k and v are in the cache
+ * already.  Rows of no request are left as they were.  Pages that no row
+ * sees (behind a window) are not read and may have been given back. */
+typedef struct {
+  int32_t dtype;      /* CEV_F32 or CEV_BF16: q, k, v, out */
+  int32_t n_q_heads;  /* hq */
+  int32_t n_kv_heads; /* hkv; hq / hkv is 1, 2, 4 or 8 */
+  int32_t head_dim;   /* 128 or 256 (f32: 128) */
+  int32_t n_requests; /* 1..4096 */
+  int32_t t;          /* packed rows of q and out */
+  int32_t max_new;    /* no request has more new tokens; 1..t */
+  int32_t page_size;  /* a power of two, 16..1024 */
+  int32_t n_pages;
+  int32_t max_pages;  /* entries of a request's row of the block table */
+  int32_t window;     /* 0: none */
+  int32_t sinks;      /* first tokens that stay visible behind a window */
+  float scale;
+  int32_t reserved;
+  int64_t q_stride_t, q_stride_h;
+  int64_t kc_stride_p, kc_stride_t, kc_stride_h;
+  int64_t vc_stride_p, vc_stride_t, vc_stride_h;
+  int64_t o_stride_t, o_stride_h;
+  int64_t bt_stride;
+} cev_paged_desc;
+
+/* Fills d with dense strides, max_new = t, no window and scale =
+ * 1/sqrt(head_dim). */
+int32_t cev_paged_desc_init(cev_paged_desc* d, int32_t dtype, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t n_requests,
+                            int32_t t, int32_t page_size, int32_t n_pages, int32_t max_pages);
+
+/* Bytes of the work buffer (host only): the list of work items that
+ * cev_paged_plan makes on the device from the lengths, and the partial
+ * results of rows whose keys are split over several workgroups.  16-byte
+ * aligned; a plan and the attention calls that use it run one after the
+ * other. */
+int32_t cev_paged_work_size(const cev_paged_desc* d, size_t* bytes);
+
+/* Makes the work list in `work` from cu (n_requests + 1) and lengths
+ * (n_requests).  A cu or length that is out of its bounds makes the
+ * attention calls write NaN to every row. */
+int32_t cev_paged_plan(const cev_paged_desc* d, const int32_t* cu, const int32_t* lengths, void* work, size_t work_bytes, cev_stream stream);
+
+/* The attention over one layer's caches.  d may differ from the plan's in
+ * its strides and scale only; with any other plan in `work` every row of out
+ * is NaN, and a row that sees a page outside [0, n_pages) is NaN. */
+int32_t cev_paged_attention(const cev_paged_desc* d, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                            void* out, void* work, size_t work_bytes, cev_stream stream);
+
+/* ------------------------------------------------------------------ */
 /* Table builders (host only). */
 
 /* The packed pass of engine.rs:365-442.  Plans p = 0..n_plans-1 in plan

@@ -24,6 +24,7 @@ __all__ = [
     "GatedDeltaNet",
     "CEV_BF16", "CEV_F32", "CevError", "Block", "Span", "BlockTable", "AttnPlan", "PackedAttention",
     "packed_attention", "qknorm_rope", "rope_table", "Rotary", "device_info", "synth",
+    "paged_tables", "free_ring", "RotaryAngles", "rope", "PagedAttention",
     "Blas", "linear", "gather_rows", "D3Readout", "PrefixStore", "qknorm_rope_kv",
 ]
 
@@ -676,3 +677,9 @@ class GatedDeltaNet:
             s_out = torch.empty((B, nv, dk, dv), dtype=torch.float32, device=mixed.device)
         calls().gdn(self.desc, mixed, z, b, a, conv_w, neg_a, dt_bias, norm_w, conv_in, s_in, y, conv_out, s_out, self.workspace, stream)
         return y, conv_out, s_out
+
+
+# ---------------------------------------------------------------------------
+# Paged caches
+
+from .paged import PagedAttention, RotaryAngles, free_ring, paged_tables, rope  # noqa: E402

@@ -20,6 +20,7 @@ CEV_ERR_SPACE = -4
 CEV_F32 = 0
 CEV_BF16 = 1
 CEV_MAX_SPANS = 4
+CEV_ROPE_PLAIN, CEV_ROPE_LINEAR, CEV_ROPE_YARN, CEV_ROPE_WAVELENGTH = range(4)
 CEV_ATTN_SCRATCH_BYTES = 64 << 20
 CEV_LINEAR_WORKSPACE_BYTES = 32 << 20
 
@@ -86,6 +87,37 @@ class GdnDesc(C.Structure):
     ]
 
 
+class RopeScaling(C.Structure):
+    _fields_ = [
+        ("kind", i32), ("rotary_dim", i32), ("theta", C.c_double), ("factor", C.c_double), ("original", C.c_double),
+        ("low", C.c_double), ("high", C.c_double), ("attention_factor", C.c_double),
+    ]
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [
+        ("dtype", i32), ("n_q_heads", i32), ("n_kv_heads", i32), ("head_dim", i32), ("t", i32), ("rotary_dim", i32),
+        ("interleaved", i32), ("transposed", i32), ("factor", C.c_float), ("page_size", i32), ("n_slots", i32), ("reserved", i32),
+        ("qi_stride_t", i64), ("qi_stride_h", i64),
+        ("ki_stride_t", i64), ("ki_stride_h", i64),
+        ("vi_stride_t", i64), ("vi_stride_h", i64),
+        ("qo_stride_t", i64), ("qo_stride_h", i64),
+        ("ko_stride_p", i64), ("ko_stride_t", i64), ("ko_stride_h", i64),
+        ("vo_stride_p", i64), ("vo_stride_t", i64), ("vo_stride_h", i64),
+    ]
+
+
+class PagedDesc(C.Structure):
+    _fields_ = [
+        ("dtype", i32), ("n_q_heads", i32), ("n_kv_heads", i32), ("head_dim", i32), ("n_requests", i32), ("t", i32), ("max_new", i32),
+        ("page_size", i32), ("n_pages", i32), ("max_pages", i32), ("window", i32), ("sinks", i32), ("scale", C.c_float), ("reserved", i32),
+        ("q_stride_t", i64), ("q_stride_h", i64),
+        ("kc_stride_p", i64), ("kc_stride_t", i64), ("kc_stride_h", i64),
+        ("vc_stride_p", i64), ("vc_stride_t", i64), ("vc_stride_h", i64),
+        ("o_stride_t", i64), ("o_stride_h", i64), ("bt_stride", i64),
+    ]
+
+
 P = C.c_void_p
 Pi32 = C.POINTER(i32)
 PBlock = C.POINTER(Block)
@@ -115,6 +147,14 @@ SIGNATURES = {
     "cev_linear": (i32, [P, i32, i32, i64, i64, i64, P, i64, P, i64, C.c_float, P, i64, P, C.c_size_t, P]),
     "cev_linear_form": (i32, [i32, i64, i64, i64, C.c_size_t, Pi32]),
     "cev_gather_rows": (i32, [i32, i32, i64, i64, P, i64, i64, P, P, i64, P]),
+    "cev_paged_tables": (i32, [i32, i32, i32, i32, i32, P, P, P, i64, P, P, P, P, P, P, P, P]),
+    "cev_rope_angles": (i32, [C.POINTER(RopeScaling), C.POINTER(C.c_uint64), C.POINTER(C.c_float)]),
+    "cev_rope_desc_init": (i32, [C.POINTER(RopeDesc), i32, i32, i32, i32, i32, i32, i32, i32]),
+    "cev_rope": (i32, [C.POINTER(RopeDesc), P, P, P, P, P, P, P, P, P, P]),
+    "cev_paged_desc_init": (i32, [C.POINTER(PagedDesc), i32, i32, i32, i32, i32, i32, i32, i32, i32]),
+    "cev_paged_work_size": (i32, [C.POINTER(PagedDesc), C.POINTER(C.c_size_t)]),
+    "cev_paged_plan": (i32, [C.POINTER(PagedDesc), P, P, P, C.c_size_t, P]),
+    "cev_paged_attention": (i32, [C.POINTER(PagedDesc), P, P, P, P, P, P, C.c_size_t, P]),
     "cev_table_from_plans": (i32, [i32, Pi32, Pi32, Pi32, i32, Pi32, Pi32, PBlock, i32, Pi32, Pi32, i32, Pi32, Pi32]),
     "cev_table_from_rows": (i32, [i32, i32, i32, i32, Pi32, PBlock, i32]),
     "cev_table_from_slots": (i32, [i32, Pi32, Pi32, Pi32, i32, Pi32, Pi32, Pi32, i32, PBlock, i32, Pi32, Pi32, Pi32, i32, Pi32, Pi32]),

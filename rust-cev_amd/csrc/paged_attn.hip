@@ -1,0 +1,541 @@
+// Attention of each request's new tokens over a paged K/V cache.
+//
+// A work item (cev_paged_plan) is up to 32 query slots (rows x the g query
+// heads of one KV head: slot -> row slot / g, head slot % g) and a run of the
+// 32-key sub-tiles that they see.  Its workgroup's four waves take the
+// sub-tiles in turn, each on its own: no barrier until their partial results
+// are joined.  Scores are computed transposed, S^T = K . Q^T, on 32x32 MFMA
+// tiles, so a lane holds 16 keys of one query row and the softmax's running
+// max and sum stay in its registers; O^T = V^T . P^T follows with P as the B
+// operand.
+//
+// K and V go from HBM straight into this wave's own LDS (buffer_load ... lds,
+// 1 KB an instruction), one or two sub-tiles ahead.  A page's base is a scalar
+// 64-bit address (page ids are wave-uniform), so the cache may have any size;
+// keys past the end, in pages behind the window or not visible to any row of
+// the item get an offset out of the resource's range and read as zero.
+//
+// Items of one tile whose keys are split write partial results (f32); the last
+// of them to arrive (a counter per tile and KV head) joins all in their order,
+// so the result does not depend on who is last.
+#include "attn_device.h"
+#include "paged.h"
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * 64;
+
+struct PagedArgs {
+  const void *q, *kc, *vc;
+  const int32_t* bt;
+  void* out;
+  char* work;
+  size_t items_off, counters_off, records_off;
+  int64_t q_st, q_sh, kc_sp, kc_st, kc_sh, vc_sp, vc_st, vc_sh, o_st, o_sh, bt_stride;
+  int32_t hkv, g, t, n_requests, page_shift, n_pages, max_pages, window, sinks;
+  float scale_log2;
+  uint32_t sig;
+};
+
+// Workgroup b writes NaN over its share of out's rows.
+template <typename T, int D>
+__device__ void paged_poison(const PagedArgs& a) {
+  const int64_t G = gridDim.x;
+  const int64_t r0 = (int64_t)blockIdx.x * a.t / G, r1 = (int64_t)(blockIdx.x + 1) * a.t / G;
+  const int64_t per_row = (int64_t)a.hkv * a.g * D;
+  for (int64_t i = threadIdx.x; i < (r1 - r0) * per_row; i += blockDim.x) {
+    const int64_t r = r0 + i / per_row, h = (i % per_row) / D, e = i % D;
+    ((T*)a.out)[r * a.o_st + h * a.o_sh + e] = (T)__builtin_nanf("");
+  }
+}
+
+// f32 values as sums of three bf16 parts and the six large part products
+// (see fan_attn.hip).
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void bf16_parts(const float* x, bf16x8* p) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    f32x2 r = {x[e], x[e + 1]};
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const bf16x2 b = __builtin_convertvector(r, bf16x2);
+      p[i][e] = b[0];
+      p[i][e + 1] = b[1];
+      r = r - __builtin_convertvector(b, f32x2);
+    }
+  }
+}
+__device__ __forceinline__ f32x16 parts_mma(const bf16x8* a, const bf16x8* b, f32x16 c) {
+#pragma unroll
+  for (int o = 2; o >= 0; --o)
+#pragma unroll
+    for (int i = 0; i <= o; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[o - i], c, 0, 0, 0);
+  return c;
+}
+
+// 16-byte block of row `row` that block blk of K is stored at: a row's blocks
+// are permuted so that the operand reads (16 rows at once) meet every bank.
+__device__ __forceinline__ int k_place(int blk, int row) { return blk ^ (row & 15); }
+// of V: bf16 is read transposed, four rows x four blocks at once; f32 by two
+// half waves whose rows differ in bit 2.
+template <typename T>
+__device__ __forceinline__ int v_place(int blk, int row) {
+  return sizeof(T) == 2 ? blk ^ ((row & 3) << 2) : blk ^ (((row >> 2) & 1) << 3);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) void paged_attn_kernel(PagedArgs a) {
+  using F = Frag<T, D>;
+  constexpr bool BF = sizeof(T) == 2;
+  constexpr int NDT = D / 32;
+  constexpr int kRB = D * (int)sizeof(T);        // bytes of one key row
+  constexpr int kTile = kPagedKeys * kRB;        // K or V of a sub-tile
+  constexpr int kLoads = kTile / 1024;           // 1 KB loads of it
+  constexpr int NB = kRB == 256 ? 2 : 1;         // sub-tiles of K and of V in LDS
+  constexpr int kRows = 1024 / kRB, kBlk = kRB / 16;  // rows of one load, 16-byte blocks of a row
+  constexpr int RS = D + 4;                      // row stride (floats) of a partial result in LDS
+  constexpr int kRing = kWaves * 2 * NB * kTile, kOut = kWaves * 32 * RS * 4;
+  __shared__ __align__(16) char lds[kRing > kOut ? kRing : kOut];
+  __shared__ float2 ml[kWaves * 32];
+  __shared__ int32_t last_s;
+
+  const PagedHeader* const hdr = (const PagedHeader*)a.work;
+  const int32_t n_items = hdr->n_items;
+  if (hdr->sig != a.sig || hdr->bad != 0) {
+    paged_poison<T, D>(a);
+    return;
+  }
+  const int item = blockIdx.x / (uint32_t)a.hkv, kvh = blockIdx.x - item * a.hkv;
+  if (item >= n_items) return;
+  const PagedItem it = ((const PagedItem*)(a.work + a.items_off))[item];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i32(tid >> 6);
+  const int n = lane & 31, u = lane >> 5;
+  const int gs = __builtin_ctz(a.g);
+  const bool ok = (n >> gs) < it.n_rows;
+  const int row = it.row0 + (ok ? n >> gs : 0), head = kvh * a.g + (n & (a.g - 1));
+  const int pos = ok ? it.pos0 + (n >> gs) : -1;
+  const int pos1 = it.pos0 + it.n_rows - 1;
+  const PagedSpan span = paged_span<kPagedKeys>(it.pos0, pos1, a.window, a.sinks);
+
+  // ---- Q, as the B operand
+  const T* const qrow = (const T*)a.q + (int64_t)row * a.q_st + (int64_t)head * a.q_sh;
+  F fr;
+  bf16x8 qp[BF ? 1 : D / 16][3];
+  auto load_q8 = [&](int st, float* x) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const f32x4 v = ok ? *(const f32x4*)(qrow + 16 * st + 8 * u + e) : f32x4{};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[e + j] = v[j];
+    }
+  };
+  if constexpr (BF) {
+    fr.load_q(qrow, ok, u);
+  } else {
+#pragma unroll
+    for (int st = 0; st < D / 16; ++st) {
+      float x[8];
+      load_q8(st, x);
+      bf16_parts(x, qp[st]);
+    }
+  }
+
+  // ---- this wave's sub-tiles: c_begin + wave, + kWaves, ...
+  const int c_end = it.c_end;
+  auto first_key = [&](int c) { return kPagedKeys * (c < span.sinks ? c : c - span.sinks + span.first); };
+  const int32_t* const bt = a.bt + it.req * a.bt_stride;
+  const uint64_t kbase = (uint64_t)((const T*)a.kc + kvh * a.kc_sh), vbase = (uint64_t)((const T*)a.vc + kvh * a.vc_sh);
+  const int kr = uniform_i32((int)(a.kc_st * (int64_t)sizeof(T))), vr = uniform_i32((int)(a.vc_st * (int64_t)sizeof(T)));
+  // Lane l keeps the two page ids of this wave's sub-tile 64 b + l of the
+  // current batch b (a page of 16 keys holds half a sub-tile).
+  int batch_first = 0, page_a = 0, page_b = 0;
+  auto load_pages = [&](int c0) {
+    batch_first = c0;
+    const int c = min(c0 + kWaves * lane, c_end - 1);
+    const int j = first_key(max(c, 0));
+    // (the last sub-tile may reach beyond the block table's last page)
+    page_a = bt[min(j >> a.page_shift, a.max_pages - 1)];
+    page_b = bt[min((j + 16) >> a.page_shift, a.max_pages - 1)];
+  };
+  bool bad_page = false;
+  char* const ring = lds + wave * 2 * NB * kTile;
+  const int lds_ring = (int)(size_t)(const __attribute__((address_space(3))) char*)ring;
+  // Row of a load's lane within the sub-tile, and its block there.
+  const int ld_row = lane / kBlk, ld_blk = lane % kBlk;
+
+  // K (which = 0) or V (1) of sub-tile c into buffer buf; past the end: zeros.
+  auto fetch = [&](int c, int which, int buf) {
+    const bool real = c < c_end;
+    if (real && which == 0 && c >= batch_first + kWaves * 64) load_pages(c);
+    const int key0 = real ? first_key(c) : 0;
+    const int l = real ? (c - batch_first) / kWaves : 0;
+    const int stride = which ? vr : kr;
+    const int64_t page_bytes = (which ? a.vc_sp : a.kc_sp) * (int64_t)sizeof(T);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int first = key0 + 16 * half;
+      // keys that some row of the item sees
+      const bool seen = real && first < span.end && !(first >= span.skip_lo && first + 16 <= span.skip_hi);
+      int page = half ? __builtin_amdgcn_readlane(page_b, l) : __builtin_amdgcn_readlane(page_a, l);
+      const bool in = (uint32_t)page < (uint32_t)a.n_pages;
+      bad_page |= seen && !in;
+      page = in ? page : 0;
+      const uint64_t base = (which ? vbase : kbase) + (uint64_t)(page * page_bytes) + (uint64_t)((first & ((1 << a.page_shift) - 1)) * (int64_t)stride);
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)uniform_u64(base), (short)0, uniform_i32(seen && in ? 16 * stride : 0), kBufferWord3);
+#pragma unroll
+      for (int i = 0; i < kLoads / 2; ++i) {
+        const int r = half * 16 + kRows * i + ld_row;  // row of the sub-tile
+        const int key = key0 + r;
+        const bool load = key < span.end && !(key >= span.skip_lo && key < span.skip_hi);
+        const int blk = which ? v_place<T>(ld_blk, r) : k_place(ld_blk, r);
+        const int off = load ? (r - half * 16) * stride + (blk << 4) : INT32_MAX;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(ring + (which * NB + buf) * kTile + 1024 * (half * (kLoads / 2) + i)), 16, off, 0, 0, 0);
+      }
+    }
+  };
+
+  f32x16 o[NDT];
+  float m_run, l_run;
+  auto reset = [&] {
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[dt] = f32x16{};
+    m_run = -1e30f;
+    l_run = 0.0f;
+  };
+  reset();
+  int voff[NDT];
+  if constexpr (BF) {
+    const int i = lane & 15, rr = i >> 2, blk = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) voff[dt] = (4 * u + rr) * kRB + (v_place<T>(4 * dt + blk, rr) << 4) + 8 * (i & 1);
+  }
+  // A value of V in buffer buf.
+  auto v_at = [&](int buf, int key, int col) -> T* {
+    return (T*)(ring + (NB + buf) * kTile + key * kRB + (v_place<T>(col * (int)sizeof(T) / 16, key) << 4)) + col % (16 / (int)sizeof(T));
+  };
+
+  // f32: an infinite value (or one above bf16's range) has no parts.  A wave
+  // that ends with anything non-finite walks its keys again on the f32 unit.
+  bool exact = false;
+  for (;;) {
+    int c = it.c_begin + wave;
+    if (c < c_end) {
+    load_pages(c);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      fetch(c + b * kWaves, 0, b);
+      fetch(c + b * kWaves, 1, b);
+    }
+    auto step = [&](int buf) {
+      const int key0 = first_key(c);
+      // K of this sub-tile has landed once only later loads are in flight
+      pipe::wait_vmcnt<(2 * NB - 1) * kLoads>();
+      asm volatile("" ::: "memory");
+      f32x16 s = f32x16{};
+      const char* const kt = ring + buf * kTile + n * kRB;
+#pragma unroll
+      for (int st = 0; st < D / 16; ++st) {
+        if constexpr (BF) {
+          fr.qk_mfma(*(const bf16x8*)(kt + (k_place(2 * st + u, n) << 4)), st, s);
+        } else {
+          float x[8];
+          *(f32x4*)x = *(const f32x4*)(kt + (k_place(4 * st + 2 * u, n) << 4));
+          *(f32x4*)(x + 4) = *(const f32x4*)(kt + (k_place(4 * st + 2 * u + 1, n) << 4));
+          if (!exact) {
+            bf16x8 kp[3];
+            bf16_parts(x, kp);
+            s = parts_mma(kp, qp[st], s);
+          } else {
+            float q[8];
+            load_q8(st, q);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], q[e], s, 0, 0, 0);
+          }
+        }
+      }
+      asm volatile("" ::: "memory");
+      const bool masked = key0 + kPagedKeys - 1 > it.pos0 ||
+                          (a.window > 0 && key0 <= pos1 - a.window && key0 + kPagedKeys > a.sinks);
+      auto visible = [&](int key) { return (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.sinks)); };
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const bool vis = visible(key0 + 8 * (i >> 2) + 4 * u + (i & 3));
+          s[i] = vis ? s[i] : -INFINITY;
+        }
+      }
+      // (s is made: K's buffer is free for the sub-tile NB ahead)
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(c + NB * kWaves, 0, buf);
+      __builtin_amdgcn_sched_barrier(0);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
+      const float m_cand = pair_max(mx) * a.scale_log2;
+      const bool grow = m_cand > m_run + kRescale;
+      if (__ballot(grow)) {
+        const float m_new = grow ? m_cand : m_run;
+        const float alpha = fast_exp2(m_run - m_new);
+        m_run = m_new;
+        l_run *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) o[dt] *= alpha;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = fast_exp2(__builtin_fmaf(s[i], a.scale_log2, -m_run));
+      typename F::P p;
+      F::make_p(s, p, l_run);
+      pipe::wait_vmcnt<(2 * NB - 1) * kLoads>();
+      asm volatile("" ::: "memory");
+      if (masked) {
+        // 0 times an infinity or NaN is NaN: a key that only some of the rows
+        // see must not reach the others.  Such values are added to the rows
+        // that see them and are zero for the products below.
+        const f32x4* const vt = (const f32x4*)(ring + (NB + buf) * kTile);
+        uint32_t odd = 0;
+#pragma unroll
+        for (int i = 0; i < kTile / 1024; ++i) {
+          const f32x4 w = vt[64 * i + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t x = __float_as_uint(w[e]);
+            odd |= (uint32_t)((x & 0x7f800000u) == 0x7f800000u);
+            if (BF) odd |= (uint32_t)((x & 0x7f80u) == 0x7f80u);
+          }
+        }
+        if (__ballot(odd != 0)) {
+          for (int kk = 0; kk < kPagedKeys; ++kk) {
+            float pk = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pk = i == (kk >> 3) * 4 + (kk & 3) ? s[i] : pk;
+            const float other = swap_half(pk);
+            if (((kk >> 2) & 1) != u) pk = other;
+            const bool vis = visible(key0 + kk);
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float v = (float)*v_at(buf, kk, 32 * dt + 8 * (i >> 2) + 4 * u + (i & 3));
+                const bool finite = (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u;
+                o[dt][i] += (finite | !vis) ? 0.0f : pk * v;
+              }
+          }
+          wave_lds_sync();
+          for (int i = lane; i < kPagedKeys * D; i += 64) {
+            T* const x = (T*)(ring + (NB + buf) * kTile) + i;
+            const float v = (float)*x;
+            if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) *x = (T)0.0f;
+          }
+          wave_lds_sync();
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+      }
+      if constexpr (BF) {
+        const int va = lds_ring + (NB + buf) * kTile;
+        constexpr int kGrp = 4;
+        pipe::i32x2 f[2][kGrp][2];
+        auto issue = [&](auto g_c) {
+          constexpr int G = decltype(g_c)::value;
+          static_for<kGrp>([&](auto e_c) {
+            constexpr int E = decltype(e_c)::value, J = G * kGrp + E;
+            constexpr int OFF = 16 * (J / NDT) * kRB;
+            f[G & 1][E][0] = pipe::read_tr<OFF>(va + voff[J % NDT]);
+            f[G & 1][E][1] = pipe::read_tr<OFF + 8 * kRB>(va + voff[J % NDT]);
+          });
+        };
+        issue(std::integral_constant<int, 0>{});
+        static_for<F::NPV / kGrp>([&](auto g_c) {
+          constexpr int G = decltype(g_c)::value;
+          static_for<kGrp>([&](auto e_c) {
+            constexpr int E = decltype(e_c)::value;
+            pipe::wait_tr<0>(f[G & 1][E][0], f[G & 1][E][1]);
+          });
+          if constexpr (G + 1 < F::NPV / kGrp) issue(std::integral_constant<int, G + 1>{});
+          static_for<kGrp>([&](auto e_c) {
+            constexpr int E = decltype(e_c)::value;
+            const bf16x4 lo = __builtin_bit_cast(bf16x4, f[G & 1][E][0]), hi = __builtin_bit_cast(bf16x4, f[G & 1][E][1]);
+            F::pv_mfma(bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, G * kGrp + E, p, o);
+          });
+        });
+      } else if (!exact) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = p.v[8 * h + e];
+          bf16x8 pp[3];
+          bf16_parts(x, pp);
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) {
+            // B slot 8 u' + e of half h is key 16 h + 8 (e / 4) + 4 u' + e % 4
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (float)*v_at(buf, 16 * h + 8 * (e >> 2) + 4 * u + (e & 3), dt * 32 + n);
+            bf16x8 vp[3];
+            bf16_parts(x, vp);
+            o[dt] = parts_mma(vp, pp, o[dt]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt)
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32((float)*v_at(buf, 8 * (i >> 2) + 4 * u + (i & 3), dt * 32 + n), ((const float*)&p)[i], o[dt], 0, 0, 0);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(c + NB * kWaves, 1, buf);
+      __builtin_amdgcn_sched_barrier(0);
+      c += kWaves;
+    };
+    while (c < c_end) {
+      step(0);
+      if constexpr (NB == 2) {
+        if (c >= c_end) break;
+        step(1);
+      }
+    }
+    // loads past the end still write zeros into LDS
+    pipe::wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    }
+    if constexpr (BF) break;
+    float t = l_run * 0.0f + m_run * 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t += o[dt][i] * 0.0f;
+    if (exact || !__any(!(t == 0.0f))) break;
+    exact = true;
+    reset();
+  }
+
+  // ---- join the waves' partial results through LDS
+  const float l = pair_sum(l_run) + (bad_page ? __builtin_nanf("") : 0.0f);
+  __syncthreads();  // every wave is done with its part of the ring
+  float* const ob = (float*)lds;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4)
+      *(f32x4*)(ob + (wave * 32 + n) * RS + dt * 32 + 8 * q4 + 4 * u) = f32x4{o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]};
+  if (u == 0) ml[wave * 32 + n] = make_float2(m_run, l);
+  __syncthreads();
+  const int slots = it.n_rows << gs;
+  constexpr int kCols = D / 4;  // 4-column units of a slot
+  const bool split = it.n_parts > 1;
+  // records of the tile's parts, [slot][D] then [slot] (m, l)
+  constexpr int kRec = kPagedSlots * (D + 2);
+  float* const rec0 = (float*)(a.work + a.records_off) + ((int64_t)it.rec * a.hkv + kvh) * kRec;
+  const int64_t rec_step = (int64_t)a.hkv * kRec;
+  auto put = [&](int slot, int col, const f32x4& x, float L) {
+    T* const op = (T*)a.out + (int64_t)(it.row0 + (slot >> gs)) * a.o_st + (int64_t)(kvh * a.g + (slot & (a.g - 1))) * a.o_sh + col;
+    // a row that sees no key is 0; a sum that is NaN makes its row NaN
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = L == 0.0f ? 0.0f : x[e] / L;
+    store_vec4<T>(op, v);
+  };
+  for (int i = tid; i < slots * kCols; i += kThreads) {
+    const int slot = i / kCols, col = 4 * (i % kCols);
+    float M = -INFINITY, L = 0.0f;
+    f32x4 x = f32x4{};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, ml[w * 32 + slot].x);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float2 v = ml[w * 32 + slot];
+      const float f = fast_exp2(v.x - M);
+      L += f * v.y;
+      x += f * *(const f32x4*)(ob + (w * 32 + slot) * RS + col);
+    }
+    if (!split) {
+      put(slot, col, x, L);
+    } else {
+      float* const rec = rec0 + it.part * rec_step;
+      *(f32x4*)(rec + slot * D + col) = x;
+      if (col == 0) *(float2*)(rec + kPagedSlots * D + 2 * slot) = make_float2(M, L);
+    }
+  }
+  if (!split) return;
+  __threadfence();
+  __syncthreads();
+  int32_t* const counter = (int32_t*)(a.work + a.counters_off) + (int64_t)it.split * a.hkv + kvh;
+  if (tid == 0) last_s = atomicAdd(counter, 1) == it.n_parts - 1;
+  __syncthreads();
+  if (!last_s) return;
+  __threadfence();
+  for (int i = tid; i < slots * kCols; i += kThreads) {
+    const int slot = i / kCols, col = 4 * (i % kCols);
+    float M = -INFINITY, L = 0.0f;
+    f32x4 x = f32x4{};
+    for (int p = 0; p < it.n_parts; ++p) M = fmaxf(M, rec0[p * rec_step + kPagedSlots * D + 2 * slot]);
+    for (int p = 0; p < it.n_parts; ++p) {
+      const float* const rec = rec0 + p * rec_step;
+      const float2 v = *(const float2*)(rec + kPagedSlots * D + 2 * slot);
+      const float f = fast_exp2(v.x - M);
+      L += f * v.y;
+      x += f * *(const f32x4*)(rec + slot * D + col);
+    }
+    put(slot, col, x, L);
+  }
+  if (tid == 0) *counter = 0;  // for the next call with this plan
+}
+
+template <typename T, int D>
+int32_t launch(const PagedArgs& a, int32_t items, hipStream_t stream) {
+  hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)((int64_t)items * a.hkv)), dim3(kThreads), 0, stream, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return cev_fail(CEV_ERR_HIP, "paged attention launch: %s", hipGetErrorString(e));
+  return CEV_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t cev_paged_attention(const cev_paged_desc* d, const void* q, const void* k_cache, const void* v_cache,
+                                       const int32_t* block_table, void* out, void* work, size_t work_bytes, cev_stream stream) {
+  PagedBounds b;
+  const int32_t rc = cev_paged_bounds(d, &b);
+  if (rc) return rc;
+  CEV_CHECK_ARG(q && k_cache && v_cache && block_table && out && work, "cev_paged_attention: null argument");
+  CEV_CHECK_ARG((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)work) & 15) == 0 &&
+                    ((uintptr_t)block_table & 3) == 0,
+                "cev_paged_attention: device buffers must be 16-byte aligned");
+  if (work_bytes < b.bytes) return cev_fail(CEV_ERR_SPACE, "cev_paged_attention: work buffer of %zu bytes, %zu needed", work_bytes, b.bytes);
+  PagedArgs a;
+  a.q = q;
+  a.kc = k_cache;
+  a.vc = v_cache;
+  a.bt = block_table;
+  a.out = out;
+  a.work = (char*)work;
+  a.items_off = b.items_off;
+  a.counters_off = b.counters_off;
+  a.records_off = b.records_off;
+  a.q_st = d->q_stride_t;
+  a.q_sh = d->q_stride_h;
+  a.kc_sp = d->kc_stride_p;
+  a.kc_st = d->kc_stride_t;
+  a.kc_sh = d->kc_stride_h;
+  a.vc_sp = d->vc_stride_p;
+  a.vc_st = d->vc_stride_t;
+  a.vc_sh = d->vc_stride_h;
+  a.o_st = d->o_stride_t;
+  a.o_sh = d->o_stride_h;
+  a.bt_stride = d->bt_stride;
+  a.hkv = d->n_kv_heads;
+  a.g = d->n_q_heads / d->n_kv_heads;
+  a.t = d->t;
+  a.n_requests = d->n_requests;
+  a.page_shift = __builtin_ctz((unsigned)d->page_size);
+  a.n_pages = d->n_pages;
+  a.max_pages = d->max_pages;
+  a.window = d->window;
+  a.sinks = d->sinks;
+  a.scale_log2 = d->scale * 1.4426950408889634f;
+  a.sig = b.sig;
+  const hipStream_t s = (hipStream_t)stream;
+  if (d->dtype == CEV_F32) return launch<float, 128>(a, b.items, s);
+  return d->head_dim == 128 ? launch<__bf16, 128>(a, b.items, s) : launch<__bf16, 256>(a, b.items, s);
+}

@@ -18,7 +18,9 @@
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 
+#include <initializer_list>
 #include <string>
+#include <utility>
 
 #include "../../include/cev_hip.h"
 
@@ -35,6 +37,11 @@ struct Api {
   decltype(&cev_linear) linear;
   decltype(&cev_gather_rows) gather_rows;
   decltype(&cev_gdn_forward) gdn_forward;
+  decltype(&cev_paged_tables) paged_tables;
+  decltype(&cev_rope_desc_init) rope_desc_init;
+  decltype(&cev_rope) rope;
+  decltype(&cev_paged_plan) paged_plan;
+  decltype(&cev_paged_attention) paged_attention;
   decltype(&cev_last_error) last_error;
 } api;
 PyObject* cev_error = nullptr;  // cev_hip.CevError
@@ -363,6 +370,197 @@ PyObject* py_gdn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// The operands of a paged-cache call: all on one GPU, which is current (and
+// whose current stream is taken) for the call.
+struct OnDevice {
+  c10::OptionalDeviceGuard guard;
+  c10::Device device = c10::Device(c10::kCPU);
+  OnDevice(const char* call, std::initializer_list<std::pair<const char*, const at::Tensor*>> ts) {
+    const char* first = nullptr;
+    for (const auto& [name, t] : ts) {
+      if (!t) continue;
+      if (!t->is_cuda()) raise_cev(CEV_ERR_INVALID, std::string(call) + ": " + name + " must be on the GPU");
+      if (!first) {
+        first = name;
+        device = t->device();
+      } else if (t->device() != device) {
+        raise_cev(CEV_ERR_INVALID, std::string(call) + ": " + name + " and " + first + " are on different devices");
+      }
+    }
+    guard.reset_device(device);
+  }
+  void* stream(PyObject* o) const { return o == Py_None ? (void*)c10::hip::getCurrentHIPStream(device.index()).stream() : stream_of(o); }
+};
+
+void want(bool ok, const char* call, const std::string& msg) {
+  if (!ok) raise_cev(CEV_ERR_INVALID, std::string(call) + ": " + msg);
+}
+void want_i32(const char* call, const char* name, const at::Tensor* t, int64_t size) {
+  if (!t) return;
+  want(t->scalar_type() == at::kInt && t->dim() == 1 && t->is_contiguous() && t->size(0) == size, call,
+       std::string(name) + " must be contiguous int32 of " + std::to_string(size) + " values");
+}
+int32_t fits_i32(const char* call, const char* name, int64_t x) {
+  want(x >= INT32_MIN && x <= INT32_MAX, call, std::string(name) + " " + std::to_string(x) + " does not fit 32 bits");
+  return (int32_t)x;
+}
+// The block table's row stride.
+int64_t block_table_stride(const char* call, const at::Tensor& bt, int64_t n_requests) {
+  want(bt.scalar_type() == at::kInt && bt.dim() == 2 && bt.size(0) == n_requests && bt.size(1) >= 1 && (bt.size(1) == 1 || bt.stride(1) == 1), call,
+       "block_table must be int32 (" + std::to_string(n_requests) + ", pages) with unit last stride");
+  return n_requests == 1 ? bt.size(1) : bt.stride(0);
+}
+
+// paged_tables(lengths, new_len, block_table, page_size, cu, pos, slots, n_pages, free, ring, lengths_out, ring_out, stream)
+PyObject* py_paged_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    need_args(n, 13);
+    const char* const me = "paged_tables";
+    const at::Tensor &len = tensor(a[0], "lengths"), &add = tensor(a[1], "new_len"), &bt = tensor(a[2], "block_table"),
+                     &cu = tensor(a[4], "cu"), &pos = tensor(a[5], "pos"), &slots = tensor(a[6], "slots"), &ring = tensor(a[9], "ring"),
+                     &len_out = tensor(a[10], "lengths_out"), &ring_out = tensor(a[11], "ring_out");
+    const at::Tensor* const free = tensor_or_none(a[8], "free");
+    want(len.dim() == 1, me, "lengths must be int32 (requests)");
+    const int64_t R = len.size(0);
+    want_i32(me, "lengths", &len, R);
+    want_i32(me, "new_len", &add, R);
+    want_i32(me, "lengths_out", &len_out, R);
+    want_i32(me, "cu", &cu, R + 1);
+    want(pos.dim() == 1, me, "pos must be int32 (tokens)");
+    want_i32(me, "pos", &pos, pos.size(0));
+    want_i32(me, "slots", &slots, pos.size(0));
+    want_i32(me, "ring", &ring, 4);
+    want_i32(me, "ring_out", &ring_out, 4);
+    const int64_t n_pages = as_int(a[7]), page_size = as_int(a[3]);
+    want_i32(me, "free", free, n_pages);
+    const int64_t stride = block_table_stride(me, bt, R);
+    const OnDevice dev(me, {{"lengths", &len}, {"new_len", &add}, {"block_table", &bt}, {"cu", &cu}, {"pos", &pos}, {"slots", &slots},
+                            {"ring", &ring}, {"lengths_out", &len_out}, {"ring_out", &ring_out}, {"free", free}});
+    void* const s = dev.stream(a[12]);
+    const int32_t r32 = fits_i32(me, "requests", R), ps = fits_i32(me, "page_size", page_size), np = fits_i32(me, "n_pages", n_pages),
+                  mp = fits_i32(me, "pages of a request", bt.size(1)), mt = fits_i32(me, "tokens", pos.size(0));
+    call([&] {
+      return api.paged_tables(r32, ps, np, mp, mt, (const int32_t*)ptr(len), (const int32_t*)ptr(add), (int32_t*)ptr(bt), stride,
+                              (int32_t*)ptr(free), (const int32_t*)ptr(ring), (int32_t*)ptr(len_out), (int32_t*)ptr(ring_out),
+                              (int32_t*)ptr(cu), (int32_t*)ptr(pos), (int32_t*)ptr(slots), s);
+    });
+  });
+}
+
+// rope(q_in, k_in, v_in, pos, steps, rotary_dim, factor, interleaved, transposed, slots, q_out, k_out, v_out, stream)
+PyObject* py_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    need_args(n, 14);
+    const char* const me = "rope";
+    const at::Tensor &q = tensor(a[0], "q_in"), &k = tensor(a[1], "k_in"), &pos = tensor(a[3], "pos"), &steps = tensor(a[4], "steps"),
+                     &qo = tensor(a[10], "q_out"), &ko = tensor(a[11], "k_out");
+    const at::Tensor *const v = tensor_or_none(a[2], "v_in"), *const slots = tensor_or_none(a[9], "slots"),
+                     *const vo = tensor_or_none(a[12], "v_out");
+    want(q.dim() == 3 && k.dim() == 3 && k.size(0) == q.size(0) && k.size(2) == q.size(2), me, "q_in must be (t, hq, d) and k_in (t, hkv, d)");
+    const int64_t t = q.size(0), rotary = as_int(a[5]);
+    const int dt = dtype_code(q);
+    const at::Tensor* const all[] = {&q, &k, v, &qo, &ko, vo};
+    for (const at::Tensor* x : all) {
+      if (!x) continue;
+      want(x->scalar_type() == q.scalar_type(), me, "q, k and v must share the dtype");
+      rows_contiguous(*x);
+    }
+    want(qo.sizes().equals(q.sizes()), me, "q_out must have q_in's shape");
+    want((v == nullptr) == (vo == nullptr), me, "v_in and v_out go together");
+    want(!v || v->sizes().equals(k.sizes()), me, "v_in must have k_in's shape");
+    want_i32(me, "pos", &pos, t);
+    want_i32(me, "slots", slots, t);
+    want(steps.scalar_type() == at::kLong && steps.is_contiguous() && steps.numel() == rotary / 2, me, "steps must be the rotary_dim / 2 values of RotaryAngles");
+    int64_t page = 0, n_slots = 0;
+    for (const at::Tensor* x : {&ko, vo}) {
+      if (!x) continue;
+      if (!slots) {
+        want(x->sizes().equals(k.sizes()), me, "k_out and v_out must have k_in's shape");
+      } else {
+        want(x->dim() == 4 && x->size(2) == k.size(1) && x->size(3) == k.size(2) && x->size(0) == ko.size(0) && x->size(1) == ko.size(1), me,
+             "with slots k_out and v_out must be (pages, page_size, hkv, d) caches");
+        page = x->size(1);
+        n_slots = x->size(0) * x->size(1);
+      }
+    }
+    cev_rope_desc d;
+    check(api.rope_desc_init(&d, dt, fits_i32(me, "q heads", q.size(1)), fits_i32(me, "kv heads", k.size(1)), fits_i32(me, "head_dim", q.size(2)),
+                             fits_i32(me, "tokens", t), fits_i32(me, "rotary_dim", rotary), fits_i32(me, "page_size", page),
+                             fits_i32(me, "slots", n_slots)));
+    d.factor = (float)as_double(a[6]);
+    d.interleaved = as_bool(a[7]) ? 1 : 0;
+    d.transposed = as_bool(a[8]) ? 1 : 0;
+    d.qi_stride_t = q.stride(0), d.qi_stride_h = q.stride(1);
+    d.ki_stride_t = k.stride(0), d.ki_stride_h = k.stride(1);
+    d.qo_stride_t = qo.stride(0), d.qo_stride_h = qo.stride(1);
+    if (v) d.vi_stride_t = v->stride(0), d.vi_stride_h = v->stride(1);
+    const int s0 = slots ? 1 : 0;  // a cache's strides follow its page stride
+    d.ko_stride_p = slots ? ko.stride(0) : 0, d.ko_stride_t = ko.stride(s0), d.ko_stride_h = ko.stride(s0 + 1);
+    if (vo) d.vo_stride_p = slots ? vo->stride(0) : 0, d.vo_stride_t = vo->stride(s0), d.vo_stride_h = vo->stride(s0 + 1);
+    const OnDevice dev(me, {{"q_in", &q}, {"k_in", &k}, {"v_in", v}, {"pos", &pos}, {"steps", &steps}, {"slots", slots}, {"q_out", &qo},
+                            {"k_out", &ko}, {"v_out", vo}});
+    void* const s = dev.stream(a[13]);
+    call([&] {
+      return api.rope(&d, ptr(q), ptr(k), ptr(v), (const int32_t*)ptr(pos), (const uint64_t*)ptr(steps), (const int32_t*)ptr(slots), ptr(qo),
+                      ptr(ko), ptr(vo), s);
+    });
+  });
+}
+
+const cev_paged_desc* paged_desc(const Bytes& b) {
+  if (b.b.len != (Py_ssize_t)sizeof(cev_paged_desc)) raise_py(PyExc_TypeError, "desc must be a PagedDesc");
+  return (const cev_paged_desc*)b.b.buf;
+}
+
+// paged_plan(desc, cu, lengths, work, stream)
+PyObject* py_paged_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    need_args(n, 5);
+    const char* const me = "paged attention plan";
+    const Bytes desc(a[0], false);
+    const cev_paged_desc d = *paged_desc(desc);
+    const at::Tensor &cu = tensor(a[1], "cu"), &len = tensor(a[2], "lengths"), &work = tensor(a[3], "work");
+    want_i32(me, "cu", &cu, (int64_t)d.n_requests + 1);
+    want_i32(me, "lengths", &len, d.n_requests);
+    const OnDevice dev(me, {{"work", &work}, {"cu", &cu}, {"lengths", &len}});
+    void* const s = dev.stream(a[4]);
+    call([&] { return api.paged_plan(&d, (const int32_t*)ptr(cu), (const int32_t*)ptr(len), ptr(work), work.nbytes(), s); });
+  });
+}
+
+// paged_attention(desc, q, k_cache, v_cache, block_table, out, work, stream): with the tensors' strides in desc's place
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    need_args(n, 8);
+    const char* const me = "paged attention";
+    const Bytes desc(a[0], false);
+    cev_paged_desc d = *paged_desc(desc);
+    const at::Tensor &q = tensor(a[1], "q"), &kc = tensor(a[2], "k_cache"), &vc = tensor(a[3], "v_cache"), &bt = tensor(a[4], "block_table"),
+                     &out = tensor(a[5], "out"), &work = tensor(a[6], "work");
+    const auto type = d.dtype == CEV_BF16 ? at::kBFloat16 : at::kFloat;
+    for (const at::Tensor* x : {&q, &kc, &vc, &out}) {
+      want(x->scalar_type() == type, me, "q, the caches and out must be of the type it was made for");
+      rows_contiguous(*x);
+    }
+    for (const at::Tensor* x : {&q, &out})
+      want(x->dim() == 3 && x->size(0) == d.t && x->size(1) == d.n_q_heads && x->size(2) == d.head_dim, me,
+           "q and out must be (" + std::to_string(d.t) + ", " + std::to_string(d.n_q_heads) + ", " + std::to_string(d.head_dim) + ")");
+    for (const at::Tensor* x : {&kc, &vc})
+      want(x->dim() == 4 && x->size(0) == d.n_pages && x->size(1) == d.page_size && x->size(2) == d.n_kv_heads && x->size(3) == d.head_dim, me,
+           "the caches must be (" + std::to_string(d.n_pages) + ", " + std::to_string(d.page_size) + ", " + std::to_string(d.n_kv_heads) + ", " +
+               std::to_string(d.head_dim) + ")");
+    d.bt_stride = block_table_stride(me, bt, d.n_requests);
+    want(bt.size(1) == d.max_pages, me, "block_table must have " + std::to_string(d.max_pages) + " entries a request");
+    d.q_stride_t = q.stride(0), d.q_stride_h = q.stride(1);
+    d.o_stride_t = out.stride(0), d.o_stride_h = out.stride(1);
+    d.kc_stride_p = kc.stride(0), d.kc_stride_t = kc.stride(1), d.kc_stride_h = kc.stride(2);
+    d.vc_stride_p = vc.stride(0), d.vc_stride_t = vc.stride(1), d.vc_stride_h = vc.stride(2);
+    const OnDevice dev(me, {{"work", &work}, {"q", &q}, {"k_cache", &kc}, {"v_cache", &vc}, {"block_table", &bt}, {"out", &out}});
+    void* const s = dev.stream(a[7]);
+    call([&] { return api.paged_attention(&d, ptr(q), ptr(kc), ptr(vc), (const int32_t*)ptr(bt), ptr(out), ptr(work), work.nbytes(), s); });
+  });
+}
+
 // bind(error_class, {symbol: address})
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&] {
@@ -384,6 +582,11 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     get("cev_linear", api.linear);
     get("cev_gather_rows", api.gather_rows);
     get("cev_gdn_forward", api.gdn_forward);
+    get("cev_paged_tables", api.paged_tables);
+    get("cev_rope_desc_init", api.rope_desc_init);
+    get("cev_rope", api.rope);
+    get("cev_paged_plan", api.paged_plan);
+    get("cev_paged_attention", api.paged_attention);
     get("cev_last_error", api.last_error);
     Py_INCREF(a[0]);
     cev_error = a[0];
@@ -392,7 +595,8 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define CEV_METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {CEV_METHOD(bind),   CEV_METHOD(qknorm_rope), CEV_METHOD(attention),   CEV_METHOD(rms_norm), CEV_METHOD(swiglu),
-                         CEV_METHOD(linear), CEV_METHOD(gather_rows), CEV_METHOD(gdn), {nullptr, nullptr, 0, nullptr}};
+                         CEV_METHOD(linear), CEV_METHOD(gather_rows), CEV_METHOD(gdn), CEV_METHOD(paged_tables), CEV_METHOD(rope),
+                         CEV_METHOD(paged_plan), CEV_METHOD(paged_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_cev_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
