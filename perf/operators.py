@@ -403,12 +403,12 @@ def run(s):
             if not case["store"]:
                 q, k = cev.rope(s["q"], s["k"], s["pos"], s["rot"], interleaved=case["interleaved"], transposed=True)
                 return {"q": q, "k": k}
-            q, _ = cev.rope(s["q"], s["k"], s["pos"], s["rot"], interleaved=case["interleaved"], v_in=s["v"], k_out=s["k_cache"],
+            q, _, _ = cev.rope(s["q"], s["k"], s["pos"], s["rot"], interleaved=case["interleaved"], v_in=s["v"], k_out=s["k_cache"],
                             v_out=s["v_cache"], slots=s["slots"])
             return {"q": q, "k_cache": s["k_cache"], "v_cache": s["v_cache"]}
         q, lengths = s["q"], s["lengths"]
         if kind == "step":
-            q, _ = cev.rope(q, s["k"], s["pos"], s["rot"], v_in=s["v"], k_out=s["k_cache"], v_out=s["v_cache"], slots=s["slots"])
+            q, _, _ = cev.rope(q, s["k"], s["pos"], s["rot"], v_in=s["v"], k_out=s["k_cache"], v_out=s["v_cache"], slots=s["slots"])
             lengths = s["lengths_out"]
         attention = s["attention"]
         attention.plan(s["cu"], lengths)
