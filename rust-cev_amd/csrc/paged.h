@@ -27,7 +27,7 @@ static_assert(sizeof(PagedHeader) == 16 && sizeof(PagedItem) == 48, "work buffer
 
 constexpr int kPagedSlots = 32;     // query slots (rows x heads of a group) of an item
 constexpr int kPagedKeys = 32;      // keys of a sub-tile
-constexpr int kPagedTarget = 512;   // workgroups that a launch is split into (two for each CU)
+constexpr int kPagedTarget = 4096;   // workgroups that a launch is split into (two for each CU)
 constexpr int kPagedMaxRequests = 4096;
 
 // What a descriptor bounds: sizes and offsets of the work buffer's parts.

@@ -50,6 +50,17 @@ __device__ void paged_poison(const PagedArgs& a) {
   }
 }
 
+// Partial results go between workgroups of any XCD: stores past the XCD's own
+// L2 and loads past it (relaxed atomics of agent scope).  Fences in their place
+// write back and drop the whole L2: a decoding batch's attention took 334 us
+// with 512 parts and 1019 with 4096.
+__device__ __forceinline__ void put_shared(float* p, float2 v) {
+  __hip_atomic_store((uint64_t*)p, __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get_shared(const float* p) {
+  return __builtin_bit_cast(float2, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
 // f32 values as sums of three bf16 parts and the six large part products
 // (see fan_attn.hip).
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -84,15 +95,41 @@ __device__ __forceinline__ int v_place(int blk, int row) {
   return sizeof(T) == 2 ? blk ^ ((row & 3) << 2) : blk ^ (((row >> 2) & 1) << 3);
 }
 
+// Operand reads through asm: the compiler places a wait for every load in
+// flight before each LDS read that it emits itself (it cannot tell the
+// buffers apart), which would drain the fetches ahead.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+template <int OFF>
+__device__ __forceinline__ i32x4 read_b128(int vaddr) {
+  static_assert(OFF >= 0 && OFF < 65536, "ds offset field");
+  i32x4 r;
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(vaddr), "i"(OFF) : "memory");
+  return r;
+}
+template <int OFF>
+__device__ __forceinline__ float read_b32(int vaddr) {
+  static_assert(OFF >= 0 && OFF < 65536, "ds offset field");
+  float r;
+  asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(r) : "v"(vaddr), "i"(OFF) : "memory");
+  return r;
+}
+// Every LDS read has returned, and r holds its value.
+template <typename R>
+__device__ __forceinline__ void wait_read(R& r) {
+  asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(r));
+}
+
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) void paged_attn_kernel(PagedArgs a) {
+constexpr int kMinWaves = sizeof(T) == 2 && D == 128 ? 2 : 1;
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWaves<T, D>))) void paged_attn_kernel(PagedArgs a) {
   using F = Frag<T, D>;
   constexpr bool BF = sizeof(T) == 2;
   constexpr int NDT = D / 32;
   constexpr int kRB = D * (int)sizeof(T);        // bytes of one key row
   constexpr int kTile = kPagedKeys * kRB;        // K or V of a sub-tile
   constexpr int kLoads = kTile / 1024;           // 1 KB loads of it
-  constexpr int NB = kRB == 256 ? 2 : 1;         // sub-tiles of K and of V in LDS
+  constexpr int NB = 1;         // sub-tiles of K and of V in LDS
   constexpr int kRows = 1024 / kRB, kBlk = kRB / 16;  // rows of one load, 16-byte blocks of a row
   constexpr int RS = D + 4;                      // row stride (floats) of a partial result in LDS
   constexpr int kRing = kWaves * 2 * NB * kTile, kOut = kWaves * 32 * RS * 4;
@@ -161,21 +198,30 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) v
   bool bad_page = false;
   char* const ring = lds + wave * 2 * NB * kTile;
   const int lds_ring = (int)(size_t)(const __attribute__((address_space(3))) char*)ring;
-  // Row of a load's lane within the sub-tile, and its block there.
+  // Byte offset of this lane's 16 bytes in load i of either half of a sub-tile.
   const int ld_row = lane / kBlk, ld_blk = lane % kBlk;
+  int k_at[kLoads / 2], v_at_off[kLoads / 2];
+#pragma unroll
+  for (int i = 0; i < kLoads / 2; ++i) {
+    const int r = kRows * i + ld_row;
+    k_at[i] = r * kr + (k_place(ld_blk, r) << 4);
+    v_at_off[i] = r * vr + (v_place<T>(ld_blk, r) << 4);
+  }
 
   // K (which = 0) or V (1) of sub-tile c into buffer buf; past the end: zeros.
-  auto fetch = [&](int c, int which, int buf) {
+  auto fetch = [&](int c, auto which_c, int buf) {
+    constexpr int which = decltype(which_c)::value;
     const bool real = c < c_end;
     if (real && which == 0 && c >= batch_first + kWaves * 64) load_pages(c);
     const int key0 = real ? first_key(c) : 0;
     const int l = real ? (c - batch_first) / kWaves : 0;
     const int stride = which ? vr : kr;
     const int64_t page_bytes = (which ? a.vc_sp : a.kc_sp) * (int64_t)sizeof(T);
+    // every key of it is seen by some row of the item
+    const bool full = key0 + kPagedKeys <= span.end && !(key0 < span.skip_hi && key0 + kPagedKeys > span.skip_lo);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int first = key0 + 16 * half;
-      // keys that some row of the item sees
       const bool seen = real && first < span.end && !(first >= span.skip_lo && first + 16 <= span.skip_hi);
       int page = half ? __builtin_amdgcn_readlane(page_b, l) : __builtin_amdgcn_readlane(page_a, l);
       const bool in = (uint32_t)page < (uint32_t)a.n_pages;
@@ -183,17 +229,20 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) v
       page = in ? page : 0;
       const uint64_t base = (which ? vbase : kbase) + (uint64_t)(page * page_bytes) + (uint64_t)((first & ((1 << a.page_shift) - 1)) * (int64_t)stride);
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)uniform_u64(base), (short)0, uniform_i32(seen && in ? 16 * stride : 0), kBufferWord3);
+      char* const to = ring + (which * NB + buf) * kTile + half * (kTile / 2);
 #pragma unroll
       for (int i = 0; i < kLoads / 2; ++i) {
-        const int r = half * 16 + kRows * i + ld_row;  // row of the sub-tile
-        const int key = key0 + r;
-        const bool load = key < span.end && !(key >= span.skip_lo && key < span.skip_hi);
-        const int blk = which ? v_place<T>(ld_blk, r) : k_place(ld_blk, r);
-        const int off = load ? (r - half * 16) * stride + (blk << 4) : INT32_MAX;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(ring + (which * NB + buf) * kTile + 1024 * (half * (kLoads / 2) + i)), 16, off, 0, 0, 0);
+        int off = which ? v_at_off[i] : k_at[i];
+        if (!full) {
+          const int key = first + kRows * i + ld_row;
+          off = key < span.end && !(key >= span.skip_lo && key < span.skip_hi) ? off : INT32_MAX;
+        }
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(to + 1024 * i), 16, off, 0, 0, 0);
       }
     }
   };
+  using K_c = std::integral_constant<int, 0>;
+  using V_c = std::integral_constant<int, 1>;
 
   f32x16 o[NDT];
   float m_run, l_run;
@@ -204,11 +253,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) v
     l_run = 0.0f;
   };
   reset();
-  int voff[NDT];
-  if constexpr (BF) {
+  // Byte offsets of the operand reads within a sub-tile of K and of V.
+  int koff[8], voff[NDT];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) koff[j] = n * kRB + (k_place(BF ? 2 * j + u : 4 * (j >> 1) + 2 * u + (j & 1), n) << 4);
+  {
     const int i = lane & 15, rr = i >> 2, blk = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) voff[dt] = (4 * u + rr) * kRB + (v_place<T>(4 * dt + blk, rr) << 4) + 8 * (i & 1);
+    for (int dt = 0; dt < NDT; ++dt)
+      voff[dt] = BF ? (4 * u + rr) * kRB + (v_place<T>(4 * dt + blk, rr) << 4) + 8 * (i & 1)
+                    : 4 * u * kRB + (v_place<T>(8 * dt + n / 4, 4 * u) << 4) + 4 * (n & 3);
   }
   // A value of V in buffer buf.
   auto v_at = [&](int buf, int key, int col) -> T* {
@@ -224,8 +278,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) v
     load_pages(c);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      fetch(c + b * kWaves, 0, b);
-      fetch(c + b * kWaves, 1, b);
+      fetch(c + b * kWaves, K_c{}, b);
+      fetch(c + b * kWaves, V_c{}, b);
     }
     auto step = [&](int buf) {
       const int key0 = first_key(c);
@@ -233,27 +287,47 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) v
       pipe::wait_vmcnt<(2 * NB - 1) * kLoads>();
       asm volatile("" ::: "memory");
       f32x16 s = f32x16{};
-      const char* const kt = ring + buf * kTile + n * kRB;
-#pragma unroll
-      for (int st = 0; st < D / 16; ++st) {
+      // K operands in groups of four 16-byte reads, one group ahead of the MFMAs
+      constexpr int kKGrp = 4, kKReads = kRB / 32;
+      i32x4 kf[2][kKGrp];
+      const int ka = lds_ring + buf * kTile;
+      auto k_issue = [&](auto g_c) {
+        constexpr int G = decltype(g_c)::value;
+        static_for<kKGrp>([&](auto e_c) {
+          constexpr int J = G * kKGrp + decltype(e_c)::value;
+          // block 2 J + u (bf16), 4 (J / 2) + 2 u + J % 2 (f32); bit 4 of a block's place is its own
+          kf[G & 1][decltype(e_c)::value] = read_b128<(J / 8) * 256>(ka + koff[J % 8]);
+        });
+      };
+      k_issue(std::integral_constant<int, 0>{});
+      static_for<kKReads / kKGrp>([&](auto g_c) {
+        constexpr int G = decltype(g_c)::value;
+        static_for<kKGrp>([&](auto e_c) { wait_read(kf[G & 1][decltype(e_c)::value]); });
+        if constexpr (G + 1 < kKReads / kKGrp) k_issue(std::integral_constant<int, G + 1>{});
         if constexpr (BF) {
-          fr.qk_mfma(*(const bf16x8*)(kt + (k_place(2 * st + u, n) << 4)), st, s);
+          static_for<kKGrp>([&](auto e_c) {
+            constexpr int E = decltype(e_c)::value;
+            fr.qk_mfma(__builtin_bit_cast(bf16x8, kf[G & 1][E]), G * kKGrp + E, s);
+          });
         } else {
-          float x[8];
-          *(f32x4*)x = *(const f32x4*)(kt + (k_place(4 * st + 2 * u, n) << 4));
-          *(f32x4*)(x + 4) = *(const f32x4*)(kt + (k_place(4 * st + 2 * u + 1, n) << 4));
-          if (!exact) {
-            bf16x8 kp[3];
-            bf16_parts(x, kp);
-            s = parts_mma(kp, qp[st], s);
-          } else {
-            float q[8];
-            load_q8(st, q);
+          static_for<kKGrp / 2>([&](auto e_c) {
+            constexpr int E = decltype(e_c)::value, st = G * kKGrp / 2 + E;
+            float x[8];
+            __builtin_memcpy(x, &kf[G & 1][2 * E], 16);
+            __builtin_memcpy(x + 4, &kf[G & 1][2 * E + 1], 16);
+            if (!exact) {
+              bf16x8 kp[3];
+              bf16_parts(x, kp);
+              s = parts_mma(kp, qp[st], s);
+            } else {
+              float q[8];
+              load_q8(st, q);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], q[e], s, 0, 0, 0);
-          }
+              for (int e = 0; e < 8; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], q[e], s, 0, 0, 0);
+            }
+          });
         }
-      }
+      });
       asm volatile("" ::: "memory");
       const bool masked = key0 + kPagedKeys - 1 > it.pos0 ||
                           (a.window > 0 && key0 <= pos1 - a.window && key0 + kPagedKeys > a.sinks);
@@ -267,7 +341,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) v
       }
       // (s is made: K's buffer is free for the sub-tile NB ahead)
       __builtin_amdgcn_sched_barrier(0);
-      fetch(c + NB * kWaves, 0, buf);
+      fetch(c + NB * kWaves, K_c{}, buf);
       __builtin_amdgcn_sched_barrier(0);
       float mx = -INFINITY;
 #pragma unroll
@@ -358,34 +432,43 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) v
             F::pv_mfma(bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, G * kGrp + E, p, o);
           });
         });
-      } else if (!exact) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = p.v[8 * h + e];
-          bf16x8 pp[3];
-          bf16_parts(x, pp);
-#pragma unroll
-          for (int dt = 0; dt < NDT; ++dt) {
-            // B slot 8 u' + e of half h is key 16 h + 8 (e / 4) + 4 u' + e % 4
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (float)*v_at(buf, 16 * h + 8 * (e >> 2) + 4 * u + (e & 3), dt * 32 + n);
-            bf16x8 vp[3];
-            bf16_parts(x, vp);
-            o[dt] = parts_mma(vp, pp, o[dt]);
-          }
-        }
       } else {
+        // V values of step j = 4 h + dt, keys 16 h + 8 (e / 4) + 4 u + e % 4 of
+        // column 32 dt + n, one step ahead of the MFMAs
+        float vf[2][8];
+        const int va = lds_ring + (NB + buf) * kTile;
+        auto v_issue = [&](auto j_c) {
+          constexpr int J = decltype(j_c)::value, H = J / NDT, DT = J % NDT;
+          static_for<8>([&](auto e_c) {
+            constexpr int E = decltype(e_c)::value;
+            vf[J & 1][E] = read_b32<(16 * H + 8 * (E >> 2) + (E & 3)) * kRB>(va + voff[DT]);
+          });
+        };
+        bf16x8 pp[3];
+        v_issue(std::integral_constant<int, 0>{});
+        static_for<2 * NDT>([&](auto j_c) {
+          constexpr int J = decltype(j_c)::value, H = J / NDT, DT = J % NDT;
+          static_for<8>([&](auto e_c) { wait_read(vf[J & 1][decltype(e_c)::value]); });
+          if constexpr (J + 1 < 2 * NDT) v_issue(std::integral_constant<int, J + 1>{});
+          if (!exact) {
+            if constexpr (DT == 0) {
+              float x[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+              for (int e = 0; e < 8; ++e) x[e] = p.v[8 * H + e];
+              bf16_parts(x, pp);
+            }
+            bf16x8 vp[3];
+            bf16_parts(vf[J & 1], vp);
+            o[DT] = parts_mma(vp, pp, o[DT]);
+          } else {
 #pragma unroll
-          for (int dt = 0; dt < NDT; ++dt)
-            o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32((float)*v_at(buf, 8 * (i >> 2) + 4 * u + (i & 3), dt * 32 + n), ((const float*)&p)[i], o[dt], 0, 0, 0);
+            for (int e = 0; e < 8; ++e) o[DT] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[J & 1][e], p.v[8 * H + e], o[DT], 0, 0, 0);
+          }
+        });
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
-      fetch(c + NB * kWaves, 1, buf);
+      fetch(c + NB * kWaves, V_c{}, buf);
       __builtin_amdgcn_sched_barrier(0);
       c += kWaves;
     };
@@ -454,29 +537,32 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) v
       put(slot, col, x, L);
     } else {
       float* const rec = rec0 + it.part * rec_step;
-      *(f32x4*)(rec + slot * D + col) = x;
-      if (col == 0) *(float2*)(rec + kPagedSlots * D + 2 * slot) = make_float2(M, L);
+      put_shared(rec + slot * D + col, float2{x[0], x[1]});
+      put_shared(rec + slot * D + col + 2, float2{x[2], x[3]});
+      if (col == 0) put_shared(rec + kPagedSlots * D + 2 * slot, float2{M, L});
     }
   }
   if (!split) return;
-  __threadfence();
+  // The stores have reached memory before the workgroup counts itself.
+  __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   int32_t* const counter = (int32_t*)(a.work + a.counters_off) + (int64_t)it.split * a.hkv + kvh;
-  if (tid == 0) last_s = atomicAdd(counter, 1) == it.n_parts - 1;
+  if (tid == 0) last_s = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.n_parts - 1;
   __syncthreads();
   if (!last_s) return;
-  __threadfence();
   for (int i = tid; i < slots * kCols; i += kThreads) {
     const int slot = i / kCols, col = 4 * (i % kCols);
     float M = -INFINITY, L = 0.0f;
     f32x4 x = f32x4{};
-    for (int p = 0; p < it.n_parts; ++p) M = fmaxf(M, rec0[p * rec_step + kPagedSlots * D + 2 * slot]);
     for (int p = 0; p < it.n_parts; ++p) {
       const float* const rec = rec0 + p * rec_step;
-      const float2 v = *(const float2*)(rec + kPagedSlots * D + 2 * slot);
-      const float f = fast_exp2(v.x - M);
-      L += f * v.y;
-      x += f * *(const f32x4*)(rec + slot * D + col);
+      const float2 v = get_shared(rec + kPagedSlots * D + 2 * slot);
+      const float2 y = get_shared(rec + slot * D + col), z = get_shared(rec + slot * D + col + 2);
+      const float m = fmaxf(M, v.x);
+      const float f = fast_exp2(v.x - m), f0 = fast_exp2(M - m);
+      M = m;
+      L = L * f0 + f * v.y;
+      x = x * f0 + f * f32x4{y.x, y.y, z.x, z.y};
     }
     put(slot, col, x, L);
   }
