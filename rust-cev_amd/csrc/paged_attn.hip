@@ -1,5 +1,6 @@
 // Attention of each request's new tokens over a paged K/V cache.
 //
+// This file: requests with few new rows (one token to a short question).
 // A work item (cev_paged_plan) is up to 32 query slots (rows x the g query
 // heads of one KV head: slot -> row slot / g, head slot % g) and a run of the
 // 32-key sub-tiles that they see.  Its workgroup's four waves take the
@@ -15,28 +16,16 @@
 // keys past the end, in pages behind the window or not visible to any row of
 // the item get an offset out of the resource's range and read as zero.
 //
-// Items of one tile whose keys are split write partial results (f32); the last
-// of them to arrive (a counter per tile and KV head) joins all in their order,
-// so the result does not depend on who is last.
-#include "attn_device.h"
-#include "paged.h"
+// Pieces of a tile whose keys lie in several workgroups' runs write partial
+// results (f32); the last of them to arrive (a counter per tile and KV head)
+// joins all in their order, so the result does not depend on who is last.
+#include "paged_device.h"
 
 namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
-
-struct PagedArgs {
-  const void *q, *kc, *vc;
-  const int32_t* bt;
-  void* out;
-  char* work;
-  size_t items_off, counters_off, records_off;
-  int64_t q_st, q_sh, kc_sp, kc_st, kc_sh, vc_sp, vc_st, vc_sh, o_st, o_sh, bt_stride;
-  int32_t hkv, g, t, n_requests, page_shift, n_pages, max_pages, window, sinks;
-  float scale_log2;
-  uint32_t sig;
-};
+constexpr int kKeys = ::kPagedKeys[kPagedFew], kSlots = ::kPagedSlots[kPagedFew];
 
 // Workgroup b writes NaN over its share of out's rows.
 template <typename T, int D>
@@ -127,7 +116,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   constexpr bool BF = sizeof(T) == 2;
   constexpr int NDT = D / 32;
   constexpr int kRB = D * (int)sizeof(T);        // bytes of one key row
-  constexpr int kTile = kPagedKeys * kRB;        // K or V of a sub-tile
+  constexpr int kTile = kKeys * kRB;        // K or V of a sub-tile
   constexpr int kLoads = kTile / 1024;           // 1 KB loads of it
   constexpr int NB = 1;         // sub-tiles of K and of V in LDS
   constexpr int kRows = 1024 / kRB, kBlk = kRB / 16;  // rows of one load, 16-byte blocks of a row
@@ -138,14 +127,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   __shared__ int32_t last_s;
 
   const PagedHeader* const hdr = (const PagedHeader*)a.work;
-  const int32_t n_items = hdr->n_items;
   if (hdr->sig != a.sig || hdr->bad != 0) {
     paged_poison<T, D>(a);
     return;
   }
-  const int item = blockIdx.x / (uint32_t)a.hkv, kvh = blockIdx.x - item * a.hkv;
-  if (item >= n_items) return;
-  const PagedItem it = ((const PagedItem*)(a.work + a.items_off))[item];
+  const int run = blockIdx.x / (uint32_t)a.hkv, kvh = blockIdx.x - run * a.hkv;
+  if (run >= uniform_i32(hdr->n_parts[kPagedFew])) return;
+  int item_end;
+  for (int item = paged_first_item(a, run, item_end); item < item_end; ++item) {
+  const PagedItem it = paged_item(a, item);
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i32(tid >> 6);
   const int n = lane & 31, u = lane >> 5;
   const int gs = __builtin_ctz(a.g);
@@ -153,7 +143,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   const int row = it.row0 + (ok ? n >> gs : 0), head = kvh * a.g + (n & (a.g - 1));
   const int pos = ok ? it.pos0 + (n >> gs) : -1;
   const int pos1 = it.pos0 + it.n_rows - 1;
-  const PagedSpan span = paged_span<kPagedKeys>(it.pos0, pos1, a.window, a.sinks);
+  const PagedSpan span = paged_span(kKeys, it.pos0, pos1, a.window, a.sinks);
 
   // ---- Q, as the B operand
   const T* const qrow = (const T*)a.q + (int64_t)row * a.q_st + (int64_t)head * a.q_sh;
@@ -180,7 +170,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
 
   // ---- this wave's sub-tiles: c_begin + wave, + kWaves, ...
   const int c_end = it.c_end;
-  auto first_key = [&](int c) { return kPagedKeys * (c < span.sinks ? c : c - span.sinks + span.first); };
+  auto first_key = [&](int c) { return kKeys * (c < span.sinks ? c : c - span.sinks + span.first); };
   const int32_t* const bt = a.bt + it.req * a.bt_stride;
   const uint64_t kbase = (uint64_t)((const T*)a.kc + kvh * a.kc_sh), vbase = (uint64_t)((const T*)a.vc + kvh * a.vc_sh);
   const int kr = uniform_i32((int)(a.kc_st * (int64_t)sizeof(T))), vr = uniform_i32((int)(a.vc_st * (int64_t)sizeof(T)));
@@ -218,7 +208,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     const int stride = which ? vr : kr;
     const int64_t page_bytes = (which ? a.vc_sp : a.kc_sp) * (int64_t)sizeof(T);
     // every key of it is seen by some row of the item
-    const bool full = key0 + kPagedKeys <= span.end && !(key0 < span.skip_hi && key0 + kPagedKeys > span.skip_lo);
+    const bool full = key0 + kKeys <= span.end && !(key0 < span.skip_hi && key0 + kKeys > span.skip_lo);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int first = key0 + 16 * half;
@@ -329,14 +319,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
         }
       });
       asm volatile("" ::: "memory");
-      const bool masked = key0 + kPagedKeys - 1 > it.pos0 ||
-                          (a.window > 0 && key0 <= pos1 - a.window && key0 + kPagedKeys > a.sinks);
+      const bool masked = key0 + kKeys - 1 > it.pos0 ||
+                          (a.window > 0 && key0 <= pos1 - a.window && key0 + kKeys > a.sinks);
       auto visible = [&](int key) { return (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.sinks)); };
       if (masked) {
+        // bounds of the register's place, 8 (i / 4) + i % 4
+        const int k0 = key0 + 4 * (fresh_lane_id() >> 5), hi = pos - k0;
+        const int lo = a.window == 0 || pos < a.window ? INT32_MIN : pos - a.window - k0, first = a.sinks - k0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const bool vis = visible(key0 + 8 * (i >> 2) + 4 * u + (i & 3));
-          s[i] = vis ? s[i] : -INFINITY;
+          const int at = 8 * (i >> 2) + (i & 3);
+          s[i] = (at <= hi) & ((at > lo) | (at < first)) ? s[i] : -INFINITY;
         }
       }
       // (s is made: K's buffer is free for the sub-tile NB ahead)
@@ -365,7 +358,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       if (masked) {
         // 0 times an infinity or NaN is NaN: a key that only some of the rows
         // see must not reach the others.  Such values are added to the rows
-        // that see them and are zero for the products below.
+        // that see them (whatever their weight) and are zeros for the products.
         const f32x4* const vt = (const f32x4*)(ring + (NB + buf) * kTile);
         uint32_t odd = 0;
 #pragma unroll
@@ -379,12 +372,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
           }
         }
         if (__ballot(odd != 0)) {
-          for (int kk = 0; kk < kPagedKeys; ++kk) {
-            float pk = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pk = i == (kk >> 3) * 4 + (kk & 3) ? s[i] : pk;
-            const float other = swap_half(pk);
-            if (((kk >> 2) & 1) != u) pk = other;
+#pragma unroll 1
+          for (int kk = 0; kk < kKeys; ++kk) {
             const bool vis = visible(key0 + kk);
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt)
@@ -392,11 +381,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
               for (int i = 0; i < 16; ++i) {
                 const float v = (float)*v_at(buf, kk, 32 * dt + 8 * (i >> 2) + 4 * u + (i & 3));
                 const bool finite = (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u;
-                o[dt][i] += (finite | !vis) ? 0.0f : pk * v;
+                o[dt][i] += (finite | !vis) ? 0.0f : v;
               }
           }
           wave_lds_sync();
-          for (int i = lane; i < kPagedKeys * D; i += 64) {
+          for (int i = lane; i < kKeys * D; i += 64) {
             T* const x = (T*)(ring + (NB + buf) * kTile) + i;
             const float v = (float)*x;
             if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) *x = (T)0.0f;
@@ -507,9 +496,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   __syncthreads();
   const int slots = it.n_rows << gs;
   constexpr int kCols = D / 4;  // 4-column units of a slot
-  const bool split = it.n_parts > 1;
+  const bool split = it.n_pieces > 1;
   // records of the tile's parts, [slot][D] then [slot] (m, l)
-  constexpr int kRec = kPagedSlots * (D + 2);
+  constexpr int kRec = kSlots * (D + 2);
   float* const rec0 = (float*)(a.work + a.records_off) + ((int64_t)it.rec * a.hkv + kvh) * kRec;
   const int64_t rec_step = (int64_t)a.hkv * kRec;
   auto put = [&](int slot, int col, const f32x4& x, float L) {
@@ -536,27 +525,30 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     if (!split) {
       put(slot, col, x, L);
     } else {
-      float* const rec = rec0 + it.part * rec_step;
+      float* const rec = rec0 + it.piece * rec_step;
       put_shared(rec + slot * D + col, float2{x[0], x[1]});
       put_shared(rec + slot * D + col + 2, float2{x[2], x[3]});
-      if (col == 0) put_shared(rec + kPagedSlots * D + 2 * slot, float2{M, L});
+      if (col == 0) put_shared(rec + kSlots * D + 2 * slot, float2{M, L});
     }
   }
-  if (!split) return;
-  // The stores have reached memory before the workgroup counts itself.
+  // A split tile's stores have reached memory before the workgroup counts
+  // itself; and the ring is the next item's.
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
+  if (!split) continue;
   int32_t* const counter = (int32_t*)(a.work + a.counters_off) + (int64_t)it.split * a.hkv + kvh;
-  if (tid == 0) last_s = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.n_parts - 1;
+  if (tid == 0) last_s = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.n_pieces - 1;
   __syncthreads();
-  if (!last_s) return;
+  const bool last = last_s;
+  __syncthreads();
+  if (!last) continue;
   for (int i = tid; i < slots * kCols; i += kThreads) {
     const int slot = i / kCols, col = 4 * (i % kCols);
     float M = -INFINITY, L = 0.0f;
     f32x4 x = f32x4{};
-    for (int p = 0; p < it.n_parts; ++p) {
+    for (int p = 0; p < it.n_pieces; ++p) {
       const float* const rec = rec0 + p * rec_step;
-      const float2 v = get_shared(rec + kPagedSlots * D + 2 * slot);
+      const float2 v = get_shared(rec + kSlots * D + 2 * slot);
       const float2 y = get_shared(rec + slot * D + col), z = get_shared(rec + slot * D + col + 2);
       const float m = fmaxf(M, v.x);
       const float f = fast_exp2(v.x - m), f0 = fast_exp2(M - m);
@@ -567,11 +559,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     put(slot, col, x, L);
   }
   if (tid == 0) *counter = 0;  // for the next call with this plan
+  }
 }
 
 template <typename T, int D>
-int32_t launch(const PagedArgs& a, int32_t items, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)((int64_t)items * a.hkv)), dim3(kThreads), 0, stream, a);
+int32_t launch(const PagedArgs& a, int32_t target, hipStream_t stream) {
+  hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)(target * a.hkv)), dim3(kThreads), 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return cev_fail(CEV_ERR_HIP, "paged attention launch: %s", hipGetErrorString(e));
   return CEV_OK;
@@ -596,9 +589,6 @@ extern "C" int32_t cev_paged_attention(const cev_paged_desc* d, const void* q, c
   a.bt = block_table;
   a.out = out;
   a.work = (char*)work;
-  a.items_off = b.items_off;
-  a.counters_off = b.counters_off;
-  a.records_off = b.records_off;
   a.q_st = d->q_stride_t;
   a.q_sh = d->q_stride_h;
   a.kc_sp = d->kc_stride_p;
@@ -613,7 +603,6 @@ extern "C" int32_t cev_paged_attention(const cev_paged_desc* d, const void* q, c
   a.hkv = d->n_kv_heads;
   a.g = d->n_q_heads / d->n_kv_heads;
   a.t = d->t;
-  a.n_requests = d->n_requests;
   a.page_shift = __builtin_ctz((unsigned)d->page_size);
   a.n_pages = d->n_pages;
   a.max_pages = d->max_pages;
@@ -621,7 +610,19 @@ extern "C" int32_t cev_paged_attention(const cev_paged_desc* d, const void* q, c
   a.sinks = d->sinks;
   a.scale_log2 = d->scale * 1.4426950408889634f;
   a.sig = b.sig;
+  auto list = [&](int i) {
+    a.first_off = b.list[i].first_off;
+    a.items_off = b.list[i].items_off;
+    a.counters_off = b.list[i].counters_off;
+    a.records_off = b.list[i].records_off;
+    return b.list[i].target;
+  };
   const hipStream_t s = (hipStream_t)stream;
-  if (d->dtype == CEV_F32) return launch<float, 128>(a, b.items, s);
-  return d->head_dim == 128 ? launch<__bf16, 128>(a, b.items, s) : launch<__bf16, 256>(a, b.items, s);
+  if (const int32_t target = list(kPagedMany)) {
+    const int32_t rc = cev_paged_tile_launch(a, target, s);
+    if (rc) return rc;
+  }
+  const int32_t target = list(kPagedFew);
+  if (d->dtype == CEV_F32) return launch<float, 128>(a, target, s);
+  return d->head_dim == 128 ? launch<__bf16, 128>(a, target, s) : launch<__bf16, 256>(a, target, s);
 }

@@ -9,6 +9,12 @@ namespace {
 
 bool power_of_two(int32_t x) { return x > 0 && (x & (x - 1)) == 0; }
 
+// Workgroups that the keys of a launch are shared out to: as many as run at
+// once (256 CUs; two workgroups of the first kernel share one for bf16 heads
+// of 128, by their LDS).
+constexpr int32_t kFewWorkgroups128 = 512, kFewWorkgroups = 256, kManyWorkgroups = 256;
+constexpr int32_t kFewSlots = 128;
+
 size_t align_up(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // FNV-1a over the fields that a plan depends on.
@@ -87,21 +93,40 @@ int32_t cev_paged_bounds(const cev_paged_desc* d, PagedBounds* b) {
       return cev_fail(CEV_ERR_UNSUPPORTED, "paged attention: cache token stride %lld outside [head_dim, %lld]", (long long)s, (long long)row_max);
   CEV_CHECK_ARG(d->bt_stride >= 0 && (d->n_requests == 1 || d->bt_stride >= d->max_pages), "paged attention: block table stride %lld",
                 (long long)d->bt_stride);
-  b->rows = kPagedSlots / g;
-  b->target = kPagedTarget / d->n_kv_heads > 0 ? kPagedTarget / d->n_kv_heads : 1;
-  const int64_t by_request = (int64_t)d->n_requests * ((d->max_new + b->rows - 1) / b->rows);
-  const int64_t by_rows = d->t / b->rows + (int64_t)d->n_requests;
-  const int64_t items = (by_request < by_rows ? by_request : by_rows) + b->target;
-  if (items * d->n_kv_heads > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "paged attention: %lld work items are too many", (long long)items);
-  b->items = (int32_t)items;
   b->max_len = d->max_pages * d->page_size;
   b->sig = signature(d);
-  b->items_off = 256;
-  b->counters_off = align_up(b->items_off + sizeof(PagedItem) * (size_t)items);
-  b->records_off = align_up(b->counters_off + 4 * (size_t)b->target * d->n_kv_heads);
-  // a launch has at most `target` parts beyond one for each split tile, and
-  // at most `target` split tiles
-  b->bytes = b->records_off + 2 * (size_t)b->target * d->n_kv_heads * kPagedSlots * (d->head_dim + 2) * sizeof(float);
+  // Rows of requests with more than kFewSlots slots go to the kernel whose
+  // workgroups share their keys among 256 slots.
+  const bool tiles = d->dtype == CEV_BF16 && d->head_dim == 128;
+  const int32_t few = tiles ? kFewSlots / g : INT32_MAX;
+  size_t at = 256;
+  for (int i = 0; i < kPagedLists; ++i) {
+    PagedListBounds& l = b->list[i];
+    l.rows = kPagedSlots[i] / g;
+    l.min_new = i == kPagedFew ? 1 : few;
+    if (i == kPagedMany) l.min_new = few == INT32_MAX ? INT32_MAX : few + 1;
+    l.max_new = i == kPagedFew && few < d->max_new ? few : d->max_new;
+    const int32_t cus = i == kPagedFew ? (tiles ? kFewWorkgroups128 : kFewWorkgroups) : kManyWorkgroups;
+    l.target = cus / d->n_kv_heads > 0 ? cus / d->n_kv_heads : 1;
+    int64_t items = 0;
+    if (l.max_new >= l.min_new) {
+      // whole tiles, and a cut for each workgroup after the first
+      const int64_t by_request = (int64_t)d->n_requests * ((l.max_new + l.rows - 1) / l.rows);
+      const int64_t by_rows = d->t / l.rows + (int64_t)d->n_requests;
+      items = (by_request < by_rows ? by_request : by_rows) + l.target;
+      if (items > INT32_MAX / 2) return cev_fail(CEV_ERR_UNSUPPORTED, "paged attention: %lld work items are too many", (long long)items);
+    } else {
+      l.target = 0;
+    }
+    l.items = (int32_t)items;
+    l.first_off = at;
+    l.items_off = align_up(l.first_off + 4 * ((size_t)l.target + 1));
+    l.counters_off = align_up(l.items_off + sizeof(PagedItem) * (size_t)items);
+    // a cut makes at most one more split tile and two more pieces
+    l.records_off = align_up(l.counters_off + 4 * (size_t)l.target * d->n_kv_heads);
+    at = align_up(l.records_off + 2 * (size_t)l.target * d->n_kv_heads * kPagedSlots[i] * (d->head_dim + 2) * sizeof(float));
+  }
+  b->bytes = at;
   return CEV_OK;
 }
 

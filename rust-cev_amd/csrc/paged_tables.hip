@@ -206,26 +206,25 @@ __global__ __launch_bounds__(kThreads) void paged_tables_kernel(TablesArgs a) {
 }
 
 // --------------------------------------------------------------------------
-// The attention's work list.
+// The attention's work lists.
 
 struct PlanArgs {
   const int32_t *cu, *lengths;
   char* work;
-  size_t items_off, counters_off;
-  int32_t n_requests, t, max_new, max_len, window, sinks, rows, target, max_items, n_counters;
+  PagedListBounds list[kPagedLists];
+  int32_t n_requests, t, max_new, max_len, window, sinks, hkv;
   uint32_t sig;
 };
 
-// Key sub-tiles of tile `tile` of the list: tiles of one request follow one
-// another, the requests in order.
-struct Tile {
-  int32_t row0, n_rows, pos0, req, total;
-};
+// A part of a workgroup is at least this many sub-tiles, so that its start and
+// its partial result stay small beside it.
+constexpr int kMinPart = 8;
 
-// One workgroup.  Two passes over the tiles (runs of `rows` query rows of a
-// request): the sum of their key sub-tiles gives the length of a part, so that
-// the launch's keys are cut into about `target` parts of the same length for
-// each KV head; then every tile's parts are listed.
+// One workgroup.  A list's tiles (runs of query rows of a request), one after
+// the other, are a row of key sub-tiles; it is cut into as many runs of equal
+// length as workgroups run at once, and every piece of a tile that lies in one
+// run is an item.  So all workgroups end together whatever the lengths, and a
+// tile is split only where a cut falls.
 __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
   __shared__ int32_t tiles_s[kPagedMaxRequests + 1];  // tiles before each request's
   __shared__ int32_t row_s[kPagedMaxRequests], n_s[kPagedMaxRequests], pos_s[kPagedMaxRequests];
@@ -235,99 +234,113 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
   const int R = a.n_requests, per = (R + kThreads - 1) / kThreads;
   if (tid == 0) bad_s = 0;
   __syncthreads();
-  int32_t n_tiles[kPerThread];
-  int64_t x[1] = {0}, total[1];
+  int32_t rows[kPerThread];
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
     const int r = tid * per + i;
-    n_tiles[i] = 0;
+    rows[i] = 0;
     if (i < per && r < R) {
       const int32_t row = a.cu[r], end = a.cu[r + 1], len = a.lengths[r];
       const int64_t n = (int64_t)end - row;
       const bool bad = row < 0 || end > a.t || n < 0 || n > a.max_new || len < n || len > a.max_len;
       if (bad) bad_s = 1;
+      rows[i] = bad ? 0 : (int32_t)n;
       row_s[r] = row;
-      n_s[r] = bad ? 0 : (int32_t)n;
-      pos_s[r] = bad ? 0 : len - (int32_t)n;
-      n_tiles[i] = bad ? 0 : (int32_t)((n + a.rows - 1) / a.rows);
+      n_s[r] = rows[i];
+      pos_s[r] = bad ? 0 : len - rows[i];
     }
-    x[0] += n_tiles[i];
   }
-  exclusive_sums(x, total, part);
-  int32_t before = (int32_t)x[0];
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    const int r = tid * per + i;
-    if (i < per && r < R) tiles_s[r] = before;
-    before += n_tiles[i];
-  }
-  const int32_t all = (int32_t)total[0];
-  if (tid == 0) tiles_s[R] = all;
-  for (int i = tid; i < a.n_counters; i += kThreads) ((int32_t*)(a.work + a.counters_off))[i] = 0;
-  __syncthreads();
   PagedHeader* const h = (PagedHeader*)a.work;
-  if (bad_s) {
-    if (tid == 0) *h = PagedHeader{a.sig, 1, 0, 0};
-    return;
-  }
-
-  auto tile = [&](int i) {
-    int lo = 0, hi = R;  // tiles_s[lo] <= i < tiles_s[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (tiles_s[mid] <= i) lo = mid; else hi = mid;
-    }
-    // (requests without tiles share their start with the one that has it)
-    const int32_t at = (i - tiles_s[lo]) * a.rows;
-    Tile t;
-    t.row0 = row_s[lo] + at;
-    t.n_rows = min(a.rows, n_s[lo] - at);
-    t.pos0 = pos_s[lo] + at;
-    t.req = lo;
-    t.total = paged_span<kPagedKeys>(t.pos0, t.pos0 + t.n_rows - 1, a.window, a.sinks).total;
-    return t;
-  };
-  int64_t sum[1] = {0};
-  for (int i = tid; i < all; i += kThreads) sum[0] += tile(i).total;
-  exclusive_sums(sum, total, part);
-  // at least 8 sub-tiles a part, so that its start and its partial result
-  // stay small beside it
-  const int32_t len = (int32_t)max((total[0] + a.target - 1) / a.target, (int64_t)8);
-
-  PagedItem* const items = (PagedItem*)(a.work + a.items_off);
-  int64_t base[3] = {0, 0, 0};  // items, records, split tiles listed so far
-  for (int i0 = 0; i0 < all; i0 += kThreads) {
-    const int i = i0 + tid;
-    Tile t{};
-    int32_t n = 0;
-    if (i < all) {
-      t = tile(i);
-      n = (t.total + len - 1) / len;
-    }
-    int64_t y[3] = {n, n > 1 ? n : 0, n > 1 ? 1 : 0}, sums[3];
-    exclusive_sums(y, sums, part);
-    for (int k = 0; k < n; ++k) {
-      const int64_t at = base[0] + y[0] + k;
-      if (at < a.max_items) {
-        PagedItem it;
-        it.row0 = t.row0;
-        it.n_rows = t.n_rows;
-        it.pos0 = t.pos0;
-        it.req = t.req;
-        it.c_begin = (int32_t)((int64_t)k * t.total / n);
-        it.c_end = (int32_t)((int64_t)(k + 1) * t.total / n);
-        it.part = k;
-        it.n_parts = n;
-        it.rec = (int32_t)(base[1] + y[1]);
-        it.split = (int32_t)(base[2] + y[2]);
-        it.reserved0 = it.reserved1 = 0;
-        items[at] = it;
-      }
-    }
+  int32_t n_parts[kPagedLists];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) base[k] += sums[k];
+  for (int list = 0; list < kPagedLists; ++list) {
+    const PagedListBounds& l = a.list[list];
+    n_parts[list] = 0;
+    if (l.max_new < l.min_new) continue;
+    int64_t x[1] = {0}, total[1];
+    int32_t n_tiles[kPerThread];
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      n_tiles[i] = rows[i] >= l.min_new && rows[i] <= l.max_new ? (rows[i] + l.rows - 1) / l.rows : 0;
+      x[0] += n_tiles[i];
+    }
+    exclusive_sums(x, total, part);
+    int32_t before = (int32_t)x[0];
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      const int r = tid * per + i;
+      if (i < per && r < R) tiles_s[r] = before;
+      before += n_tiles[i];
+    }
+    const int32_t all = (int32_t)total[0];
+    if (tid == 0) tiles_s[R] = all;
+    __syncthreads();
+    if (bad_s) break;  // (rows of a request beyond its bounds)
+
+    // tile i of the list; its sub-tiles in c_end
+    auto tile = [&](int i) {
+      int lo = 0, hi = R;  // tiles_s[lo] <= i < tiles_s[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tiles_s[mid] <= i) lo = mid; else hi = mid;
+      }
+      // (requests without tiles share their start with the one that has it)
+      const int32_t at = (i - tiles_s[lo]) * l.rows;
+      PagedItem t{};
+      t.row0 = row_s[lo] + at;
+      t.n_rows = min(l.rows, n_s[lo] - at);
+      t.pos0 = pos_s[lo] + at;
+      t.req = lo;
+      t.c_end = paged_span(kPagedKeys[list], t.pos0, t.pos0 + t.n_rows - 1, a.window, a.sinks).total;
+      return t;
+    };
+    int64_t sum[1] = {0};
+    for (int i = tid; i < all; i += kThreads) sum[0] += tile(i).c_end;
+    exclusive_sums(sum, total, part);
+    const int64_t T = total[0], P = min((T + kMinPart - 1) / kMinPart, (int64_t)l.target);
+
+    int32_t* const first = (int32_t*)(a.work + l.first_off);
+    PagedItem* const items = (PagedItem*)(a.work + l.items_off);
+    int64_t units = 0, base[3] = {0, 0, 0};  // sub-tiles; items, partial results and split tiles so far
+    for (int i0 = 0; i0 < all; i0 += kThreads) {
+      const int i = i0 + tid;
+      PagedItem t{};
+      if (i < all) t = tile(i);
+      int64_t u[1] = {t.c_end}, u_all[1];
+      exclusive_sums(u, u_all, part);
+      const int64_t from = units + u[0], to = from + t.c_end;
+      // run r is [r T / P, (r + 1) T / P): the one that `from` lies in, and the last one
+      const int64_t r0 = t.c_end ? ((from + 1) * P - 1) / T : 0, r1 = t.c_end ? (to * P - 1) / T : -1;
+      const int64_t n = r1 - r0 + 1;
+      int64_t y[3] = {n, n > 1 ? n : 0, n > 1 ? 1 : 0}, sums[3];
+      exclusive_sums(y, sums, part);
+      const int32_t total_units = t.c_end;
+      t.n_pieces = (int32_t)n;
+      t.rec = (int32_t)(base[1] + y[1]);
+      t.split = (int32_t)(base[2] + y[2]);
+      for (int64_t r = r0; r <= r1; ++r) {
+        const int64_t begin = r * T / P, end = (r + 1) * T / P, at = base[0] + y[0] + (r - r0);
+        t.c_begin = (int32_t)(max(begin, from) - from);
+        t.c_end = (int32_t)min(end - from, (int64_t)total_units);
+        t.piece = (int32_t)(r - r0);
+        if (at < l.items) {
+          items[at] = t;
+          if (begin >= from) first[r] = (int32_t)at;
+        }
+      }
+      units += u_all[0];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) base[k] += sums[k];
+    }
+    if (tid == 0) {
+      first[P] = (int32_t)base[0];
+      if (base[0] > l.items) bad_s = 1;
+    }
+    for (int i = tid; i < (int)base[2] * a.hkv; i += kThreads) ((int32_t*)(a.work + l.counters_off))[i] = 0;
+    n_parts[list] = (int32_t)P;
+    __syncthreads();
   }
-  if (tid == 0) *h = PagedHeader{a.sig, base[0] > a.max_items ? 1 : 0, (int32_t)base[0], 0};
+  if (tid == 0) *h = PagedHeader{a.sig, bad_s, {bad_s ? 0 : n_parts[0], bad_s ? 0 : n_parts[1]}};
 }
 
 }  // namespace
@@ -384,18 +397,14 @@ extern "C" int32_t cev_paged_plan(const cev_paged_desc* d, const int32_t* cu, co
   a.cu = cu;
   a.lengths = lengths;
   a.work = (char*)work;
-  a.items_off = b.items_off;
-  a.counters_off = b.counters_off;
+  for (int i = 0; i < kPagedLists; ++i) a.list[i] = b.list[i];
   a.n_requests = d->n_requests;
   a.t = d->t;
   a.max_new = d->max_new;
   a.max_len = b.max_len;
   a.window = d->window;
   a.sinks = d->sinks;
-  a.rows = b.rows;
-  a.target = b.target;
-  a.max_items = b.items;
-  a.n_counters = b.target * d->n_kv_heads;
+  a.hkv = d->n_kv_heads;
   a.sig = b.sig;
   hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, a);
   const hipError_t e = hipGetLastError();

@@ -1,0 +1,472 @@
+// Attention over a paged K/V cache for requests with many new rows (prompts,
+// chunks of prompts): bf16, d = 128.
+//
+// A workgroup's 8 waves x 32 query slots hold 256 / g rows of one request times
+// the g query heads of one KV head, and share the 64-key chunks that it walks:
+// a chunk is read once for 256 slots, where the kernel of few rows
+// (paged_attn.hip) reads it for every 32 and is bound by L2 there.  The loop is
+// packed_attn.hip's: S^T = K . Q^T of one 32-key sub-tile runs beside the
+// softmax of the one before, then O^T += V^T . P^T, with waves 4-7 one region
+// ahead of waves 0-3; it differs in
+//   - the fetch: a wave's 8 rows of a chunk lie in one page, whose 64-bit base
+//     is scalar, so the cache may have any size;
+//   - the softmax argument: scale * log2 e times the f32 score less the row's
+//     maximum in one FMA.  (Q scaled and rounded to bf16 beforehand would save
+//     the FMA, and adds as much error as the probabilities' own rounding.)
+//   - the masks: by position, from the row's last key, the window and the first
+//     tokens that stay visible;
+//   - infinities and NaN of V that only some of a chunk's rows see.
+// Pieces of a split tile are joined as in paged_attn.hip.
+#include "attn_pipe.h"
+#include "paged_device.h"
+
+namespace {
+
+using namespace pipe;
+
+constexpr int kWaves = 8;
+constexpr int kThreads = kWaves * 64;
+constexpr int kKeys = kPagedKeys[kPagedMany], kSlots = kPagedSlots[kPagedMany];
+constexpr int D = 128, NDT = D / 32;
+static_assert(kSlots == kWaves * 32 && kKeys == 64 && kTileBytes == kKeys * 2 * D, "tile layout");
+
+// Cache policy of loads and stores that go past the XCD's own L2 (sc1).
+constexpr int kPastL2 = 16;
+
+// This lane's half of the wave, computed afresh (opaque to hoisting).
+__device__ __forceinline__ int fresh_half() { return fresh_lane_id() >> 5; }
+
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_tile_kernel(PagedArgs a) {
+  using F = Frag<__bf16, D>;
+  using P = F::P;
+  using Sched = Schedule<true>;
+  static_assert(F::NQK == 8 && F::NPV == 8, "unit layout below");
+  __shared__ __align__(16) char lds[2 * kBuf * kTileBytes];
+  __shared__ int32_t odd_s, bad_s, last_s;
+
+  const PagedHeader* const hdr = (const PagedHeader*)a.work;
+  if (hdr->sig != a.sig || hdr->bad != 0) return;  // the other kernel writes NaN
+  const int run = blockIdx.x / (uint32_t)a.hkv, kvh = blockIdx.x - run * a.hkv;
+  if (run >= uniform_i32(hdr->n_parts[kPagedMany])) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i32(tid >> 6);
+  const int n = lane & 31, u = lane >> 5;
+  const int gs = __builtin_ctz(a.g);
+
+  // Per-lane LDS addresses of the operand reads; the sub-tile and half are
+  // immediates.  They move on by one buffer a chunk (12 adds beside 32 MFMAs; a
+  // body for each of the four buffers, with the buffer as an immediate, leaves
+  // the loop in four places, and O and the scores were copied between them:
+  // 1.7 KB a lane of spills).
+  const int lds_base = (int)(size_t)(const __attribute__((address_space(3))) char*)lds;
+  int koff[F::NQK], voff[NDT];
+#pragma unroll
+  for (int st = 0; st < F::NQK; ++st) koff[st] = lds_base + n * kRowBytes + (k_slot(2 * st + u, n) << 4);
+  {
+    const int i = lane & 15, g16 = (lane >> 4) & 1, rr = i >> 2;
+    const int blk = 2 * g16 + ((i & 3) >> 1);  // 16-byte block of the read, within a 64-byte slice
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+      voff[dt] = lds_base + kVBase + (4 * u + rr) * kRowBytes + (v_slot(4 * dt + blk, rr) << 4) + 8 * (i & 1);
+  }
+  struct VFrag {
+    i32x2 lo, hi;
+  };
+  auto v_issue = [&](auto kt_c, auto j_c) {
+    constexpr int KT = decltype(kt_c)::value, J = decltype(j_c)::value;
+    constexpr int OFF = (KT * 32 + 16 * (J / NDT)) * kRowBytes;
+    return VFrag{read_tr<OFF>(voff[J % NDT]), read_tr<OFF + 8 * kRowBytes>(voff[J % NDT])};
+  };
+  auto v_ready = [](VFrag& f, auto j_c) {
+    wait_tr<Sched::wait_b(decltype(j_c)::value)>(f.lo, f.hi);
+    const bf16x4 lo = __builtin_bit_cast(bf16x4, f.lo), hi = __builtin_bit_cast(bf16x4, f.hi);
+    return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+  auto k_issue = [&](auto kt_c, auto st_c) { return read_b128<decltype(kt_c)::value * 32 * kRowBytes>(koff[decltype(st_c)::value]); };
+  auto k_ready = [](KFrag& r, auto st_c) {
+    wait_b128<Sched::wait_a(decltype(st_c)::value)>(r);
+    return __builtin_bit_cast(bf16x8, r);
+  };
+
+  // Cache rows of this KV head.  A wave fetches rows 8 w .. 8 w + 7 of K and of
+  // V of a chunk, four rows (1 KB) an instruction.
+  const uint64_t kbase = (uint64_t)((const __bf16*)a.kc + kvh * a.kc_sh), vbase = (uint64_t)((const __bf16*)a.vc + kvh * a.vc_sh);
+  const int kr = uniform_i32((int)(2 * a.kc_st)), vr = uniform_i32((int)(2 * a.vc_st));
+  int kat[2], vat[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = 8 * wave + 4 * r + (lane >> 4), blk = lane & 15;
+    kat[r] = (4 * r + (lane >> 4)) * kr + (k_slot(blk, row) << 4);
+    vat[r] = (4 * r + (lane >> 4)) * vr + (v_slot(blk, row) << 4);
+  }
+
+  int item_end;
+  for (int item = paged_first_item(a, run, item_end); item < item_end; ++item) {
+    const PagedItem it = paged_item(a, item);
+    const int pos1 = it.pos0 + it.n_rows - 1;
+    const PagedSpan span = paged_span(kKeys, it.pos0, pos1, a.window, a.sinks);
+    // Query slot (wave, n) holds row slot / g of the tile and query head slot % g:
+    // the rows of a short tile fill the first waves.
+    const int rit = (wave * 32 + n) >> gs;
+    const bool row_ok = rit < it.n_rows;
+    const int pos = row_ok ? it.pos0 + rit : -1;
+    const int w_row0 = (wave * 32) >> gs, w_row1 = min((wave * 32 + 31) >> gs, it.n_rows - 1);
+    const bool wave_active = w_row0 < it.n_rows;
+    const int w_pos0 = it.pos0 + w_row0, w_pos1 = it.pos0 + w_row1;  // this wave's rows
+
+    F fr;
+    {
+      const int row = it.row0 + (row_ok ? rit : 0), head = kvh * a.g + (n & (a.g - 1));
+      fr.load_q((const __bf16*)a.q + (int64_t)row * a.q_st + (int64_t)head * a.q_sh, row_ok, u);
+    }
+    if (tid == 0) odd_s = bad_s = 0;
+
+    const int c0 = it.c_begin, nc = it.c_end - it.c_begin;  // chunks [c0, c0 + nc) of the tile's stream
+    auto first_key = [&](int i) {
+      const int c = c0 + i;
+      return kKeys * (c < span.sinks ? c : c - span.sinks + span.first);
+    };
+    const int32_t* const bt = a.bt + it.req * a.bt_stride;
+    // Lane l keeps the page of this wave's rows of chunk 64 b + l of the
+    // current batch b.
+    int batch_first = 0, page_l = 0;
+    auto load_pages = [&](int i) {
+      batch_first = i;
+      const int j = first_key(min(i + lane, nc - 1)) + 8 * wave;
+      // (the last chunk may reach beyond the block table's last page)
+      page_l = bt[min(j >> a.page_shift, a.max_pages - 1)];
+    };
+    load_pages(0);
+    bool bad_page = false;
+
+    // Chunk i into its buffer, i mod kBuf; past the end: zeros.
+    auto fetch = [&](int i) {
+      const int buf = i % kBuf;
+      const bool real = i < nc;
+      if (real && i >= batch_first + 64) load_pages(i);
+      const int key0 = (real ? first_key(i) : 0) + 8 * wave;  // first of this wave's rows
+      const int l = real ? i - batch_first : 0;
+      // keys that some row of the tile sees
+      const bool seen = real && key0 < span.end && !(key0 >= span.skip_lo && key0 + 8 <= span.skip_hi);
+      const bool full = key0 + 8 <= span.end && !(key0 < span.skip_hi && key0 + 8 > span.skip_lo);
+      int page = __builtin_amdgcn_readlane(page_l, l);
+      const bool in = (uint32_t)page < (uint32_t)a.n_pages;
+      bad_page |= seen && !in;
+      page = in ? page : 0;
+      const int off = key0 & ((1 << a.page_shift) - 1);
+      const uint64_t kp = kbase + 2 * (uint64_t)(page * a.kc_sp) + (uint64_t)(off * (int64_t)kr);
+      const uint64_t vp = vbase + 2 * (uint64_t)(page * a.vc_sp) + (uint64_t)(off * (int64_t)vr);
+      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)uniform_u64(kp), (short)0, uniform_i32(seen && in ? 8 * kr : 0), kBufferWord3);
+      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)uniform_u64(vp), (short)0, uniform_i32(seen && in ? 8 * vr : 0), kBufferWord3);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        int ka = kat[r], va = vat[r];
+        if (!full) {
+          const int key = key0 + 4 * r + (lane >> 4);
+          const bool load = key < span.end && !(key >= span.skip_lo && key < span.skip_hi);
+          ka = load ? ka : INT32_MAX;
+          va = load ? va : INT32_MAX;
+        }
+        const int dst = buf * kTileBytes + (8 * wave + 4 * r) * kRowBytes;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)(lds + dst), 16, ka, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(lds + kVBase + dst), 16, va, 0, 0, 0);
+      }
+    };
+    constexpr int kLoadsPerChunk = 4;
+
+    // Whether a chunk from key0 on holds a key that some row of positions
+    // [p0, p1] does not see.
+    auto masked = [&](int key0, int p0, int p1) {
+      return key0 + kKeys - 1 > p0 || (a.window > 0 && key0 <= p1 - a.window && key0 + kKeys > a.sinks);
+    };
+    // 0 times an infinity or NaN is NaN: a key that only some of the rows see
+    // must not reach the others.  Where the rows differ in what they see of chunk
+    // i, such values among the V rows that this wave fetched (landed by now)
+    // become zeros; after the loop they are added to the rows that see them.
+    auto clean = [&](int i) {
+      if (i >= nc || !masked(first_key(i), it.pos0, pos1)) return;
+      i32x4* const v = (i32x4*)(lds + kVBase + i % kBuf * kTileBytes + 8 * wave * kRowBytes);
+      bool odd = false;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        i32x4 x = v[64 * r + lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool hi = (x[e] & 0x7f800000) == 0x7f800000, lo = (x[e] & 0x7f80) == 0x7f80;
+          odd |= hi | lo;
+          x[e] &= (hi ? 0 : (int)0xffff0000) | (lo ? 0 : 0xffff);
+        }
+        if (odd) v[64 * r + lane] = x;
+      }
+      if (__ballot(odd) && lane == 0) *(volatile int32_t*)&odd_s = 1;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
+    auto mask_sub = [&](f32x16& s, int key0) {
+      // bounds of the register's place, 8 (i / 4) + i % 4 (constants to compare
+      // with, where the keys themselves would be 16 values to hold)
+      const int k0 = key0 + 4 * fresh_half(), hi = pos - k0;
+      const int lo = a.window == 0 || pos < a.window ? INT32_MIN : pos - a.window - k0, first = a.sinks - k0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int at = 8 * (i >> 2) + (i & 3);
+        s[i] = (at <= hi) & ((at > lo) | (at < first)) ? s[i] : -INFINITY;
+      }
+    };
+
+    f32x16 o[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[dt] = f32x16{};
+    // m_run: a maximum that the row reached, in base-2 softmax units (0 until
+    // it has seen a key, m_set); rows that never see one keep l = 0.
+    float m_run = 0.0f, l_run = 0.0f;
+    bool m_set = false;
+    const float c = a.scale_log2;
+
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) fetch(k);
+    wait_vmcnt<kLoadsPerChunk * (kAhead - 2)>();  // chunks 0 and 1 landed
+    lds_barrier();                                // (the flags are clear)
+    clean(0);
+    clean(1);
+    lds_barrier();
+
+    f32x16 sa, sb;
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    constexpr int KPF = Sched::KPF, VPF = Sched::VPF;
+    KFrag kf[KPF];
+    if (wave_active) {
+      // Sub-tile 0: its row maximum (over both lane halves) is the first m_run.
+      sa = f32x16{};
+#pragma unroll
+      for (int st = 0; st < F::NQK; ++st)
+        fr.qk_mfma(*(const bf16x8*)(lds + (koff[st] - lds_base)), st, sa);
+      if (masked(first_key(0), w_pos0, w_pos1)) mask_sub(sa, first_key(0));
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sa[i]);
+      const float m0 = pair_max(mx) * c;
+      m_set = m0 > -INFINITY;
+      m_run = m_set ? m0 : 0.0f;
+      // The first body's K reads (sub-tile 1 of chunk 0), waited for in full, so
+      // that its counted waits see no fewer reads than a steady-state body's.
+      static_for<KPF>([&](auto f_c) { kf[decltype(f_c)::value] = k_issue(I1{}, f_c); });
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    VFrag vf[VPF];
+    P p;
+    const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
+    // Region A of sub-tile KT of this chunk: the next sub-tile's scores on the
+    // MFMA unit beside this one's probabilities, then the check of the row's
+    // maximum.  (The last sub-tile also scores one past the end, never used.)
+    auto region_a = [&](auto kt_c) {
+      constexpr int kt = decltype(kt_c)::value;
+      using KTN_c = std::integral_constant<int, 1 - kt>;
+      f32x16& s = kt == 0 ? sa : sb;
+      f32x16& sn = kt == 0 ? sb : sa;
+      float rs = 0.0f;
+      static_for<F::NQK>([&](auto st_c) {
+        constexpr int st = decltype(st_c)::value;
+        if constexpr (st == 0)
+          sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_ready(kf[0], st_c), fr.q[0], f32x16{}, 0, 0, 0);
+        else
+          fr.qk_mfma(k_ready(kf[st % KPF], st_c), st, sn);
+        if constexpr (st + KPF < F::NQK) kf[st % KPF] = k_issue(KTN_c{}, std::integral_constant<int, st + KPF>{});
+        if constexpr (st >= F::NQK - VPF)
+          vf[st - (F::NQK - VPF)] = v_issue(kt_c, std::integral_constant<int, st - (F::NQK - VPF)>{});
+        const float e0 = fast_exp2(__builtin_fmaf(s[2 * st], c, -m_run));
+        const float e1 = fast_exp2(__builtin_fmaf(s[2 * st + 1], c, -m_run));
+        const bf16x2 pr = {(__bf16)e0, (__bf16)e1};
+        p.h[st / 4][2 * (st % 4)] = pr[0];
+        p.h[st / 4][2 * (st % 4) + 1] = pr[1];
+        rs = __builtin_amdgcn_fdot2_f32_bf16(pr, one, rs, false);
+        pin(rs);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      // The probabilities stand as long as their sum stays within kMaxP.
+      // Otherwise, or for a row with no maximum yet, the row moves its maximum
+      // (a set one only when it grew by more than kRescale).  No LDS operation,
+      // so the counted waits of region B still hold.
+      if (__ballot((rs > kMaxP) | !m_set)) {
+        float ml = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ml = fmaxf(ml, s[i]);
+        const float cand = pair_max(ml) * c, delta = cand - m_run;
+        const bool move = m_set ? delta > kRescale : cand > -INFINITY;
+        const float alpha = m_set && move ? fast_exp2(-delta) : 1.0f;
+        m_set = m_set | move;
+        m_run = move ? cand : m_run;
+        l_run *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) o[dt] *= alpha;
+        rs = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            const bf16x2 pr = {(__bf16)fast_exp2(__builtin_fmaf(s[8 * h + j], c, -m_run)),
+                               (__bf16)fast_exp2(__builtin_fmaf(s[8 * h + j + 1], c, -m_run))};
+            p.h[h][j] = pr[0];
+            p.h[h][j + 1] = pr[1];
+            rs = __builtin_amdgcn_fdot2_f32_bf16(pr, one, rs, false);
+          }
+      }
+      l_run += rs;
+    };
+    // Region B of sub-tile KT of chunk i: P.V, the next region's first K reads
+    // (it scores sub-tile KT of the next chunk), then the mask of the next scores.
+    auto region_b = [&](auto kt_c, int i) {
+      constexpr int kt = decltype(kt_c)::value;
+      f32x16& sn = kt == 0 ? sb : sa;
+      static_for<F::NPV>([&](auto j_c) {
+        constexpr int j = decltype(j_c)::value;
+        F::pv_mfma(v_ready(vf[j % VPF], j_c), j, p, o);
+        if constexpr (j + VPF < F::NPV) vf[j % VPF] = v_issue(kt_c, std::integral_constant<int, j + VPF>{});
+        if constexpr (j >= F::NPV - KPF) kf[j - (F::NPV - KPF)] = k_issue(kt_c, std::integral_constant<int, j - (F::NPV - KPF)>{});
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      const int in = i + kt;  // chunk of the next scores
+      if (in < nc && masked(first_key(in), w_pos0, w_pos1)) mask_sub(sn, first_key(in) + 32 * (1 - kt));
+    };
+    const bool lead = wave >= kWaves / 2;
+    if (wave_active && lead) region_a(I0{});
+#pragma unroll 1
+    for (int i = 0; i < nc; ++i) {
+      fetch(i + kAhead);
+      const int next = i % kBuf == kBuf - 1 ? -kAhead * kTileBytes : kTileBytes;  // to the next chunk's buffer
+      if (wave_active) {
+        if (!lead) region_a(I0{});
+#pragma unroll
+        for (int st = 0; st < F::NQK; ++st) koff[st] += next;
+        region_b(I0{}, i);
+        region_a(I1{});
+        region_b(I1{}, i);
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) voff[dt] += next;
+        if (lead && i + 1 < nc) region_a(I0{});
+      }
+      // Chunk i + 2 must have landed before the barrier; chunk i + kAhead may
+      // stay in flight.
+      wait_vmcnt<kLoadsPerChunk * (kAhead - 2)>();
+      clean(i + 2);
+      __builtin_amdgcn_s_barrier();
+    }
+    // Fetches past the end still write zeros into LDS: drain them, and the last
+    // body's K reads of a sub-tile past the end, before LDS is used again.
+    wait_vmcnt<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (wave_active) {
+      // back to the first buffer
+#pragma unroll
+      for (int st = 0; st < F::NQK; ++st) koff[st] -= nc % kBuf * kTileBytes;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) voff[dt] -= nc % kBuf * kTileBytes;
+    }
+
+    if (bad_page && lane == 0) *(volatile int32_t*)&bad_s = 1;  // one wave's finding
+    __syncthreads();
+    if (*(volatile int32_t*)&odd_s && wave_active) {
+#pragma unroll 1
+      for (int i = 0; i < nc; ++i) {
+        if (!masked(first_key(i), it.pos0, pos1)) continue;
+#pragma unroll 1
+        for (int kk = 0; kk < kKeys; ++kk) {
+          const int key = first_key(i) + kk;
+          if (key >= span.end || (key >= span.skip_lo && key < span.skip_hi)) continue;
+          const int page = bt[key >> a.page_shift];
+          if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
+          const __bf16* const v = (const __bf16*)(vbase + 2 * (uint64_t)(page * a.vc_sp + (key & ((1 << a.page_shift) - 1)) * a.vc_st)) + 4 * u;
+          const bool vis = (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.sinks));
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const bf16x4 x = *(const bf16x4*)(v + 32 * (j / 4) + 8 * (j % 4));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y = (float)x[e];
+              const bool finite = (__float_as_uint(y) & 0x7f800000u) != 0x7f800000u;
+              o[j / 4][4 * (j % 4) + e] += (finite | !vis) ? 0.0f : y;
+            }
+          }
+        }
+      }
+    }
+    float l = pair_sum(l_run) + (*(volatile int32_t*)&bad_s ? __builtin_nanf("") : 0.0f);
+
+    const bool split = it.n_pieces > 1;
+    // Partial results: [wave][16 vectors of 4 columns][lane], then (m, l) of
+    // each slot.
+    constexpr int kRec = kSlots * (D + 2);
+    float* const rec0 = (float*)(a.work + a.records_off) + ((int64_t)it.rec * a.hkv + kvh) * kRec;
+    const int64_t rec_step = (int64_t)a.hkv * kRec;
+    auto record = [&](int piece) {
+      return __builtin_amdgcn_make_buffer_rsrc((void*)uniform_u64((uint64_t)(rec0 + piece * rec_step)), (short)0, kRec * 4, kBufferWord3);
+    };
+    const int vec0 = wave * 16 * 1024 + lane * 16, ml0 = kSlots * D * 4 + (wave * 32 + n) * 8;
+    if (split) {
+      const __amdgpu_buffer_rsrc_t rs = record(it.piece);
+      if (wave_active) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          __builtin_amdgcn_raw_buffer_store_b128(
+              __builtin_bit_cast(decltype(__builtin_amdgcn_raw_buffer_load_b128(rs, 0, 0, 0)),
+                                 f32x4{o[v / 4][4 * (v % 4)], o[v / 4][4 * (v % 4) + 1], o[v / 4][4 * (v % 4) + 2], o[v / 4][4 * (v % 4) + 3]}),
+              rs, vec0 + 1024 * v, 0, kPastL2);
+        const float2 w = make_float2(m_set ? m_run : -1e30f, l);
+        if (u == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(decltype(__builtin_amdgcn_raw_buffer_load_b64(rs, 0, 0, 0)), w), rs, ml0, 0, kPastL2);
+      }
+      // The stores have reached memory before the workgroup counts itself.
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      int32_t* const counter = (int32_t*)(a.work + a.counters_off) + (int64_t)it.split * a.hkv + kvh;
+      if (tid == 0) {
+        last_s = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.n_pieces - 1;
+        if (last_s) *counter = 0;  // for the next call with this plan
+      }
+      __syncthreads();
+      const bool last = last_s;
+      __syncthreads();
+      if (!last) continue;
+      float M = -INFINITY;
+      l = 0.0f;
+      for (int q = 0; q < it.n_pieces; ++q) {
+        const __amdgpu_buffer_rsrc_t rq = record(q);
+        const float2 w = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rq, ml0, 0, kPastL2));
+        const float m = fmaxf(M, w.x), f0 = fast_exp2(M - m), f = fast_exp2(w.x - m);
+        M = m;
+        l = l * f0 + f * w.y;
+        if (wave_active) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const f32x4 x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rq, vec0 + 1024 * v, 0, kPastL2));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float y = o[v / 4][4 * (v % 4) + e];
+              o[v / 4][4 * (v % 4) + e] = q == 0 ? f * x[e] : y * f0 + f * x[e];
+            }
+          }
+        }
+      }
+    }
+    if (row_ok) {
+      __bf16* const op = (__bf16*)a.out + (int64_t)(it.row0 + rit) * a.o_st + (int64_t)(kvh * a.g + (n & (a.g - 1))) * a.o_sh;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = l == 0.0f ? 0.0f : o[v / 4][4 * (v % 4) + e] * inv;
+        store_vec4<__bf16>(op + (v / 4) * 32 + 8 * (v % 4) + 4 * u, x);
+      }
+    }
+    __syncthreads();  // the ring and the flags are the next item's
+  }
+}
+
+}  // namespace
+
+int32_t cev_paged_tile_launch(const PagedArgs& a, int32_t target, void* stream) {
+  hipLaunchKernelGGL(paged_tile_kernel, dim3((unsigned)(target * a.hkv)), dim3(kThreads), 0, (hipStream_t)stream, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return cev_fail(CEV_ERR_HIP, "paged attention launch: %s", hipGetErrorString(e));
+  return CEV_OK;
+}
