@@ -16,8 +16,8 @@ constexpr int kPagedSlots[kPagedLists] = {32, 256};  // query slots (rows x head
 constexpr int kPagedKeys[kPagedLists] = {32, 64};    // keys of a sub-tile
 
 // The work buffer: this header, then for each list the first item of every
-// workgroup, the items, one arrival counter for every (split tile, KV head),
-// and the split tiles' partial results.
+// workgroup's run, all items, one arrival counter for every (split tile, KV
+// head), and the split tiles' partial results.
 struct PagedHeader {
   uint32_t sig;                   // signature of the descriptor that the plan was made for
   int32_t bad;                    // not 0: a length, offset or count was out of its bounds
@@ -25,11 +25,13 @@ struct PagedHeader {
 };
 
 // One work item: a run of query rows of one request (a tile) and a run of the
-// key sub-tiles that they see.  A workgroup walks its items in order.
+// key sub-tiles that they see.  A workgroup walks its run's items in order.
 struct PagedItem {
   int32_t row0, n_rows, pos0, req;         // first packed row, rows, position of the first
   int32_t c_begin, c_end, piece, n_pieces; // key sub-tiles [c_begin, c_end) of the tile's stream
-  int32_t rec, split, reserved0, reserved1;  // first partial result and counter of a split tile
+  int32_t rec, split;                      // first partial result and counter of a split tile
+  int32_t next;                            // the run's next item, -1 behind the last
+  int32_t reserved;
 };
 static_assert(sizeof(PagedHeader) == 16 && sizeof(PagedItem) == 48, "work buffer layout");
 

@@ -39,17 +39,6 @@ __device__ void paged_poison(const PagedArgs& a) {
   }
 }
 
-// Partial results go between workgroups of any XCD: stores past the XCD's own
-// L2 and loads past it (relaxed atomics of agent scope).  Fences in their place
-// write back and drop the whole L2: a decoding batch's attention took 334 us
-// with 512 parts and 1019 with 4096.
-__device__ __forceinline__ void put_shared(float* p, float2 v) {
-  __hip_atomic_store((uint64_t*)p, __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float2 get_shared(const float* p) {
-  return __builtin_bit_cast(float2, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-}
-
 // f32 values as sums of three bf16 parts and the six large part products
 // (see fan_attn.hip).
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -121,21 +110,27 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   constexpr int NB = 1;         // sub-tiles of K and of V in LDS
   constexpr int kRows = 1024 / kRB, kBlk = kRB / 16;  // rows of one load, 16-byte blocks of a row
   constexpr int RS = D + 4;                      // row stride (floats) of a partial result in LDS
-  constexpr int kRing = kWaves * 2 * NB * kTile, kOut = kWaves * 32 * RS * 4;
-  __shared__ __align__(16) char lds[kRing > kOut ? kRing : kOut];
+  constexpr int kRing = kWaves * 2 * NB * kTile, kOut = kWaves * 32 * RS * 4, kBody = kRing > kOut ? kRing : kOut;
+  // Q of 512-byte rows (f32: its parts) lies in LDS, shared by the waves: with
+  // it in registers O is moved to and from the accumulation registers at every
+  // rescale, and at d = 256 spilled.
+  constexpr bool kQInLds = kRB == 512;
+  constexpr int kQSteps = D / 16 * (BF ? 1 : 3);  // operands of 1 KB
+  __shared__ __align__(16) char lds[kBody + (kQInLds ? kQSteps * 1024 : 0)];
   __shared__ float2 ml[kWaves * 32];
   __shared__ int32_t last_s;
 
-  const PagedHeader* const hdr = (const PagedHeader*)a.work;
-  if (hdr->sig != a.sig || hdr->bad != 0) {
+  const int run = blockIdx.x / (uint32_t)a.hkv, kvh = blockIdx.x - run * a.hkv;
+  PagedWalk walk(a, run);
+  int n_parts;
+  if (!paged_plan_ok(a, kPagedFew, n_parts)) {
     paged_poison<T, D>(a);
     return;
   }
-  const int run = blockIdx.x / (uint32_t)a.hkv, kvh = blockIdx.x - run * a.hkv;
-  if (run >= uniform_i32(hdr->n_parts[kPagedFew])) return;
-  int item_end;
-  for (int item = paged_first_item(a, run, item_end); item < item_end; ++item) {
-  const PagedItem it = paged_item(a, item);
+  if (run >= n_parts) return;
+  for (bool more = true; more;) {
+  const PagedItem it = walk.item();
+  more = it.next >= 0;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i32(tid >> 6);
   const int n = lane & 31, u = lane >> 5;
   const int gs = __builtin_ctz(a.g);
@@ -148,7 +143,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   // ---- Q, as the B operand
   const T* const qrow = (const T*)a.q + (int64_t)row * a.q_st + (int64_t)head * a.q_sh;
   F fr;
-  bf16x8 qp[BF ? 1 : D / 16][3];
   auto load_q8 = [&](int st, float* x) {
 #pragma unroll
     for (int e = 0; e < 8; e += 4) {
@@ -157,14 +151,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       for (int j = 0; j < 4; ++j) x[e + j] = v[j];
     }
   };
-  if constexpr (BF) {
+  if constexpr (!kQInLds) {
     fr.load_q(qrow, ok, u);
   } else {
 #pragma unroll
-    for (int st = 0; st < D / 16; ++st) {
-      float x[8];
-      load_q8(st, x);
-      bf16_parts(x, qp[st]);
+    for (int i = 0; i < D / 16 / kWaves; ++i) {
+      const int st = wave * (D / 16 / kWaves) + i;
+      if constexpr (BF) {
+        const bf16x8 z = {};
+        *(bf16x8*)(lds + kBody + st * 1024 + lane * 16) = ok ? *(const bf16x8*)(qrow + 16 * st + 8 * u) : z;
+      } else {
+        float x[8];
+        load_q8(st, x);
+        bf16x8 parts[3];
+        bf16_parts(x, parts);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *(bf16x8*)(lds + kBody + (3 * st + k) * 1024 + lane * 16) = parts[k];
+      }
     }
   }
 
@@ -243,6 +246,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     l_run = 0.0f;
   };
   reset();
+  const int lds_q = (int)(size_t)(const __attribute__((address_space(3))) char*)lds + kBody + lane * 16;
   // Byte offsets of the operand reads within a sub-tile of K and of V.
   int koff[8], voff[NDT];
 #pragma unroll
@@ -266,6 +270,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     int c = it.c_begin + wave;
     if (c < c_end) {
     load_pages(c);
+    }
+    if constexpr (kQInLds)
+      if (!exact) __syncthreads();  // Q is in LDS
+    if (c < c_end) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       fetch(c + b * kWaves, K_c{}, b);
@@ -277,46 +285,55 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       pipe::wait_vmcnt<(2 * NB - 1) * kLoads>();
       asm volatile("" ::: "memory");
       f32x16 s = f32x16{};
-      // K operands in groups of four 16-byte reads, one group ahead of the MFMAs
-      constexpr int kKGrp = 4, kKReads = kRB / 32;
-      i32x4 kf[2][kKGrp];
+      // K operands (and Q's of 512-byte rows) in groups, one group ahead of the
+      // MFMAs: two steps of 16 head-dim values, at d = 128 in bf16 four.
+      constexpr int kSteps = kQInLds ? 2 : 4, kKReads = BF ? 1 : 2, kQReads = kQInLds ? (BF ? 1 : 3) : 0;
+      i32x4 kf[2][kSteps * kKReads], qf[2][kSteps * kQReads + 1];
       const int ka = lds_ring + buf * kTile;
       auto k_issue = [&](auto g_c) {
         constexpr int G = decltype(g_c)::value;
-        static_for<kKGrp>([&](auto e_c) {
-          constexpr int J = G * kKGrp + decltype(e_c)::value;
-          // block 2 J + u (bf16), 4 (J / 2) + 2 u + J % 2 (f32); bit 4 of a block's place is its own
-          kf[G & 1][decltype(e_c)::value] = read_b128<(J / 8) * 256>(ka + koff[J % 8]);
+        static_for<kSteps * kKReads>([&](auto e_c) {
+          // read J is block 2 J + u (bf16), 4 (J / 2) + 2 u + J % 2 (f32); bit 4 of a block's place is its own
+          constexpr int E = decltype(e_c)::value, J = G * kSteps * kKReads + E;
+          kf[G & 1][E] = read_b128<(J / 8) * 256>(ka + koff[J % 8]);
+        });
+        static_for<kSteps * kQReads>([&](auto e_c) {
+          constexpr int E = decltype(e_c)::value;
+          qf[G & 1][E] = read_b128<(G * kSteps * kQReads + E) * 1024>(lds_q);
         });
       };
       k_issue(std::integral_constant<int, 0>{});
-      static_for<kKReads / kKGrp>([&](auto g_c) {
+      static_for<D / 16 / kSteps>([&](auto g_c) {
         constexpr int G = decltype(g_c)::value;
-        static_for<kKGrp>([&](auto e_c) { wait_read(kf[G & 1][decltype(e_c)::value]); });
-        if constexpr (G + 1 < kKReads / kKGrp) k_issue(std::integral_constant<int, G + 1>{});
-        if constexpr (BF) {
-          static_for<kKGrp>([&](auto e_c) {
-            constexpr int E = decltype(e_c)::value;
-            fr.qk_mfma(__builtin_bit_cast(bf16x8, kf[G & 1][E]), G * kKGrp + E, s);
-          });
-        } else {
-          static_for<kKGrp / 2>([&](auto e_c) {
-            constexpr int E = decltype(e_c)::value, st = G * kKGrp / 2 + E;
+        static_for<kSteps * kKReads>([&](auto e_c) { wait_read(kf[G & 1][decltype(e_c)::value]); });
+        static_for<kSteps * kQReads>([&](auto e_c) { wait_read(qf[G & 1][decltype(e_c)::value]); });
+        if constexpr (G + 1 < D / 16 / kSteps) k_issue(std::integral_constant<int, G + 1>{});
+        static_for<kSteps>([&](auto e_c) {
+          constexpr int E = decltype(e_c)::value, st = G * kSteps + E;
+          if constexpr (BF) {
+            const bf16x8 k = __builtin_bit_cast(bf16x8, kf[G & 1][E]);
+            if constexpr (kQInLds)
+              s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, __builtin_bit_cast(bf16x8, qf[G & 1][E]), s, 0, 0, 0);
+            else
+              fr.qk_mfma(k, st, s);
+          } else {
             float x[8];
             __builtin_memcpy(x, &kf[G & 1][2 * E], 16);
             __builtin_memcpy(x + 4, &kf[G & 1][2 * E + 1], 16);
             if (!exact) {
-              bf16x8 kp[3];
+              bf16x8 kp[3], qp[3];
               bf16_parts(x, kp);
-              s = parts_mma(kp, qp[st], s);
+#pragma unroll
+              for (int k = 0; k < 3; ++k) qp[k] = __builtin_bit_cast(bf16x8, qf[G & 1][3 * E + k]);
+              s = parts_mma(kp, qp, s);
             } else {
               float q[8];
               load_q8(st, q);
 #pragma unroll
               for (int e = 0; e < 8; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], q[e], s, 0, 0, 0);
             }
-          });
-        }
+          }
+        });
       });
       asm volatile("" ::: "memory");
       const bool masked = key0 + kKeys - 1 > it.pos0 ||
@@ -497,10 +514,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   const int slots = it.n_rows << gs;
   constexpr int kCols = D / 4;  // 4-column units of a slot
   const bool split = it.n_pieces > 1;
-  // records of the tile's parts, [slot][D] then [slot] (m, l)
+  // partial results of the tile's pieces, [slot][D] then [slot] (m, l)
   constexpr int kRec = kSlots * (D + 2);
   float* const rec0 = (float*)(a.work + a.records_off) + ((int64_t)it.rec * a.hkv + kvh) * kRec;
-  const int64_t rec_step = (int64_t)a.hkv * kRec;
+  auto record = [&](int piece) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)uniform_u64((uint64_t)(rec0 + (int64_t)piece * a.hkv * kRec)), (short)0, kRec * 4, kBufferWord3);
+  };
   auto put = [&](int slot, int col, const f32x4& x, float L) {
     T* const op = (T*)a.out + (int64_t)(it.row0 + (slot >> gs)) * a.o_st + (int64_t)(kvh * a.g + (slot & (a.g - 1))) * a.o_sh + col;
     // a row that sees no key is 0; a sum that is NaN makes its row NaN
@@ -509,6 +528,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     for (int e = 0; e < 4; ++e) v[e] = L == 0.0f ? 0.0f : x[e] / L;
     store_vec4<T>(op, v);
   };
+  const __amdgpu_buffer_rsrc_t mine = record(it.piece);
+  const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc((void*)uniform_u64((uint64_t)rec0), (short)0, uniform_i32(it.n_pieces * a.hkv * kRec * 4), kBufferWord3);
   for (int i = tid; i < slots * kCols; i += kThreads) {
     const int slot = i / kCols, col = 4 * (i % kCols);
     float M = -INFINITY, L = 0.0f;
@@ -525,10 +546,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     if (!split) {
       put(slot, col, x, L);
     } else {
-      float* const rec = rec0 + it.piece * rec_step;
-      put_shared(rec + slot * D + col, float2{x[0], x[1]});
-      put_shared(rec + slot * D + col + 2, float2{x[2], x[3]});
-      if (col == 0) put_shared(rec + kSlots * D + 2 * slot, float2{M, L});
+      put_past_l2(mine, (slot * D + col) * 4, x);
+      if (col == 0) put_past_l2(mine, (kSlots * D + 2 * slot) * 4, make_float2(M, L));
     }
   }
   // A split tile's stores have reached memory before the workgroup counts
@@ -542,22 +561,64 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   const bool last = last_s;
   __syncthreads();
   if (!last) continue;
-  for (int i = tid; i < slots * kCols; i += kThreads) {
-    const int slot = i / kCols, col = 4 * (i % kCols);
+  // Threads -> (group of pieces, 4-column unit): with few rows several groups
+  // walk the pieces, kBatch at a time, and meet in LDS.
+  constexpr int kBatch = 8;
+  const int units = slots * kCols;
+  int groups = 1;
+  while (groups < 8 && 2 * groups * units <= kThreads && 2 * groups < it.n_pieces) groups *= 2;
+  for (int i0 = 0; i0 < units; i0 += kThreads) {
+    const int i = i0 + tid, unit = i % units, group = i / units;
+    const int slot = unit / kCols, col = 4 * (unit % kCols);
     float M = -INFINITY, L = 0.0f;
     f32x4 x = f32x4{};
-    for (int p = 0; p < it.n_pieces; ++p) {
-      const float* const rec = rec0 + p * rec_step;
-      const float2 v = get_shared(rec + kSlots * D + 2 * slot);
-      const float2 y = get_shared(rec + slot * D + col), z = get_shared(rec + slot * D + col + 2);
-      const float m = fmaxf(M, v.x);
-      const float f = fast_exp2(v.x - m), f0 = fast_exp2(M - m);
-      M = m;
-      L = L * f0 + f * v.y;
-      x = x * f0 + f * f32x4{y.x, y.y, z.x, z.y};
+    if (group < groups) {
+      for (int p0 = group; p0 < it.n_pieces; p0 += kBatch * groups) {
+        f32x4 y[kBatch];
+        float2 w[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+          const int at = min(p0 + b * groups, it.n_pieces - 1) * (int)(a.hkv * kRec * 4);
+          y[b] = get4_past_l2(all, at + (slot * D + col) * 4);
+          w[b] = get2_past_l2(all, at + (kSlots * D + 2 * slot) * 4);
+        }
+        float m = M;
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) m = fmaxf(m, w[b].x);
+        const float f0 = fast_exp2(M - m);
+        M = m;
+        L *= f0;
+        x *= f0;
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+          const float f = p0 + b * groups < it.n_pieces ? fast_exp2(w[b].x - m) : 0.0f;
+          if (f > 0.0f || w[b].y != w[b].y) {
+            L += f * w[b].y;
+            x += f * y[b];
+          }
+        }
+      }
+      if (groups > 1) {
+        *(f32x4*)(ob + (group * units + unit) * 8) = x;
+        *(float2*)(ob + (group * units + unit) * 8 + 4) = make_float2(M, L);
+      }
     }
-    put(slot, col, x, L);
+    if (groups > 1) {
+      __syncthreads();
+      if (group == 0) {
+        for (int k = 1; k < groups; ++k) {
+          const float2 w = *(const float2*)(ob + (k * units + unit) * 8 + 4);
+          const f32x4 y = *(const f32x4*)(ob + (k * units + unit) * 8);
+          const float m = fmaxf(M, w.x), f0 = fast_exp2(M - m), f = fast_exp2(w.x - m);
+          M = m;
+          L = L * f0 + f * w.y;
+          x = x * f0 + f * y;
+        }
+      }
+    }
+    if (group == 0) put(slot, col, x, L);
   }
+  __syncthreads();
   if (tid == 0) *counter = 0;  // for the next call with this plan
   }
 }

@@ -120,7 +120,7 @@ int32_t cev_paged_bounds(const cev_paged_desc* d, PagedBounds* b) {
     }
     l.items = (int32_t)items;
     l.first_off = at;
-    l.items_off = align_up(l.first_off + 4 * ((size_t)l.target + 1));
+    l.items_off = align_up(l.first_off + sizeof(PagedItem) * (size_t)l.target);
     l.counters_off = align_up(l.items_off + sizeof(PagedItem) * (size_t)items);
     // a cut makes at most one more split tile and two more pieces
     l.records_off = align_up(l.counters_off + 4 * (size_t)l.target * d->n_kv_heads);

@@ -216,15 +216,17 @@ struct PlanArgs {
   uint32_t sig;
 };
 
-// A part of a workgroup is at least this many sub-tiles, so that its start and
-// its partial result stay small beside it.
-constexpr int kMinPart = 8;
+// What an item costs beside its sub-tiles (its start, and its partial or final
+// result), in sub-tiles; and the least that a run is worth, in the same.
+constexpr int kItemCost = 8, kMinRun = 16;
+static_assert(kMinRun > kItemCost, "no run without a sub-tile");
 
 // One workgroup.  A list's tiles (runs of query rows of a request), one after
-// the other, are a row of key sub-tiles; it is cut into as many runs of equal
-// length as workgroups run at once, and every piece of a tile that lies in one
-// run is an item.  So all workgroups end together whatever the lengths, and a
-// tile is split only where a cut falls.
+// the other, are a row of key sub-tiles, each tile kItemCost longer than its
+// own; it is cut into as many runs of equal length as workgroups run at once,
+// and every piece of a tile that lies in one run is an item.  So all workgroups
+// end together whatever the lengths, and a tile is split only where a cut
+// falls.
 __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
   __shared__ int32_t tiles_s[kPagedMaxRequests + 1];  // tiles before each request's
   __shared__ int32_t row_s[kPagedMaxRequests], n_s[kPagedMaxRequests], pos_s[kPagedMaxRequests];
@@ -295,47 +297,48 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
       return t;
     };
     int64_t sum[1] = {0};
-    for (int i = tid; i < all; i += kThreads) sum[0] += tile(i).c_end;
+    for (int i = tid; i < all; i += kThreads) sum[0] += tile(i).c_end + kItemCost;
     exclusive_sums(sum, total, part);
-    const int64_t T = total[0], P = min((T + kMinPart - 1) / kMinPart, (int64_t)l.target);
+    // (a run is longer than a tile's cost, so sub-tiles lie in every run)
+    const int64_t T = total[0], P = T == 0 ? 0 : max(min(T / kMinRun, (int64_t)l.target), (int64_t)1);
 
-    int32_t* const first = (int32_t*)(a.work + l.first_off);
+    PagedItem* const first = (PagedItem*)(a.work + l.first_off);
     PagedItem* const items = (PagedItem*)(a.work + l.items_off);
-    int64_t units = 0, base[3] = {0, 0, 0};  // sub-tiles; items, partial results and split tiles so far
+    int64_t units = 0, base[3] = {0, 0, 0};  // length so far; items, partial results and split tiles
     for (int i0 = 0; i0 < all; i0 += kThreads) {
       const int i = i0 + tid;
       PagedItem t{};
       if (i < all) t = tile(i);
-      int64_t u[1] = {t.c_end}, u_all[1];
+      const int32_t n_sub = t.c_end;
+      int64_t u[1] = {n_sub ? n_sub + kItemCost : 0}, u_all[1];
       exclusive_sums(u, u_all, part);
-      const int64_t from = units + u[0], to = from + t.c_end;
-      // run r is [r T / P, (r + 1) T / P): the one that `from` lies in, and the last one
-      const int64_t r0 = t.c_end ? ((from + 1) * P - 1) / T : 0, r1 = t.c_end ? (to * P - 1) / T : -1;
+      // run r is [r T / P, (r + 1) T / P); a tile's cost comes before its sub-tiles
+      const int64_t from = units + u[0], keys = from + kItemCost, to = keys + n_sub;
+      const int64_t r0 = n_sub ? ((keys + 1) * P - 1) / T : 0, r1 = n_sub ? (to * P - 1) / T : -1;
       const int64_t n = r1 - r0 + 1;
       int64_t y[3] = {n, n > 1 ? n : 0, n > 1 ? 1 : 0}, sums[3];
       exclusive_sums(y, sums, part);
-      const int32_t total_units = t.c_end;
       t.n_pieces = (int32_t)n;
       t.rec = (int32_t)(base[1] + y[1]);
       t.split = (int32_t)(base[2] + y[2]);
       for (int64_t r = r0; r <= r1; ++r) {
         const int64_t begin = r * T / P, end = (r + 1) * T / P, at = base[0] + y[0] + (r - r0);
-        t.c_begin = (int32_t)(max(begin, from) - from);
-        t.c_end = (int32_t)min(end - from, (int64_t)total_units);
+        t.c_begin = (int32_t)(max(begin, keys) - keys);
+        t.c_end = (int32_t)(min(end, to) - keys);
         t.piece = (int32_t)(r - r0);
+        // the run goes on with the next tile when that tile's sub-tiles begin in it
+        t.next = to + kItemCost < end && i + 1 < all ? (int32_t)at + 1 : -1;
+        // it begins here when no tile before has sub-tiles in it
         if (at < l.items) {
           items[at] = t;
-          if (begin >= from) first[r] = (int32_t)at;
+          if (begin >= from) first[r] = t;
         }
       }
       units += u_all[0];
 #pragma unroll
       for (int k = 0; k < 3; ++k) base[k] += sums[k];
     }
-    if (tid == 0) {
-      first[P] = (int32_t)base[0];
-      if (base[0] > l.items) bad_s = 1;
-    }
+    if (tid == 0 && base[0] > l.items) bad_s = 1;
     for (int i = tid; i < (int)base[2] * a.hkv; i += kThreads) ((int32_t*)(a.work + l.counters_off))[i] = 0;
     n_parts[list] = (int32_t)P;
     __syncthreads();

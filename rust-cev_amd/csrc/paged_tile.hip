@@ -30,9 +30,6 @@ constexpr int kKeys = kPagedKeys[kPagedMany], kSlots = kPagedSlots[kPagedMany];
 constexpr int D = 128, NDT = D / 32;
 static_assert(kSlots == kWaves * 32 && kKeys == 64 && kTileBytes == kKeys * 2 * D, "tile layout");
 
-// Cache policy of loads and stores that go past the XCD's own L2 (sc1).
-constexpr int kPastL2 = 16;
-
 // This lane's half of the wave, computed afresh (opaque to hoisting).
 __device__ __forceinline__ int fresh_half() { return fresh_lane_id() >> 5; }
 
@@ -44,10 +41,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   __shared__ __align__(16) char lds[2 * kBuf * kTileBytes];
   __shared__ int32_t odd_s, bad_s, last_s;
 
-  const PagedHeader* const hdr = (const PagedHeader*)a.work;
-  if (hdr->sig != a.sig || hdr->bad != 0) return;  // the other kernel writes NaN
   const int run = blockIdx.x / (uint32_t)a.hkv, kvh = blockIdx.x - run * a.hkv;
-  if (run >= uniform_i32(hdr->n_parts[kPagedMany])) return;
+  PagedWalk walk(a, run);
+  int n_parts;
+  if (!paged_plan_ok(a, kPagedMany, n_parts)) return;  // the other kernel writes NaN
+  if (run >= n_parts) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i32(tid >> 6);
   const int n = lane & 31, u = lane >> 5;
   const int gs = __builtin_ctz(a.g);
@@ -99,9 +97,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     vat[r] = (4 * r + (lane >> 4)) * vr + (v_slot(blk, row) << 4);
   }
 
-  int item_end;
-  for (int item = paged_first_item(a, run, item_end); item < item_end; ++item) {
-    const PagedItem it = paged_item(a, item);
+  for (bool more = true; more;) {
+    const PagedItem it = walk.item();
+    more = it.next >= 0;
     const int pos1 = it.pos0 + it.n_rows - 1;
     const PagedSpan span = paged_span(kKeys, it.pos0, pos1, a.window, a.sinks);
     // Query slot (wave, n) holds row slot / g of the tile and query head slot % g:
@@ -406,13 +404,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       if (wave_active) {
 #pragma unroll
         for (int v = 0; v < 16; ++v)
-          __builtin_amdgcn_raw_buffer_store_b128(
-              __builtin_bit_cast(decltype(__builtin_amdgcn_raw_buffer_load_b128(rs, 0, 0, 0)),
-                                 f32x4{o[v / 4][4 * (v % 4)], o[v / 4][4 * (v % 4) + 1], o[v / 4][4 * (v % 4) + 2], o[v / 4][4 * (v % 4) + 3]}),
-              rs, vec0 + 1024 * v, 0, kPastL2);
-        const float2 w = make_float2(m_set ? m_run : -1e30f, l);
-        if (u == 0)
-          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(decltype(__builtin_amdgcn_raw_buffer_load_b64(rs, 0, 0, 0)), w), rs, ml0, 0, kPastL2);
+          put_past_l2(rs, vec0 + 1024 * v,
+                      f32x4{o[v / 4][4 * (v % 4)], o[v / 4][4 * (v % 4) + 1], o[v / 4][4 * (v % 4) + 2], o[v / 4][4 * (v % 4) + 3]});
+        if (u == 0) put_past_l2(rs, ml0, make_float2(m_set ? m_run : -1e30f, l));
       }
       // The stores have reached memory before the workgroup counts itself.
       __builtin_amdgcn_s_waitcnt(0);
@@ -430,14 +424,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       l = 0.0f;
       for (int q = 0; q < it.n_pieces; ++q) {
         const __amdgpu_buffer_rsrc_t rq = record(q);
-        const float2 w = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rq, ml0, 0, kPastL2));
+        const float2 w = get2_past_l2(rq, ml0);
         const float m = fmaxf(M, w.x), f0 = fast_exp2(M - m), f = fast_exp2(w.x - m);
         M = m;
         l = l * f0 + f * w.y;
         if (wave_active) {
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            const f32x4 x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rq, vec0 + 1024 * v, 0, kPastL2));
+            const f32x4 x = get4_past_l2(rq, vec0 + 1024 * v);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float y = o[v / 4][4 * (v % 4) + e];
