@@ -26,10 +26,19 @@ from typing import Optional
 from ._abi import CEV_BF16, CEV_F32, CEV_ROPE_LINEAR, CEV_ROPE_PLAIN, CEV_ROPE_WAVELENGTH, CEV_ROPE_YARN, CevError, PagedDesc, RopeScaling, calls, check, lib
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(stream):
     """Allocations for work on `stream` (None: the current one)."""
     import torch
-    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+    return _HERE if stream is None else torch.cuda.stream(stream)
+
+
+def _like(x):
+    """A contiguous tensor of x's shape and type, without values."""
+    import torch
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _i32(name: str, value) -> int:
@@ -107,16 +116,13 @@ def rope(q_in, k_in, pos, rot: RotaryAngles, interleaved: bool = False, transpos
     nothing, and no two tokens may have the same one.  transposed: the gradient
     of q_in and k_in from that of q_out and k_out.  Outputs may be their
     inputs.  Returns (q_out, k_out), with v_in also v_out."""
-    import torch
     if slots is not None and (k_out is None or (v_in is not None and v_out is None)):
         raise CevError(-1, "rope: slots need caches to store into")
-    with _on(stream):
-        if q_out is None:
-            q_out = torch.empty(tuple(q_in.shape), dtype=q_in.dtype, device=q_in.device)
-        if k_out is None:
-            k_out = torch.empty(tuple(k_in.shape), dtype=k_in.dtype, device=k_in.device)
-        if v_in is not None and v_out is None:
-            v_out = torch.empty(tuple(v_in.shape), dtype=v_in.dtype, device=v_in.device)
+    if q_out is None or k_out is None or (v_in is not None and v_out is None):
+        with _on(stream):
+            q_out = _like(q_in) if q_out is None else q_out
+            k_out = _like(k_in) if k_out is None else k_out
+            v_out = _like(v_in) if v_in is not None and v_out is None else v_out
     calls().rope(q_in, k_in, v_in, pos, rot.steps, rot.rotary_dim, rot.factor, interleaved, transposed, slots, q_out, k_out, v_out, stream)
     return (q_out, k_out) if v_in is None else (q_out, k_out, v_out)
 
@@ -161,9 +167,8 @@ class PagedAttention:
         return self
 
     def __call__(self, q, k_cache, v_cache, block_table, out=None, stream=None):
-        import torch
         if out is None:
             with _on(stream):
-                out = torch.empty(tuple(q.shape), dtype=q.dtype, device=q.device)
+                out = _like(q)
         calls().paged_attention(self.desc, q, k_cache, v_cache, block_table, out, self.work, stream)
         return out

@@ -98,7 +98,7 @@ __device__ __forceinline__ void wait_read(R& r) {
 }
 
 template <typename T, int D>
-constexpr int kMinWaves = sizeof(T) == 2 && D == 128 ? 2 : 1;
+constexpr int kMinWaves = 2;
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWaves<T, D>))) void paged_attn_kernel(PagedArgs a) {
   using F = Frag<T, D>;
@@ -191,16 +191,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   bool bad_page = false;
   char* const ring = lds + wave * 2 * NB * kTile;
   const int lds_ring = (int)(size_t)(const __attribute__((address_space(3))) char*)ring;
-  // Byte offset of this lane's 16 bytes in load i of either half of a sub-tile.
+  // Row (of load 0 of a half) and block there of this lane's 16 bytes.
   const int ld_row = lane / kBlk, ld_blk = lane % kBlk;
-  int k_at[kLoads / 2], v_at_off[kLoads / 2];
-#pragma unroll
-  for (int i = 0; i < kLoads / 2; ++i) {
-    const int r = kRows * i + ld_row;
-    k_at[i] = r * kr + (k_place(ld_blk, r) << 4);
-    v_at_off[i] = r * vr + (v_place<T>(ld_blk, r) << 4);
-  }
-
   // K (which = 0) or V (1) of sub-tile c into buffer buf; past the end: zeros.
   auto fetch = [&](int c, auto which_c, int buf) {
     constexpr int which = decltype(which_c)::value;
@@ -225,7 +217,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       char* const to = ring + (which * NB + buf) * kTile + half * (kTile / 2);
 #pragma unroll
       for (int i = 0; i < kLoads / 2; ++i) {
-        int off = which ? v_at_off[i] : k_at[i];
+        const int r = kRows * i + ld_row;
+        int off = r * stride + ((which ? v_place<T>(ld_blk, r) : k_place(ld_blk, r)) << 4);
         if (!full) {
           const int key = first + kRows * i + ld_row;
           off = key < span.end && !(key >= span.skip_lo && key < span.skip_hi) ? off : INT32_MAX;

@@ -114,7 +114,10 @@ int32_t cev_paged_bounds(const cev_paged_desc* d, PagedBounds* b) {
       const int64_t by_request = (int64_t)d->n_requests * ((l.max_new + l.rows - 1) / l.rows);
       const int64_t by_rows = d->t / l.rows + (int64_t)d->n_requests;
       items = (by_request < by_rows ? by_request : by_rows) + l.target;
-      if (items > INT32_MAX / 2) return cev_fail(CEV_ERR_UNSUPPORTED, "paged attention: %lld work items are too many", (long long)items);
+      // the plan counts the tiles' sub-tiles, and eight more for each, in 32 bits
+      if ((items - l.target) * ((int64_t)b->max_len / kPagedKeys[i] + 16) > INT32_MAX)
+        return cev_fail(CEV_ERR_UNSUPPORTED, "paged attention: %lld tiles of query rows over %d keys are too many for one call",
+                        (long long)(items - l.target), b->max_len);
     } else {
       l.target = 0;
     }

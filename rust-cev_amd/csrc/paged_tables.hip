@@ -5,42 +5,64 @@
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWaves = kThreads / 64;
-constexpr int kPerThread = kPagedMaxRequests / kThreads;  // requests of a thread
-constexpr int kTokens = 4;                                // packed rows of a thread and round
+// Sums of lower lanes' values by lane moves within rows of 16 lanes and then
+// across rows (a bpermute a step takes ten times as long).  Sums saturate, so
+// that counts out of their bounds stay so.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+__device__ __forceinline__ uint32_t wave_inclusive(uint32_t x) {
+  x = add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false));  // row_shr:1
+  x = add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false));  // row_shr:2
+  x = add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false));  // row_shr:4
+  x = add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false));  // row_shr:8
+  x = add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false));  // row_bcast:15 to rows 1 and 3
+  x = add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false));  // row_bcast:31 to rows 2 and 3
+  return x;
+}
 
-// Sums of the values of all lower lanes and waves (and of the whole
-// workgroup), N values at once.  `part` holds kWaves * N values; two barriers.
-template <int N>
-__device__ __forceinline__ void exclusive_sums(int64_t (&x)[N], int64_t (&total)[N], int64_t* part) {
+// N values at once: each becomes the sum of those of all lower threads, total
+// that of the whole workgroup.  `part` holds N values a wave; two barriers.
+template <int W, int N>
+__device__ __forceinline__ void exclusive_sums(uint32_t (&x)[N], uint32_t (&total)[N], uint32_t* part) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t own[N];
+  uint32_t own[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     own[k] = x[k];
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const int64_t y = __shfl_up(x[k], s, 64);
-      if (lane >= s) x[k] += y;
-    }
-    if (lane == 63) part[wave * N + k] = x[k];
+    x[k] = wave_inclusive(x[k]);
+    if constexpr (W == 1)
+      total[k] = (uint32_t)__builtin_amdgcn_readlane((int)x[k], 63);
+    else if (lane == 63)
+      part[wave * N + k] = x[k];
   }
-  __syncthreads();
+  if constexpr (W > 1) {
+    __syncthreads();
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    int64_t before = 0, all = 0;
+    for (int k = 0; k < N; ++k) {
+      uint32_t before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const int64_t p = part[w * N + k];
-      before += w < wave ? p : 0;
-      all += p;
+      for (int w = 0; w < W; ++w) {
+        const uint32_t p = part[w * N + k];
+        before = add_sat(before, w < wave ? p : 0);
+        all = add_sat(all, p);
+      }
+      x[k] = add_sat(x[k], before);
+      total[k] = all;
     }
-    x[k] += before - own[k];
-    total[k] = all;
+    __syncthreads();
   }
-  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) x[k] = x[k] == UINT32_MAX ? x[k] : x[k] - own[k];
 }
+
+// Workgroups of W waves for up to 64 W PER requests.
+template <typename Fn>
+int32_t by_requests(int32_t n_requests, bool small, Fn&& launch) {
+  if (n_requests <= 64 && small) return launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+  if (n_requests <= 512) return launch(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
+  return launch(std::integral_constant<int, 8>{}, std::integral_constant<int, kPagedMaxRequests / 512>{});
+}
+
+constexpr int kTokens = 4;  // packed rows of a thread and round
 
 struct TablesArgs {
   const int32_t *lengths, *new_len, *ring;
@@ -57,30 +79,31 @@ struct TablesArgs {
 // the two ranges never meet in a ring of n_pages places).  Only the new
 // lengths and the new ring state may lie in their inputs' place; the last
 // workgroup to have read the inputs writes those.
-__global__ __launch_bounds__(kThreads) void paged_tables_kernel(TablesArgs a) {
-  __shared__ int32_t cu_s[kPagedMaxRequests + 1];
-  __shared__ int32_t len_s[kPagedMaxRequests];
-  __shared__ int32_t first_s[kPagedMaxRequests];  // pages taken before this request's; ended: -1 - (pages given back before)
-  __shared__ int64_t part[kWaves * 3];
+template <int W, int PER>
+__global__ __launch_bounds__(64 * W) void paged_tables_kernel(TablesArgs a) {
+  constexpr int kThreads = 64 * W, kMax = kThreads * PER;
+  __shared__ int32_t cu_s[kMax + 1];
+  __shared__ int32_t len_s[kMax];
+  __shared__ int32_t first_s[kMax];  // pages taken before this request's; ended: -1 - (pages given back before)
+  __shared__ uint32_t part[W * 3];
   __shared__ int32_t status_s, last_s;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int R = a.n_requests, per = (R + kThreads - 1) / kThreads;
+  const int R = a.n_requests;
   const int page = 1 << a.page_shift;
   if (tid == 0) status_s = 0;
-  const int64_t head = a.ring[0], count = a.ring[1];
-  int32_t len[kPerThread], add[kPerThread];
-  int64_t x[3] = {0, 0, 0};  // new tokens, pages taken, pages given back
+  const int32_t head = a.ring[0], count = a.ring[1];
+  int32_t len[PER], add[PER];
+  uint32_t x[3] = {0, 0, 0};  // new tokens, pages taken, pages given back
   int bad = 0;
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    const int r = tid * per + i;
-    const bool ok = i < per && r < R;
-    len[i] = ok ? a.lengths[r] : 0;
-    add[i] = ok ? a.new_len[r] : 0;
+  for (int i = 0; i < PER; ++i) {
+    const int r = tid * PER + i;
+    len[i] = r < R ? a.lengths[r] : 0;
+    add[i] = r < R ? a.new_len[r] : 0;
   }
   const int32_t max_len = a.max_pages << a.page_shift;
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
+  for (int i = 0; i < PER; ++i) {
     if (len[i] < 0 || len[i] > max_len || add[i] < -1) {
       bad |= 8;
       len[i] = add[i] = 0;
@@ -91,35 +114,36 @@ __global__ __launch_bounds__(kThreads) void paged_tables_kernel(TablesArgs a) {
     }
     const int32_t have = (len[i] + page - 1) >> a.page_shift;
     if (add[i] < 0) {
-      x[2] += a.free_pages ? have : 0;
+      x[2] = add_sat(x[2], a.free_pages ? have : 0);
     } else {
-      x[0] += add[i];
-      x[1] += a.free_pages ? ((len[i] + add[i] + page - 1) >> a.page_shift) - have : 0;
+      x[0] = add_sat(x[0], add[i]);
+      x[1] = add_sat(x[1], a.free_pages ? ((len[i] + add[i] + page - 1) >> a.page_shift) - have : 0);
     }
   }
-  int64_t total[3];
-  exclusive_sums(x, total, part);
-  if (total[0] > a.max_tokens) bad |= 1;
+  uint32_t total[3];
+  exclusive_sums<W>(x, total, part);
+  if (total[0] > (uint32_t)a.max_tokens) bad |= 1;
   if (a.free_pages) {
     if (head < 0 || head >= a.n_pages || count < 0 || count > a.n_pages)
       bad |= 8;
-    else if (total[1] > count)
+    else if (total[1] > (uint32_t)count)
       bad |= 4;
-    else if (count + total[2] > a.n_pages)
+    else if (total[2] > (uint32_t)(a.n_pages - count))
       bad |= 8;
   }
+  if (W == 1) __syncthreads();  // (status_s is clear; the sums' barriers do it otherwise)
   if (bad) atomicOr(&status_s, bad);
   __syncthreads();
   const int status = status_s;
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    const int r = tid * per + i;
-    if (i < per && r < R) {
+  for (int i = 0; i < PER; ++i) {
+    const int r = tid * PER + i;
+    if (r < R) {
       const int32_t have = (len[i] + page - 1) >> a.page_shift;
       cu_s[r] = status ? 0 : (int32_t)x[0];
       len_s[r] = len[i];
       if (add[i] < 0) {
-        first_s[r] = (int32_t)(-1 - x[2]);
+        first_s[r] = (int32_t)(-1 - (int32_t)x[2]);
         x[2] += a.free_pages ? have : 0;
       } else {
         first_s[r] = (int32_t)x[1];
@@ -134,6 +158,11 @@ __global__ __launch_bounds__(kThreads) void paged_tables_kernel(TablesArgs a) {
 
   if (blockIdx.x == 0)
     for (int r = tid; r <= R; r += kThreads) a.cu[r] = cu_s[r];
+  // Place i of the ring, counted from its head: i < 2 n_pages - head.
+  auto place = [&](uint32_t i) {
+    const uint32_t at = (uint32_t)head + i;
+    return at >= (uint32_t)a.n_pages ? at - (uint32_t)a.n_pages : at;
+  };
 
   // Rows: kTokens in a row to a thread; its first one's request by bisection.
   const int64_t step = (int64_t)gridDim.x * kThreads * kTokens;
@@ -146,42 +175,40 @@ __global__ __launch_bounds__(kThreads) void paged_tables_kernel(TablesArgs a) {
         if (cu_s[mid] <= i0) r = mid; else hi = mid;
       }
     }
-    int32_t p[kTokens], sl[kTokens];
+    int32_t p[kTokens], id[kTokens];
+    int32_t* entry[kTokens];  // of a new page's first token
 #pragma unroll
     for (int k = 0; k < kTokens; ++k) {
       const int i = (int)i0 + k;
       p[k] = 0;
-      sl[k] = -1;
+      id[k] = -1;
+      entry[k] = nullptr;
       if (i0 + k < n) {
         while (cu_s[r + 1] <= i) ++r;
         p[k] = len_s[r] + i - cu_s[r];
         const int32_t j = p[k] >> a.page_shift, have = (len_s[r] + page - 1) >> a.page_shift;
-        int32_t* const entry = a.block_table + r * a.bt_stride + j;
-        int32_t id;
-        if (a.free_pages && j >= have) {
-          id = a.free_pages[(head + first_s[r] + (j - have)) % a.n_pages];
-          if ((p[k] & (page - 1)) == 0) *entry = id;
-        } else {
-          id = *entry;
-        }
-        sl[k] = (uint32_t)id < (uint32_t)a.n_pages ? (id << a.page_shift) + (p[k] & (page - 1)) : -1;
+        int32_t* const e = a.block_table + r * a.bt_stride + j;
+        const bool fresh = a.free_pages && j >= have;
+        id[k] = *(fresh ? a.free_pages + place((uint32_t)(first_s[r] + (j - have))) : e);
+        entry[k] = fresh && (p[k] & (page - 1)) == 0 ? e : nullptr;
       }
     }
 #pragma unroll
     for (int k = 0; k < kTokens; ++k)
       if (i0 + k < a.max_tokens) {
         a.pos[i0 + k] = p[k];
-        a.slots[i0 + k] = sl[k];
+        a.slots[i0 + k] = (uint32_t)id[k] < (uint32_t)a.n_pages ? (id[k] << a.page_shift) + (p[k] & (page - 1)) : -1;
+        if (entry[k]) *entry[k] = id[k];
       }
   }
 
   // Pages of the requests that ended: a wave to a request.
   if (status == 0 && a.free_pages && total[2] > 0)
-    for (int r = blockIdx.x * kWaves + (tid >> 6); r < R; r += gridDim.x * kWaves)
+    for (int r = blockIdx.x * W + (tid >> 6); r < R; r += gridDim.x * W)
       if (first_s[r] < 0) {
         const int32_t have = (len_s[r] + page - 1) >> a.page_shift;
         for (int j = lane; j < have; j += 64)
-          a.free_pages[(head + count + (-1 - first_s[r]) + j) % a.n_pages] = a.block_table[r * a.bt_stride + j];
+          a.free_pages[place((uint32_t)count + (uint32_t)(-1 - first_s[r]) + (uint32_t)j)] = a.block_table[r * a.bt_stride + j];
       }
 
   if (gridDim.x > 1) {
@@ -198,8 +225,9 @@ __global__ __launch_bounds__(kThreads) void paged_tables_kernel(TablesArgs a) {
       a.lengths_out[r] = first_s[r] < 0 ? 0 : len_s[r] + cu_s[r + 1] - cu_s[r];
   }
   if (tid == 0) {
-    a.ring_out[0] = (int32_t)(status || !a.free_pages ? head : (head + total[1]) % a.n_pages);
-    a.ring_out[1] = (int32_t)(status || !a.free_pages ? count : count - total[1] + total[2]);
+    const bool same = status || !a.free_pages;
+    a.ring_out[0] = same ? head : (int32_t)place(total[1]);
+    a.ring_out[1] = same ? count : count - (int32_t)total[1] + (int32_t)total[2];
     a.ring_out[2] = status;
     a.ring_out[3] = 0;
   }
@@ -217,31 +245,39 @@ struct PlanArgs {
 };
 
 // What an item costs beside its sub-tiles (its start, and its partial or final
-// result), in sub-tiles; and the least that a run is worth, in the same.
-constexpr int kItemCost = 8, kMinRun = 16;
-static_assert(kMinRun > kItemCost, "no run without a sub-tile");
+// result), in sub-tiles.
+constexpr int kItemCost = 8;
+// Sub-tiles of a piece where there are workgroups enough for all (joining the
+// pieces costs about as much as 16 sub-tiles: one token after 301 keys 9.8 us in
+// one piece, 11.1 us in two).
+constexpr int kPiece[kPagedLists] = {16, 32};
 
-// One workgroup.  A list's tiles (runs of query rows of a request), one after
-// the other, are a row of key sub-tiles, each tile kItemCost longer than its
-// own; it is cut into as many runs of equal length as workgroups run at once,
-// and every piece of a tile that lies in one run is an item.  So all workgroups
-// end together whatever the lengths, and a tile is split only where a cut
-// falls.
-__global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
-  __shared__ int32_t tiles_s[kPagedMaxRequests + 1];  // tiles before each request's
-  __shared__ int32_t row_s[kPagedMaxRequests], n_s[kPagedMaxRequests], pos_s[kPagedMaxRequests];
-  __shared__ int64_t part[kWaves * 3];
+// One workgroup.  A list's tiles are runs of query rows of a request.  When
+// there are workgroups enough for every tile in pieces of kPiece sub-tiles, each
+// piece is a run of its own.  Otherwise the tiles, one after the other, each
+// kItemCost longer than its sub-tiles, are cut into as many runs of equal length
+// as workgroups run at once, and every piece of a tile that lies in one run is
+// an item: all workgroups end together whatever the lengths, and a tile is split
+// only where a cut falls.
+//
+// Sums of sub-tiles are 32-bit: cev_paged_bounds refuses shapes beyond.
+template <int W, int PER>
+__global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
+  constexpr int kThreads = 64 * W, kMax = kThreads * PER;
+  __shared__ int32_t tiles_s[kMax + 1];  // tiles before each request's
+  __shared__ int32_t row_s[kMax], n_s[kMax], pos_s[kMax];
+  __shared__ uint32_t part[W * 3];
   __shared__ int32_t bad_s;
   const int tid = threadIdx.x;
-  const int R = a.n_requests, per = (R + kThreads - 1) / kThreads;
+  const int R = a.n_requests;
   if (tid == 0) bad_s = 0;
   __syncthreads();
-  int32_t rows[kPerThread];
+  int32_t rows[PER];
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    const int r = tid * per + i;
+  for (int i = 0; i < PER; ++i) {
+    const int r = tid * PER + i;
     rows[i] = 0;
-    if (i < per && r < R) {
+    if (r < R) {
       const int32_t row = a.cu[r], end = a.cu[r + 1], len = a.lengths[r];
       const int64_t n = (int64_t)end - row;
       const bool bad = row < 0 || end > a.t || n < 0 || n > a.max_new || len < n || len > a.max_len;
@@ -259,25 +295,26 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
     const PagedListBounds& l = a.list[list];
     n_parts[list] = 0;
     if (l.max_new < l.min_new) continue;
-    int64_t x[1] = {0}, total[1];
-    int32_t n_tiles[kPerThread];
+    uint32_t x[1] = {0}, total[1];
+    int32_t n_tiles[PER];
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
+    for (int i = 0; i < PER; ++i) {
       n_tiles[i] = rows[i] >= l.min_new && rows[i] <= l.max_new ? (rows[i] + l.rows - 1) / l.rows : 0;
       x[0] += n_tiles[i];
     }
-    exclusive_sums(x, total, part);
+    exclusive_sums<W>(x, total, part);
     int32_t before = (int32_t)x[0];
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-      const int r = tid * per + i;
-      if (i < per && r < R) tiles_s[r] = before;
+    for (int i = 0; i < PER; ++i) {
+      const int r = tid * PER + i;
+      if (r < R) tiles_s[r] = before;
       before += n_tiles[i];
     }
     const int32_t all = (int32_t)total[0];
     if (tid == 0) tiles_s[R] = all;
     __syncthreads();
     if (bad_s) break;  // (rows of a request beyond its bounds)
+    if (all == 0) continue;
 
     // tile i of the list; its sub-tiles in c_end
     auto tile = [&](int i) {
@@ -296,51 +333,66 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
       t.c_end = paged_span(kPagedKeys[list], t.pos0, t.pos0 + t.n_rows - 1, a.window, a.sinks).total;
       return t;
     };
-    int64_t sum[1] = {0};
-    for (int i = tid; i < all; i += kThreads) sum[0] += tile(i).c_end + kItemCost;
-    exclusive_sums(sum, total, part);
-    // (a run is longer than a tile's cost, so sub-tiles lie in every run)
-    const int64_t T = total[0], P = T == 0 ? 0 : max(min(T / kMinRun, (int64_t)l.target), (int64_t)1);
+    uint32_t sum[2] = {0, 0}, sums[2];  // length of all tiles; pieces of them
+    for (int i = tid; i < all; i += kThreads) {
+      const uint32_t n_sub = (uint32_t)tile(i).c_end;
+      sum[0] += n_sub + kItemCost;
+      sum[1] += (n_sub + kPiece[list] - 1) / kPiece[list];
+    }
+    exclusive_sums<W>(sum, sums, part);
+    const bool pieces = sums[1] <= (uint32_t)l.target;
+    // length of a run (longer than a tile's cost, so sub-tiles lie in every one)
+    const uint32_t len = max((sums[0] + (uint32_t)l.target - 1) / (uint32_t)l.target, (uint32_t)kItemCost + 1);
+    const int32_t P = (int32_t)(pieces ? sums[1] : (sums[0] + len - 1) / len);
 
     PagedItem* const first = (PagedItem*)(a.work + l.first_off);
     PagedItem* const items = (PagedItem*)(a.work + l.items_off);
-    int64_t units = 0, base[3] = {0, 0, 0};  // length so far; items, partial results and split tiles
+    uint32_t units = 0, base[3] = {0, 0, 0};  // length so far; items, partial results and split tiles
     for (int i0 = 0; i0 < all; i0 += kThreads) {
       const int i = i0 + tid;
       PagedItem t{};
       if (i < all) t = tile(i);
-      const int32_t n_sub = t.c_end;
-      int64_t u[1] = {n_sub ? n_sub + kItemCost : 0}, u_all[1];
-      exclusive_sums(u, u_all, part);
-      // run r is [r T / P, (r + 1) T / P); a tile's cost comes before its sub-tiles
-      const int64_t from = units + u[0], keys = from + kItemCost, to = keys + n_sub;
-      const int64_t r0 = n_sub ? ((keys + 1) * P - 1) / T : 0, r1 = n_sub ? (to * P - 1) / T : -1;
-      const int64_t n = r1 - r0 + 1;
-      int64_t y[3] = {n, n > 1 ? n : 0, n > 1 ? 1 : 0}, sums[3];
-      exclusive_sums(y, sums, part);
+      const uint32_t n_sub = (uint32_t)t.c_end;
+      uint32_t u[1] = {n_sub ? n_sub + kItemCost : 0}, u_all[1];
+      exclusive_sums<W>(u, u_all, part);
+      // run r is [r len, (r + 1) len); a tile's cost comes before its sub-tiles
+      const uint32_t from = units + u[0], keys = from + kItemCost, to = keys + n_sub;
+      const uint32_t r0 = keys / len, r1 = n_sub ? (to - 1) / len : 0;
+      const uint32_t n = !n_sub ? 0 : pieces ? (n_sub + kPiece[list] - 1) / kPiece[list] : r1 - r0 + 1;
+      uint32_t y[3] = {n, n > 1 ? n : 0, n > 1 ? 1u : 0u}, y_all[3];
+      exclusive_sums<W>(y, y_all, part);
       t.n_pieces = (int32_t)n;
       t.rec = (int32_t)(base[1] + y[1]);
       t.split = (int32_t)(base[2] + y[2]);
-      for (int64_t r = r0; r <= r1; ++r) {
-        const int64_t begin = r * T / P, end = (r + 1) * T / P, at = base[0] + y[0] + (r - r0);
-        t.c_begin = (int32_t)(max(begin, keys) - keys);
-        t.c_end = (int32_t)(min(end, to) - keys);
-        t.piece = (int32_t)(r - r0);
-        // the run goes on with the next tile when that tile's sub-tiles begin in it
-        t.next = to + kItemCost < end && i + 1 < all ? (int32_t)at + 1 : -1;
-        // it begins here when no tile before has sub-tiles in it
-        if (at < l.items) {
+      for (uint32_t k = 0; k < n; ++k) {
+        const uint32_t at = base[0] + y[0] + k, begin = (r0 + k) * len, end = begin + len;
+        t.piece = (int32_t)k;
+        if (pieces) {
+          t.c_begin = (int32_t)(k * n_sub / n);
+          t.c_end = (int32_t)((k + 1) * n_sub / n);
+          t.next = -1;
+        } else {
+          t.c_begin = (int32_t)(max(begin, keys) - keys);
+          t.c_end = (int32_t)(min(end, to) - keys);
+          // the run goes on with the next tile when that tile's sub-tiles begin in it
+          t.next = to + kItemCost < end && i + 1 < all ? (int32_t)at + 1 : -1;
+        }
+        if (at < (uint32_t)l.items) {
           items[at] = t;
-          if (begin >= from) first[r] = t;
+          // a run begins here when no tile before has sub-tiles in it
+          if (pieces)
+            first[at] = t;
+          else if (begin >= from)
+            first[r0 + k] = t;
         }
       }
       units += u_all[0];
 #pragma unroll
-      for (int k = 0; k < 3; ++k) base[k] += sums[k];
+      for (int k = 0; k < 3; ++k) base[k] += y_all[k];
     }
-    if (tid == 0 && base[0] > l.items) bad_s = 1;
+    if (tid == 0 && base[0] > (uint32_t)l.items) bad_s = 1;
     for (int i = tid; i < (int)base[2] * a.hkv; i += kThreads) ((int32_t*)(a.work + l.counters_off))[i] = 0;
-    n_parts[list] = (int32_t)P;
+    n_parts[list] = P;
     __syncthreads();
   }
   if (tid == 0) *h = PagedHeader{a.sig, bad_s, {bad_s ? 0 : n_parts[0], bad_s ? 0 : n_parts[1]}};
@@ -381,11 +433,15 @@ extern "C" int32_t cev_paged_tables(int32_t n_requests, int32_t page_size, int32
   a.n_pages = n_pages;
   a.max_pages = max_pages;
   a.max_tokens = max_tokens;
-  const int64_t grid = ((int64_t)max_tokens + kThreads * kTokens - 1) / (kThreads * kTokens);
-  hipLaunchKernelGGL(paged_tables_kernel, dim3((unsigned)(grid < 1 ? 1 : grid > 256 ? 256 : grid)), dim3(kThreads), 0, (hipStream_t)stream, a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return cev_fail(CEV_ERR_HIP, "paged tables launch: %s", hipGetErrorString(e));
-  return CEV_OK;
+  return by_requests(n_requests, max_tokens <= 64 * kTokens, [&](auto w_c, auto per_c) {
+    constexpr int W = decltype(w_c)::value, PER = decltype(per_c)::value, rows = 64 * W * kTokens;
+    const int64_t grid = ((int64_t)max_tokens + rows - 1) / rows;
+    hipLaunchKernelGGL((paged_tables_kernel<W, PER>), dim3((unsigned)(grid < 1 ? 1 : grid > 256 ? 256 : grid)), dim3(64 * W), 0,
+                       (hipStream_t)stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return cev_fail(CEV_ERR_HIP, "paged tables launch: %s", hipGetErrorString(e));
+    return (int32_t)CEV_OK;
+  });
 }
 
 extern "C" int32_t cev_paged_plan(const cev_paged_desc* d, const int32_t* cu, const int32_t* lengths, void* work, size_t work_bytes,
@@ -409,8 +465,13 @@ extern "C" int32_t cev_paged_plan(const cev_paged_desc* d, const int32_t* cu, co
   a.sinks = d->sinks;
   a.hkv = d->n_kv_heads;
   a.sig = b.sig;
-  hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return cev_fail(CEV_ERR_HIP, "paged plan launch: %s", hipGetErrorString(e));
-  return CEV_OK;
+  // one wave where a lane has a few tiles at most
+  const int64_t tiles = (int64_t)b.list[kPagedFew].items - b.list[kPagedFew].target + b.list[kPagedMany].items - b.list[kPagedMany].target;
+  return by_requests(d->n_requests, tiles <= 256, [&](auto w_c, auto per_c) {
+    constexpr int W = decltype(w_c)::value, PER = decltype(per_c)::value;
+    hipLaunchKernelGGL((paged_plan_kernel<W, PER>), dim3(1), dim3(64 * W), 0, (hipStream_t)stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return cev_fail(CEV_ERR_HIP, "paged plan launch: %s", hipGetErrorString(e));
+    return (int32_t)CEV_OK;
+  });
 }

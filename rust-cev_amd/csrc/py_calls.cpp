@@ -392,9 +392,11 @@ struct OnDevice {
   void* stream(PyObject* o) const { return o == Py_None ? (void*)c10::hip::getCurrentHIPStream(device.index()).stream() : stream_of(o); }
 };
 
-void want(bool ok, const char* call, const std::string& msg) {
-  if (!ok) raise_cev(CEV_ERR_INVALID, std::string(call) + ": " + msg);
-}
+// (a macro: the message is put together only when it is raised)
+#define want(ok, call, msg)                                                     \
+  do {                                                                          \
+    if (!(ok)) raise_cev(CEV_ERR_INVALID, std::string(call) + ": " + (msg));    \
+  } while (0)
 void want_i32(const char* call, const char* name, const at::Tensor* t, int64_t size) {
   if (!t) return;
   want(t->scalar_type() == at::kInt && t->dim() == 1 && t->is_contiguous() && t->size(0) == size, call,
@@ -447,7 +449,8 @@ PyObject* py_paged_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// rope(q_in, k_in, v_in, pos, steps, rotary_dim, factor, interleaved, transposed, slots, q_out, k_out, v_out, stream)
+// rope(q_in, k_in, v_in, pos, steps, rotary_dim, factor, interleaved, transposed, slots, q_out, k_out, v_out, stream): all on
+// one GPU, outputs given
 PyObject* py_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&] {
     need_args(n, 14);
