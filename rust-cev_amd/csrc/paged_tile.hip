@@ -123,65 +123,78 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       const int c = c0 + i;
       return kKeys * (c < span.sinks ? c : c - span.sinks + span.first);
     };
+    // Chunks of the part before lo and from hi on hold keys that not all rows
+    // at positions [p0, p1] see (those before lo may also be seen by all).
+    auto unmasked = [&](int p0, int p1, int& lo, int& hi) {
+      // the chunks of the window start at stream place span.sinks; the last key
+      // of the one at place c is first_key + 63
+      hi = span.sinks + (p0 + 1) / kKeys - span.first - c0;
+      lo = 0;
+      if (a.window > 0 && p1 >= a.window) lo = span.sinks + (p1 - a.window) / kKeys + 1 - span.first - c0;
+    };
+    int w_lo, w_hi, t_lo, t_hi;  // of this wave's rows, and of all of the tile's
+    unmasked(w_pos0, w_pos1, w_lo, w_hi);
+    unmasked(it.pos0, pos1, t_lo, t_hi);
+
     const int32_t* const bt = a.bt + it.req * a.bt_stride;
-    // Lane l keeps the page of this wave's rows of chunk 64 b + l of the
-    // current batch b.
-    int batch_first = 0, page_l = 0;
+    // Lane l keeps the addresses of this wave's rows of K and of V of chunk 64 b +
+    // l of the current batch b, and whether they are fetched at all.
+    int batch_first = 0, k_lo = 0, k_hi = 0, v_lo = 0, v_hi = 0, fetched = 0;
+    bool bad_page = false;
     auto load_pages = [&](int i) {
       batch_first = i;
-      const int j = first_key(min(i + lane, nc - 1)) + 8 * wave;
+      const int key0 = first_key(min(i + lane, nc - 1)) + 8 * wave;
       // (the last chunk may reach beyond the block table's last page)
-      page_l = bt[min(j >> a.page_shift, a.max_pages - 1)];
+      int page = bt[min(key0 >> a.page_shift, a.max_pages - 1)];
+      // rows that some row of the tile sees
+      const bool seen = key0 < span.end && !(key0 >= span.skip_lo && key0 + 8 <= span.skip_hi);
+      const bool in = (uint32_t)page < (uint32_t)a.n_pages;
+      bad_page |= __any(seen && !in);
+      fetched = seen && in ? 8 : 0;
+      page = in ? page : 0;
+      const int64_t off = key0 & ((1 << a.page_shift) - 1);
+      const uint64_t kp = kbase + 2 * (uint64_t)(page * a.kc_sp + off * a.kc_st), vp = vbase + 2 * (uint64_t)(page * a.vc_sp + off * a.vc_st);
+      k_lo = (int)(uint32_t)kp, k_hi = (int)(uint32_t)(kp >> 32);
+      v_lo = (int)(uint32_t)vp, v_hi = (int)(uint32_t)(vp >> 32);
     };
     load_pages(0);
-    bool bad_page = false;
 
     // Chunk i into its buffer, i mod kBuf; past the end: zeros.
     auto fetch = [&](int i) {
-      const int buf = i % kBuf;
       const bool real = i < nc;
       if (real && i >= batch_first + 64) load_pages(i);
-      const int key0 = (real ? first_key(i) : 0) + 8 * wave;  // first of this wave's rows
       const int l = real ? i - batch_first : 0;
-      // keys that some row of the tile sees
-      const bool seen = real && key0 < span.end && !(key0 >= span.skip_lo && key0 + 8 <= span.skip_hi);
-      const bool full = key0 + 8 <= span.end && !(key0 < span.skip_hi && key0 + 8 > span.skip_lo);
-      int page = __builtin_amdgcn_readlane(page_l, l);
-      const bool in = (uint32_t)page < (uint32_t)a.n_pages;
-      bad_page |= seen && !in;
-      page = in ? page : 0;
-      const int off = key0 & ((1 << a.page_shift) - 1);
-      const uint64_t kp = kbase + 2 * (uint64_t)(page * a.kc_sp) + (uint64_t)(off * (int64_t)kr);
-      const uint64_t vp = vbase + 2 * (uint64_t)(page * a.vc_sp) + (uint64_t)(off * (int64_t)vr);
-      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)uniform_u64(kp), (short)0, uniform_i32(seen && in ? 8 * kr : 0), kBufferWord3);
-      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)uniform_u64(vp), (short)0, uniform_i32(seen && in ? 8 * vr : 0), kBufferWord3);
+      const int rows = real ? __builtin_amdgcn_readlane(fetched, l) : 0;
+      const uint64_t kp = (uint32_t)__builtin_amdgcn_readlane(k_lo, l) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(k_hi, l) << 32;
+      const uint64_t vp = (uint32_t)__builtin_amdgcn_readlane(v_lo, l) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(v_hi, l) << 32;
+      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)kp, (short)0, rows * kr, kBufferWord3);
+      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)vp, (short)0, rows * vr, kBufferWord3);
+      int ka[2] = {kat[0], kat[1]}, va[2] = {vat[0], vat[1]};
+      if (i >= t_hi || i < t_lo) {  // it may hold keys that no row sees
+        const int key0 = (real ? first_key(i) : 0) + 8 * wave;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        int ka = kat[r], va = vat[r];
-        if (!full) {
+        for (int r = 0; r < 2; ++r) {
           const int key = key0 + 4 * r + (lane >> 4);
           const bool load = key < span.end && !(key >= span.skip_lo && key < span.skip_hi);
-          ka = load ? ka : INT32_MAX;
-          va = load ? va : INT32_MAX;
+          ka[r] = load ? ka[r] : INT32_MAX;
+          va[r] = load ? va[r] : INT32_MAX;
         }
-        const int dst = buf * kTileBytes + (8 * wave + 4 * r) * kRowBytes;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)(lds + dst), 16, ka, 0, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(lds + kVBase + dst), 16, va, 0, 0, 0);
+      }
+      char* const dst = lds + i % kBuf * kTileBytes + 8 * wave * kRowBytes;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)(dst + 4 * r * kRowBytes), 16, ka[r], 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(dst + kVBase + 4 * r * kRowBytes), 16, va[r], 0, 0, 0);
       }
     };
     constexpr int kLoadsPerChunk = 4;
 
-    // Whether a chunk from key0 on holds a key that some row of positions
-    // [p0, p1] does not see.
-    auto masked = [&](int key0, int p0, int p1) {
-      return key0 + kKeys - 1 > p0 || (a.window > 0 && key0 <= p1 - a.window && key0 + kKeys > a.sinks);
-    };
     // 0 times an infinity or NaN is NaN: a key that only some of the rows see
     // must not reach the others.  Where the rows differ in what they see of chunk
     // i, such values among the V rows that this wave fetched (landed by now)
     // become zeros; after the loop they are added to the rows that see them.
     auto clean = [&](int i) {
-      if (i >= nc || !masked(first_key(i), it.pos0, pos1)) return;
+      if (i >= nc || (i >= t_lo && i < t_hi)) return;
       i32x4* const v = (i32x4*)(lds + kVBase + i % kBuf * kTileBytes + 8 * wave * kRowBytes);
       bool odd = false;
 #pragma unroll
@@ -238,7 +251,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
       for (int st = 0; st < F::NQK; ++st)
         fr.qk_mfma(*(const bf16x8*)(lds + (koff[st] - lds_base)), st, sa);
-      if (masked(first_key(0), w_pos0, w_pos1)) mask_sub(sa, first_key(0));
+      if (0 >= w_hi || 0 < w_lo) mask_sub(sa, first_key(0));
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sa[i]);
@@ -323,16 +336,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         __builtin_amdgcn_sched_barrier(0);
       });
       const int in = i + kt;  // chunk of the next scores
-      if (in < nc && masked(first_key(in), w_pos0, w_pos1)) mask_sub(sn, first_key(in) + 32 * (1 - kt));
+      if (in < w_lo || in >= w_hi) mask_sub(sn, first_key(in) + 32 * (1 - kt));
     };
     const bool lead = wave >= kWaves / 2;
     if (wave_active && lead) region_a(I0{});
 #pragma unroll 1
     for (int i = 0; i < nc; ++i) {
-      fetch(i + kAhead);
       const int next = i % kBuf == kBuf - 1 ? -kAhead * kTileBytes : kTileBytes;  // to the next chunk's buffer
+      if (wave_active && !lead) region_a(I0{});
+      fetch(i + kAhead);
       if (wave_active) {
-        if (!lead) region_a(I0{});
 #pragma unroll
         for (int st = 0; st < F::NQK; ++st) koff[st] += next;
         region_b(I0{}, i);
@@ -365,7 +378,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     if (*(volatile int32_t*)&odd_s && wave_active) {
 #pragma unroll 1
       for (int i = 0; i < nc; ++i) {
-        if (!masked(first_key(i), it.pos0, pos1)) continue;
+        if (i >= t_lo && i < t_hi) continue;
 #pragma unroll 1
         for (int kk = 0; kk < kKeys; ++kk) {
           const int key = first_key(i) + kk;
