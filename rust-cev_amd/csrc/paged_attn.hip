@@ -91,6 +91,24 @@ __device__ __forceinline__ float read_b32(int vaddr) {
   asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(r) : "v"(vaddr), "i"(OFF) : "memory");
   return r;
 }
+template <int N, typename R>
+__device__ __forceinline__ void pass_through(R& r) {
+  asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(r) : "i"(N));
+}
+// All LDS reads but the last N have returned, and the values given are there.
+template <int N, typename... R>
+__device__ __forceinline__ void wait_reads(R&... r) {
+  static_assert(N >= 0 && N < 16, "lgkmcnt range");
+  (void)std::initializer_list<int>{(pass_through<N>(r), 0)...};
+}
+// Six MFMAs with the vector instructions of the region spread between them.
+__device__ __forceinline__ void beside_mfmas() {
+#pragma unroll
+  for (int i = 0; i < 6; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // one MFMA
+    __builtin_amdgcn_sched_group_barrier(0x2, 8, 0);  // eight VALU instructions
+  }
+}
 // Every LDS read has returned, and r holds its value.
 template <typename R>
 __device__ __forceinline__ void wait_read(R& r) {
@@ -111,12 +129,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   constexpr int kRows = 1024 / kRB, kBlk = kRB / 16;  // rows of one load, 16-byte blocks of a row
   constexpr int RS = D + 4;                      // row stride (floats) of a partial result in LDS
   constexpr int kRing = kWaves * 2 * NB * kTile, kOut = kWaves * 32 * RS * 4, kBody = kRing > kOut ? kRing : kOut;
-  // Q of 512-byte rows (f32: its parts) lies in LDS, shared by the waves: with
-  // it in registers O is moved to and from the accumulation registers at every
-  // rescale, and at d = 256 spilled.
-  constexpr bool kQInLds = kRB == 512;
-  constexpr int kQSteps = D / 16 * (BF ? 1 : 3);  // operands of 1 KB
-  __shared__ __align__(16) char lds[kBody + (kQInLds ? kQSteps * 1024 : 0)];
+  // Q of d = 256 lies in LDS, shared by the waves (with it in registers O is
+  // moved to and from the accumulation registers, and some of it spilled).
+  constexpr bool kQInLds = BF && D == 256;
+  __shared__ __align__(16) char lds[kBody + (kQInLds ? D / 16 * 1024 : 0)];
   __shared__ float2 ml[kWaves * 32];
   __shared__ int32_t last_s;
 
@@ -151,23 +167,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       for (int j = 0; j < 4; ++j) x[e + j] = v[j];
     }
   };
-  if constexpr (!kQInLds) {
+  bf16x8 qp[BF ? 1 : D / 16][3];  // f32: the parts of q[16 st + 8 u ..]
+  if constexpr (!BF) {
+#pragma unroll
+    for (int st = 0; st < D / 16; ++st) {
+      float x[8];
+      load_q8(st, x);
+      bf16_parts(x, qp[st]);
+    }
+  } else if constexpr (!kQInLds) {
     fr.load_q(qrow, ok, u);
   } else {
 #pragma unroll
     for (int i = 0; i < D / 16 / kWaves; ++i) {
       const int st = wave * (D / 16 / kWaves) + i;
-      if constexpr (BF) {
-        const bf16x8 z = {};
-        *(bf16x8*)(lds + kBody + st * 1024 + lane * 16) = ok ? *(const bf16x8*)(qrow + 16 * st + 8 * u) : z;
-      } else {
-        float x[8];
-        load_q8(st, x);
-        bf16x8 parts[3];
-        bf16_parts(x, parts);
-#pragma unroll
-        for (int k = 0; k < 3; ++k) *(bf16x8*)(lds + kBody + (3 * st + k) * 1024 + lane * 16) = parts[k];
-      }
+      const bf16x8 z = {};
+      *(bf16x8*)(lds + kBody + st * 1024 + lane * 16) = ok ? *(const bf16x8*)(qrow + 16 * st + 8 * u) : z;
     }
   }
 
@@ -256,17 +271,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     return (T*)(ring + (NB + buf) * kTile + key * kRB + (v_place<T>(col * (int)sizeof(T) / 16, key) << 4)) + col % (16 / (int)sizeof(T));
   };
 
-  // f32: an infinite value (or one above bf16's range) has no parts.  A wave
-  // that ends with anything non-finite walks its keys again on the f32 unit.
-  bool exact = false;
-  for (;;) {
+  // This wave's sub-tiles.  f32: an infinite value (or one above bf16's range)
+  // has no parts; a wave that ends with anything non-finite walks its keys again
+  // on the f32 unit (exact).
+  auto pass = [&](auto exact_c) {
+    constexpr bool kExact = decltype(exact_c)::value;
     int c = it.c_begin + wave;
-    if (c < c_end) {
-    load_pages(c);
-    }
-    if constexpr (kQInLds)
-      if (!exact) __syncthreads();  // Q is in LDS
-    if (c < c_end) {
+    if (c < c_end) load_pages(c);
+    if constexpr (kQInLds) __syncthreads();  // Q is in LDS
+    if (c >= c_end) return;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       fetch(c + b * kWaves, K_c{}, b);
@@ -278,56 +291,85 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       pipe::wait_vmcnt<(2 * NB - 1) * kLoads>();
       asm volatile("" ::: "memory");
       f32x16 s = f32x16{};
-      // K operands (and Q's of 512-byte rows) in groups, one group ahead of the
-      // MFMAs: two steps of 16 head-dim values, at d = 128 in bf16 four.
-      constexpr int kSteps = kQInLds ? 2 : 4, kKReads = BF ? 1 : 2, kQReads = kQInLds ? (BF ? 1 : 3) : 0;
-      i32x4 kf[2][kSteps * kKReads], qf[2][kSteps * kQReads + 1];
       const int ka = lds_ring + buf * kTile;
-      auto k_issue = [&](auto g_c) {
-        constexpr int G = decltype(g_c)::value;
-        static_for<kSteps * kKReads>([&](auto e_c) {
-          // read J is block 2 J + u (bf16), 4 (J / 2) + 2 u + J % 2 (f32); bit 4 of a block's place is its own
-          constexpr int E = decltype(e_c)::value, J = G * kSteps * kKReads + E;
-          kf[G & 1][E] = read_b128<(J / 8) * 256>(ka + koff[J % 8]);
-        });
-        static_for<kSteps * kQReads>([&](auto e_c) {
-          constexpr int E = decltype(e_c)::value;
-          qf[G & 1][E] = read_b128<(G * kSteps * kQReads + E) * 1024>(lds_q);
-        });
-      };
-      k_issue(std::integral_constant<int, 0>{});
-      static_for<D / 16 / kSteps>([&](auto g_c) {
-        constexpr int G = decltype(g_c)::value;
-        static_for<kSteps * kKReads>([&](auto e_c) { wait_read(kf[G & 1][decltype(e_c)::value]); });
-        static_for<kSteps * kQReads>([&](auto e_c) { wait_read(qf[G & 1][decltype(e_c)::value]); });
-        if constexpr (G + 1 < D / 16 / kSteps) k_issue(std::integral_constant<int, G + 1>{});
-        static_for<kSteps>([&](auto e_c) {
-          constexpr int E = decltype(e_c)::value, st = G * kSteps + E;
-          if constexpr (BF) {
+      if constexpr (BF) {
+        // K operands (and Q's of d = 256) in groups, one group ahead of the MFMAs
+        constexpr int kSteps = kQInLds ? 2 : 4, kQReads = kQInLds ? 1 : 0;
+        i32x4 kf[2][kSteps], qf[2][kSteps * kQReads + 1];
+        auto k_issue = [&](auto g_c) {
+          constexpr int G = decltype(g_c)::value;
+          static_for<kSteps>([&](auto e_c) {
+            // read J is block 2 J + u; bit 4 of a block's place is its own
+            constexpr int E = decltype(e_c)::value, J = G * kSteps + E;
+            kf[G & 1][E] = read_b128<(J / 8) * 256>(ka + koff[J % 8]);
+          });
+          static_for<kSteps * kQReads>([&](auto e_c) {
+            constexpr int E = decltype(e_c)::value;
+            qf[G & 1][E] = read_b128<(G * kSteps + E) * 1024>(lds_q);
+          });
+        };
+        k_issue(std::integral_constant<int, 0>{});
+        static_for<D / 16 / kSteps>([&](auto g_c) {
+          constexpr int G = decltype(g_c)::value;
+          static_for<kSteps>([&](auto e_c) { wait_read(kf[G & 1][decltype(e_c)::value]); });
+          static_for<kSteps * kQReads>([&](auto e_c) { wait_read(qf[G & 1][decltype(e_c)::value]); });
+          if constexpr (G + 1 < D / 16 / kSteps) k_issue(std::integral_constant<int, G + 1>{});
+          static_for<kSteps>([&](auto e_c) {
+            constexpr int E = decltype(e_c)::value, st = G * kSteps + E;
             const bf16x8 k = __builtin_bit_cast(bf16x8, kf[G & 1][E]);
             if constexpr (kQInLds)
               s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, __builtin_bit_cast(bf16x8, qf[G & 1][E]), s, 0, 0, 0);
             else
               fr.qk_mfma(k, st, s);
+          });
+        });
+      } else {
+        // Step st: two reads (blocks 4 st + 2 u and the next), the parts of their
+        // values, six MFMAs.  A step's parts are made beside the MFMAs of the one
+        // before; its reads are two steps ahead.
+        i32x4 kf[3][2];
+        bf16x8 kp[2][3];
+        auto k_issue = [&](auto st_c) {
+          constexpr int ST = decltype(st_c)::value;
+          static_for<2>([&](auto e_c) {
+            constexpr int E = decltype(e_c)::value, J = 2 * ST + E;
+            kf[ST % 3][E] = read_b128<(J / 8) * 256>(ka + koff[J % 8]);
+          });
+        };
+        auto values = [&](auto st_c, float* x) {
+          constexpr int ST = decltype(st_c)::value;
+          __builtin_memcpy(x, &kf[ST % 3][0], 16);
+          __builtin_memcpy(x + 4, &kf[ST % 3][1], 16);
+        };
+        k_issue(std::integral_constant<int, 0>{});
+        k_issue(std::integral_constant<int, 1>{});
+        wait_reads<2>(kf[0][0], kf[0][1]);
+        if constexpr (!kExact) {
+          float x[8];
+          values(std::integral_constant<int, 0>{}, x);
+          bf16_parts(x, kp[0]);
+        }
+        static_for<D / 16>([&](auto st_c) {
+          constexpr int ST = decltype(st_c)::value;
+          if constexpr (ST + 2 < D / 16) k_issue(std::integral_constant<int, ST + 2>{});
+          if constexpr (ST + 1 < D / 16) wait_reads<(ST + 2 < D / 16 ? 2 : 0)>(kf[(ST + 1) % 3][0], kf[(ST + 1) % 3][1]);
+          float x[8];
+          if constexpr (kExact) {
+            float q[8];
+            values(st_c, x);
+            load_q8(ST, q);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], q[e], s, 0, 0, 0);
           } else {
-            float x[8];
-            __builtin_memcpy(x, &kf[G & 1][2 * E], 16);
-            __builtin_memcpy(x + 4, &kf[G & 1][2 * E + 1], 16);
-            if (!exact) {
-              bf16x8 kp[3], qp[3];
-              bf16_parts(x, kp);
-#pragma unroll
-              for (int k = 0; k < 3; ++k) qp[k] = __builtin_bit_cast(bf16x8, qf[G & 1][3 * E + k]);
-              s = parts_mma(kp, qp, s);
-            } else {
-              float q[8];
-              load_q8(st, q);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], q[e], s, 0, 0, 0);
+            if constexpr (ST + 1 < D / 16) {
+              values(std::integral_constant<int, ST + 1>{}, x);
+              bf16_parts(x, kp[(ST + 1) & 1]);
             }
+            s = parts_mma(kp[ST & 1], qp[ST], s);
+            beside_mfmas();
           }
         });
-      });
+      }
       asm volatile("" ::: "memory");
       const bool masked = key0 + kKeys - 1 > it.pos0 ||
                           (a.window > 0 && key0 <= pos1 - a.window && key0 + kKeys > a.sinks);
@@ -433,35 +475,43 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
         });
       } else {
         // V values of step j = 4 h + dt, keys 16 h + 8 (e / 4) + 4 u + e % 4 of
-        // column 32 dt + n, one step ahead of the MFMAs
-        float vf[2][8];
+        // column 32 dt + n: as above
+        float vf[3][8];
         const int va = lds_ring + (NB + buf) * kTile;
         auto v_issue = [&](auto j_c) {
           constexpr int J = decltype(j_c)::value, H = J / NDT, DT = J % NDT;
           static_for<8>([&](auto e_c) {
             constexpr int E = decltype(e_c)::value;
-            vf[J & 1][E] = read_b32<(16 * H + 8 * (E >> 2) + (E & 3)) * kRB>(va + voff[DT]);
+            vf[J % 3][E] = read_b32<(16 * H + 8 * (E >> 2) + (E & 3)) * kRB>(va + voff[DT]);
           });
         };
-        bf16x8 pp[3];
+        constexpr int kSteps = 2 * NDT;
+        bf16x8 pp[2][3], vp[2][3];
         v_issue(std::integral_constant<int, 0>{});
-        static_for<2 * NDT>([&](auto j_c) {
-          constexpr int J = decltype(j_c)::value, H = J / NDT, DT = J % NDT;
-          static_for<8>([&](auto e_c) { wait_read(vf[J & 1][decltype(e_c)::value]); });
-          if constexpr (J + 1 < 2 * NDT) v_issue(std::integral_constant<int, J + 1>{});
-          if (!exact) {
-            if constexpr (DT == 0) {
-              float x[8];
+        v_issue(std::integral_constant<int, 1>{});
+        if constexpr (!kExact) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = p.v[8 * H + e];
-              bf16_parts(x, pp);
-            }
-            bf16x8 vp[3];
-            bf16_parts(vf[J & 1], vp);
-            o[DT] = parts_mma(vp, pp, o[DT]);
+          for (int h = 0; h < 2; ++h) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = p.v[8 * h + e];
+            bf16_parts(x, pp[h]);
+          }
+        }
+        wait_reads<8>(vf[0][0], vf[0][1], vf[0][2], vf[0][3], vf[0][4], vf[0][5], vf[0][6], vf[0][7]);
+        if constexpr (!kExact) bf16_parts(vf[0], vp[0]);
+        static_for<kSteps>([&](auto j_c) {
+          constexpr int J = decltype(j_c)::value, H = J / NDT, DT = J % NDT, N = (J + 1) % 3;
+          if constexpr (J + 2 < kSteps) v_issue(std::integral_constant<int, J + 2>{});
+          if constexpr (J + 1 < kSteps)
+            wait_reads<(J + 2 < kSteps ? 8 : 0)>(vf[N][0], vf[N][1], vf[N][2], vf[N][3], vf[N][4], vf[N][5], vf[N][6], vf[N][7]);
+          if constexpr (kExact) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[DT] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[J % 3][e], p.v[8 * H + e], o[DT], 0, 0, 0);
           } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) o[DT] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[J & 1][e], p.v[8 * H + e], o[DT], 0, 0, 0);
+            if constexpr (J + 1 < kSteps) bf16_parts(vf[N], vp[(J + 1) & 1]);
+            o[DT] = parts_mma(vp[J & 1], pp[H], o[DT]);
+            beside_mfmas();
           }
         });
       }
@@ -481,16 +531,18 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     // loads past the end still write zeros into LDS
     pipe::wait_vmcnt<0>();
     asm volatile("" ::: "memory");
-    }
-    if constexpr (BF) break;
+  };
+  pass(std::false_type{});
+  if constexpr (!BF) {
     float t = l_run * 0.0f + m_run * 0.0f;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) t += o[dt][i] * 0.0f;
-    if (exact || !__any(!(t == 0.0f))) break;
-    exact = true;
-    reset();
+    if (__any(!(t == 0.0f))) {
+      reset();
+      pass(std::true_type{});
+    }
   }
 
   // ---- join the waves' partial results through LDS
