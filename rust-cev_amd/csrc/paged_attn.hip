@@ -606,62 +606,84 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   const bool last = last_s;
   __syncthreads();
   if (!last) continue;
-  // Threads -> (group of pieces, 4-column unit): with few rows several groups
-  // walk the pieces, kBatch at a time, and meet in LDS.
-  constexpr int kBatch = 8;
+  // Threads -> (group of pieces, 4-column units kThreads apart): with few rows
+  // several groups walk the pieces and meet in LDS.  All loads of kUnits x
+  // kBatch partial results are in flight at once: a trip past the L2 takes
+  // 1.5 us (with one unit at a time the joining of three pieces of 32 slots took
+  // 6 us at d = 128, 12 us at d = 256).
+  constexpr int kUnits = BF && D == 128 ? 2 : 4, kBatch = 4;
   const int units = slots * kCols;
   int groups = 1;
   while (groups < 8 && 2 * groups * units <= kThreads && 2 * groups < it.n_pieces) groups *= 2;
-  for (int i0 = 0; i0 < units; i0 += kThreads) {
-    const int i = i0 + tid, unit = i % units, group = i / units;
-    const int slot = unit / kCols, col = 4 * (unit % kCols);
-    float M = -INFINITY, L = 0.0f;
-    f32x4 x = f32x4{};
+  const int group = groups > 1 ? tid / units : 0, unit0 = groups > 1 ? tid % units : tid;
+  for (int i0 = 0; i0 < units; i0 += kUnits * kThreads) {
+    float M[kUnits], L[kUnits];
+    f32x4 x[kUnits];
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      M[k] = -INFINITY;
+      L[k] = 0.0f;
+      x[k] = f32x4{};
+    }
     if (group < groups) {
       for (int p0 = group; p0 < it.n_pieces; p0 += kBatch * groups) {
-        f32x4 y[kBatch];
-        float2 w[kBatch];
+        f32x4 y[kUnits][kBatch];
+        float2 w[kUnits][kBatch];
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-          const int at = min(p0 + b * groups, it.n_pieces - 1) * (int)(a.hkv * kRec * 4);
-          y[b] = get4_past_l2(all, at + (slot * D + col) * 4);
-          w[b] = get2_past_l2(all, at + (kSlots * D + 2 * slot) * 4);
+        for (int k = 0; k < kUnits; ++k) {
+          // (units beyond the last, and pieces beyond theirs, read the last again)
+          const int unit = min(i0 + unit0 + k * kThreads, units - 1), slot = unit / kCols, col = 4 * (unit % kCols);
+          if (k > 0 && i0 + k * kThreads >= units) break;
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int at = min(p0 + b * groups, it.n_pieces - 1) * (int)(a.hkv * kRec * 4);
+            y[k][b] = get4_past_l2(all, at + (slot * D + col) * 4);
+            w[k][b] = get2_past_l2(all, at + (kSlots * D + 2 * slot) * 4);
+          }
         }
-        float m = M;
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) m = fmaxf(m, w[b].x);
-        const float f0 = fast_exp2(M - m);
-        M = m;
-        L *= f0;
-        x *= f0;
+        for (int k = 0; k < kUnits; ++k) {
+          if (k > 0 && i0 + k * kThreads >= units) break;
+          float m = M[k];
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-          const float f = p0 + b * groups < it.n_pieces ? fast_exp2(w[b].x - m) : 0.0f;
-          if (f > 0.0f || w[b].y != w[b].y) {
-            L += f * w[b].y;
-            x += f * y[b];
+          for (int b = 0; b < kBatch; ++b) m = fmaxf(m, w[k][b].x);
+          const float f0 = fast_exp2(M[k] - m);
+          M[k] = m;
+          L[k] *= f0;
+          x[k] *= f0;
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const float f = p0 + b * groups < it.n_pieces ? fast_exp2(w[k][b].x - m) : 0.0f;
+            if (f > 0.0f || w[k][b].y != w[k][b].y) {
+              L[k] += f * w[k][b].y;
+              x[k] += f * y[k][b];
+            }
           }
         }
       }
       if (groups > 1) {
-        *(f32x4*)(ob + (group * units + unit) * 8) = x;
-        *(float2*)(ob + (group * units + unit) * 8 + 4) = make_float2(M, L);
+        *(f32x4*)(ob + (group * units + unit0) * 8) = x[0];
+        *(float2*)(ob + (group * units + unit0) * 8 + 4) = make_float2(M[0], L[0]);
       }
     }
     if (groups > 1) {
       __syncthreads();
       if (group == 0) {
         for (int k = 1; k < groups; ++k) {
-          const float2 w = *(const float2*)(ob + (k * units + unit) * 8 + 4);
-          const f32x4 y = *(const f32x4*)(ob + (k * units + unit) * 8);
-          const float m = fmaxf(M, w.x), f0 = fast_exp2(M - m), f = fast_exp2(w.x - m);
-          M = m;
-          L = L * f0 + f * w.y;
-          x = x * f0 + f * y;
+          const float2 w = *(const float2*)(ob + (k * units + unit0) * 8 + 4);
+          const f32x4 y = *(const f32x4*)(ob + (k * units + unit0) * 8);
+          const float m = fmaxf(M[0], w.x), f0 = fast_exp2(M[0] - m), f = fast_exp2(w.x - m);
+          M[0] = m;
+          L[0] = L[0] * f0 + f * w.y;
+          x[0] = x[0] * f0 + f * y;
         }
       }
     }
-    if (group == 0) put(slot, col, x, L);
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      const int unit = i0 + unit0 + k * kThreads;
+      if (group == 0 && unit < units) put(unit / kCols, 4 * (unit % kCols), x[k], L[k]);
+    }
   }
   __syncthreads();
   if (tid == 0) *counter = 0;  // for the next call with this plan
