@@ -647,6 +647,25 @@ def test_attention_of_a_long_prompt(gpu, kind, hq, hkv, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,d", [("bf16", 128), ("bf16", 256), ("f32", 128)])
+@pytest.mark.parametrize("requests,past_hi,new_hi", [(40, 700, 1), (70, 300, 9), (9, 1500, 200), (200, 40, 3), (3, 60, 900), (33, 2500, 2)])
+def test_attention_of_more_work_than_workgroups(gpu, kind, d, requests, past_hi, new_hi):
+    """Sixteen KV heads leave 16 or 32 workgroups a head: tiles in rounds, cut
+    ones, shared-out ones.  Twice with one plan: the same bits."""
+    import torch
+    rng = random.Random(requests)
+    past = [rng.choice([0, rng.randint(0, past_hi), past_hi]) for _ in range(requests)]
+    new = [rng.choice([1, new_hi, rng.randint(0, new_hi)]) for _ in range(requests)]
+    p = _Paged(gpu, past, new, 16, 16, d, kind, 16, seed=requests)
+    for kw in ({}, dict(window=50, sinks=5)):
+        att = p.attention(**kw)
+        att.plan(p.cu, p.lengths)
+        out = att(p.q, p.k, p.v, p.table, out=torch.full_like(p.q, 5.0))
+        p.check(out, **kw)
+        assert torch.equal(att(p.q, p.k, p.v, p.table, out=torch.full_like(p.q, 5.0)), out)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind,hq,hkv,d", SHAPES)
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("which", ["k", "v"])
