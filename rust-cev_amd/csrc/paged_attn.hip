@@ -115,8 +115,10 @@ __device__ __forceinline__ void wait_read(R& r) {
   asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(r));
 }
 
+// Waves a SIMD that registers are left for: two workgroups of bf16 d = 128 share
+// a CU, the others' LDS holds one.
 template <typename T, int D>
-constexpr int kMinWaves = 2;
+constexpr int kMinWaves = sizeof(T) == 2 && D == 128 ? 2 : 1;
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWaves<T, D>))) void paged_attn_kernel(PagedArgs a) {
   using F = Frag<T, D>;
@@ -125,10 +127,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   constexpr int kRB = D * (int)sizeof(T);        // bytes of one key row
   constexpr int kTile = kKeys * kRB;        // K or V of a sub-tile
   constexpr int kLoads = kTile / 1024;           // 1 KB loads of it
-  constexpr int NB = 1;         // sub-tiles of K and of V in LDS
   constexpr int kRows = 1024 / kRB, kBlk = kRB / 16;  // rows of one load, 16-byte blocks of a row
   constexpr int RS = D + 4;                      // row stride (floats) of a partial result in LDS
-  constexpr int kRing = kWaves * 2 * NB * kTile, kOut = kWaves * 32 * RS * 4, kBody = kRing > kOut ? kRing : kOut;
+  constexpr int kRing = kWaves * 2 * kTile, kOut = kWaves * 32 * RS * 4, kBody = kRing > kOut ? kRing : kOut;
   // Q of d = 256 lies in LDS, shared by the waves (with it in registers O is
   // moved to and from the accumulation registers, and some of it spilled).
   constexpr bool kQInLds = BF && D == 256;
@@ -156,34 +157,32 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   const int pos1 = it.pos0 + it.n_rows - 1;
   const PagedSpan span = paged_span(kKeys, it.pos0, pos1, a.window, a.sinks);
 
-  // ---- Q, as the B operand
+  // ---- Q, as the B operand; zeros in slots without a row
   const T* const qrow = (const T*)a.q + (int64_t)row * a.q_st + (int64_t)head * a.q_sh;
   F fr;
-  auto load_q8 = [&](int st, float* x) {
-#pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-      const f32x4 v = ok ? *(const f32x4*)(qrow + 16 * st + 8 * u + e) : f32x4{};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[e + j] = v[j];
-    }
+  auto load_q8 = [&](int st, f32x4* x) {
+    x[0] = ok ? *(const f32x4*)(qrow + 16 * st + 8 * u) : f32x4{};
+    x[1] = ok ? *(const f32x4*)(qrow + 16 * st + 8 * u + 4) : f32x4{};
   };
   bf16x8 qp[BF ? 1 : D / 16][3];  // f32: the parts of q[16 st + 8 u ..]
   if constexpr (!BF) {
 #pragma unroll
     for (int st = 0; st < D / 16; ++st) {
+      f32x4 q[2];
       float x[8];
-      load_q8(st, x);
+      load_q8(st, q);
+      __builtin_memcpy(x, q, 32);
       bf16_parts(x, qp[st]);
     }
-  } else if constexpr (!kQInLds) {
-    fr.load_q(qrow, ok, u);
-  } else {
+  } else if constexpr (kQInLds) {
 #pragma unroll
     for (int i = 0; i < D / 16 / kWaves; ++i) {
       const int st = wave * (D / 16 / kWaves) + i;
       const bf16x8 z = {};
       *(bf16x8*)(lds + kBody + st * 1024 + lane * 16) = ok ? *(const bf16x8*)(qrow + 16 * st + 8 * u) : z;
     }
+  } else {
+    fr.load_q(qrow, ok, u);
   }
 
   // ---- this wave's sub-tiles: c_begin + wave, + kWaves, ...
@@ -204,12 +203,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     page_b = bt[min((j + 16) >> a.page_shift, a.max_pages - 1)];
   };
   bool bad_page = false;
-  char* const ring = lds + wave * 2 * NB * kTile;
+  char* const ring = lds + wave * 2 * kTile;
   const int lds_ring = (int)(size_t)(const __attribute__((address_space(3))) char*)ring;
   // Row (of load 0 of a half) and block there of this lane's 16 bytes.
   const int ld_row = lane / kBlk, ld_blk = lane % kBlk;
-  // K (which = 0) or V (1) of sub-tile c into buffer buf; past the end: zeros.
-  auto fetch = [&](int c, auto which_c, int buf) {
+  // K (which = 0) or V (1) of sub-tile c into its buffer; past the end: zeros.
+  auto fetch = [&](int c, auto which_c) {
     constexpr int which = decltype(which_c)::value;
     const bool real = c < c_end;
     if (real && which == 0 && c >= batch_first + kWaves * 64) load_pages(c);
@@ -229,7 +228,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       page = in ? page : 0;
       const uint64_t base = (which ? vbase : kbase) + (uint64_t)(page * page_bytes) + (uint64_t)((first & ((1 << a.page_shift) - 1)) * (int64_t)stride);
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)uniform_u64(base), (short)0, uniform_i32(seen && in ? 16 * stride : 0), kBufferWord3);
-      char* const to = ring + (which * NB + buf) * kTile + half * (kTile / 2);
+      char* const to = ring + which * kTile + half * (kTile / 2);
 #pragma unroll
       for (int i = 0; i < kLoads / 2; ++i) {
         const int r = kRows * i + ld_row;
@@ -266,9 +265,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       voff[dt] = BF ? (4 * u + rr) * kRB + (v_place<T>(4 * dt + blk, rr) << 4) + 8 * (i & 1)
                     : 4 * u * kRB + (v_place<T>(8 * dt + n / 4, 4 * u) << 4) + 4 * (n & 3);
   }
-  // A value of V in buffer buf.
-  auto v_at = [&](int buf, int key, int col) -> T* {
-    return (T*)(ring + (NB + buf) * kTile + key * kRB + (v_place<T>(col * (int)sizeof(T) / 16, key) << 4)) + col % (16 / (int)sizeof(T));
+  // A value of V.
+  auto v_at = [&](int key, int col) -> T* {
+    return (T*)(ring + kTile + key * kRB + (v_place<T>(col * (int)sizeof(T) / 16, key) << 4)) + col % (16 / (int)sizeof(T));
   };
 
   // This wave's sub-tiles.  f32: an infinite value (or one above bf16's range)
@@ -280,18 +279,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     if (c < c_end) load_pages(c);
     if constexpr (kQInLds) __syncthreads();  // Q is in LDS
     if (c >= c_end) return;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      fetch(c + b * kWaves, K_c{}, b);
-      fetch(c + b * kWaves, V_c{}, b);
-    }
-    auto step = [&](int buf) {
+    fetch(c, K_c{});
+    fetch(c, V_c{});
+    auto step = [&] {
       const int key0 = first_key(c);
       // K of this sub-tile has landed once only later loads are in flight
-      pipe::wait_vmcnt<(2 * NB - 1) * kLoads>();
+      pipe::wait_vmcnt<kLoads>();
       asm volatile("" ::: "memory");
       f32x16 s = f32x16{};
-      const int ka = lds_ring + buf * kTile;
+      const int ka = lds_ring;
       if constexpr (BF) {
         // K operands (and Q's of d = 256) in groups, one group ahead of the MFMAs
         constexpr int kSteps = kQInLds ? 2 : 4, kQReads = kQInLds ? 1 : 0;
@@ -356,8 +352,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
           float x[8];
           if constexpr (kExact) {
             float q[8];
+            f32x4 q4[2];
             values(st_c, x);
-            load_q8(ST, q);
+            load_q8(ST, q4);
+            __builtin_memcpy(q, q4, 32);
 #pragma unroll
             for (int e = 0; e < 8; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], q[e], s, 0, 0, 0);
           } else {
@@ -384,9 +382,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
           s[i] = (at <= hi) & ((at > lo) | (at < first)) ? s[i] : -INFINITY;
         }
       }
-      // (s is made: K's buffer is free for the sub-tile NB ahead)
+      // (s is made: K's buffer is free for the next sub-tile)
       __builtin_amdgcn_sched_barrier(0);
-      fetch(c + NB * kWaves, K_c{}, buf);
+      fetch(c + kWaves, K_c{});
       __builtin_amdgcn_sched_barrier(0);
       float mx = -INFINITY;
 #pragma unroll
@@ -405,13 +403,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       for (int i = 0; i < 16; ++i) s[i] = fast_exp2(__builtin_fmaf(s[i], a.scale_log2, -m_run));
       typename F::P p;
       F::make_p(s, p, l_run);
-      pipe::wait_vmcnt<(2 * NB - 1) * kLoads>();
+      pipe::wait_vmcnt<kLoads>();
       asm volatile("" ::: "memory");
       if (masked) {
         // 0 times an infinity or NaN is NaN: a key that only some of the rows
         // see must not reach the others.  Such values are added to the rows
         // that see them (whatever their weight) and are zeros for the products.
-        const f32x4* const vt = (const f32x4*)(ring + (NB + buf) * kTile);
+        const f32x4* const vt = (const f32x4*)(ring + kTile);
         uint32_t odd = 0;
 #pragma unroll
         for (int i = 0; i < kTile / 1024; ++i) {
@@ -431,14 +429,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
             for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
-                const float v = (float)*v_at(buf, kk, 32 * dt + 8 * (i >> 2) + 4 * u + (i & 3));
+                const float v = (float)*v_at(kk, 32 * dt + 8 * (i >> 2) + 4 * u + (i & 3));
                 const bool finite = (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u;
                 o[dt][i] += (finite | !vis) ? 0.0f : v;
               }
           }
           wave_lds_sync();
           for (int i = lane; i < kKeys * D; i += 64) {
-            T* const x = (T*)(ring + (NB + buf) * kTile) + i;
+            T* const x = (T*)(ring + kTile) + i;
             const float v = (float)*x;
             if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) *x = (T)0.0f;
           }
@@ -447,7 +445,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
         }
       }
       if constexpr (BF) {
-        const int va = lds_ring + (NB + buf) * kTile;
+        const int va = lds_ring + kTile;
         constexpr int kGrp = 4;
         pipe::i32x2 f[2][kGrp][2];
         auto issue = [&](auto g_c) {
@@ -477,7 +475,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
         // V values of step j = 4 h + dt, keys 16 h + 8 (e / 4) + 4 u + e % 4 of
         // column 32 dt + n: as above
         float vf[3][8];
-        const int va = lds_ring + (NB + buf) * kTile;
+        const int va = lds_ring + kTile;
         auto v_issue = [&](auto j_c) {
           constexpr int J = decltype(j_c)::value, H = J / NDT, DT = J % NDT;
           static_for<8>([&](auto e_c) {
@@ -517,17 +515,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
-      fetch(c + NB * kWaves, V_c{}, buf);
+      fetch(c + kWaves, V_c{});
       __builtin_amdgcn_sched_barrier(0);
       c += kWaves;
     };
-    while (c < c_end) {
-      step(0);
-      if constexpr (NB == 2) {
-        if (c >= c_end) break;
-        step(1);
-      }
-    }
+    while (c < c_end) step();
     // loads past the end still write zeros into LDS
     pipe::wait_vmcnt<0>();
     asm volatile("" ::: "memory");

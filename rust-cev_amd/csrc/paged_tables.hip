@@ -242,18 +242,36 @@ struct PlanArgs {
   PagedListBounds list[kPagedLists];
   int32_t n_requests, t, max_new, max_len, window, sinks, hkv;
   uint32_t sig;
+  bool bf16, two_a_cu;
 };
 
 // What an item costs beside its sub-tiles (its start, and its partial or final
 // result), in sub-tiles.
 constexpr int kItemCost = 8;
-// Sub-tiles of a piece where there are workgroups enough for all (joining the
-// pieces costs about as much as 16 sub-tiles: one token after 301 keys 9.8 us in
-// one piece, 11.1 us in two).
-constexpr int kPiece[kPagedLists] = {16, 32};
+// Pieces of a tile of n_sub sub-tiles where there are workgroups enough for all.
+// A piece's sub-tiles take r us each, and joining the pieces takes j us for each
+// of them (the last workgroup reads them past its L2), so the best length is near
+// sqrt(n_sub j / r); the waves of the kernel of few rows take four sub-tiles at
+// once, and up to two of those a wave are not worth a join.  Of a tile that fills
+// at most half of its slots less is read.  `by` makes the pieces longer.  One
+// request, us, against pieces of 16 sub-tiles of the first kernel, 32 of the second:
+//   one row, 4 heads a KV head, after  1023 / 4095 keys
+//     bf16 d = 128   8.3 (11.4) / 11.0 (12.1)
+//     bf16 d = 256  11.1 (16.5) / 14.8 (17.2)    f32  12.5 (23.4) / 15.7 (23.6)
+//   32 slots of bf16 d = 128 in 1024 / 4096 keys   13.5 (16.1) / 18.0 (18.1)
+//   256 slots of the second kernel                 30.8 (35.9) / 44.9 (69.0)
+__device__ __forceinline__ uint32_t piece_count(int list, bool bf16, bool half_filled, uint32_t n_sub, float by) {
+  const float n = (float)n_sub, root = __builtin_amdgcn_sqrtf(n);
+  float len;
+  if (list == kPagedMany)
+    len = 2.0f * root;
+  else
+    len = n_sub <= 8 ? 8.0f : fmaxf(4.0f, 4.0f * rintf((half_filled ? 0.125f : 0.25f) * (bf16 ? 1.4f : 0.7f) * root));
+  return 1 + (uint32_t)((n - 1.0f) * __builtin_amdgcn_rcpf(by * len));
+}
 
 // One workgroup.  A list's tiles are runs of query rows of a request.  When
-// there are workgroups enough for every tile in pieces of kPiece sub-tiles, each
+// there are workgroups enough for every tile in pieces of the best length, each
 // piece is a run of its own.  Otherwise the tiles, one after the other, each
 // kItemCost longer than its sub-tiles, are cut into as many runs of equal length
 // as workgroups run at once, and every piece of a tile that lies in one run is
@@ -266,7 +284,7 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
   constexpr int kThreads = 64 * W, kMax = kThreads * PER;
   __shared__ int32_t tiles_s[kMax + 1];  // tiles before each request's
   __shared__ int32_t row_s[kMax], n_s[kMax], pos_s[kMax];
-  __shared__ uint32_t part[W * 3];
+  __shared__ uint32_t part[W * 4];
   __shared__ int32_t bad_s;
   const int tid = threadIdx.x;
   const int R = a.n_requests;
@@ -333,17 +351,28 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
       t.c_end = paged_span(kPagedKeys[list], t.pos0, t.pos0 + t.n_rows - 1, a.window, a.sinks).total;
       return t;
     };
-    uint32_t sum[2] = {0, 0}, sums[2];  // length of all tiles; pieces of them
+    // length of all tiles; pieces of them, of twice and of four times the length
+    uint32_t sum[4] = {0, 0, 0, 0}, sums[4];
     for (int i = tid; i < all; i += kThreads) {
-      const uint32_t n_sub = (uint32_t)tile(i).c_end;
+      const PagedItem t = tile(i);
+      const uint32_t n_sub = (uint32_t)t.c_end;
       sum[0] += n_sub + kItemCost;
-      sum[1] += (n_sub + kPiece[list] - 1) / kPiece[list];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) sum[1 + k] += piece_count(list, a.bf16, 2 * t.n_rows <= l.rows, n_sub, (float)(1 << k));
     }
     exclusive_sums<W>(sum, sums, part);
-    const bool pieces = sums[1] <= (uint32_t)l.target;
+    // Two workgroups of few rows of bf16 d = 128 share a CU: short pieces are made
+    // longer before that (16 requests of one token after 1023: 15.5 us, 18.1 with
+    // two a CU), long ones are not (4 requests of 32 rows after 4064: 29.4 us with
+    // two a CU, 35.6 in longer pieces).
+    const bool two = list == kPagedFew && a.two_a_cu;
+    const uint32_t target = (uint32_t)l.target, alone = two ? target / 2 : target;
+    const int by = sums[1] <= alone ? 0 : sums[2] <= alone ? 1 : two && sums[3] <= alone && sums[0] <= 24 * sums[3] ? 2 : 1;
+    const uint32_t n_pieces = by == 0 ? sums[1] : by == 1 ? sums[2] : sums[3];
+    const bool pieces = n_pieces <= target;
     // length of a run (longer than a tile's cost, so sub-tiles lie in every one)
-    const uint32_t len = max((sums[0] + (uint32_t)l.target - 1) / (uint32_t)l.target, (uint32_t)kItemCost + 1);
-    const int32_t P = (int32_t)(pieces ? sums[1] : (sums[0] + len - 1) / len);
+    const uint32_t len = max((sums[0] + target - 1) / target, (uint32_t)kItemCost + 1);
+    const int32_t P = (int32_t)(pieces ? n_pieces : (sums[0] + len - 1) / len);
 
     PagedItem* const first = (PagedItem*)(a.work + l.first_off);
     PagedItem* const items = (PagedItem*)(a.work + l.items_off);
@@ -358,7 +387,7 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
       // run r is [r len, (r + 1) len); a tile's cost comes before its sub-tiles
       const uint32_t from = units + u[0], keys = from + kItemCost, to = keys + n_sub;
       const uint32_t r0 = keys / len, r1 = n_sub ? (to - 1) / len : 0;
-      const uint32_t n = !n_sub ? 0 : pieces ? (n_sub + kPiece[list] - 1) / kPiece[list] : r1 - r0 + 1;
+      const uint32_t n = !n_sub ? 0 : pieces ? piece_count(list, a.bf16, 2 * t.n_rows <= l.rows, n_sub, (float)(1 << by)) : r1 - r0 + 1;
       uint32_t y[3] = {n, n > 1 ? n : 0, n > 1 ? 1u : 0u}, y_all[3];
       exclusive_sums<W>(y, y_all, part);
       t.n_pieces = (int32_t)n;
@@ -465,6 +494,8 @@ extern "C" int32_t cev_paged_plan(const cev_paged_desc* d, const int32_t* cu, co
   a.sinks = d->sinks;
   a.hkv = d->n_kv_heads;
   a.sig = b.sig;
+  a.bf16 = d->dtype == CEV_BF16;
+  a.two_a_cu = a.bf16 && d->head_dim == 128;
   // one wave where a lane has a few tiles at most
   const int64_t tiles = (int64_t)b.list[kPagedFew].items - b.list[kPagedFew].target + b.list[kPagedMany].items - b.list[kPagedMany].target;
   return by_requests(d->n_requests, tiles <= 256, [&](auto w_c, auto per_c) {

@@ -433,23 +433,42 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       const bool last = last_s;
       __syncthreads();
       if (!last) continue;
-      float M = -INFINITY;
-      l = 0.0f;
-      for (int q = 0; q < it.n_pieces; ++q) {
-        const __amdgpu_buffer_rsrc_t rq = record(q);
-        const float2 w = get2_past_l2(rq, ml0);
-        const float m = fmaxf(M, w.x), f0 = fast_exp2(M - m), f = fast_exp2(w.x - m);
-        M = m;
-        l = l * f0 + f * w.y;
-        if (wave_active) {
+      // Half of the columns at a time; the next piece is on its way while one is
+      // added (a trip past the L2 takes longer than the adding).
+      if (wave_active) {
 #pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const f32x4 x = get4_past_l2(rq, vec0 + 1024 * v);
+        for (int half = 0; half < 2; ++half) {
+          f32x4 x[2][8];
+          float2 w[2];
+          auto get = [&](int q, f32x4* to, float2& to_w) {
+            const __amdgpu_buffer_rsrc_t rq = record(min(q, it.n_pieces - 1));
+            to_w = get2_past_l2(rq, ml0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float y = o[v / 4][4 * (v % 4) + e];
-              o[v / 4][4 * (v % 4) + e] = q == 0 ? f * x[e] : y * f0 + f * x[e];
-            }
+            for (int v = 0; v < 8; ++v) to[v] = get4_past_l2(rq, vec0 + 1024 * (8 * half + v));
+          };
+          float M = -1e30f;
+          l = 0.0f;
+          o[2 * half] = o[2 * half + 1] = f32x16{};
+          auto add = [&](const f32x4* from, const float2& from_w) {
+            const float m = fmaxf(M, from_w.x), f0 = fast_exp2(M - m), f = fast_exp2(from_w.x - m);
+            M = m;
+            l = l * f0 + f * from_w.y;
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int dt = 2 * half + v / 4, at = 4 * (v % 4) + e;
+                o[dt][at] = o[dt][at] * f0 + f * from[v][e];
+              }
+          };
+          get(0, x[0], w[0]);
+          for (int q = 0;;) {
+            get(q + 1, x[1], w[1]);
+            add(x[0], w[0]);
+            if (++q == it.n_pieces) break;
+            get(q + 1, x[0], w[0]);
+            add(x[1], w[1]);
+            if (++q == it.n_pieces) break;
           }
         }
       }
