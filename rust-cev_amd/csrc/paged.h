@@ -37,9 +37,8 @@ static_assert(sizeof(PagedHeader) == 16 && sizeof(PagedItem) == 48, "work buffer
 
 struct PagedListBounds {
   int32_t rows;      // query rows of a tile
-  int32_t target;    // most workgroups, for each KV head
+  int32_t target;    // most workgroups, for each KV head (0: no request can be in the list)
   int32_t items;     // most items
-  int32_t min_new, max_new;  // requests of the list: min_new <= new rows <= max_new (none: max_new < min_new)
   size_t first_off, items_off, counters_off, records_off;
 };
 // What a descriptor bounds: sizes and offsets of the work buffer's parts.

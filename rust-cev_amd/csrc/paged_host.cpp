@@ -13,7 +13,6 @@ bool power_of_two(int32_t x) { return x > 0 && (x & (x - 1)) == 0; }
 // once (256 CUs; two workgroups of the first kernel share one for bf16 heads
 // of 128, by their LDS).
 constexpr int32_t kFewWorkgroups128 = 512, kFewWorkgroups = 256, kManyWorkgroups = 256;
-constexpr int32_t kFewSlots = 128;
 
 size_t align_up(size_t x) { return (x + 255) & ~(size_t)255; }
 
@@ -95,31 +94,31 @@ int32_t cev_paged_bounds(const cev_paged_desc* d, PagedBounds* b) {
                 (long long)d->bt_stride);
   b->max_len = d->max_pages * d->page_size;
   b->sig = signature(d);
-  // Rows of requests with more than kFewSlots slots go to the kernel whose
-  // workgroups share their keys among 256 slots.
+  // bf16 heads of 128 have a kernel for requests of more rows than one tile of
+  // the first kernel holds; the plan decides which kernel takes them.
   const bool tiles = d->dtype == CEV_BF16 && d->head_dim == 128;
-  const int32_t few = tiles ? kFewSlots / g : INT32_MAX;
   size_t at = 256;
   for (int i = 0; i < kPagedLists; ++i) {
     PagedListBounds& l = b->list[i];
     l.rows = kPagedSlots[i] / g;
-    l.min_new = i == kPagedFew ? 1 : few;
-    if (i == kPagedMany) l.min_new = few == INT32_MAX ? INT32_MAX : few + 1;
-    l.max_new = i == kPagedFew && few < d->max_new ? few : d->max_new;
-    const int32_t cus = i == kPagedFew ? (tiles ? kFewWorkgroups128 : kFewWorkgroups) : kManyWorkgroups;
-    l.target = cus / d->n_kv_heads > 0 ? cus / d->n_kv_heads : 1;
+    l.target = 0;
     int64_t items = 0;
-    if (l.max_new >= l.min_new) {
+    if (i == kPagedFew || (tiles && d->max_new > kPagedSlots[kPagedFew] / g)) {
+      const int32_t cus = i == kPagedMany ? kManyWorkgroups : tiles ? kFewWorkgroups128 : kFewWorkgroups;
+      l.target = cus / d->n_kv_heads > 0 ? cus / d->n_kv_heads : 1;
       // whole tiles, and a cut for each workgroup after the first
-      const int64_t by_request = (int64_t)d->n_requests * ((l.max_new + l.rows - 1) / l.rows);
-      const int64_t by_rows = d->t / l.rows + (int64_t)d->n_requests;
-      items = (by_request < by_rows ? by_request : by_rows) + l.target;
+      auto most = [&](int32_t max_new) {
+        const int64_t by_request = (int64_t)d->n_requests * ((max_new + l.rows - 1) / l.rows);
+        const int64_t by_rows = d->t / l.rows + (int64_t)d->n_requests;
+        return by_request < by_rows ? by_request : by_rows;
+      };
+      items = most(d->max_new) + l.target;
       // the plan counts the tiles' sub-tiles, and eight more for each, in 32 bits
-      if ((items - l.target) * ((int64_t)b->max_len / kPagedKeys[i] + 16) > INT32_MAX)
+      // (much work in requests of many rows is not left to the first kernel)
+      const int64_t counted = most(i == kPagedFew && tiles && d->max_new > l.rows ? l.rows : d->max_new);
+      if (counted * ((int64_t)b->max_len / kPagedKeys[i] + 16) > INT32_MAX)
         return cev_fail(CEV_ERR_UNSUPPORTED, "paged attention: %lld tiles of query rows over %d keys are too many for one call",
-                        (long long)(items - l.target), b->max_len);
-    } else {
-      l.target = 0;
+                        (long long)counted, b->max_len);
     }
     l.items = (int32_t)items;
     l.first_off = at;

@@ -9,13 +9,28 @@ namespace {
 // across rows (a bpermute a step takes ten times as long).  Sums saturate, so
 // that counts out of their bounds stay so.
 __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
-__device__ __forceinline__ uint32_t wave_inclusive(uint32_t x) {
-  x = add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false));  // row_shr:1
-  x = add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false));  // row_shr:2
-  x = add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false));  // row_shr:4
-  x = add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false));  // row_shr:8
-  x = add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false));  // row_bcast:15 to rows 1 and 3
-  x = add_sat(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false));  // row_bcast:31 to rows 2 and 3
+template <typename Op>
+__device__ __forceinline__ uint32_t wave_inclusive(uint32_t x, Op op) {
+  x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false));  // row_shr:1
+  x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false));  // row_shr:2
+  x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false));  // row_shr:4
+  x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false));  // row_shr:8
+  x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false));  // row_bcast:15 to rows 1 and 3
+  x = op(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false));  // row_bcast:31 to rows 2 and 3
+  return x;
+}
+
+// The largest of the workgroup's values.  `part` holds a value a wave; two barriers.
+template <int W>
+__device__ __forceinline__ uint32_t largest(uint32_t x, uint32_t* part) {
+  x = (uint32_t)__builtin_amdgcn_readlane((int)wave_inclusive(x, [](uint32_t a, uint32_t b) { return max(a, b); }), 63);
+  if constexpr (W > 1) {
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) x = max(x, part[w]);
+    __syncthreads();
+  }
   return x;
 }
 
@@ -28,7 +43,7 @@ __device__ __forceinline__ void exclusive_sums(uint32_t (&x)[N], uint32_t (&tota
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     own[k] = x[k];
-    x[k] = wave_inclusive(x[k]);
+    x[k] = wave_inclusive(x[k], add_sat);
     if constexpr (W == 1)
       total[k] = (uint32_t)__builtin_amdgcn_readlane((int)x[k], 63);
     else if (lane == 63)
@@ -245,6 +260,18 @@ struct PlanArgs {
   bool bf16, two_a_cu;
 };
 
+// Requests of more rows than a tile of the first kernel (32 slots) go to the
+// second from this many of the first kernel's sub-tiles for each of its
+// workgroups on.  With fewer the first has more workgroups at work; with more it
+// is bound by reading the keys once for every 32 slots.  First and second kernel
+// (32 query over 8 KV heads, us):
+//   1 request of 256 slots and  2048 keys (8 sub-tiles a workgroup)   20.9  35.1
+//   4 requests of  64 slots and  4096 keys (16)                       25.4  31.8
+//   16 requests of 64 slots and  2048 keys (32)                       34.6  32.8
+//   64 requests of 48 slots and   512 keys (32)                       48.5  36.4
+//   64 requests of 64 slots and  2048 keys (128)                       193   112
+constexpr int kFewWork = 32;
+static_assert((int64_t)kFewWork * 512 < 1 << 18, "the sum's clip");
 // What an item costs beside its sub-tiles (its start, and its partial or final
 // result), in sub-tiles.
 constexpr int kItemCost = 8;
@@ -253,25 +280,26 @@ constexpr int kItemCost = 8;
 // of them (the last workgroup reads them past its L2), so the best length is near
 // sqrt(n_sub j / r); the waves of the kernel of few rows take four sub-tiles at
 // once, and up to two of those a wave are not worth a join.  Of a tile that fills
-// at most half of its slots less is read.  `by` makes the pieces longer.  One
+// at most half of its slots less is read.  piece_rate: one over the length.  One
 // request, us, against pieces of 16 sub-tiles of the first kernel, 32 of the second:
 //   one row, 4 heads a KV head, after  1023 / 4095 keys
 //     bf16 d = 128   8.3 (11.4) / 11.0 (12.1)
 //     bf16 d = 256  11.1 (16.5) / 14.8 (17.2)    f32  12.5 (23.4) / 15.7 (23.6)
 //   32 slots of bf16 d = 128 in 1024 / 4096 keys   13.5 (16.1) / 18.0 (18.1)
 //   256 slots of the second kernel                 30.8 (35.9) / 44.9 (69.0)
-__device__ __forceinline__ uint32_t piece_count(int list, bool bf16, bool half_filled, uint32_t n_sub, float by) {
-  const float n = (float)n_sub, root = __builtin_amdgcn_sqrtf(n);
+__device__ __forceinline__ float piece_rate(int list, bool bf16, bool half_filled, uint32_t n_sub) {
+  const float root = __builtin_amdgcn_sqrtf((float)n_sub);
   float len;
   if (list == kPagedMany)
     len = 2.0f * root;
   else
     len = n_sub <= 8 ? 8.0f : fmaxf(4.0f, 4.0f * rintf((half_filled ? 0.125f : 0.25f) * (bf16 ? 1.4f : 0.7f) * root));
-  return 1 + (uint32_t)((n - 1.0f) * __builtin_amdgcn_rcpf(by * len));
+  return __builtin_amdgcn_rcpf(len);
 }
+__device__ __forceinline__ uint32_t piece_count(uint32_t n_sub, float rate) { return 1 + (uint32_t)((float)(n_sub - 1) * rate); }
 
 // One workgroup.  A list's tiles are runs of query rows of a request.  When
-// there are workgroups enough for every tile in pieces of the best length, each
+// there are workgroups enough for every tile in pieces of a good length, each
 // piece is a run of its own.  Otherwise the tiles, one after the other, each
 // kItemCost longer than its sub-tiles, are cut into as many runs of equal length
 // as workgroups run at once, and every piece of a tile that lies in one run is
@@ -308,17 +336,36 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
   }
   PagedHeader* const h = (PagedHeader*)a.work;
   int32_t n_parts[kPagedLists];
+  // Requests of more rows than a tile of the first kernel go to the second one,
+  // which reads their keys once for 256 slots, unless the first one's workgroups
+  // have little work with them: it shares a request out to many more.
+  int32_t few_rows = INT32_MAX;
+  if (a.list[kPagedMany].target > 0) {
+    const PagedListBounds& l = a.list[kPagedFew];
+    uint32_t work[1] = {0}, all_work[1];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (rows[i] <= l.rows) continue;
+      const int32_t pos0 = pos_s[tid * PER + i], pos1 = pos0 + rows[i] - 1;
+      const int64_t n_sub = (int64_t)paged_span(kPagedKeys[kPagedFew], pos0, pos0 + l.rows - 1, a.window, a.sinks).total +
+                            paged_span(kPagedKeys[kPagedFew], pos1 - l.rows + 1, pos1, a.window, a.sinks).total;
+      work[0] += (uint32_t)min((int64_t)1 << 18, ((rows[i] + l.rows - 1) / l.rows * n_sub) >> 1);
+    }
+    exclusive_sums<W>(work, all_work, part);
+    if (all_work[0] >= (uint32_t)(kFewWork * l.target)) few_rows = l.rows;
+  }
 #pragma unroll
   for (int list = 0; list < kPagedLists; ++list) {
     const PagedListBounds& l = a.list[list];
     n_parts[list] = 0;
-    if (l.max_new < l.min_new) continue;
-    uint32_t x[1] = {0}, total[1];
+    if (l.target == 0) continue;
+    uint32_t x[2] = {0, 0}, total[2];  // tiles, requests
     int32_t n_tiles[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      n_tiles[i] = rows[i] >= l.min_new && rows[i] <= l.max_new ? (rows[i] + l.rows - 1) / l.rows : 0;
+      n_tiles[i] = (rows[i] <= few_rows) == (list == kPagedFew) ? (rows[i] + l.rows - 1) / l.rows : 0;
       x[0] += n_tiles[i];
+      x[1] += n_tiles[i] > 0;
     }
     exclusive_sums<W>(x, total, part);
     int32_t before = (int32_t)x[0];
@@ -352,13 +399,15 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
       return t;
     };
     // length of all tiles; pieces of them, of twice and of four times the length
-    uint32_t sum[4] = {0, 0, 0, 0}, sums[4];
+    uint32_t sum[4] = {0, 0, 0, 0}, sums[4], longest = 0;
     for (int i = tid; i < all; i += kThreads) {
       const PagedItem t = tile(i);
       const uint32_t n_sub = (uint32_t)t.c_end;
       sum[0] += n_sub + kItemCost;
+      longest = max(longest, n_sub);
+      const float rate = piece_rate(list, a.bf16, 2 * t.n_rows <= l.rows, n_sub);
 #pragma unroll
-      for (int k = 0; k < 3; ++k) sum[1 + k] += piece_count(list, a.bf16, 2 * t.n_rows <= l.rows, n_sub, (float)(1 << k));
+      for (int k = 0; k < 3; ++k) sum[1 + k] += piece_count(n_sub, rate / (float)(1 << k));
     }
     exclusive_sums<W>(sum, sums, part);
     // Two workgroups of few rows of bf16 d = 128 share a CU: short pieces are made
@@ -369,10 +418,25 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
     const uint32_t target = (uint32_t)l.target, alone = two ? target / 2 : target;
     const int by = sums[1] <= alone ? 0 : sums[2] <= alone ? 1 : two && sums[3] <= alone && sums[0] <= 24 * sums[3] ? 2 : 1;
     const uint32_t n_pieces = by == 0 ? sums[1] : by == 1 ? sums[2] : sums[3];
-    const bool pieces = n_pieces <= target;
+    const float shorter = by == 0 ? 1.0f : by == 1 ? 0.5f : 0.25f;
+    bool pieces = n_pieces <= target;
     // length of a run (longer than a tile's cost, so sub-tiles lie in every one)
     const uint32_t len = max((sums[0] + target - 1) / target, (uint32_t)kItemCost + 1);
-    const int32_t P = (int32_t)(pieces ? n_pieces : (sums[0] + len - 1) / len);
+    // Tiles of one request that walk the same keys at once read them from memory
+    // once.  Where requests have several tiles, pieces of one length for all tiles
+    // are taken before cuts, if they are at most half as long again as the runs
+    // (d = 128, 12 requests of 9 to 24 rows in 256 to 2048 keys: 26.4 us, 32.9 in
+    // cuts; d = 256, 4 requests of 40 rows in 4096 keys: 42.6 us, 63.8 in cuts).
+    // f32 is bound by its arithmetic and loses by the longer pieces (6 requests of
+    // 9 to 24 rows in 500 to 8000 keys: 68.5 us, 62.0 in cuts).
+    uint32_t same = 0;
+    if (!pieces && list == kPagedFew && a.bf16 && (uint32_t)all <= target && (uint32_t)all > total[1]) {
+      longest = largest<W>(longest, part);
+      const uint32_t spare = target - (uint32_t)all, n_sub = sums[0] - (uint32_t)(all * kItemCost);
+      same = spare ? min((n_sub + spare - 1) / spare, longest) : longest;
+      pieces = 2 * same <= 3 * len;
+      if (!pieces) same = 0;
+    }
 
     PagedItem* const first = (PagedItem*)(a.work + l.first_off);
     PagedItem* const items = (PagedItem*)(a.work + l.items_off);
@@ -387,18 +451,25 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
       // run r is [r len, (r + 1) len); a tile's cost comes before its sub-tiles
       const uint32_t from = units + u[0], keys = from + kItemCost, to = keys + n_sub;
       const uint32_t r0 = keys / len, r1 = n_sub ? (to - 1) / len : 0;
-      const uint32_t n = !n_sub ? 0 : pieces ? piece_count(list, a.bf16, 2 * t.n_rows <= l.rows, n_sub, (float)(1 << by)) : r1 - r0 + 1;
+      uint32_t n = 0;
+      if (n_sub && !pieces)
+        n = r1 - r0 + 1;
+      else if (n_sub && same)
+        n = (n_sub + same - 1) / same;
+      else if (n_sub)
+        n = piece_count(n_sub, piece_rate(list, a.bf16, 2 * t.n_rows <= l.rows, n_sub) * shorter);
       uint32_t y[3] = {n, n > 1 ? n : 0, n > 1 ? 1u : 0u}, y_all[3];
       exclusive_sums<W>(y, y_all, part);
       t.n_pieces = (int32_t)n;
       t.rec = (int32_t)(base[1] + y[1]);
       t.split = (int32_t)(base[2] + y[2]);
+      const float step = (float)n_sub * __builtin_amdgcn_rcpf((float)n);
       for (uint32_t k = 0; k < n; ++k) {
         const uint32_t at = base[0] + y[0] + k, begin = (r0 + k) * len, end = begin + len;
         t.piece = (int32_t)k;
         if (pieces) {
-          t.c_begin = (int32_t)(k * n_sub / n);
-          t.c_end = (int32_t)((k + 1) * n_sub / n);
+          t.c_begin = k ? t.c_end : 0;
+          t.c_end = (int32_t)(k + 1 < n ? (uint32_t)((float)(k + 1) * step) : n_sub);
           t.next = -1;
         } else {
           t.c_begin = (int32_t)(max(begin, keys) - keys);
@@ -421,7 +492,7 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
     }
     if (tid == 0 && base[0] > (uint32_t)l.items) bad_s = 1;
     for (int i = tid; i < (int)base[2] * a.hkv; i += kThreads) ((int32_t*)(a.work + l.counters_off))[i] = 0;
-    n_parts[list] = P;
+    n_parts[list] = (int32_t)(pieces ? base[0] : (sums[0] + len - 1) / len);
     __syncthreads();
   }
   if (tid == 0) *h = PagedHeader{a.sig, bad_s, {bad_s ? 0 : n_parts[0], bad_s ? 0 : n_parts[1]}};
@@ -497,7 +568,8 @@ extern "C" int32_t cev_paged_plan(const cev_paged_desc* d, const int32_t* cu, co
   a.bf16 = d->dtype == CEV_BF16;
   a.two_a_cu = a.bf16 && d->head_dim == 128;
   // one wave where a lane has a few tiles at most
-  const int64_t tiles = (int64_t)b.list[kPagedFew].items - b.list[kPagedFew].target + b.list[kPagedMany].items - b.list[kPagedMany].target;
+  const PagedListBounds& most = b.list[b.list[kPagedMany].target ? kPagedMany : kPagedFew];
+  const int64_t tiles = (int64_t)most.items - most.target;
   return by_requests(d->n_requests, tiles <= 256, [&](auto w_c, auto per_c) {
     constexpr int W = decltype(w_c)::value, PER = decltype(per_c)::value;
     hipLaunchKernelGGL((paged_plan_kernel<W, PER>), dim3(1), dim3(64 * W), 0, (hipStream_t)stream, a);

@@ -706,6 +706,93 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(gpu, kind, hq, hkv, d, v
             assert bool(rows.isnan().all())
 
 
+class _Many(_Paged):
+    """The same, with one more request behind them of so many rows that the plan
+    sends all requests of more than 32 query slots to the kernel of many rows.
+    Its own rows are only looked at for being finite."""
+
+    def __init__(self, dev, past, new, hq, hkv, d, kind, page, window=0, **kw):
+        rows, target = 32 * hkv // hq, max(1, 512 // hkv)
+        each = max(1, (window + rows - 1) // 32) if window else 64  # sub-tiles that a tile sees at least
+        super().__init__(dev, [*past, window or 2048], [*new, rows * (32 * target // each + 2)], hq, hkv, d, kind, page, **kw)
+
+    def run(self, out=None, stream=None, **kw):
+        import torch
+        att = self.attention(**kw)
+        out = torch.full_like(self.q, 5.0) if out is None else out
+        att.plan(self.cu, self.lengths, stream=stream)
+        assert int(att.work[12:16].view(torch.int32)) > 0  # workgroups of the second list
+        return att(self.q, self.k, self.v, self.table, out=out, stream=stream)
+
+    def check(self, out, what="", **kw):
+        out, all_new = out.clone(), self.new
+        rows = slice(sum(all_new[:-1]), sum(all_new))
+        assert bool(out[rows].isfinite().all())
+        out[rows] = 5.0
+        self.new = all_new[:-1]
+        super().check(out, what, **kw)
+        self.new = all_new
+
+
+MANY_SHAPES = [("bf16", 8, 2, 128), ("bf16", 4, 4, 128), ("bf16", 16, 2, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,hq,hkv,d", MANY_SHAPES)
+@pytest.mark.parametrize("past,new,page,window,sinks", [
+    ([0, 7, 100], [37, 0, 50], 16, 0, 0), ([0, 0, 31, 64], [33, 64, 65, 257], 16, 0, 0), ([129, 1000, 0], [70, 1, 130], 64, 0, 0),
+    ([20011], [40], 1024, 0, 0), ([0, 130, 700, 33], [50, 40, 300, 2], 16, 1, 0), ([0, 130, 700], [50, 40, 70], 16, 7, 3),
+    ([0, 130, 700], [50, 40, 70], 32, 33, 4), ([10, 1000], [500, 40], 16, 64, 200), ([0, 3000], [100, 100], 16, 1000, 70)])
+def test_attention_of_many_rows(gpu, kind, hq, hkv, d, past, new, page, window, sinks):
+    import torch
+    kw = dict(window=window, sinks=sinks) if window else {}
+    p = _Many(gpu, past, new, hq, hkv, d, kind, page, seed=len(past) + page, pad=2, window=window)
+    out = p.run(**kw)
+    p.check(out, **kw)
+    assert torch.equal(p.run(**kw), out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,hq,hkv,d", MANY_SHAPES)
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_values_that_one_of_many_rows_does_not_see(gpu, kind, hq, hkv, d, value, which):
+    import torch
+    past, new, at = [70], [90], 70 + 41
+    for kw in ({}, dict(window=20, sinks=2)):
+        p = _Many(gpu, past, new, hq, hkv, d, kind, 16, seed=11, window=kw.get("window", 0))
+        clean = p.run(**kw)[:90]
+        cache = getattr(p, which)
+        page, off = int(p.table[0, at // 16]), at % 16
+        if which == "v":
+            cache[page, off, 0, 5] = value
+        else:
+            cache[page, off, 0] = value
+        out = p.run(**kw)[:90]
+        g = hq // hkv
+        sees = torch.zeros(90, dtype=torch.bool, device=gpu)
+        sees[41: 41 + kw.get("window", 90)] = True
+        assert torch.equal(out[~sees], clean[~sees]) and torch.equal(out[:, g:], clean[:, g:])
+        rows = out[sees][:, :g]
+        if which == "v":
+            col = rows[..., 5].float()
+            assert bool((col.isnan() if math.isnan(value) else col == value).all())
+            assert torch.equal(rows[..., torch.arange(d) != 5], clean[sees][:, :g][..., torch.arange(d) != 5])
+        elif math.isnan(value):
+            assert bool(rows.isnan().all())
+
+
+@pytest.mark.gpu
+def test_bad_pages_of_many_rows(gpu):
+    """A page outside the cache that only the later rows of a request see, and one in a request of its own."""
+    p = _Many(gpu, [20, 100], [60, 70], 8, 2, 128, "bf16", 16)
+    want = p.run()
+    p.table[0, 4], p.table[1, 0] = p.n_pages, -1
+    out = p.run()
+    assert bool(out[60:130].isnan().all()) and bool(out[44:60].isnan().all())
+    assert bool((out[130:] == want[130:]).all())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_attention_of_large_scores(gpu, kind):
