@@ -39,14 +39,14 @@ __device__ __forceinline__ bool paged_plan_ok(const PagedArgs& a, int list, int&
 // workgroups and 1019 with 4096.
 constexpr int kPastL2 = 16;
 
-__device__ __forceinline__ void put_past_l2(__amdgpu_buffer_rsrc_t rs, int at, const f32x4& v) {
-  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(decltype(__builtin_amdgcn_raw_buffer_load_b128(rs, 0, 0, 0)), v), rs, at, 0, kPastL2);
+__device__ __forceinline__ void put_past_l2(__amdgpu_buffer_rsrc_t rs, int at, const f32x4& v, int scalar_at = 0) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(decltype(__builtin_amdgcn_raw_buffer_load_b128(rs, 0, 0, 0)), v), rs, at, scalar_at, kPastL2);
 }
 __device__ __forceinline__ void put_past_l2(__amdgpu_buffer_rsrc_t rs, int at, const float2& v) {
   __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(decltype(__builtin_amdgcn_raw_buffer_load_b64(rs, 0, 0, 0)), v), rs, at, 0, kPastL2);
 }
-__device__ __forceinline__ f32x4 get4_past_l2(__amdgpu_buffer_rsrc_t rs, int at) {
-  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, kPastL2));
+__device__ __forceinline__ f32x4 get4_past_l2(__amdgpu_buffer_rsrc_t rs, int at, int scalar_at = 0) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at, scalar_at, kPastL2));
 }
 __device__ __forceinline__ float2 get2_past_l2(__amdgpu_buffer_rsrc_t rs, int at) {
   return __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, kPastL2));

@@ -97,30 +97,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     vat[r] = (4 * r + (lane >> 4)) * vr + (v_slot(blk, row) << 4);
   }
 
-  for (bool more = true; more;) {
-    const PagedItem it = walk.item();
-    more = it.next >= 0;
-    const int pos1 = it.pos0 + it.n_rows - 1;
-    const PagedSpan span = paged_span(kKeys, it.pos0, pos1, a.window, a.sinks);
-    // Query slot (wave, n) holds row slot / g of the tile and query head slot % g:
-    // the rows of a short tile fill the first waves.
-    const int rit = (wave * 32 + n) >> gs;
-    const bool row_ok = rit < it.n_rows;
-    const int pos = row_ok ? it.pos0 + rit : -1;
-    const int w_row0 = (wave * 32) >> gs, w_row1 = min((wave * 32 + 31) >> gs, it.n_rows - 1);
-    const bool wave_active = w_row0 < it.n_rows;
-    const int w_pos0 = it.pos0 + w_row0, w_pos1 = it.pos0 + w_row1;  // this wave's rows
-
-    F fr;
-    {
-      const int row = it.row0 + (row_ok ? rit : 0), head = kvh * a.g + (n & (a.g - 1));
-      fr.load_q((const __bf16*)a.q + (int64_t)row * a.q_st + (int64_t)head * a.q_sh, row_ok, u);
-    }
-    if (tid == 0) odd_s = bad_s = 0;
-
-    const int c0 = it.c_begin, nc = it.c_end - it.c_begin;  // chunks [c0, c0 + nc) of the tile's stream
-    auto first_key = [&](int i) {
-      const int c = c0 + i;
+  // The current item's state, of this wave where it says so.
+  PagedItem it;
+  PagedSpan span;
+  int pos, w_pos0, w_pos1, w_lo, w_hi, t_lo, t_hi, nc;  // last position that the lane's row sees; unmasked() below
+  bool row_ok, wave_active;
+  const int32_t* bt;
+  F fr;
+  // chunks [it.c_begin, it.c_begin + nc) of the tile's stream
+  auto first_key = [&](int i) {
+      const int c = it.c_begin + i;
       return kKeys * (c < span.sinks ? c : c - span.sinks + span.first);
     };
     // Chunks of the part before lo and from hi on hold keys that not all rows
@@ -128,15 +114,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     auto unmasked = [&](int p0, int p1, int& lo, int& hi) {
       // the chunks of the window start at stream place span.sinks; the last key
       // of the one at place c is first_key + 63
-      hi = span.sinks + (p0 + 1) / kKeys - span.first - c0;
+      hi = span.sinks + (p0 + 1) / kKeys - span.first - it.c_begin;
       lo = 0;
-      if (a.window > 0 && p1 >= a.window) lo = span.sinks + (p1 - a.window) / kKeys + 1 - span.first - c0;
+      if (a.window > 0 && p1 >= a.window) lo = span.sinks + (p1 - a.window) / kKeys + 1 - span.first - it.c_begin;
     };
-    int w_lo, w_hi, t_lo, t_hi;  // of this wave's rows, and of all of the tile's
-    unmasked(w_pos0, w_pos1, w_lo, w_hi);
-    unmasked(it.pos0, pos1, t_lo, t_hi);
-
-    const int32_t* const bt = a.bt + it.req * a.bt_stride;
     // Lane l keeps the addresses of this wave's rows of K and of V of chunk 64 b +
     // l of the current batch b, and whether they are fetched at all.
     int batch_first = 0, k_lo = 0, k_hi = 0, v_lo = 0, v_hi = 0, fetched = 0;
@@ -157,8 +138,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       k_lo = (int)(uint32_t)kp, k_hi = (int)(uint32_t)(kp >> 32);
       v_lo = (int)(uint32_t)vp, v_hi = (int)(uint32_t)(vp >> 32);
     };
-    load_pages(0);
-
     // Chunk i into its buffer, i mod kBuf; past the end: zeros.
     auto fetch = [&](int i) {
       const bool real = i < nc;
@@ -195,18 +174,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     // become zeros; after the loop they are added to the rows that see them.
     auto clean = [&](int i) {
       if (i >= nc || (i >= t_lo && i < t_hi)) return;
-      i32x4* const v = (i32x4*)(lds + kVBase + i % kBuf * kTileBytes + 8 * wave * kRowBytes);
+      const int at = kVBase + i % kBuf * kTileBytes + 8 * wave * kRowBytes + lane * 16;
+      i32x4* const v = (i32x4*)(lds + at);
+      KFrag vr[2] = {read_b128<0>(lds_base + at), read_b128<1024>(lds_base + at)};
+      wait_b128<1>(vr[0]);
+      wait_b128<0>(vr[1]);
       bool odd = false;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        i32x4 x = v[64 * r + lane];
+        i32x4 x = __builtin_bit_cast(i32x4, vr[r]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const bool hi = (x[e] & 0x7f800000) == 0x7f800000, lo = (x[e] & 0x7f80) == 0x7f80;
           odd |= hi | lo;
           x[e] &= (hi ? 0 : (int)0xffff0000) | (lo ? 0 : 0xffff);
         }
-        if (odd) v[64 * r + lane] = x;
+        if (odd) v[64 * r] = x;
       }
       if (__ballot(odd) && lane == 0) *(volatile int32_t*)&odd_s = 1;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -223,6 +206,42 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       }
     };
 
+  // Takes the run's next item and asks for its Q, its pages and its first chunks.
+  auto begin = [&] {
+    it = walk.item();
+    const int pos1 = it.pos0 + it.n_rows - 1;
+    span = paged_span(kKeys, it.pos0, pos1, a.window, a.sinks);
+    nc = it.c_end - it.c_begin;
+    // Query slot (wave, n) holds row slot / g of the tile and query head slot % g:
+    // the rows of a short tile fill the first waves.
+    const int rit = (wave * 32 + n) >> gs;
+    row_ok = rit < it.n_rows;
+    pos = row_ok ? it.pos0 + rit : -1;
+    const int w_row0 = (wave * 32) >> gs, w_row1 = min((wave * 32 + 31) >> gs, it.n_rows - 1);
+    wave_active = w_row0 < it.n_rows;
+    w_pos0 = it.pos0 + w_row0, w_pos1 = it.pos0 + w_row1;
+    unmasked(w_pos0, w_pos1, w_lo, w_hi);    // of this wave's rows
+    unmasked(it.pos0, pos1, t_lo, t_hi);     // of all of the tile's
+    bt = a.bt + it.req * a.bt_stride;
+    bad_page = false;
+    load_pages(0);
+    const int row = it.row0 + (row_ok ? rit : 0), head = kvh * a.g + (n & (a.g - 1));
+    fr.load_q((const __bf16*)a.q + (int64_t)row * a.q_st + (int64_t)head * a.q_sh, row_ok, u);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) fetch(k);
+    __builtin_amdgcn_sched_barrier(0);
+    // Q is waited for here, where only the chunks are behind it.
+#pragma unroll
+    for (int st = 0; st < F::NQK; ++st) {
+      i32x4 x = __builtin_bit_cast(i32x4, fr.q[st]);
+      asm volatile("" : "+v"(x));
+      fr.q[st] = __builtin_bit_cast(bf16x8, x);
+    }
+  };
+  if (tid == 0) odd_s = bad_s = 0;
+  begin();
+  for (;;) {
     f32x16 o[NDT];
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) o[dt] = f32x16{};
@@ -232,8 +251,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     bool m_set = false;
     const float c = a.scale_log2;
 
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) fetch(k);
     wait_vmcnt<kLoadsPerChunk * (kAhead - 2)>();  // chunks 0 and 1 landed
     lds_barrier();                                // (the flags are clear)
     clean(0);
@@ -248,9 +265,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     if (wave_active) {
       // Sub-tile 0: its row maximum (over both lane halves) is the first m_run.
       sa = f32x16{};
-#pragma unroll
-      for (int st = 0; st < F::NQK; ++st)
-        fr.qk_mfma(*(const bf16x8*)(lds + (koff[st] - lds_base)), st, sa);
+      KFrag k0[F::NQK];
+      static_for<F::NQK>([&](auto st_c) { k0[decltype(st_c)::value] = k_issue(I0{}, st_c); });
+      static_for<F::NQK>([&](auto st_c) {
+        constexpr int st = decltype(st_c)::value;
+        wait_b128<F::NQK - 1 - st>(k0[st]);
+        fr.qk_mfma(__builtin_bit_cast(bf16x8, k0[st]), st, sa);
+      });
       if (0 >= w_hi || 0 < w_lo) mask_sub(sa, first_key(0));
       float mx = -INFINITY;
 #pragma unroll
@@ -402,6 +423,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     }
     float l = pair_sum(l_run) + (*(volatile int32_t*)&bad_s ? __builtin_nanf("") : 0.0f);
 
+    bool write = row_ok;
     const bool split = it.n_pieces > 1;
     // Partial results: [wave][16 vectors of 4 columns][lane], then (m, l) of
     // each slot.
@@ -417,8 +439,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       if (wave_active) {
 #pragma unroll
         for (int v = 0; v < 16; ++v)
-          put_past_l2(rs, vec0 + 1024 * v,
-                      f32x4{o[v / 4][4 * (v % 4)], o[v / 4][4 * (v % 4) + 1], o[v / 4][4 * (v % 4) + 2], o[v / 4][4 * (v % 4) + 3]});
+          put_past_l2(rs, vec0, f32x4{o[v / 4][4 * (v % 4)], o[v / 4][4 * (v % 4) + 1], o[v / 4][4 * (v % 4) + 2], o[v / 4][4 * (v % 4) + 3]}, 1024 * v);
         if (u == 0) put_past_l2(rs, ml0, make_float2(m_set ? m_run : -1e30f, l));
       }
       // The stores have reached memory before the workgroup counts itself.
@@ -432,10 +453,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       __syncthreads();
       const bool last = last_s;
       __syncthreads();
-      if (!last) continue;
-      // Half of the columns at a time; the next piece is on its way while one is
+      write = write && last;
+      // The last one: half of the columns at a time; the next piece is on its way while one is
       // added (a trip past the L2 takes longer than the adding).
-      if (wave_active) {
+      if (last && wave_active) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           f32x4 x[2][8];
@@ -444,7 +465,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
             const __amdgpu_buffer_rsrc_t rq = record(min(q, it.n_pieces - 1));
             to_w = get2_past_l2(rq, ml0);
 #pragma unroll
-            for (int v = 0; v < 8; ++v) to[v] = get4_past_l2(rq, vec0 + 1024 * (8 * half + v));
+            for (int v = 0; v < 8; ++v) to[v] = get4_past_l2(rq, vec0, 1024 * (8 * half + v));
           };
           float M = -1e30f;
           l = 0.0f;
@@ -473,18 +494,33 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
       }
     }
-    if (row_ok) {
-      __bf16* const op = (__bf16*)a.out + (int64_t)(it.row0 + rit) * a.o_st + (int64_t)(kvh * a.g + (n & (a.g - 1))) * a.o_sh;
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    // The row's 16-byte vectors: a half wave holds four columns of each eight, and
+    // the halves exchange theirs of two vectors.
+    i32x4 res[8];
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        float x[4];
+    for (int w = 0; w < 8; ++w) {
+      int x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = l == 0.0f ? 0.0f : o[v / 4][4 * (v % 4) + e] * inv;
-        store_vec4<__bf16>(op + (v / 4) * 32 + 8 * (v % 4) + 4 * u, x);
+      for (int e = 0; e < 4; ++e) {
+        const float x0 = o[w / 2][8 * (w % 2) + 2 * e], x1 = o[w / 2][8 * (w % 2) + 2 * e + 1];
+        const bf16x2 y = {(__bf16)(l == 0.0f ? 0.0f : x0 * inv), (__bf16)(l == 0.0f ? 0.0f : x1 * inv)};
+        x[e] = __builtin_bit_cast(int, y);
       }
+      const auto r0 = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false), r1 = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+      res[w] = i32x4{(int)r0[0], (int)r1[0], (int)r0[1], (int)r1[1]};
     }
-    __syncthreads();  // the ring and the flags are the next item's
+    __bf16* const op = (__bf16*)a.out + (int64_t)(it.row0 + ((wave * 32 + n) >> gs)) * a.o_st + (int64_t)(kvh * a.g + (n & (a.g - 1))) * a.o_sh + 8 * u;
+    // The next item's first chunks come while this one's rows are written.
+    lds_barrier();  // every wave has read the flags
+    if (tid == 0) odd_s = bad_s = 0;
+    const bool more = it.next >= 0;
+    if (more) begin();
+    if (write) {
+#pragma unroll
+      for (int w = 0; w < 8; ++w) *(i32x4*)(op + 32 * (w / 2) + 16 * (w % 2)) = res[w];
+    }
+    if (!more) break;
   }
 }
 
