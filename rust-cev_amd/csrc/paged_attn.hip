@@ -229,16 +229,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       const uint64_t base = (which ? vbase : kbase) + (uint64_t)(page * page_bytes) + (uint64_t)((first & ((1 << a.page_shift) - 1)) * (int64_t)stride);
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)uniform_u64(base), (short)0, uniform_i32(seen && in ? 16 * stride : 0), kBufferWord3);
       char* const to = ring + which * kTile + half * (kTile / 2);
+      // (the two cases apart, or every load is a branch of its own)
+      auto loads = [&](auto full_c) {
 #pragma unroll
-      for (int i = 0; i < kLoads / 2; ++i) {
-        const int r = kRows * i + ld_row;
-        int off = r * stride + ((which ? v_place<T>(ld_blk, r) : k_place(ld_blk, r)) << 4);
-        if (!full) {
-          const int key = first + kRows * i + ld_row;
-          off = key < span.end && !(key >= span.skip_lo && key < span.skip_hi) ? off : INT32_MAX;
+        for (int i = 0; i < kLoads / 2; ++i) {
+          const int r = kRows * i + ld_row;
+          int off = r * stride + ((which ? v_place<T>(ld_blk, r) : k_place(ld_blk, r)) << 4);
+          if (!decltype(full_c)::value) {
+            const int key = first + r;
+            off = ((key < span.end) & !((key >= span.skip_lo) & (key < span.skip_hi))) ? off : INT32_MAX;
+          }
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(to + 1024 * i), 16, off, 0, 0, 0);
         }
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(to + 1024 * i), 16, off, 0, 0, 0);
-      }
+      };
+      if (full)
+        loads(std::true_type{});
+      else
+        loads(std::false_type{});
     }
   };
   using K_c = std::integral_constant<int, 0>;
