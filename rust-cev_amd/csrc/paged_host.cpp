@@ -82,8 +82,9 @@ int32_t cev_paged_bounds(const cev_paged_desc* d, PagedBounds* b) {
                            {d->o_stride_t, d->t},        {d->o_stride_h, hq}};
   for (const auto& s : st) {
     CEV_CHECK_ARG(cev_stride_fits(s[0], s[1]), "paged attention: stride %lld of %lld rows", (long long)s[0], (long long)s[1]);
-    if (s[0] % al) return cev_fail(CEV_ERR_UNSUPPORTED, "paged attention: strides must be multiples of %lld elements", (long long)al);
+    if (s[1] > 1 && s[0] % al) return cev_fail(CEV_ERR_UNSUPPORTED, "paged attention: strides must be multiples of %lld elements", (long long)al);
   }
+  CEV_CHECK_ARG((hq == 1 || d->o_stride_h >= d->head_dim) && (d->t == 1 || d->o_stride_t >= d->head_dim), "paged attention: rows of out overlap");
   // a buffer resource spans 16 rows of a page
   const int64_t row_max = (INT32_MAX / 2) / 16 / esz;
   const int64_t rows[] = {d->kc_stride_t, d->vc_stride_t};

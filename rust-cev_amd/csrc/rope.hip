@@ -163,19 +163,23 @@ extern "C" int32_t cev_rope(const cev_rope_desc* d, const void* q_in, const void
     return cev_fail(CEV_ERR_UNSUPPORTED, "cev_rope: rotary_dim %d (a multiple of 16 up to head_dim %d)", d->rotary_dim, d->head_dim);
   CEV_CHECK_ARG(d->factor == d->factor && d->factor >= -3.0e38f && d->factor <= 3.0e38f, "cev_rope: factor must be finite");
   const int64_t t = d->t, hq = d->n_q_heads, hkv = d->n_kv_heads, al = d->dtype == CEV_BF16 ? 8 : 4;
-  // rows of a k or v output: the tokens', or a page's (the pages number at most n_slots)
-  const int64_t rows = slots ? d->page_size : t, pages = slots ? d->n_slots : 1;
+  // rows of a k or v output: the tokens', or a page's
+  const int64_t rows = slots ? d->page_size : t, pages = slots && d->page_size > 0 ? ((int64_t)d->n_slots + d->page_size - 1) / d->page_size : 1;
   const int64_t st[][2] = {{d->qi_stride_t, t},    {d->qi_stride_h, hq},  {d->ki_stride_t, t},     {d->ki_stride_h, hkv}, {d->vi_stride_t, t},
                            {d->vi_stride_h, hkv},  {d->qo_stride_t, t},   {d->qo_stride_h, hq},    {d->ko_stride_p, pages}, {d->ko_stride_t, rows},
                            {d->ko_stride_h, hkv},  {d->vo_stride_p, pages}, {d->vo_stride_t, rows}, {d->vo_stride_h, hkv}};
   for (const auto& s : st) {
     CEV_CHECK_ARG(cev_stride_fits(s[0], s[1]), "cev_rope: stride %lld of %lld rows", (long long)s[0], (long long)s[1]);
-    if (s[0] % al) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_rope: strides must be multiples of %lld elements", (long long)al);
+    if (s[1] > 1 && s[0] % al) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_rope: strides must be multiples of %lld elements", (long long)al);
   }
   if (slots) {
     CEV_CHECK_ARG(d->n_slots >= 0, "cev_rope: %d slots", d->n_slots);
     CEV_CHECK_ARG(d->page_size >= 1 && (d->page_size & (d->page_size - 1)) == 0, "cev_rope: page_size %d is not a power of two", d->page_size);
   }
+  const int64_t outs[][2] = {{d->qo_stride_t, t}, {d->qo_stride_h, hq}, {d->ko_stride_p, pages}, {d->ko_stride_t, rows}, {d->ko_stride_h, hkv},
+                             {v_out ? d->vo_stride_p : INT64_MAX, pages}, {v_out ? d->vo_stride_t : INT64_MAX, rows}, {v_out ? d->vo_stride_h : INT64_MAX, hkv}};
+  for (const auto& s : outs)
+    CEV_CHECK_ARG(s[1] <= 1 || s[0] >= d->head_dim, "cev_rope: rows of an output overlap");
   if (d->t == 0 || d->n_q_heads + d->n_kv_heads == 0) return CEV_OK;
   CEV_CHECK_ARG(pos && steps, "cev_rope: null pos or steps");
   CEV_CHECK_ARG(d->n_q_heads == 0 || (q_in && q_out), "cev_rope: null q buffers");

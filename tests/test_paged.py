@@ -59,6 +59,18 @@ def test_paged_descriptors_out_of_bounds_are_refused(cev, kw, code):
     assert _abi.lib().cev_last_error()
 
 
+@pytest.mark.parametrize("kw", [dict(o_stride_t=0), dict(o_stride_h=64), dict(o_stride_h=0)])
+def test_overlapping_rows_of_out_are_refused(cev, kw):
+    assert _work_size(_paged_desc(**kw))[0] == -1
+
+
+def test_strides_of_single_rows_do_not_count(cev):
+    """A tensor's stride over a dimension of size one may be anything."""
+    assert _work_size(_paged_desc(t=1, q_stride_t=3, o_stride_t=1))[0] == 0
+    assert _work_size(_paged_desc(hq=1, hkv=1, q_stride_h=1, o_stride_h=0, kc_stride_h=5, vc_stride_h=1))[0] == 0
+    assert _work_size(_paged_desc(n_pages=1, kc_stride_p=1, vc_stride_p=7))[0] == 0
+
+
 def test_paged_calls_check_their_buffers(cev):
     L, d = _abi.lib(), _paged_desc()
     n = _work_size(d)[1]
@@ -111,6 +123,13 @@ def test_rope_calls_are_checked(cev):
         assert run(_rope_desc(), bad) == -1, i
     assert L.cev_rope(None, *ok, None) == -1
     assert run(_rope_desc(t=0), [None] * 9) == 0 and run(_rope_desc(n_q_heads=0, n_kv_heads=0), [None] * 9) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(qo_stride_t=0), dict(qo_stride_h=64), dict(ko_stride_h=64), dict(vo_stride_t=0), dict(vo_stride_p=0),
+                                dict(ko_stride_p=64)])
+def test_overlapping_rows_of_rope_are_refused(cev, kw):
+    ok = [C.c_void_p(4096)] * 9
+    assert _abi.lib().cev_rope(C.byref(_rope_desc(**kw)), *ok, None) == -1
 
 
 @pytest.mark.parametrize("scaling,args", [("none", {}), ("linear", dict(factor=8.0)), ("yarn", dict(factor=4.0, original=32768)),
@@ -704,6 +723,96 @@ def test_values_that_a_row_does_not_see_do_not_reach_it(gpu, kind, hq, hkv, d, v
             assert same(out, clean, sees, slice(0, g), torch.arange(d) != 5)
         elif math.isnan(value):
             assert bool(rows.isnan().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,d", [("bf16", 128), ("bf16", 256), ("f32", 128)])
+@pytest.mark.parametrize("requests,past_hi,new_hi", [(513, 90, 2), (700, 40, 1), (4096, 20, 2)])
+def test_attention_of_many_requests(gpu, kind, d, requests, past_hi, new_hi):
+    rng = random.Random(requests)
+    past = [rng.randint(0, past_hi) for _ in range(requests)]
+    p = _Paged(gpu, past, [rng.randint(0, new_hi) for _ in range(requests)], 2, 1, d, kind, 16, seed=requests, pad=1)
+    p.check(p.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,hq,hkv,d", [("bf16", 6, 3, 128), ("bf16", 40, 5, 128), ("bf16", 300, 300, 128), ("bf16", 14, 7, 256), ("f32", 3, 3, 128),
+                                           ("bf16", 1, 1, 128)])
+def test_attention_of_odd_head_counts(gpu, kind, hq, hkv, d):
+    """KV heads that do not divide the workgroups, and more heads than those."""
+    p = _Paged(gpu, [0, 200, 33], [40, 1, 9], hq, hkv, d, kind, 16, seed=hkv, pad=2)
+    for kw in ({}, dict(window=2 ** 31 - 1), dict(window=30, sinks=2 ** 31 - 1)):
+        p.check(p.run(**kw), kw, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,many", [("bf16", False), ("bf16", True), ("f32", False)])
+def test_attention_in_place_of_q(gpu, kind, many):
+    import torch
+    p = (_Many if many else _Paged)(gpu, [0, 3000, 33], [40, 70, 1], 8, 2, 128, kind, 16, seed=2)
+    want = p.run()
+    assert torch.equal(p.run(out=p.q), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,hq,hkv,d", [("bf16", 8, 2, 128), ("bf16", 4, 2, 256), ("f32", 4, 2, 128)])
+def test_requests_that_share_pages(gpu, kind, hq, hkv, d):
+    """A common beginning lies in the same pages, and one page is twice in a request's table."""
+    p = _Paged(gpu, [100, 130, 64], [3, 1, 20], hq, hkv, d, kind, 16, seed=4)
+    p.table[1, :6] = p.table[0, :6]
+    p.table[2, 3] = p.table[2, 1]
+    p.check(p.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_two_graphs_of_one_object(gpu, kind):
+    """A graph of a decoding step and one of a chunk's, of the same work buffer,
+    replayed in turn, with eager calls and other lengths between."""
+    import torch
+    p = _Paged(gpu, [700, 40, 2000], [1, 33, 5], 8, 2, 128, kind, 16, seed=13, pad=3)
+    att, out = p.attention(), torch.empty_like(p.q)
+    att.plan(p.cu, p.lengths)(p.q, p.k, p.v, p.table, out=out)
+    torch.cuda.synchronize()
+    steps = ([700, 40, 2000], [1, 33, 5]), ([701, 0, 1998], [1, 1, 7])
+    graphs = []
+    sets = [tuple(torch.tensor(x, dtype=torch.int32, device=gpu) for x in (np.concatenate([[0], np.cumsum(new)]), np.add(past, new))) for past, new in steps]
+    for cu, lengths in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            att.plan(cu, lengths)
+            att(p.q, p.k, p.v, p.table, out=out)
+    for i in (0, 1, 1, 0, 2, 1, 0):
+        out.fill_(5.0)
+        if i == 2:
+            att.plan(*sets[0])(p.q, p.k, p.v, p.table, out=out)
+            i = 0
+        else:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        p.past, p.new = steps[i]
+        p.check(out, i)
+
+
+@pytest.mark.gpu
+def test_tables_and_rope_on_another_stream(gpu):
+    import torch
+    s = torch.cuda.Stream()
+    a, b = (_Tables(gpu, [5, 40, 0, 17], 16, 8, 9, seed=3, max_tokens=20) for _ in range(2))
+    new = [3, -1, 8, 1]
+    torch.cuda.synchronize()
+    want = a.expect(new)
+    a.step(new)
+    b.step(new, stream=s)
+    a.check(want)
+    b.check(want)
+    rot = cev_hip.RotaryAngles(1e6, 128, gpu)
+    q, k = torch.randn(20, 4, 128, device=gpu), torch.randn(20, 2, 128, device=gpu)
+    here = cev_hip.rope(q, k, a.pos, rot)
+    torch.cuda.synchronize()
+    there = cev_hip.rope(q, k, a.pos, rot, stream=s)
+    s.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(here, there))
 
 
 class _Many(_Paged):
