@@ -359,13 +359,14 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
     const PagedListBounds& l = a.list[list];
     n_parts[list] = 0;
     if (l.target == 0) continue;
-    uint32_t x[2] = {0, 0}, total[2];  // tiles, requests
+    uint32_t x[3] = {0, 0, 0}, total[3];  // tiles, requests, rows
     int32_t n_tiles[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       n_tiles[i] = (rows[i] <= few_rows) == (list == kPagedFew) ? (rows[i] + l.rows - 1) / l.rows : 0;
       x[0] += n_tiles[i];
       x[1] += n_tiles[i] > 0;
+      x[2] += n_tiles[i] > 0 ? rows[i] : 0;
     }
     exclusive_sums<W>(x, total, part);
     int32_t before = (int32_t)x[0];
@@ -420,8 +421,13 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
     const uint32_t n_pieces = by == 0 ? sums[1] : by == 1 ? sums[2] : sums[3];
     const float shorter = by == 0 ? 1.0f : by == 1 ? 0.5f : 0.25f;
     bool pieces = n_pieces <= target;
-    // length of a run (longer than a tile's cost, so sub-tiles lie in every one)
-    const uint32_t len = max((sums[0] + target - 1) / target, (uint32_t)kItemCost + 1);
+    // Length of a run in cuts (longer than a tile's cost, so sub-tiles lie in every
+    // one).  Tiles of few rows stream their keys as fast with one run a CU and have
+    // fewer joins (64 decoding requests of 64 to 8192 keys 186 us, 196 with two a
+    // CU), fuller ones do not (64 requests of 8 rows of 4 heads in 512 keys 30.1 us,
+    // 27.4 with two).
+    const uint32_t runs = 2 * total[2] <= (uint32_t)(all * l.rows) ? alone : target;
+    const uint32_t len = max((sums[0] + runs - 1) / runs, (uint32_t)kItemCost + 1);
     // Tiles of one request that walk the same keys at once read them from memory
     // once.  Where requests have several tiles, pieces of one length for all tiles
     // are taken before cuts, if they are at most half as long again as the runs
