@@ -134,8 +134,9 @@ class PagedAttention:
     max_new: no request has more new tokens in a step (default t).  window: a
     row sees that many last keys, itself among them, and the first `sinks`
     ones; 0: all.  plan() makes the step's work list from cu and lengths on the
-    device; every call until the next plan() uses it.  The object's workspace
-    serves one step at a time."""
+    device; every call until the next plan() uses it.  out may be q.  The object
+    is made on the current stream, which other streams wait for as for a
+    tensor; its workspace serves one step at a time."""
 
     def __init__(self, q, k_cache, block_table, max_new: Optional[int] = None, window: int = 0, sinks: int = 0, scale: Optional[float] = None):
         import torch

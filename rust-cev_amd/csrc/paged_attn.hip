@@ -11,10 +11,31 @@
 // operand.
 //
 // K and V go from HBM straight into this wave's own LDS (buffer_load ... lds,
-// 1 KB an instruction), one or two sub-tiles ahead.  A page's base is a scalar
+// 1 KB an instruction), one sub-tile ahead: K of the next one is asked for when
+// its scores are made, V when its products are.  A page's base is a scalar
 // 64-bit address (page ids are wave-uniform), so the cache may have any size;
 // keys past the end, in pages behind the window or not visible to any row of
 // the item get an offset out of the resource's range and read as zero.
+//
+// Rounding: scores, sums, the running maximum and O are f32; bf16 probabilities
+// are rounded to bf16 for the product (at most 2^-8 of each weight, no more than
+// the output's own rounding is off by), and their sum is that of the rounded
+// ones, so that a row's weights add up to one.
+//
+// What bounds it, alone on the card, us:
+//   bf16 d = 128  64 requests of one token, 64 to 8192 keys, 8 KV heads: 186, for
+//                 1077 MB 5.8 TB/s: HBM
+//   bf16 d = 128  one token after 300 keys: 8.8, a chain of trips: the list's item,
+//                 page ids, K, scores, V, the pieces' join; a launch is 3.5
+//   bf16 d = 256  28 requests of 1 to 8 rows and 4 of 64, 100 to 4096 keys: 91.  K and
+//                 V of 276 MB come from HBM once (3.0 TB/s), and tiles of one request
+//                 again from the L2 (585 MB into LDS); a round of the four waves'
+//                 sub-tiles takes 7000 cycles, of which 4000 are spent handing
+//                 32 loads of 1 KB a wave to a CU that holds one workgroup (its LDS)
+//   f32           12 chunks of 17 to 41 rows, 256 to 2048 keys: 58, of which a
+//                 quarter are the items' starts and joins; a round of 9100 cycles has 3000
+//                 of MFMAs, the rest makes bf16 parts of K and V beside them and
+//                 hands over the loads
 //
 // Pieces of a tile whose keys lie in several workgroups' runs write partial
 // results (f32); the last of them to arrive (a counter per tile and KV head)

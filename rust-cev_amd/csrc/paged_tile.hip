@@ -17,6 +17,13 @@
 //     tokens that stay visible;
 //   - infinities and NaN of V that only some of a chunk's rows see.
 // Pieces of a split tile are joined as in paged_attn.hip.
+//
+// Bound by the matrix cores and the softmax beside them: a chunk of 64 keys takes
+// 4100 cycles of a workgroup (2048 of MFMAs a SIMD).  4 chunks of 450 rows after 12000
+// to 32000 keys (32 over 8 heads) 556 us, 990 TFLOP/s; 7600 rows that see 1024 keys
+// and the first four 185 us, 710 TFLOP/s: a tile of 19 chunks has 15000 cycles of its
+// own (first scores and their maximum 5000, a chunk's masks, the rows' stores).
+// Without the fetch the chunks' call took 478 of 569 us, without the exponentials 536.
 #include "attn_pipe.h"
 #include "paged_device.h"
 
