@@ -27,11 +27,10 @@
 //                 1077 MB 5.8 TB/s: HBM
 //   bf16 d = 128  one token after 300 keys: 8.8, a chain of trips: the list's item,
 //                 page ids, K, scores, V, the pieces' join; a launch is 3.5
-//   bf16 d = 256  28 requests of 1 to 8 rows and 4 of 64, 100 to 4096 keys: 91.  K and
-//                 V of 276 MB come from HBM once (3.0 TB/s), and tiles of one request
-//                 again from the L2 (585 MB into LDS); a round of the four waves'
-//                 sub-tiles takes 7000 cycles, of which 4000 are spent handing
-//                 32 loads of 1 KB a wave to a CU that holds one workgroup (its LDS)
+//   bf16 d = 256  28 requests of 1 to 8 rows and 4 of 64, 100 to 4096 keys: 91, for
+//                 560 MB 6.1 TB/s of HBM and MALL.  276 MB would do: the tiles of
+//                 one request read its keys each for themselves.  Of a round's 7000
+//                 cycles 4000 are spent handing out loads that wait for room
 //   f32           12 chunks of 17 to 41 rows, 256 to 2048 keys: 58, of which a
 //                 quarter are the items' starts and joins; a round of 9100 cycles has 3000
 //                 of MFMAs, the rest makes bf16 parts of K and V beside them and
