@@ -629,7 +629,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   // several groups walk the pieces and meet in LDS.  All loads of kUnits x
   // kBatch partial results are in flight at once: a trip past the L2 takes
   // 1.5 us (with one unit at a time the joining of three pieces of 32 slots took
-  // 6 us at d = 128, 12 us at d = 256).
+  // 6 us at d = 128, 12 us at d = 256).  Two units of bf16 d = 128, whose registers
+  // two workgroups share: with four, 16 requests of 32 rows in 1024 keys took 26.5 us,
+  // 24.9 with two.
   constexpr int kUnits = BF && D == 128 ? 2 : 4, kBatch = 4;
   const int units = slots * kCols;
   int groups = 1;
