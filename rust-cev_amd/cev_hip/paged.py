@@ -118,13 +118,12 @@ def rope(q_in, k_in, pos, rot: RotaryAngles, interleaved: bool = False, transpos
     inputs.  Returns (q_out, k_out), with v_in also v_out."""
     if slots is not None and (k_out is None or (v_in is not None and v_out is None)):
         raise CevError(-1, "rope: slots need caches to store into")
-    if q_out is None or k_out is None or (v_in is not None and v_out is None):
+    if stream is not None:  # (outputs that the call makes come from the current stream's pool)
         with _on(stream):
             q_out = _like(q_in) if q_out is None else q_out
             k_out = _like(k_in) if k_out is None else k_out
             v_out = _like(v_in) if v_in is not None and v_out is None else v_out
-    calls().rope(q_in, k_in, v_in, pos, rot.steps, rot.rotary_dim, rot.factor, interleaved, transposed, slots, q_out, k_out, v_out, stream)
-    return (q_out, k_out) if v_in is None else (q_out, k_out, v_out)
+    return calls().rope(q_in, k_in, v_in, pos, rot.steps, rot.rotary_dim, rot.factor, interleaved, transposed, slots, q_out, k_out, v_out, stream)
 
 
 class PagedAttention:

@@ -14,6 +14,7 @@
 #include <Python.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/ops/empty_like.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
@@ -449,16 +450,26 @@ PyObject* py_paged_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// rope(q_in, k_in, v_in, pos, steps, rotary_dim, factor, interleaved, transposed, slots, q_out, k_out, v_out, stream): all on
-// one GPU, outputs given
+// An output, or a contiguous tensor like x where none is given (from the
+// current stream's pool: calls on another stream give theirs).
+const at::Tensor& output(PyObject* o, const char* name, const at::Tensor& x, at::Tensor& made) {
+  if (o != Py_None) return tensor(o, name);
+  made = at::empty_like(x, at::MemoryFormat::Contiguous);
+  return made;
+}
+
+// rope(q_in, k_in, v_in, pos, steps, rotary_dim, factor, interleaved, transposed, slots, q_out, k_out, v_out, stream) -> the
+// outputs, v's with v_in: all on one GPU
 PyObject* py_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded([&] {
+  PyObject* result = nullptr;
+  PyObject* const done = guarded([&] {
     need_args(n, 14);
     const char* const me = "rope";
-    const at::Tensor &q = tensor(a[0], "q_in"), &k = tensor(a[1], "k_in"), &pos = tensor(a[3], "pos"), &steps = tensor(a[4], "steps"),
-                     &qo = tensor(a[10], "q_out"), &ko = tensor(a[11], "k_out");
-    const at::Tensor *const v = tensor_or_none(a[2], "v_in"), *const slots = tensor_or_none(a[9], "slots"),
-                     *const vo = tensor_or_none(a[12], "v_out");
+    const at::Tensor &q = tensor(a[0], "q_in"), &k = tensor(a[1], "k_in"), &pos = tensor(a[3], "pos"), &steps = tensor(a[4], "steps");
+    const at::Tensor *const v = tensor_or_none(a[2], "v_in"), *const slots = tensor_or_none(a[9], "slots");
+    at::Tensor made[3];
+    const at::Tensor &qo = output(a[10], "q_out", q, made[0]), &ko = output(a[11], "k_out", k, made[1]);
+    const at::Tensor* const vo = v ? &output(a[12], "v_out", *v, made[2]) : tensor_or_none(a[12], "v_out");
     want(q.dim() == 3 && k.dim() == 3 && k.size(0) == q.size(0) && k.size(2) == q.size(2), me, "q_in must be (t, hq, d) and k_in (t, hkv, d)");
     const int64_t t = q.size(0), rotary = as_int(a[5]);
     const int dt = dtype_code(q);
@@ -507,7 +518,15 @@ PyObject* py_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return api.rope(&d, ptr(q), ptr(k), ptr(v), (const int32_t*)ptr(pos), (const uint64_t*)ptr(steps), (const int32_t*)ptr(slots), ptr(qo),
                       ptr(ko), ptr(vo), s);
     });
+    auto object = [&](PyObject* o, const at::Tensor& x) { return o != Py_None ? Py_NewRef(o) : THPVariable_Wrap(x); };
+    result = v ? Py_BuildValue("(NNN)", object(a[10], qo), object(a[11], ko), object(a[12], *vo)) : Py_BuildValue("(NN)", object(a[10], qo), object(a[11], ko));
   });
+  if (!done) {
+    Py_XDECREF(result);
+    return nullptr;
+  }
+  Py_DECREF(done);
+  return result;
 }
 
 const cev_paged_desc* paged_desc(const Bytes& b) {
