@@ -130,7 +130,8 @@ class PagedAttention:
     """Attention of each request's new tokens, its last positions, over its
     pages (cev_paged_attention) for calls of one shape: q and out (t, hq, d),
     caches (n_pages, page_size, hkv, d), block_table (requests, pages).
-    max_new: no request has more new tokens in a step (default t).  window: a
+    max_new: no request has more new tokens in a step (default t; a decoding
+    step that says so is one launch less).  window: a
     row sees that many last keys, itself among them, and the first `sinks`
     ones; 0: all.  plan() makes the step's work list from cu and lengths on the
     device; every call until the next plan() uses it.  out may be q.  The object
