@@ -12,8 +12,9 @@ constexpr int kPagedMaxRequests = 4096;
 // The two kernels and their work lists: requests with few new rows go to the
 // first, those with many to the second (choice in cev_paged_bounds).
 constexpr int kPagedFew = 0, kPagedMany = 1, kPagedLists = 2;
-constexpr int kPagedSlots[kPagedLists] = {32, 256};  // query slots (rows x heads of a group) of a tile
-constexpr int kPagedKeys[kPagedLists] = {32, 64};    // keys of a sub-tile
+// Query slots (rows x heads of a group) of a tile and keys of a sub-tile of heads of d.
+constexpr int paged_slots(int list) { return list == kPagedFew ? 32 : 256; }
+constexpr int paged_keys(int list, int d) { return list == kPagedMany && d == 128 ? 64 : 32; }
 
 // The work buffer: this header, then for each list the first item of every
 // workgroup's run, all items, one arrival counter for every (split tile, KV
@@ -37,6 +38,7 @@ static_assert(sizeof(PagedHeader) == 16 && sizeof(PagedItem) == 48, "work buffer
 
 struct PagedListBounds {
   int32_t rows;      // query rows of a tile
+  int32_t keys;      // keys of a sub-tile
   int32_t target;    // most workgroups, for each KV head (0: no request can be in the list)
   int32_t items;     // most items
   size_t first_off, items_off, counters_off, records_off;
@@ -65,7 +67,7 @@ struct PagedArgs {
   uint32_t sig;
 };
 // The kernel of tiles of 256 query slots (paged_tile.hip).
-int32_t cev_paged_tile_launch(const PagedArgs& a, int32_t target, void* stream);
+int32_t cev_paged_tile_launch(const PagedArgs& a, int32_t d, int32_t target, void* stream);
 
 // The key sub-tiles that query rows at positions [pos0, pos1] see, in stream
 // order: `sinks` sub-tiles from key 0, then those from `first` on.  Keys from

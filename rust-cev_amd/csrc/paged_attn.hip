@@ -45,7 +45,8 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
-constexpr int kKeys = ::kPagedKeys[kPagedFew], kSlots = ::kPagedSlots[kPagedFew];
+constexpr int kKeys = 32, kSlots = paged_slots(kPagedFew);  // keys of a sub-tile
+static_assert(paged_keys(kPagedFew, 128) == kKeys && paged_keys(kPagedFew, 256) == kKeys, "the work list's sub-tiles");
 
 // Workgroup b writes NaN over its share of out's rows.
 template <typename T, int D>
@@ -768,7 +769,7 @@ extern "C" int32_t cev_paged_attention(const cev_paged_desc* d, const void* q, c
   };
   const hipStream_t s = (hipStream_t)stream;
   if (const int32_t target = list(kPagedMany)) {
-    const int32_t rc = cev_paged_tile_launch(a, target, s);
+    const int32_t rc = cev_paged_tile_launch(a, d->head_dim, target, s);
     if (rc) return rc;
   }
   const int32_t target = list(kPagedFew);

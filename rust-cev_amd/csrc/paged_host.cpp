@@ -96,17 +96,18 @@ int32_t cev_paged_bounds(const cev_paged_desc* d, PagedBounds* b) {
                 (long long)d->bt_stride);
   b->max_len = d->max_pages * d->page_size;
   b->sig = signature(d);
-  // bf16 heads of 128 have a kernel for requests of more rows than one tile of
+  // bf16 heads have a kernel for requests of more rows than one tile of
   // the first kernel holds; the plan decides which kernel takes them.
-  const bool tiles = d->dtype == CEV_BF16 && d->head_dim == 128;
+  const bool tiles = d->dtype == CEV_BF16, two = tiles && d->head_dim == 128;
   size_t at = 256;
   for (int i = 0; i < kPagedLists; ++i) {
     PagedListBounds& l = b->list[i];
-    l.rows = kPagedSlots[i] / g;
+    l.rows = paged_slots(i) / g;
+    l.keys = paged_keys(i, d->head_dim);
     l.target = 0;
     int64_t items = 0;
-    if (i == kPagedFew || (tiles && d->max_new > kPagedSlots[kPagedFew] / g)) {
-      const int32_t cus = i == kPagedMany ? kManyWorkgroups : tiles ? kFewWorkgroups128 : kFewWorkgroups;
+    if (i == kPagedFew || (tiles && d->max_new > paged_slots(kPagedFew) / g)) {
+      const int32_t cus = i == kPagedMany ? kManyWorkgroups : two ? kFewWorkgroups128 : kFewWorkgroups;
       l.target = cus / d->n_kv_heads > 0 ? cus / d->n_kv_heads : 1;
       // whole tiles, and a cut for each workgroup after the first
       auto most = [&](int32_t max_new) {
@@ -118,7 +119,7 @@ int32_t cev_paged_bounds(const cev_paged_desc* d, PagedBounds* b) {
       // the plan counts the tiles' sub-tiles, and eight more for each, in 32 bits
       // (much work in requests of many rows is not left to the first kernel)
       const int64_t counted = most(i == kPagedFew && tiles && d->max_new > l.rows ? l.rows : d->max_new);
-      if (counted * ((int64_t)b->max_len / kPagedKeys[i] + 16) > INT32_MAX)
+      if (counted * ((int64_t)b->max_len / l.keys + 16) > INT32_MAX)
         return cev_fail(CEV_ERR_UNSUPPORTED, "paged attention: %lld tiles of query rows over %d keys are too many for one call",
                         (long long)counted, b->max_len);
     }
@@ -128,7 +129,7 @@ int32_t cev_paged_bounds(const cev_paged_desc* d, PagedBounds* b) {
     l.counters_off = align_up(l.items_off + sizeof(PagedItem) * (size_t)items);
     // a cut makes at most one more split tile and two more pieces
     l.records_off = align_up(l.counters_off + 4 * (size_t)l.target * d->n_kv_heads);
-    at = align_up(l.records_off + 2 * (size_t)l.target * d->n_kv_heads * kPagedSlots[i] * (d->head_dim + 2) * sizeof(float));
+    at = align_up(l.records_off + 2 * (size_t)l.target * d->n_kv_heads * paged_slots(i) * (d->head_dim + 2) * sizeof(float));
   }
   b->bytes = at;
   return CEV_OK;

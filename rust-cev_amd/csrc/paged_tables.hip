@@ -261,22 +261,29 @@ struct PlanArgs {
   PagedListBounds list[kPagedLists];
   int32_t n_requests, t, max_new, max_len, window, sinks, hkv;
   uint32_t sig;
-  bool bf16, two_a_cu;
+  bool bf16, d128;
 };
 
 // Requests of more rows than a tile of the first kernel (32 slots) go to the
 // second from this many of the first kernel's sub-tiles for each of its
 // workgroups on.  With fewer the first has more workgroups at work; with more it
-// is bound by reading the keys once for every 32 slots.  First and second kernel
-// (32 query over 8 KV heads, us):
+// is bound by reading the keys once for every 32 slots.  First and second kernel,
+// d = 128 (32 query over 8 KV heads, us):
 //   1 request of 256 slots and  2048 keys (8 sub-tiles a workgroup)   20.6  35.5
 //   4 requests of  64 slots and  4096 keys (16)                       25.5  31.7
 //   12 requests of 128 slots and 1024 keys (24)                       25.1  26.3
 //   16 requests of 64 slots and  2048 keys (32)                       34.9  33.9
 //   64 requests of 48 slots and   512 keys (32)                       49.7  36.1
 //   64 requests of 64 slots and  2048 keys (128)                       195   117
-constexpr int kFewWork = 32;
-static_assert((int64_t)kFewWork * 512 < 1 << 18, "the sum's clip");
+// d = 256 (16 over 4):
+//   16 requests of 64 slots and 2048 keys (32)                        39.7  53.1
+//   16 requests of 128 slots and 2048 keys (64)                       48.8  58.3
+//   16 requests of 256 slots and 2048 keys (128)                      92.6  76.8
+//   64 requests of 64 slots and 2048 keys (128)                        194   156
+//   64 requests of 256 slots and 2048 keys (512)                       740   195
+//   1 request of 1024 slots and 8192 keys (128), the other way         90    121
+constexpr int few_work(bool d128) { return d128 ? 32 : 96; }
+static_assert(few_work(true) * 512 < 1 << 18 && few_work(false) * 256 < 1 << 18, "the sum's clip");
 // What an item costs beside its sub-tiles (its start, and its partial or final
 // result), in sub-tiles.  With 4, 8 and 12 (us): 12 f32 chunks 59.7, 60.4, 60.5; 32
 // requests of d = 256 95.6, 92.1, 95.0; 12 f32 chunks of 17 to 41 rows of 4 heads
@@ -294,11 +301,11 @@ constexpr int kItemCost = 8;
 //     bf16 d = 256  11.1 (16.5) / 14.8 (17.2)    f32  12.5 (23.4) / 15.7 (23.6)
 //   32 slots of bf16 d = 128 in 1024 / 4096 keys   13.5 (16.1) / 18.0 (18.1)
 //   256 slots of the second kernel                 30.8 (35.9) / 44.9 (69.0)
-__device__ __forceinline__ float piece_rate(int list, bool bf16, bool half_filled, uint32_t n_sub) {
+__device__ __forceinline__ float piece_rate(int list, bool bf16, bool d128, bool half_filled, uint32_t n_sub) {
   const float root = __builtin_amdgcn_sqrtf((float)n_sub);
   float len;
   if (list == kPagedMany)
-    len = 2.0f * root;
+    len = (d128 ? 2.0f : 2.8f) * root;
   else
     len = n_sub <= 8 ? 8.0f : fmaxf(4.0f, 4.0f * rintf((half_filled ? 0.125f : 0.25f) * (bf16 ? 1.4f : 0.7f) * root));
   return __builtin_amdgcn_rcpf(len);
@@ -356,12 +363,12 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
     for (int i = 0; i < PER; ++i) {
       if (rows[i] <= l.rows) continue;
       const int32_t pos0 = pos_s[tid * PER + i], pos1 = pos0 + rows[i] - 1;
-      const int64_t n_sub = (int64_t)paged_span(kPagedKeys[kPagedFew], pos0, pos0 + l.rows - 1, a.window, a.sinks).total +
-                            paged_span(kPagedKeys[kPagedFew], pos1 - l.rows + 1, pos1, a.window, a.sinks).total;
+      const int64_t n_sub = (int64_t)paged_span(l.keys, pos0, pos0 + l.rows - 1, a.window, a.sinks).total +
+                            paged_span(l.keys, pos1 - l.rows + 1, pos1, a.window, a.sinks).total;
       work[0] += (uint32_t)min((int64_t)1 << 18, ((rows[i] + l.rows - 1) / l.rows * n_sub) >> 1);
     }
     exclusive_sums<W>(work, all_work, part);
-    if (all_work[0] >= (uint32_t)(kFewWork * l.target)) few_rows = l.rows;
+    if (all_work[0] >= (uint32_t)(few_work(a.d128) * l.target)) few_rows = l.rows;
   }
 #pragma unroll
   for (int list = 0; list < kPagedLists; ++list) {
@@ -405,7 +412,7 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
       t.n_rows = min(l.rows, n_s[lo] - at);
       t.pos0 = pos_s[lo] + at;
       t.req = lo;
-      t.c_end = paged_span(kPagedKeys[list], t.pos0, t.pos0 + t.n_rows - 1, a.window, a.sinks).total;
+      t.c_end = paged_span(l.keys, t.pos0, t.pos0 + t.n_rows - 1, a.window, a.sinks).total;
       return t;
     };
     // length of all tiles; pieces of them, of twice and of four times the length
@@ -415,7 +422,7 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
       const uint32_t n_sub = (uint32_t)t.c_end;
       sum[0] += n_sub + kItemCost;
       longest = max(longest, n_sub);
-      const float rate = piece_rate(list, a.bf16, 2 * t.n_rows <= l.rows, n_sub);
+      const float rate = piece_rate(list, a.bf16, a.d128, 2 * t.n_rows <= l.rows, n_sub);
 #pragma unroll
       for (int k = 0; k < 3; ++k) sum[1 + k] += piece_count(n_sub, rate / (float)(1 << k));
     }
@@ -424,7 +431,7 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
     // longer before that (16 requests of one token after 1023: 15.5 us, 18.1 with
     // two a CU), long ones are not (4 requests of 32 rows after 4064: 29.4 us with
     // two a CU, 35.6 in longer pieces).
-    const bool two = list == kPagedFew && a.two_a_cu;
+    const bool two = list == kPagedFew && a.d128;
     const uint32_t target = (uint32_t)l.target, alone = two ? target / 2 : target;
     const int by = sums[1] <= alone ? 0 : sums[2] <= alone ? 1 : two && sums[3] <= alone && sums[0] <= 24 * sums[3] ? 2 : 1;
     const uint32_t n_pieces = by == 0 ? sums[1] : by == 1 ? sums[2] : sums[3];
@@ -472,7 +479,7 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
       else if (n_sub && same)
         n = (n_sub + same - 1) / same;
       else if (n_sub)
-        n = piece_count(n_sub, piece_rate(list, a.bf16, 2 * t.n_rows <= l.rows, n_sub) * shorter);
+        n = piece_count(n_sub, piece_rate(list, a.bf16, a.d128, 2 * t.n_rows <= l.rows, n_sub) * shorter);
       uint32_t y[3] = {n, n > 1 ? n : 0, n > 1 ? 1u : 0u}, y_all[3];
       exclusive_sums<W>(y, y_all, part);
       t.n_pieces = (int32_t)n;
@@ -581,7 +588,7 @@ extern "C" int32_t cev_paged_plan(const cev_paged_desc* d, const int32_t* cu, co
   a.hkv = d->n_kv_heads;
   a.sig = b.sig;
   a.bf16 = d->dtype == CEV_BF16;
-  a.two_a_cu = a.bf16 && d->head_dim == 128;
+  a.d128 = a.bf16 && d->head_dim == 128;
   // one wave where a lane has a few tiles at most
   const PagedListBounds& most = b.list[b.list[kPagedMany].target ? kPagedMany : kPagedFew];
   const int64_t tiles = (int64_t)most.items - most.target;

@@ -746,10 +746,10 @@ def test_attention_of_odd_head_counts(gpu, kind, hq, hkv, d):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("kind,many", [("bf16", False), ("bf16", True), ("f32", False)])
-def test_attention_in_place_of_q(gpu, kind, many):
+@pytest.mark.parametrize("kind,d,many", [("bf16", 128, False), ("bf16", 128, True), ("bf16", 256, False), ("bf16", 256, True), ("f32", 128, False)])
+def test_attention_in_place_of_q(gpu, kind, d, many):
     import torch
-    p = (_Many if many else _Paged)(gpu, [0, 3000, 33], [40, 70, 1], 8, 2, 128, kind, 16, seed=2)
+    p = (_Many if many else _Paged)(gpu, [0, 3000, 33], [40, 70, 1], 8, 2, d, kind, 16, seed=2)
     want = p.run()
     assert torch.equal(p.run(out=p.q), want)
 
@@ -821,9 +821,9 @@ class _Many(_Paged):
     Its own rows are only looked at for being finite."""
 
     def __init__(self, dev, past, new, hq, hkv, d, kind, page, window=0, **kw):
-        rows, target = 32 * hkv // hq, max(1, 512 // hkv)
-        each = max(1, (window + rows - 1) // 32) if window else 64  # sub-tiles that a tile sees at least
-        super().__init__(dev, [*past, window or 2048], [*new, rows * (32 * target // each + 2)], hq, hkv, d, kind, page, **kw)
+        rows, work = 32 * hkv // hq, 32 * (512 // hkv) if d == 128 else 96 * (256 // hkv)
+        each = (window + rows + 30) // 32 if window else 64  # sub-tiles that a tile sees at least
+        super().__init__(dev, [*past, window or 2048], [*new, rows * (work // each + 2)], hq, hkv, d, kind, page, **kw)
 
     def run(self, out=None, stream=None, **kw):
         import torch
@@ -843,7 +843,7 @@ class _Many(_Paged):
         self.new = all_new
 
 
-MANY_SHAPES = [("bf16", 8, 2, 128), ("bf16", 4, 4, 128), ("bf16", 16, 2, 128)]
+MANY_SHAPES = [("bf16", 8, 2, 128), ("bf16", 4, 4, 128), ("bf16", 16, 2, 128), ("bf16", 4, 2, 256), ("bf16", 8, 1, 256)]
 
 
 @pytest.mark.gpu
@@ -862,7 +862,7 @@ def test_attention_of_many_rows(gpu, kind, hq, hkv, d, past, new, page, window, 
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("kind,hq,hkv,d", MANY_SHAPES)
+@pytest.mark.parametrize("kind,hq,hkv,d", MANY_SHAPES[:4])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("which", ["k", "v"])
 def test_values_that_one_of_many_rows_does_not_see(gpu, kind, hq, hkv, d, value, which):
@@ -892,9 +892,10 @@ def test_values_that_one_of_many_rows_does_not_see(gpu, kind, hq, hkv, d, value,
 
 
 @pytest.mark.gpu
-def test_bad_pages_of_many_rows(gpu):
+@pytest.mark.parametrize("d", [128, 256])
+def test_bad_pages_of_many_rows(gpu, d):
     """A page outside the cache that only the later rows of a request see, and one in a request of its own."""
-    p = _Many(gpu, [20, 100], [60, 70], 8, 2, 128, "bf16", 16)
+    p = _Many(gpu, [20, 100], [60, 70], 8, 2, d, "bf16", 16)
     want = p.run()
     p.table[0, 4], p.table[1, 0] = p.n_pages, -1
     out = p.run()
