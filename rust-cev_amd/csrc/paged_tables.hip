@@ -276,13 +276,13 @@ struct PlanArgs {
 //   64 requests of 48 slots and   512 keys (32)                       49.7  36.1
 //   64 requests of 64 slots and  2048 keys (128)                       195   117
 // d = 256 (16 over 4):
-//   16 requests of 64 slots and 2048 keys (32)                        39.7  53.1
-//   16 requests of 128 slots and 2048 keys (64)                       48.8  58.3
-//   16 requests of 256 slots and 2048 keys (128)                      92.6  76.8
-//   64 requests of 64 slots and 2048 keys (128)                        194   156
-//   64 requests of 256 slots and 2048 keys (512)                       740   195
-//   1 request of 1024 slots and 8192 keys (128), the other way         90    121
-constexpr int few_work(bool d128) { return d128 ? 32 : 96; }
+//   16 requests of  64 slots and  2048 keys (32)                      39.7  43.4
+//   16 requests of 128 slots and  2048 keys (64)                      48.8  48.2
+//   6 requests of 70 to 164 slots and 4000 to 8000 keys (71)          93.7  80.2
+//   16 requests of 256 slots and  2048 keys (128)                     92.6  68.1
+//   64 requests of 256 slots and  2048 keys (512)                      740   155
+//   1 request of 1024 slots and   8192 keys (126), the other way        90   102
+constexpr int few_work(bool d128) { return d128 ? 32 : 64; }
 static_assert(few_work(true) * 512 < 1 << 18 && few_work(false) * 256 < 1 << 18, "the sum's clip");
 // What an item costs beside its sub-tiles (its start, and its partial or final
 // result), in sub-tiles.  With 4, 8 and 12 (us): 12 f32 chunks 59.7, 60.4, 60.5; 32

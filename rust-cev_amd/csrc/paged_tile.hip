@@ -27,8 +27,9 @@
 // and the first four 185 us, 710 TFLOP/s: a tile of 19 chunks has 15000 cycles of its
 // own (first scores and their maximum 5000, a chunk's masks, the rows' stores).
 // Without the fetch the chunks' call took 478 of 569 us, without the exponentials 536.
-// d = 256: 64 requests of 256 rows in 2048 keys (16 over 4 heads) 718 us, 720 TFLOP/s;
-// 32 slots a workgroup took 2800.
+// d = 256: 64 requests of 256 rows in 2048 keys (16 over 4 heads) 592 us, 870 TFLOP/s;
+// 32 slots a workgroup took 2800.  K reads three units ahead 718; two, and fewer
+// addresses kept, so that nothing of the loop lies in scratch, 676.
 #include "attn_pipe.h"
 #include "paged_device.h"
 
@@ -47,7 +48,7 @@ __device__ __forceinline__ int fresh_half() { return fresh_lane_id() >> 5; }
 // LDS reads of d = 256's chunk body: 16 K reads kKPF ahead of their MFMA, then 16
 // V fragments of two reads kVPF ahead, beside whose last units the next body's
 // first K reads go out.  What a unit waits for: the reads issued after its own.
-constexpr int kKPF = 3, kVPF = 3;
+constexpr int kKPF = 2, kVPF = 3;
 constexpr int wait_k256(int st) { return 15 - st < kKPF - 1 ? 15 - st : kKPF - 1; }
 constexpr int wait_v256(int unit) {
   int at[16] = {}, n = 0, wait = 0;
@@ -59,8 +60,8 @@ constexpr int wait_v256(int unit) {
   }
   return wait;
 }
-static_assert(wait_k256(0) == 2 && wait_k256(15) == 0 && wait_v256(0) == 4 && wait_v256(13) == 4 && wait_v256(14) == 3 && wait_v256(15) == 2,
-              "three fragments ahead");
+static_assert(wait_k256(0) == 1 && wait_k256(15) == 0 && wait_v256(0) == 4 && wait_v256(13) == 4 && wait_v256(14) == 2 && wait_v256(15) == 1,
+              "two K and three V fragments ahead");
 
 template <int D>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_tile_kernel(PagedArgs a) {
@@ -90,8 +91,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int lds_base = (int)(size_t)(const __attribute__((address_space(3))) char*)lds;
   // (bit 4 of a block's place is its own: the upper 128 columns of d = 256 are 256
   // bytes further)
-  // d = 256 keeps the first of each, and makes the others of their places' bits:
-  // with all kept, nine values of Q lay in scratch.
+  // d = 256 keeps the first of each, and makes the others of their places' bits
+  // (with all kept nine values of the loop lay in scratch, now a few).
   constexpr int kKoff = D == 128 ? 8 : 1, kVoff = D == 128 ? 4 : 1;
   int koff[kKoff], voff[kVoff];
 #pragma unroll
