@@ -904,6 +904,51 @@ def test_bad_pages_of_many_rows(gpu, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [128, 256])
+def test_many_rows_strides_and_far_pages(gpu, d):
+    """Caches with strides of their own whose pages lie more than 4 GiB in, rows
+    inside larger buffers, an odd block table stride, another stream."""
+    import torch
+    p = _Many(gpu, [40, 333, 0], [50, 33, 200], 8, 2, d, "bf16", 16, seed=6)
+    want = p.run()
+    n_pages = (5 << 30) // (2 * 16 * 2 * (d + 16))
+    far = torch.arange(p.n_pages, device=gpu) * (n_pages // p.n_pages - 1) + 5
+    for name in ("k", "v"):
+        wide = torch.empty(n_pages, 16, 2, d + 16, dtype=torch.bfloat16, device=gpu)[..., :d]
+        wide[far] = getattr(p, name)
+        setattr(p, name, wide)
+    p.n_pages = n_pages
+    moved = torch.where(p.table >= 0, far[p.table.clamp(min=0).long()], -1).to(torch.int32)
+    p.table = torch.full((moved.shape[0], p.max_pages + 3), -1, dtype=torch.int32, device=gpu)[:, : p.max_pages]
+    p.table.copy_(moved)
+    q = torch.zeros(p.t, 8, d + 8, dtype=torch.bfloat16, device=gpu)[..., :d]
+    q.copy_(p.q)
+    p.q = q
+    out = torch.full((p.t, 16, d), 5.0, dtype=torch.bfloat16, device=gpu)[:, ::2]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    p.run(out=out, stream=s)
+    s.synchronize()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("order", ["up", "down", "one"])
+def test_large_scores_of_many_rows(gpu, d, order):
+    """The running maximum moves, stays, or sits at one key."""
+    import torch
+    p = _Many(gpu, [800], [103], 4, 2, d, "bf16", 16, seed=3)
+    place = torch.zeros(p.n_pages, 16, device=gpu)
+    for i, page in enumerate(p.table[0, : -(-903 // 16)].tolist()):
+        place[page] = torch.arange(16, device=gpu) + 16 * i
+    size = {"up": place / 903, "down": 1 - place / 903, "one": (place == 450).float()}[order]
+    p.q.copy_(p.q.sign())
+    p.k.copy_((size[..., None, None] * 25 * p.q[0, 0].float()).to(p.k.dtype).expand_as(p.k))
+    p.check(p.run(), order)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_attention_of_large_scores(gpu, kind):
     """Scores of several hundred that rise with the key, fall, or sit at one key: the running maximum moves or stays."""
