@@ -374,7 +374,11 @@ int32_t cev_gather_rows(int32_t dtype, int32_t out_dtype, int64_t n, int64_t wid
  * ends it.  Pages that the new tokens need are taken from the free ring in
  * request order and entered in block_table; an ended request's pages go back
  * to the ring's end in request order (for later calls: none of them is
- * taken by this one) and its length becomes 0.  The ring is free_pages
+ * taken by this one) and its length becomes 0.  Entries outside [0, n_pages)
+ * are passed over, and every page is given back as often as an ended row
+ * names it: whoever lets requests share pages, or gives pages behind a window
+ * back before their request ends, enters -1 for what a request does not hold
+ * before it ends.  The ring is free_pages
  * (n_pages entries) with ring = {head, count, status, counter}: the free
  * pages are free_pages[(head + i) % n_pages], i < count.  Written:
  *   lengths_out (n_requests)  the lengths with the new tokens

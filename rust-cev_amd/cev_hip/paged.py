@@ -57,6 +57,11 @@ def paged_tables(lengths, new_len, block_table, page_size: int, cu, pos, slots, 
     offsets cu (requests + 1), each packed row's position and cache slot (0 and
     -1 behind the last row), the new lengths and the ring's new state.
 
+    A page has one holder: the ring takes back every page that an ended
+    request's row names.  Entries outside [0, n_pages) are passed over, so enter
+    -1 where a page is another request's (a shared prefix) or was given back
+    before (behind a window) and then end the request.
+
     All tensors are int32 on the GPU: lengths, new_len (requests), block_table
     (requests, pages), pos and slots (the most rows of a step), free (n_pages)
     and ring (4): [head, count, status, 0], the free pages being

@@ -1210,3 +1210,78 @@ def test_steps_on_two_streams(gpu):
     torch.cuda.synchronize()
     for (_, _, out, _), want in zip(sides, alone):
         assert torch.equal(out, want)
+
+
+# ---------------------------------------------------------------------------
+# What an ended request holds
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("requests,max_pages,page,tokens", [(5, 7, 16, 40), (90, 70, 16, 300), (700, 33, 4, 5000), (70, 300, 16, 80), (3, 700, 1, 9)])
+def test_an_ended_request_gives_back_what_its_row_names(gpu, requests, max_pages, page, tokens):
+    """Entries that are no pages (shared ones, those given back behind a
+    window) are passed over: the ring gets the others in their order, counts
+    those, and never hands a page to two requests."""
+    rng = random.Random(requests)
+    lengths = [rng.randint(0, max_pages * page) for _ in range(requests)]
+    s = _Tables(gpu, lengths, page, max_pages, spare=requests + 3, seed=requests, max_tokens=tokens, extra_stride=1)
+    held = [-(-n // page) for n in lengths]
+    bad = [-1, s.n_pages, 2 ** 31 - 1, -(2 ** 31)]
+    for r, h in enumerate(held):
+        gone = range(h) if rng.random() < 0.2 else range(0) if rng.random() < 0.2 else [j for j in range(h) if rng.random() < 0.5]
+        for j in gone:
+            s.table_np[r][j] = rng.choice(bad)
+    s.table.copy_(s.t(s.table_np))
+    new = [rng.choice([-1, -1, 0, 0]) if r else -1 for r in range(requests)]
+    given = [e for r, a in enumerate(new) if a < 0 for e in s.table_np[r][: held[r]] if 0 <= e < s.n_pages]
+    head, count = s.ring_np[:2]
+    ring = list(s.free_np)
+    for i, e in enumerate(given):
+        ring[(head + count + i) % s.n_pages] = e
+    table = [list(r) for r in s.table_np]
+    s.step(new)
+    assert s.ring.tolist() == [head, count + len(given), 0, 0] and s.free.tolist() == ring and s.table.tolist() == table
+    assert s.lengths.tolist() == [0 if a < 0 else n for a, n in zip(new, lengths)]
+    # whoever comes next gets pages that nobody holds
+    rows = [a < 0 for a in new]
+    new = [min(page * 2, tokens // requests + 1) if gone else 0 for gone in rows]
+    while sum(new) > tokens:
+        new[max(r for r, a in enumerate(new) if a)] = 0
+    s.step(new)
+    assert s.ring.tolist()[2] == 0 and min(s.slots.tolist()[: sum(new)]) >= 0
+    names = [e for r in range(requests) for e in s.table.tolist()[r][: -(-s.lengths.tolist()[r] // page)] if 0 <= e < s.n_pages]
+    assert len(set(names)) == len(names)
+    assert not set(names) & {s.free.tolist()[(s.ring.tolist()[0] + i) % s.n_pages] for i in range(s.ring.tolist()[1])}
+
+
+@pytest.mark.gpu
+def test_requests_that_shared_a_prefix_end(gpu):
+    """The first one holds the common pages; the others name them no more when they end."""
+    s = _Tables(gpu, [40, 0, 0], 16, 4, 9, seed=5, max_tokens=60)
+    common = s.table_np[0][:2]
+    for r in (1, 2):  # 32 tokens of the first one's
+        s.table[r, :2] = s.table[0, :2]
+        s.lengths[r] = 32
+    s.step([1, 10, 20])
+    assert s.ring.tolist()[2] == 0
+    s.table[1:, :2] = -1
+    s.step([0, -1, -1])
+    assert s.ring.tolist()[1:3] == [s.n_pages - 3, 0]
+    s.step([-1, 0, 0])
+    head, count, status, _ = s.ring.tolist()
+    assert (count, status) == (s.n_pages, 0) and sorted(s.free.tolist()) == list(range(s.n_pages)) and set(common) <= set(s.free.tolist())
+
+
+@pytest.mark.gpu
+def test_more_pages_given_back_than_the_ring_has_room_for(gpu):
+    """Counted without the entries that are no pages: with them the step would be refused."""
+    s = _Tables(gpu, [64, 64], 16, 4, 0, seed=5, max_tokens=8)
+    s.table_np[0][1] = s.table_np[0][3] = -1
+    s.table.copy_(s.t(s.table_np))
+    s.ring_np = [2, s.n_pages - 5, 0, 0]
+    s.ring.copy_(s.t(s.ring_np))
+    s.step([-1, -1])  # six pages, five places
+    s.check(dict(status=8))
+    s.ring[1] -= 1
+    s.step([-1, -1])
+    assert s.ring.tolist() == [2, s.n_pages, 0, 0] and s.lengths.tolist() == [0, 0]
