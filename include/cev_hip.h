@@ -392,12 +392,13 @@ int32_t cev_gather_rows(int32_t dtype, int32_t out_dtype, int64_t n, int64_t wid
  * out of its bounds.  Then nothing is taken, given back or counted (cu is
  * all 0, slots all -1), so what the step launches next finds no rows.  An
  * entry outside [0, n_pages) gives slots of -1.  lengths_out may be lengths
- * and ring_out ring; ring_out[3] must be 0 before the first call (calls
- * leave it 0).  free_pages NULL: block_table holds the new tokens' pages
+ * and ring_out ring (otherwise they do not overlap).  ring[3] must be 0 before
+ * the first call: a call with one of the two in place counts its workgroups
+ * there, and leaves it 0 as it does ring_out[3].  free_pages NULL: block_table holds the new tokens' pages
  * already, and ended requests' pages are the caller's. */
 int32_t cev_paged_tables(int32_t n_requests, int32_t page_size, int32_t n_pages, int32_t max_pages, int32_t max_tokens,
                          const int32_t* lengths, const int32_t* new_len, int32_t* block_table, int64_t bt_stride, int32_t* free_pages,
-                         const int32_t* ring, int32_t* lengths_out, int32_t* ring_out, int32_t* cu, int32_t* pos, int32_t* slots,
+                         int32_t* ring, int32_t* lengths_out, int32_t* ring_out, int32_t* cu, int32_t* pos, int32_t* slots,
                          cev_stream stream);
 
 /* Rotary angles.  Pair i of rotary_dim / 2 turns by inv_i radians a position,

@@ -66,7 +66,7 @@ def paged_tables(lengths, new_len, block_table, page_size: int, cu, pos, slots, 
     (requests, pages), pos and slots (the most rows of a step), free (n_pages)
     and ring (4): [head, count, status, 0], the free pages being
     free[(head + i) % n_pages] for i < count.  lengths_out and ring_out default
-    to lengths and ring (in place).  ring[2] is 0, or says why the step was not
+    to lengths and ring (in place); their values before the call do not matter.  ring[2] is 0, or says why the step was not
     made (cev_hip.h); its cu is then all 0.  free None: the block table holds
     the new tokens' pages already (n_pages is then required)."""
     if ring is None:

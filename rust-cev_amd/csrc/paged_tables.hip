@@ -84,6 +84,7 @@ constexpr int kTokens = 4;  // packed rows of a thread and round
 struct TablesArgs {
   const int32_t *lengths, *new_len, *ring;
   int32_t *block_table, *free_pages, *lengths_out, *ring_out, *cu, *pos, *slots;
+  int32_t* arrived;  // workgroups that have read the inputs; null: no output lies in an input's place
   int64_t bt_stride;
   int32_t n_requests, page_shift, n_pages, max_pages, max_tokens;
 };
@@ -95,7 +96,8 @@ struct TablesArgs {
 // [head + count, ...) receive the pages given back: pages are distinct, so
 // the two ranges never meet in a ring of n_pages places).  Only the new
 // lengths and the new ring state may lie in their inputs' place; the last
-// workgroup to have read the inputs writes those.
+// workgroup to have read the inputs writes those then (counted in ring[3], which
+// the caller sets up with the rest of the ring).
 //
 // Of an ended request only the entries that are pages go back (its holder enters
 // another value for what the request does not hold), so every workgroup counts
@@ -285,11 +287,13 @@ __global__ __launch_bounds__(64 * W) void paged_tables_kernel(TablesArgs a) {
         }
       }
 
-  if (gridDim.x > 1) {
+  if (a.arrived) {
     __syncthreads();
-    if (tid == 0) last_s = atomicAdd(&a.ring_out[3], 1) == (int)gridDim.x - 1;
+    if (tid == 0) last_s = atomicAdd(a.arrived, 1) == (int)gridDim.x - 1;
     __syncthreads();
     if (!last_s) return;
+  } else if (blockIdx.x > 0) {
+    return;
   }
   for (int r = tid; r < R; r += kThreads) {
     // (a status leaves the lengths as they were, also those out of bounds)
@@ -299,6 +303,7 @@ __global__ __launch_bounds__(64 * W) void paged_tables_kernel(TablesArgs a) {
       a.lengths_out[r] = first_s[r] < 0 ? 0 : len_s[r] + cu_s[r + 1] - cu_s[r];
   }
   if (tid == 0) {
+    if (a.arrived) *a.arrived = 0;
     const bool same = status || !a.free_pages;
     a.ring_out[0] = same ? head : (int32_t)place(total[1]);
     a.ring_out[1] = same ? count : count - (int32_t)total[1] + (int32_t)total[2];
@@ -579,7 +584,7 @@ __global__ __launch_bounds__(64 * W) void paged_plan_kernel(PlanArgs a) {
 
 extern "C" int32_t cev_paged_tables(int32_t n_requests, int32_t page_size, int32_t n_pages, int32_t max_pages, int32_t max_tokens,
                                     const int32_t* lengths, const int32_t* new_len, int32_t* block_table, int64_t bt_stride,
-                                    int32_t* free_pages, const int32_t* ring, int32_t* lengths_out, int32_t* ring_out, int32_t* cu,
+                                    int32_t* free_pages, int32_t* ring, int32_t* lengths_out, int32_t* ring_out, int32_t* cu,
                                     int32_t* pos, int32_t* slots, cev_stream stream) {
   CEV_CHECK_ARG(n_requests >= 1, "cev_paged_tables: %d requests", n_requests);
   if (n_requests > kPagedMaxRequests)
@@ -593,6 +598,12 @@ extern "C" int32_t cev_paged_tables(int32_t n_requests, int32_t page_size, int32
                 (long long)bt_stride);
   CEV_CHECK_ARG(lengths && new_len && block_table && ring && lengths_out && ring_out && cu, "cev_paged_tables: null argument");
   CEV_CHECK_ARG(max_tokens == 0 || (pos && slots), "cev_paged_tables: null pos or slots");
+  auto cut = [](const int32_t* x, const int32_t* y, int32_t n) {  // the same place, or apart
+    const int64_t by = (int64_t)((uintptr_t)x - (uintptr_t)y);
+    return by != 0 && by < 4 * (int64_t)n && -by < 4 * (int64_t)n;
+  };
+  CEV_CHECK_ARG(!cut(lengths, lengths_out, n_requests) && !cut(ring, ring_out, 4),
+                "cev_paged_tables: an output overlaps its input without being the same");
   TablesArgs a;
   a.lengths = lengths;
   a.new_len = new_len;
@@ -613,6 +624,7 @@ extern "C" int32_t cev_paged_tables(int32_t n_requests, int32_t page_size, int32
   return by_requests(n_requests, max_tokens <= 64 * kTokens, [&](auto w_c, auto per_c) {
     constexpr int W = decltype(w_c)::value, PER = decltype(per_c)::value, rows = 64 * W * kTokens;
     const int64_t grid = ((int64_t)max_tokens + rows - 1) / rows;
+    a.arrived = grid > 1 && (lengths == lengths_out || ring == ring_out) ? ring + 3 : nullptr;
     hipLaunchKernelGGL((paged_tables_kernel<W, PER>), dim3((unsigned)(grid < 1 ? 1 : grid > 256 ? 256 : grid)), dim3(64 * W), 0,
                        (hipStream_t)stream, a);
     const hipError_t e = hipGetLastError();

@@ -1285,3 +1285,33 @@ def test_more_pages_given_back_than_the_ring_has_room_for(gpu):
     s.ring[1] -= 1
     s.step([-1, -1])
     assert s.ring.tolist() == [2, s.n_pages, 0, 0] and s.lengths.tolist() == [0, 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("requests,room", [(9, 2000), (300, 9000)])
+@pytest.mark.parametrize("apart", ["both", "ring", "lengths"])
+def test_tables_of_many_workgroups_write_outputs_whatever_they_held(gpu, requests, room, apart):
+    """New lengths and ring state in buffers that nobody has cleared, over several steps of more than one workgroup."""
+    import torch
+    rng = random.Random(requests)
+    s = _Tables(gpu, [rng.randint(0, 60) for _ in range(requests)], 16, 20, requests * 12, seed=3, max_tokens=room)
+    for k in range(4):
+        new = [rng.choice([-1, 0, 1, 20]) for _ in range(requests)]
+        want = s.expect(new)
+        lengths = torch.full_like(s.lengths, 77) if apart != "ring" else s.lengths
+        ring = s.t([-5, 9, 3, [1, -2, 7, 2 ** 31 - 1][k]]) if apart != "lengths" else s.ring
+        cev_hip.paged_tables(s.lengths, s.t(new), s.table, 16, s.cu, s.pos, s.slots, free=s.free, ring=s.ring, lengths_out=lengths, ring_out=ring)
+        torch.cuda.synchronize()
+        assert s.ring.tolist()[3] == 0
+        s.lengths, s.ring = lengths, ring
+        s.check(want, k)
+
+
+def test_tables_outputs_that_cut_their_inputs_are_refused(cev):
+    at = lambda a: C.c_void_p(a)  # noqa: E731
+    #       requests page n_pages max_pages tokens lengths new table stride free ring lengths_out ring_out cu pos slots
+    args = [8, 16, 50, 10, 0, at(4096), at(8192), at(16384), 10, at(32768), at(65536), at(69632), at(73728), at(77824), None, None, None]
+    for i, where in ((11, 4096 + 4), (11, 4096 + 28), (11, 4096 - 28), (12, 65536 + 4), (12, 65536 - 12)):
+        bad = list(args)
+        bad[i] = at(where)
+        assert _abi.lib().cev_paged_tables(*bad) == -1 and b"overlaps" in _abi.lib().cev_last_error(), (i, where)
