@@ -109,9 +109,11 @@ int32_t cev_paged_bounds(const cev_paged_desc* d, PagedBounds* b) {
     if (i == kPagedFew || (tiles && d->max_new > paged_slots(kPagedFew) / g)) {
       const int32_t cus = i == kPagedMany ? kManyWorkgroups : two ? kFewWorkgroups128 : kFewWorkgroups;
       l.target = cus / d->n_kv_heads > 0 ? cus / d->n_kv_heads : 1;
-      // whole tiles, and a cut for each workgroup after the first
+      // whole tiles, and a cut for each workgroup after the first (no request has
+      // more new tokens than tokens)
       auto most = [&](int32_t max_new) {
-        const int64_t by_request = (int64_t)d->n_requests * ((max_new + l.rows - 1) / l.rows);
+        const int64_t new_rows = max_new < b->max_len ? max_new : b->max_len;
+        const int64_t by_request = d->n_requests * ((new_rows + l.rows - 1) / l.rows);
         const int64_t by_rows = d->t / l.rows + (int64_t)d->n_requests;
         return by_request < by_rows ? by_request : by_rows;
       };

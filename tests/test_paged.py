@@ -1315,3 +1315,17 @@ def test_tables_outputs_that_cut_their_inputs_are_refused(cev):
         bad = list(args)
         bad[i] = at(where)
         assert _abi.lib().cev_paged_tables(*bad) == -1 and b"overlaps" in _abi.lib().cev_last_error(), (i, where)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(d=256), dict(dtype=_abi.CEV_F32), dict(hq=16), dict(requests=4096)])
+def test_work_size_of_the_most_tokens(cev, kw):
+    """Up to 2^31 - 1 rows: the size counts the rows that the requests' pages hold, and never wraps."""
+    sizes = []
+    for t in (1, 9, 160, 161, 10 ** 6, 2 ** 31 - 256, 2 ** 31 - 1):
+        rc, n = _work_size(_paged_desc(t=t, **kw))
+        assert rc == 0
+        sizes.append(n)
+    # (up to t / rows + requests tiles: at t = 160 that is fewer than a tile's worth for every request)
+    assert sizes == sorted(sizes) and sizes[4] == sizes[-1] < 1 << 30
+    # pages for many more keys: too many tiles of them
+    assert _work_size(_paged_desc(t=2 ** 31 - 1, max_pages=(2 ** 31 - 1025) // 16, n_pages=1 << 27, **kw))[0] == -2
