@@ -444,7 +444,7 @@ PyObject* py_paged_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
                   mp = fits_i32(me, "pages of a request", bt.size(1)), mt = fits_i32(me, "tokens", pos.size(0));
     call([&] {
       return api.paged_tables(r32, ps, np, mp, mt, (const int32_t*)ptr(len), (const int32_t*)ptr(add), (int32_t*)ptr(bt), stride,
-                              (int32_t*)ptr(free), (const int32_t*)ptr(ring), (int32_t*)ptr(len_out), (int32_t*)ptr(ring_out),
+                              (int32_t*)ptr(free), (int32_t*)ptr(ring), (int32_t*)ptr(len_out), (int32_t*)ptr(ring_out),
                               (int32_t*)ptr(cu), (int32_t*)ptr(pos), (int32_t*)ptr(slots), s);
     });
   });
