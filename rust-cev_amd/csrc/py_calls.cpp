@@ -437,11 +437,11 @@ PyObject* py_paged_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t n_pages = as_int(a[7]), page_size = as_int(a[3]);
     want_i32(me, "free", free, n_pages);
     const int64_t stride = block_table_stride(me, bt, R);
+    const int32_t r32 = fits_i32(me, "requests", R), ps = fits_i32(me, "page_size", page_size), np = fits_i32(me, "n_pages", n_pages),
+                  mp = fits_i32(me, "pages of a request", bt.size(1)), mt = fits_i32(me, "tokens", pos.size(0));
     const OnDevice dev(me, {{"lengths", &len}, {"new_len", &add}, {"block_table", &bt}, {"cu", &cu}, {"pos", &pos}, {"slots", &slots},
                             {"ring", &ring}, {"lengths_out", &len_out}, {"ring_out", &ring_out}, {"free", free}});
     void* const s = dev.stream(a[12]);
-    const int32_t r32 = fits_i32(me, "requests", R), ps = fits_i32(me, "page_size", page_size), np = fits_i32(me, "n_pages", n_pages),
-                  mp = fits_i32(me, "pages of a request", bt.size(1)), mt = fits_i32(me, "tokens", pos.size(0));
     call([&] {
       return api.paged_tables(r32, ps, np, mp, mt, (const int32_t*)ptr(len), (const int32_t*)ptr(add), (int32_t*)ptr(bt), stride,
                               (int32_t*)ptr(free), (int32_t*)ptr(ring), (int32_t*)ptr(len_out), (int32_t*)ptr(ring_out),

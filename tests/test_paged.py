@@ -1329,3 +1329,53 @@ def test_work_size_of_the_most_tokens(cev, kw):
     assert sizes == sorted(sizes) and sizes[4] == sizes[-1] < 1 << 30
     # pages for many more keys: too many tiles of them
     assert _work_size(_paged_desc(t=2 ** 31 - 1, max_pages=(2 ** 31 - 1025) // 16, n_pages=1 << 27, **kw))[0] == -2
+
+
+@pytest.mark.parametrize("name,bad,says", [
+    ("lengths", ("i", 3, 1), "lengths must be int32"), ("lengths", ("long", 3), "lengths must be contiguous int32 of 3"),
+    ("lengths", ("i", 4), "new_len must be contiguous int32 of 4"), ("lengths", ("half", 3), "lengths must be contiguous"),
+    ("new_len", ("i", 2), "new_len must be contiguous int32 of 3"), ("new_len", ("long", 3), "new_len must be contiguous"),
+    ("block_table", ("i", 2, 4), r"block_table must be int32 \(3, pages\)"), ("block_table", ("i", 3, 0), "block_table must be"),
+    ("block_table", ("half", 3, 4), "block_table must be"), ("block_table", ("long", 3, 4), "block_table must be"), ("block_table", ("i", 12), "block_table must be"),
+    ("cu", ("i", 3), "cu must be contiguous int32 of 4"), ("cu", ("half", 4), "cu must be contiguous"), ("pos", ("half", 10), "pos must be contiguous"),
+    ("pos", ("i", 10, 1), "pos must be int32"), ("pos", ("i", 9), "slots must be contiguous int32 of 9"), ("slots", ("i", 9), "slots must be contiguous int32 of 10"),
+    ("slots", ("long", 10), "slots must be contiguous"), ("ring", ("i", 3), "ring must be contiguous int32 of 4"), ("ring", ("long", 4), "ring must be contiguous"),
+    ("free", ("long", 20), "free must be contiguous int32 of 20"), ("free", ("half", 20), "free must be contiguous"), ("n_pages", 19, "free must be contiguous int32 of 19"),
+    ("lengths_out", ("i", 4), "lengths_out must be contiguous int32 of 3"), ("ring_out", ("i", 5), "ring_out must be contiguous int32 of 4"),
+    ("page_size", 1 << 40, "page_size 1099511627776 does not fit 32 bits"), ("page_size", -(1 << 31) - 1, "page_size .* does not fit"),
+    ("ring", None, "ring is required"), ("free", None, "n_pages is required"), ("none", 0, "lengths must be on the GPU")])
+def test_paged_tables_says_which_argument_it_refuses(cev, name, bad, says):
+    """The message names the argument: a refusal for another reason (the tensors are on the CPU) is none."""
+    import torch
+
+    def tensor(kind, *shape):
+        x = torch.zeros(*shape[:-1], shape[-1] * 2, dtype=torch.int64 if kind == "long" else torch.int32)
+        return x[..., ::2] if kind == "half" else x[..., : shape[-1]].contiguous()
+    args = dict(page_size=16)
+    for k, shape in dict(lengths=(3,), new_len=(3,), block_table=(3, 4), cu=(4,), pos=(10,), slots=(10,), free=(20,), ring=(4,)).items():
+        args[k] = tensor("i", *shape)
+    if name != "none":
+        args[name] = tensor(*bad) if isinstance(bad, tuple) else bad
+    with pytest.raises(CevError, match=says) as e:
+        cev.paged_tables(**args)
+    assert e.value.code == -1
+
+
+def test_more_pages_than_32_bits_number(cev):
+    """Refused by their count, before the tensors' device is looked at."""
+    import torch
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(CevError, match="n_pages 4294967296 does not fit 32 bits") as e:
+        cev.paged_tables(i(3), i(3), i(3, 4), 16, i(4), i(10), i(10), ring=i(4), n_pages=1 << 32)
+    assert e.value.code == -1
+
+
+@pytest.mark.parametrize("change,says", [
+    (dict(window=1 << 32), "window 4294967296 does not fit 32 bits"), (dict(max_new=6), "max_new 6"), (dict(max_new=0), "max_new 0"),
+    (dict(max_new=(1 << 32) + 1), "max_new 4294967297 does not fit"), (dict(sinks=3), "first tokens that stay visible need a window"),
+    (dict(window=-1), "window -1"), (dict(scale=0.0), "scale must be"), (dict(scale=math.inf), "scale must be"), (dict(sinks=-(1 << 40)), "sinks .* does not fit")])
+def test_paged_attention_says_which_argument_it_refuses(cev, change, says):
+    import torch
+    with pytest.raises(CevError, match=says) as e:
+        cev.PagedAttention(torch.zeros(5, 4, 128), torch.zeros(3, 16, 2, 128), torch.zeros(2, 4, dtype=torch.int32), **change)
+    assert e.value.code == -1
