@@ -520,7 +520,8 @@ int32_t cev_paged_plan(const cev_paged_desc* d, const int32_t* cu, const int32_t
 
 /* The attention over one layer's caches.  d may differ from the plan's in
  * its strides and scale only; with any other plan in `work` every row of out
- * is NaN, and a row that sees a page outside [0, n_pages) is NaN. */
+ * is NaN, and a row that sees a page outside [0, n_pages) is NaN (the rows
+ * before it, and those that have left it behind their window, are not). */
 int32_t cev_paged_attention(const cev_paged_desc* d, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
                             void* out, void* work, size_t work_bytes, cev_stream stream);
 

@@ -223,7 +223,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     page_a = bt[min(j >> a.page_shift, a.max_pages - 1)];
     page_b = bt[min((j + 16) >> a.page_shift, a.max_pages - 1)];
   };
-  bool bad_page = false;
+  bool sees_bad = false;  // this lane's row sees a key of a page outside the cache
   char* const ring = lds + wave * 2 * kTile;
   const int lds_ring = (int)(size_t)(const __attribute__((address_space(3))) char*)ring;
   // Row (of load 0 of a half) and block there of this lane's 16 bytes.
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       const bool seen = real && first < span.end && !(first >= span.skip_lo && first + 16 <= span.skip_hi);
       int page = half ? __builtin_amdgcn_readlane(page_b, l) : __builtin_amdgcn_readlane(page_a, l);
       const bool in = (uint32_t)page < (uint32_t)a.n_pages;
-      bad_page |= seen && !in;
+      if (which == 0 && seen && !in) sees_bad |= (first <= pos) & ((a.window == 0) | (first + 15 > pos - a.window) | (first < a.sinks));
       page = in ? page : 0;
       const uint64_t base = (which ? vbase : kbase) + (uint64_t)(page * page_bytes) + (uint64_t)((first & ((1 << a.page_shift) - 1)) * (int64_t)stride);
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)uniform_u64(base), (short)0, uniform_i32(seen && in ? 16 * stride : 0), kBufferWord3);
@@ -566,7 +566,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   }
 
   // ---- join the waves' partial results through LDS
-  const float l = pair_sum(l_run) + (bad_page ? __builtin_nanf("") : 0.0f);
+  const float l = pair_sum(l_run) + (sees_bad ? __builtin_nanf("") : 0.0f);
   __syncthreads();  // every wave is done with its part of the ring
   float* const ob = (float*)lds;
 #pragma unroll

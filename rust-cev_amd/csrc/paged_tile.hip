@@ -533,7 +533,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
       }
     }
-    float l = pair_sum(l_run) + (*(volatile int32_t*)&bad_s ? __builtin_nanf("") : 0.0f);
+    float l = pair_sum(l_run);
+    if (*(volatile int32_t*)&bad_s && wave_active) {
+      // a page outside the cache makes the rows NaN that see it
+#pragma unroll 1
+      for (int i = 0; i < nc; ++i)
+#pragma unroll 1
+        for (int key = first_key(i), k = 0; k < kKeys / 16; ++k, key += 16) {
+          if (key >= span.end || (key >= span.skip_lo && key + 16 <= span.skip_hi)) continue;
+          const bool bad = (uint32_t)bt[key >> a.page_shift] >= (uint32_t)a.n_pages;
+          const bool vis = (key <= pos) & ((a.window == 0) | (key + 15 > pos - a.window) | (key < a.sinks));
+          l += (bad & vis) ? __builtin_nanf("") : 0.0f;
+        }
+    }
 
     bool write = row_ok;
     const bool split = it.n_pieces > 1;

@@ -1379,3 +1379,35 @@ def test_paged_attention_says_which_argument_it_refuses(cev, change, says):
     with pytest.raises(CevError, match=says) as e:
         cev.PagedAttention(torch.zeros(5, 4, 128), torch.zeros(3, 16, 2, 128), torch.zeros(2, 4, dtype=torch.int32), **change)
     assert e.value.code == -1
+
+
+def _rows_that_see(p, r, page, window, sinks):
+    """Which of request r's new rows see a key of the page-th entry of its table."""
+    rows = range(p.past[r], p.past[r] + p.new[r])
+    keys = lambda at: range(page * p.page, min((page + 1) * p.page, at + 1))  # noqa: E731
+    return [any(not window or j > at - window or j < sinks for j in keys(at)) for at in rows]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("many,kind,hq,hkv,d", [(False, *x) for x in SHAPES] + [(True, *x) for x in MANY_SHAPES])
+@pytest.mark.parametrize("page,window,sinks", [(16, 0, 0), (16, 20, 3), (32, 40, 33), (64, 50, 0)])
+def test_a_page_outside_makes_the_rows_nan_that_see_it(gpu, many, kind, hq, hkv, d, page, window, sinks):
+    """Rows of the same request before such a page, and those that have left it behind their window, are as without it."""
+    import torch
+    kw = dict(window=window, sinks=sinks) if window else {}
+    past, new = [30, 0, 200], [150, 33, 9]
+    p = _Many(gpu, past, new, hq, hkv, d, kind, page, seed=8, window=window) if many else _Paged(gpu, past, new, hq, hkv, d, kind, page, seed=8)
+    want = p.run(**kw)
+    for r, entry, value in ((0, 5, -1), (0, 0, p.n_pages), (1, 1, 2 ** 31 - 1), (2, 0, -(2 ** 31)), (2, 200 // page, p.n_pages)):
+        if entry * page >= past[r] + new[r]:
+            continue
+        old = int(p.table[r, entry])
+        p.table[r, entry] = value
+        out = p.run(**kw)
+        p.table[r, entry] = old
+        bad = torch.zeros(p.t, dtype=torch.bool, device=gpu)
+        at = sum(new[:r])
+        bad[at: at + new[r]] = torch.tensor(_rows_that_see(p, r, entry, window, sinks), device=gpu)
+        assert bool(out[bad].isnan().all()), (r, entry)
+        assert torch.equal(out[~bad], want[~bad]), (r, entry)
+        assert 0 < int(bad.sum()) < p.t or window
