@@ -477,7 +477,8 @@ int32_t cev_rope(const cev_rope_desc* d, const void* q_in, const void* k_in, con
  * sinks).  lengths include the new tokens, whose k and v are in the cache
  * already.  Rows of no request are left as they were.  Pages that no row
  * sees (behind a window) are not read and may have been given back; requests
- * may share pages.  out may be q with the same strides; rows of out do not
+ * may share pages.  Infinities and NaN of v reach the rows that see them and no
+ * others: their column is the sum of all of them, whatever their weights.  out may be q with the same strides; rows of out do not
  * overlap.  A stride over one row counts for nothing. */
 typedef struct {
   int32_t dtype;      /* CEV_F32 or CEV_BF16: q, k, v, out */

@@ -155,7 +155,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   // moved to and from the accumulation registers, and some of it spilled).
   constexpr bool kQInLds = BF && D == 256;
   __shared__ __align__(16) char lds[kBody + (kQInLds ? D / 16 * 1024 : 0)];
-  __shared__ float2 ml[kWaves * 32];
+  __shared__ float2 ml[kWaves * 32];  // of a slot: maximum, sum; below zero (or -0) with odd_v
   __shared__ int32_t last_s;
 
   const int run = blockIdx.x / (uint32_t)a.hkv, kvh = blockIdx.x - run * a.hkv;
@@ -293,10 +293,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       voff[dt] = BF ? (4 * u + rr) * kRB + (v_place<T>(4 * dt + blk, rr) << 4) + 8 * (i & 1)
                     : 4 * u * kRB + (v_place<T>(8 * dt + n / 4, 4 * u) << 4) + 4 * (n & 3);
   }
-  // A value of V.
-  auto v_at = [&](int key, int col) -> T* {
-    return (T*)(ring + kTile + key * kRB + (v_place<T>(col * (int)sizeof(T) / 16, key) << 4)) + col % (16 / (int)sizeof(T));
+  // Whether the rows differ in what they see of the sub-tile at key0.
+  auto is_masked = [&](int key0) {
+    return key0 + kKeys - 1 > it.pos0 || (a.window > 0 && key0 <= pos1 - a.window && key0 + kKeys > a.sinks);
   };
+  bool odd_v = false;  // such a sub-tile's V held infinities or NaN
 
   // This wave's sub-tiles.  f32: an infinite value (or one above bf16's range)
   // has no parts; a wave that ends with anything non-finite walks its keys again
@@ -397,9 +398,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
         });
       }
       asm volatile("" ::: "memory");
-      const bool masked = key0 + kKeys - 1 > it.pos0 ||
-                          (a.window > 0 && key0 <= pos1 - a.window && key0 + kKeys > a.sinks);
-      auto visible = [&](int key) { return (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.sinks)); };
+      const bool masked = is_masked(key0);
       if (masked) {
         // bounds of the register's place, 8 (i / 4) + i % 4
         const int k0 = key0 + 4 * (fresh_lane_id() >> 5), hi = pos - k0;
@@ -435,8 +434,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
       asm volatile("" ::: "memory");
       if (masked) {
         // 0 times an infinity or NaN is NaN: a key that only some of the rows
-        // see must not reach the others.  Such values are added to the rows
-        // that see them (whatever their weight) and are zeros for the products.
+        // see must not reach the others.  Such values are zeros for the products;
+        // the rows that see them get them when the waves' results are joined.
         const f32x4* const vt = (const f32x4*)(ring + kTile);
         uint32_t odd = 0;
 #pragma unroll
@@ -450,18 +449,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
           }
         }
         if (__ballot(odd != 0)) {
-#pragma unroll 1
-          for (int kk = 0; kk < kKeys; ++kk) {
-            const bool vis = visible(key0 + kk);
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float v = (float)*v_at(kk, 32 * dt + 8 * (i >> 2) + 4 * u + (i & 3));
-                const bool finite = (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u;
-                o[dt][i] += (finite | !vis) ? 0.0f : v;
-              }
-          }
+          odd_v = true;
           wave_lds_sync();
           for (int i = lane; i < kKeys * D; i += 64) {
             T* const x = (T*)(ring + kTile) + i;
@@ -574,7 +562,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4)
       *(f32x4*)(ob + (wave * 32 + n) * RS + dt * 32 + 8 * q4 + 4 * u) = f32x4{o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]};
-  if (u == 0) ml[wave * 32 + n] = make_float2(m_run, l);
+  if (u == 0) ml[wave * 32 + n] = make_float2(m_run, odd_v ? -l : l);
   __syncthreads();
   const int slots = it.n_rows << gs;
   constexpr int kCols = D / 4;  // 4-column units of a slot
@@ -593,8 +581,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     for (int e = 0; e < 4; ++e) v[e] = L == 0.0f ? 0.0f : x[e] / L;
     store_vec4<T>(op, v);
   };
+  auto put_odd = [&](int slot, int col, uint32_t up, uint32_t down) {
+    T* const op = (T*)a.out + (int64_t)(it.row0 + (slot >> gs)) * a.o_st + (int64_t)(kvh * a.g + (slot & (a.g - 1))) * a.o_sh + col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if ((up | down) >> e & 1) op[e] = (T)odd_or(0.0f, 1u << e, up, down);
+  };
   const __amdgpu_buffer_rsrc_t mine = record(it.piece);
   const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc((void*)uniform_u64((uint64_t)rec0), (short)0, uniform_i32(it.n_pieces * a.hkv * kRec * 4), kBufferWord3);
+  bool odd = false, odd_masked = false;
   for (int i = tid; i < slots * kCols; i += kThreads) {
     const int slot = i / kCols, col = 4 * (i % kCols);
     float M = -INFINITY, L = 0.0f;
@@ -605,14 +600,55 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     for (int w = 0; w < kWaves; ++w) {
       const float2 v = ml[w * 32 + slot];
       const float f = fast_exp2(v.x - M);
-      L += f * v.y;
+      L += f * __builtin_fabsf(v.y);
+      odd_masked |= __builtin_signbitf(v.y) != 0;
       x += f * *(const f32x4*)(ob + (w * 32 + slot) * RS + col);
     }
+    odd |= (L == L) & !finite4(x);
     if (!split) {
       put(slot, col, x, L);
     } else {
       put_past_l2(mine, (slot * D + col) * 4, x);
       if (col == 0) put_past_l2(mine, (kSlots * D + 2 * slot) * 4, make_float2(M, L));
+    }
+  }
+  // Infinities and NaN of V (see note_odd): the sub-tiles whose rows differ in what
+  // they see held some, or a row has come out so.  They go over what was written
+  // (in the loop above they took it 0.4 us).
+  if (__any(odd | odd_masked)) {
+    const bool every = __any(odd);
+    __builtin_amdgcn_s_waitcnt(0);
+#pragma unroll 1
+    for (int i = tid; i < slots * kCols; i += kThreads) {
+      const int slot = i / kCols, col = 4 * (i % kCols), row_pos = it.pos0 + (slot >> gs);
+      uint32_t up = 0, down = 0;
+#pragma unroll 1
+      for (int c = it.c_begin; c < c_end; ++c) {
+        if (!every && !is_masked(first_key(c))) continue;
+#pragma unroll 1
+        for (int first = first_key(c), half = 0; half < 2; ++half, first += 16) {
+          if (first >= span.end || (first >= span.skip_lo && first + 16 <= span.skip_hi)) continue;
+          const int page = bt[first >> a.page_shift];
+          if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
+          const T* const v = (const T*)(vbase + sizeof(T) * (uint64_t)(page * a.vc_sp + (first & ((1 << a.page_shift) - 1)) * a.vc_st)) + col;
+#pragma unroll 4
+          for (int k = 0; k < 16; ++k) {
+            const int key = first + k;
+            const bool vis = (key <= row_pos) & ((a.window == 0) | (key > row_pos - a.window) | (key < a.sinks));
+            typedef T vec4 __attribute__((ext_vector_type(4)));
+            const vec4 y = *(const vec4*)(v + k * a.vc_st);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) note_odd((float)y[e], vis, 1u << e, up, down);
+          }
+        }
+      }
+      bool nan_row = false;
+      for (int w = 0; w < kWaves; ++w) nan_row |= ml[w * 32 + slot].y != ml[w * 32 + slot].y;
+      if (nan_row) continue;
+      if (!split) put_odd(slot, col, up, down);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (split && ((up | down) >> e & 1)) put_past_l2(mine, (slot * D + col + e) * 4, odd_or(0.0f, 1u << e, up, down));
     }
   }
   // A split tile's stores have reached memory before the workgroup counts
@@ -637,6 +673,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
   const int units = slots * kCols;
   int groups = 1;
   while (groups < 8 && 2 * groups * units <= kThreads && 2 * groups < it.n_pieces) groups *= 2;
+  odd = false;
   const int group = groups > 1 ? tid / units : 0, unit0 = groups > 1 ? tid % units : tid;
   for (int i0 = 0; i0 < units; i0 += kUnits * kThreads) {
     float M[kUnits], L[kUnits];
@@ -676,10 +713,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
 #pragma unroll
           for (int b = 0; b < kBatch; ++b) {
             const float f = p0 + b * groups < it.n_pieces ? fast_exp2(w[k][b].x - m) : 0.0f;
-            if (f > 0.0f || w[k][b].y != w[k][b].y) {
-              L[k] += f * w[k][b].y;
-              x[k] += f * y[k][b];
-            }
+            L[k] += f * w[k][b].y;
+            x[k] += f * y[k][b];
           }
         }
       }
@@ -703,8 +738,30 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kMinWa
     }
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
-      const int unit = i0 + unit0 + k * kThreads;
-      if (group == 0 && unit < units) put(unit / kCols, 4 * (unit % kCols), x[k], L[k]);
+      const int unit = i0 + unit0 + k * kThreads, slot = unit / kCols, col = 4 * (unit % kCols);
+      if (group == 0 && unit < units) {
+        odd |= (L[k] == L[k]) & !finite4(x[k]);
+        put(slot, col, x[k], L[k]);
+      }
+    }
+  }
+  if (__any(odd)) {  // (the weight of a piece that has such a sum may be 0)
+    __builtin_amdgcn_s_waitcnt(0);
+#pragma unroll 1
+    for (int unit = unit0; group == 0 && unit < units; unit += kThreads) {
+      const int slot = unit / kCols, col = 4 * (unit % kCols);
+      uint32_t up = 0, down = 0;
+      bool nan_row = false;
+#pragma unroll 1
+      for (int p = 0; p < it.n_pieces; ++p) {
+        const int at = p * (int)(a.hkv * kRec * 4);
+        const f32x4 y = get4_past_l2(all, at + (slot * D + col) * 4);
+        const float l_piece = get2_past_l2(all, at + (kSlots * D + 2 * slot) * 4).y;
+        nan_row |= l_piece != l_piece;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) note_odd(y[e], true, 1u << e, up, down);
+      }
+      if (!nan_row) put_odd(slot, col, up, down);
     }
   }
   __syncthreads();

@@ -45,11 +45,33 @@ __device__ __forceinline__ void put_past_l2(__amdgpu_buffer_rsrc_t rs, int at, c
 __device__ __forceinline__ void put_past_l2(__amdgpu_buffer_rsrc_t rs, int at, const float2& v) {
   __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(decltype(__builtin_amdgcn_raw_buffer_load_b64(rs, 0, 0, 0)), v), rs, at, 0, kPastL2);
 }
+__device__ __forceinline__ void put_past_l2(__amdgpu_buffer_rsrc_t rs, int at, float v) {
+  __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(decltype(__builtin_amdgcn_raw_buffer_load_b32(rs, 0, 0, 0)), v), rs, at, 0, kPastL2);
+}
 __device__ __forceinline__ f32x4 get4_past_l2(__amdgpu_buffer_rsrc_t rs, int at, int scalar_at = 0) {
   return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at, scalar_at, kPastL2));
 }
 __device__ __forceinline__ float2 get2_past_l2(__amdgpu_buffer_rsrc_t rs, int at) {
   return __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, kPastL2));
+}
+
+// An infinity or NaN of V makes its column of every row that sees it the sum of all
+// such values, whatever their weights.  (A weight may come out as 0, for which the
+// products have NaN, and which weights do depends on how the keys were shared out.)
+// The kernels keep what they have found of a value's sum as a bit of `up` (+inf) and
+// one of `down` (-inf), both for NaN.
+__device__ __forceinline__ void note_odd(float x, bool seen, uint32_t bit, uint32_t& up, uint32_t& down) {
+  const bool odd = seen & !__builtin_isfinite(x);
+  up |= (odd & !(x < 0.0f)) ? bit : 0u;
+  down |= (odd & !(x > 0.0f)) ? bit : 0u;
+}
+// x, or the sum that was found.
+__device__ __forceinline__ float odd_or(float x, uint32_t bit, uint32_t up, uint32_t down) {
+  x = (down & bit) ? -INFINITY : x;
+  return (up & bit) ? ((down & bit) ? __builtin_nanf("") : INFINITY) : x;
+}
+__device__ __forceinline__ bool finite4(const f32x4& x) {
+  return __builtin_isfinite(x[0]) & __builtin_isfinite(x[1]) & __builtin_isfinite(x[2]) & __builtin_isfinite(x[3]);
 }
 
 }  // namespace

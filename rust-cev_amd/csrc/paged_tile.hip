@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     bool bad_page = false;
     auto load_pages = [&](int i) {
       batch_first = i;
-      const int key0 = first_key(min(i + lane, nc - 1)) + kRows * wave;
+      const int key0 = first_key(min(i + fresh_lane_id(), nc - 1)) + kRows * wave;
       // (the last chunk may reach beyond the block table's last page)
       int page = bt[min(key0 >> a.page_shift, a.max_pages - 1)];
       // rows that some row of the tile sees
@@ -200,10 +200,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)vp, (short)0, rows * vr, kBufferWord3);
       int ka[2] = {kat[0], kat[1]}, va[2] = {vat[0], vat[1]};
       if (i >= t_hi || i < t_lo) {  // it may hold keys that no row sees
-        const int key0 = (real ? first_key(i) : 0) + kRows * wave;
+        const int key0 = (real ? first_key(i) : 0) + kRows * wave + fresh_lane_id() / kBlk;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int key = key0 + kLoadRows * r + lane / kBlk;
+          const int key = key0 + kLoadRows * r;
           const bool load = key < span.end && !(key >= span.skip_lo && key < span.skip_hi);
           ka[r] = load ? ka[r] : INT32_MAX;
           va[r] = load ? va[r] : INT32_MAX;
@@ -221,10 +221,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     // 0 times an infinity or NaN is NaN: a key that only some of the rows see
     // must not reach the others.  Where the rows differ in what they see of chunk
     // i, such values among the V rows that this wave fetched (landed by now)
-    // become zeros; after the loop they are added to the rows that see them.
+    // become zeros; after the loop the rows that see them get them.
     auto clean = [&](int i) {
       if (i >= nc || (i >= t_lo && i < t_hi)) return;
-      const int at = kVBase + i % kBuf * kTileBytes + kRows * wave * kRowBytes + lane * 16;
+      const int lane = fresh_lane_id(), at = kVBase + i % kBuf * kTileBytes + kRows * wave * kRowBytes + lane * 16;
       i32x4* const v = (i32x4*)(lds + at);
       KFrag vr[2] = {read_b128<0>(lds_base + at), read_b128<1024>(lds_base + at)};
       wait_b128<1>(vr[0]);
@@ -258,6 +258,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 
   // Takes the run's next item and asks for its Q, its pages and its first chunks.
   auto begin = [&] {
+    const int lane = fresh_lane_id(), n = lane & 31, u = lane >> 5;
     it = walk.item();
     const int pos1 = it.pos0 + it.n_rows - 1;
     span = paged_span(kKeys, it.pos0, pos1, a.window, a.sinks);
@@ -506,34 +507,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       for (int dt = 0; dt < kVoff; ++dt) voff[dt] -= nc % kBuf * kTileBytes;
     }
 
+    // (computed again here, and held in no register through the loop)
+    const int lane = fresh_lane_id(), n = lane & 31, u = lane >> 5;
+    const bool one = wave == 0 && lane == 0;
     if (bad_page && lane == 0) *(volatile int32_t*)&bad_s = 1;  // one wave's finding
     __syncthreads();
-    if (*(volatile int32_t*)&odd_s && wave_active) {
-#pragma unroll 1
-      for (int i = 0; i < nc; ++i) {
-        if (i >= t_lo && i < t_hi) continue;
-#pragma unroll 1
-        for (int kk = 0; kk < kKeys; ++kk) {
-          const int key = first_key(i) + kk;
-          if (key >= span.end || (key >= span.skip_lo && key < span.skip_hi)) continue;
-          const int page = bt[key >> a.page_shift];
-          if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
-          const __bf16* const v = (const __bf16*)(vbase + 2 * (uint64_t)(page * a.vc_sp + (key & ((1 << a.page_shift) - 1)) * a.vc_st)) + 4 * u;
-          const bool vis = (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.sinks));
-#pragma unroll
-          for (int j = 0; j < 4 * NDT; ++j) {
-            const bf16x4 x = *(const bf16x4*)(v + 32 * (j / 4) + 8 * (j % 4));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float y = (float)x[e];
-              const bool finite = (__float_as_uint(y) & 0x7f800000u) != 0x7f800000u;
-              o[j / 4][4 * (j % 4) + e] += (finite | !vis) ? 0.0f : y;
-            }
-          }
-        }
-      }
-    }
     float l = pair_sum(l_run);
+    // Infinities and NaN of V (see note_odd): the tile's chunks whose rows differ in
+    // what they see held some, or a row has come out so.
+    bool odd_masked = uniform_i32(*(volatile int32_t*)&odd_s);
+    auto odd_rows = [&] {
+      float t[4] = {};
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t[e % 4] = __builtin_fmaf(o[dt][e], 0.0f, t[e % 4]);
+      return __any(row_ok & (l == l) & !((t[0] + t[1]) + (t[2] + t[3]) == 0.0f));
+    };
     if (*(volatile int32_t*)&bad_s && wave_active) {
       // a page outside the cache makes the rows NaN that see it
 #pragma unroll 1
@@ -570,12 +560,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
       int32_t* const counter = (int32_t*)(a.work + a.counters_off) + (int64_t)it.split * a.hkv + kvh;
-      if (tid == 0) {
-        last_s = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.n_pieces - 1;
-        if (last_s) *counter = 0;  // for the next call with this plan
+      if (one) {
+        // (pieces with odd_masked count in the upper half too)
+        const int before = __hip_atomic_fetch_add(counter, odd_masked ? 0x10001 : 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool all = (before & 0xffff) == it.n_pieces - 1;
+        if (all) *counter = 0;  // for the next call with this plan
+        last_s = all ? 1 + (before >> 16) : 0;
       }
       __syncthreads();
-      const bool last = last_s;
+      const int last = uniform_i32(last_s);
+      odd_masked |= last > 1;
       __syncthreads();
       write = write && last;
       // The last one: 64 columns at a time; the next piece is on its way while one is
@@ -618,6 +612,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
       }
     }
+    const bool odd_row = odd_rows();
     // The row's 16-byte vectors: a half wave holds four columns of each eight, and
     // the halves exchange theirs of two vectors.
     i32x4 res[D / 16];
@@ -635,15 +630,55 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       res[w] = i32x4{(int)r0[0], (int)r1[0], (int)r0[1], (int)r1[1]};
     }
     __bf16* const op = (__bf16*)a.out + (int64_t)(it.row0 + ((wave * 32 + n) >> gs)) * a.o_st + (int64_t)(kvh * a.g + (n & (a.g - 1))) * a.o_sh + 8 * u;
-    // The next item's first chunks come while this one's rows are written.
-    lds_barrier();  // every wave has read the flags
-    if (tid == 0) odd_s = bad_s = 0;
-    const bool more = it.next >= 0;
-    if (more) begin();
-    if (write) {
+    auto store = [&] {
 #pragma unroll
       for (int w = 0; w < D / 16; ++w) *(i32x4*)(op + 32 * (w / 2) + 16 * (w % 2)) = res[w];
+    };
+    if (__any(write) && (odd_masked || odd_row)) {
+      // They go over the rows in memory, where O no longer takes registers (changed in
+      // place it cost the loop 100 bytes a lane of scratch).
+      if (write) store();
+      __builtin_amdgcn_s_waitcnt(0);
+#pragma unroll 1
+      for (int w = 0; w < D; w += 64) {
+        uint32_t up = 0, down = 0;  // bit 4 j + e: column w + 8 j + 4 u + e
+#pragma unroll 1
+        for (int i = -it.c_begin; i < span.total - it.c_begin; ++i) {
+          if (!odd_row && i >= t_lo && i < t_hi) continue;
+#pragma unroll 1
+          for (int first = first_key(i), left = kKeys; left > 0; left -= 16, first += 16) {
+            if (first >= span.end || (first >= span.skip_lo && first + 16 <= span.skip_hi)) continue;
+            const int page = bt[first >> a.page_shift];
+            if ((uint32_t)page >= (uint32_t)a.n_pages || !__any(write & ((up & down) != ~0u))) continue;
+            const __bf16* const v = (const __bf16*)(vbase + 2 * (uint64_t)(page * a.vc_sp + (first & ((1 << a.page_shift) - 1)) * a.vc_st)) + w;
+            // sixteen rows' bytes, 32 of a lane; most hold none
+            const bf16x8 x0 = *(const bf16x8*)(v + lane / 8 * a.vc_st + lane % 8 * 8), x1 = *(const bf16x8*)(v + (8 + lane / 8) * a.vc_st + lane % 8 * 8);
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) any |= !__builtin_isfinite((float)x0[e]) | !__builtin_isfinite((float)x1[e]);
+            if (!__any(any)) continue;
+#pragma unroll 1
+            for (int at = 0; at < 16 * 8; ++at) {
+              const int key = first + at / 8;
+              const bool vis = (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.sinks));
+              const bf16x4 x = *(const bf16x4*)(v + at / 8 * a.vc_st + at % 8 * 8 + 4 * u);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) note_odd((float)x[e], vis, 1u << (4 * (at % 8) + e), up, down);
+            }
+          }
+        }
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i, up >>= 1, down >>= 1)
+          if (write & (l == l) & ((up | down) & 1)) (op - 4 * u)[w + 8 * (i / 4) + i % 4] = (__bf16)odd_or(0.0f, 1, up, down);
+      }
+      write = false;
     }
+    // The next item's first chunks come while this one's rows are written.
+    lds_barrier();  // every wave has read the flags
+    if (one) odd_s = bad_s = 0;
+    const bool more = it.next >= 0;
+    if (more) begin();
+    if (write) store();
     if (!more) break;
   }
 }

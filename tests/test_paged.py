@@ -1411,3 +1411,68 @@ def test_a_page_outside_makes_the_rows_nan_that_see_it(gpu, many, kind, hq, hkv,
         assert bool(out[bad].isnan().all()), (r, entry)
         assert torch.equal(out[~bad], want[~bad]), (r, entry)
         assert 0 < int(bad.sum()) < p.t or window
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("many,kind,hq,hkv,d", [(False, *x) for x in SHAPES] + [(True, *x) for x in MANY_SHAPES])
+@pytest.mark.parametrize("past,new,window,sinks", [([900], [40], 0, 0), ([900], [40], 300, 40), ([20011], [3], 0, 0), ([0], [130], 0, 0)])
+def test_infinities_of_v_do_not_depend_on_their_weights(gpu, many, kind, hq, hkv, d, past, new, window, sinks):
+    """Scores of several hundred at one key leave the others weights of 0.  An
+    infinity or NaN among those values still reaches each row that sees it, in
+    masked and unmasked sub-tiles, in pieces of a split request and in either
+    kernel; two infinities of different signs give NaN."""
+    import torch
+    kw = dict(window=window, sinks=sinks) if window else {}
+    p = _Many(gpu, past, new, hq, hkv, d, kind, 16, seed=3, window=window) if many else _Paged(gpu, past, new, hq, hkv, d, kind, 16, seed=3)
+    total, g = past[0] + new[0], hq // hkv
+    big = total - new[0] - 5 if past[0] else 2  # the key that takes all weight of the rows that see it
+    place = lambda j: (int(p.table[0, j // 16]), j % 16)  # noqa: E731
+    p.q[: new[0]] = p.q[: new[0]].sign()
+    p.k[p.table[0, : -(-total // 16)].long()] = 0.0
+    p.k[place(big)] = (25 * p.q[0, ::g].float()).to(p.k.dtype)
+    p.q[: new[0]] = p.q[:1, ::g].repeat_interleave(g, 1)  # every head of a group scores alike
+    rows = torch.arange(past[0], total)
+    sees = lambda j: (j <= rows) & ((window == 0) | (j > rows - window) | (j < sinks))  # noqa: E731
+    values = {0: (math.inf, 3), min(100, total - 3): (-math.inf, 5), total - 20: (math.nan, 7), total - 2: (math.inf, 9), big - 1: (math.inf, 11), big + 1: (-math.inf, 11)}
+    held = {}
+    clean = p.run(**kw)
+    p.check(clean, **kw)
+    for j, (x, col) in values.items():
+        held[j] = p.v[place(j)].clone()
+        p.v[place(j)][hkv - 1, col] = x
+    out = p.run(**kw)
+    want = clean[: new[0]].float().cpu()
+    odd = torch.zeros_like(want)
+    for j, (x, col) in values.items():
+        odd[:, -g:, col] += torch.where(sees(j)[:, None], x, 0.0)
+    got = out[: new[0]].float().cpu()
+    assert bool(((got == odd) | (got.isnan() & odd.isnan()))[odd != 0].all())
+    # (f32 walks keys again on the f32 unit where a row is not finite: within the bound of _Paged.check)
+    _, size, big_score = p.exact(0, **kw)
+    slack = 2.0 ** -18 * (1 + big_score) * size if kind == "f32" else torch.zeros_like(size)
+    assert bool(((got.double() - want.double()).abs() <= slack)[odd == 0].all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,hq,hkv,d", [("bf16", 8, 2, 128), ("bf16", 4, 2, 256), ("f32", 4, 2, 128)])
+def test_sums_that_overflow_stay_infinite(gpu, kind, hq, hkv, d):
+    """Finite values whose sum passes the type: no value that is not finite is there, and the infinity stays."""
+    import torch
+    p = _Paged(gpu, [200], [3], hq, hkv, d, kind, 16, seed=5)
+    p.q.zero_()
+    p.v[..., 4] = 3.0e38
+    out = p.run()
+    assert bool((out[..., 4] == math.inf).all())
+    p.v[..., 4] = out[..., 4] = 0.0
+    p.check(out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("many", [False, True])
+def test_a_cache_of_nan_ends_in_time(gpu, many):
+    """Nothing but NaN in V: every row is NaN, by way of the slow path of every tile."""
+    p = (_Many if many else _Paged)(gpu, [3000, 10], [70, 1], 8, 2, 128, "bf16", 16, seed=5)
+    p.v.fill_(math.nan)
+    att = p.attention()
+    att.plan(p.cu, p.lengths)
+    assert bool(att(p.q, p.k, p.v, p.table).isnan().all())
