@@ -36,7 +36,7 @@ PEAK_HBM_GBPS = 8000.0
 
 # Kernel sources each workload's measured traffic depends on (c1 is a small
 # launch: its attention kernel is fan_attn.hip's).
-K2_SOURCES = ("attn_device.h", "packed_attn.hip")
+K2_SOURCES = ("attn_device.h", "attn_pipe.h", "packed_attn.hip")
 TRAFFIC_SOURCES = {"c5gdn": ("gdn.hip",), "c5gdnrows": ("gdn.hip",), "c1": K2_SOURCES + ("fan_attn.hip",)}
 
 
