@@ -141,7 +141,8 @@ class PagedAttention:
     ones; 0: all.  plan() makes the step's work list from cu and lengths on the
     device; every call until the next plan() uses it.  out may be q.  The object
     is made on the current stream, which other streams wait for as for a
-    tensor; its workspace serves one step at a time."""
+    tensor; its workspace (17 MB for decoding steps, 85 to 152 MB for bf16
+    steps with chunks) serves one step at a time."""
 
     def __init__(self, q, k_cache, block_table, max_new: Optional[int] = None, window: int = 0, sinks: int = 0, scale: Optional[float] = None):
         import torch

@@ -1476,3 +1476,22 @@ def test_a_cache_of_nan_ends_in_time(gpu, many):
     att = p.attention()
     att.plan(p.cu, p.lengths)
     assert bool(att(p.q, p.k, p.v, p.table).isnan().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("many,kind,hq,hkv,d", [(False, *x) for x in SHAPES] + [(True, *x) for x in MANY_SHAPES])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_near_the_largest_that_are_exact(gpu, many, kind, hq, hkv, d, sign):
+    """Equal scores of 2^27.5 (d = 128) or 2^28 (256) in size: a maximum is then off by
+    up to 2^3 in the exponent, the same for all keys of a row, and the rows are means."""
+    import torch
+    p = (_Many if many else _Paged)(gpu, [700], [90], hq, hkv, d, kind, 16, seed=6)
+    p.q.fill_(2.0 ** 12)
+    p.k.fill_(sign * 2.0 ** 12)
+    out = p.run()[:90].double().cpu()
+    v = p.keys(0, p.v).cpu().repeat_interleave(hq // hkv, 1)
+    n = torch.arange(701, 791)[:, None, None]
+    mean, size = v.cumsum(0)[700:] / n, v.abs().cumsum(0)[700:] / n
+    # the weights of a row are equal, to half a step of bf16 where the two lane halves or pieces differ in their factor
+    half = HALF[kind]
+    assert bool(((out - mean).abs() <= (2 * half if kind == "bf16" else 2.0 ** -18) * size + half * mean.abs() * 1.01).all())
