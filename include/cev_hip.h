@@ -516,10 +516,9 @@ int32_t cev_paged_desc_init(cev_paged_desc* d, int32_t dtype, int32_t n_q_heads,
 /* Bytes of the work buffer (host only): the list of work items that
  * cev_paged_plan makes on the device from the lengths, and the partial
  * results of rows whose keys are split over several workgroups (with up to 256
- * KV heads f32 9 MB;
- * bf16 17 MB, with max_new above 32 / (hq / hkv) rows 85 MB at d = 128 and 152
- * MB at d = 256).  16-byte aligned; a plan and the attention calls that use it run one after the
- * other. */
+ * KV heads f32 9 MB; bf16 17 MB, with max_new above 32 / (hq / hkv) rows 85 MB
+ * at d = 128 and 152 MB at d = 256).  16-byte aligned; a plan and the attention
+ * calls that use it run one after the other. */
 int32_t cev_paged_work_size(const cev_paged_desc* d, size_t* bytes);
 
 /* Makes the work list in `work` from cu (n_requests + 1) and lengths

@@ -10,7 +10,9 @@
 constexpr int kPagedMaxRequests = 4096;
 
 // The two kernels and their work lists: requests with few new rows go to the
-// first, those with many to the second (choice in cev_paged_bounds).
+// first, those with many to the second where the plan kernel finds enough work in
+// them (few_work in paged_tables.hip; cev_paged_bounds says whether a shape has a
+// second list at all).
 constexpr int kPagedFew = 0, kPagedMany = 1, kPagedLists = 2;
 // Query slots (rows x heads of a group) of a tile and keys of a sub-tile of heads of d.
 constexpr int paged_slots(int list) { return list == kPagedFew ? 32 : 256; }

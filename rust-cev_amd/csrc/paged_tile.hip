@@ -156,105 +156,105 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   F fr;
   // chunks [it.c_begin, it.c_begin + nc) of the tile's stream
   auto first_key = [&](int i) {
-      const int c = it.c_begin + i;
-      return kKeys * (c < span.sinks ? c : c - span.sinks + span.first);
-    };
-    // Chunks of the part before lo and from hi on hold keys that not all rows
-    // at positions [p0, p1] see (those before lo may also be seen by all).
-    auto unmasked = [&](int p0, int p1, int& lo, int& hi) {
-      // the chunks of the window start at stream place span.sinks; the last key
-      // of the one at place c is first_key + kKeys - 1
-      hi = span.sinks + (p0 + 1) / kKeys - span.first - it.c_begin;
-      lo = 0;
-      if (a.window > 0 && p1 >= a.window) lo = span.sinks + (p1 - a.window) / kKeys + 1 - span.first - it.c_begin;
-    };
-    // Lane l keeps the addresses of this wave's rows of K and of V of chunk 64 b +
-    // l of the current batch b, and whether they are fetched at all.
-    int batch_first = 0, k_lo = 0, k_hi = 0, v_lo = 0, v_hi = 0, fetched = 0;
-    bool bad_page = false;
-    auto load_pages = [&](int i) {
-      batch_first = i;
-      const int key0 = first_key(min(i + fresh_lane_id(), nc - 1)) + kRows * wave;
-      // (the last chunk may reach beyond the block table's last page)
-      int page = bt[min(key0 >> a.page_shift, a.max_pages - 1)];
-      // rows that some row of the tile sees
-      const bool seen = key0 < span.end && !(key0 >= span.skip_lo && key0 + kRows <= span.skip_hi);
-      const bool in = (uint32_t)page < (uint32_t)a.n_pages;
-      bad_page |= __any(seen && !in);
-      fetched = seen && in ? kRows : 0;
-      page = in ? page : 0;
-      const int64_t off = key0 & ((1 << a.page_shift) - 1);
-      const uint64_t kp = kbase + 2 * (uint64_t)(page * a.kc_sp + off * a.kc_st), vp = vbase + 2 * (uint64_t)(page * a.vc_sp + off * a.vc_st);
-      k_lo = (int)(uint32_t)kp, k_hi = (int)(uint32_t)(kp >> 32);
-      v_lo = (int)(uint32_t)vp, v_hi = (int)(uint32_t)(vp >> 32);
-    };
-    // Chunk i into its buffer, i mod kBuf; past the end: zeros.
-    auto fetch = [&](int i) {
-      const bool real = i < nc;
-      if (real && i >= batch_first + 64) load_pages(i);
-      const int l = real ? i - batch_first : 0;
-      const int rows = real ? __builtin_amdgcn_readlane(fetched, l) : 0;
-      const uint64_t kp = (uint32_t)__builtin_amdgcn_readlane(k_lo, l) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(k_hi, l) << 32;
-      const uint64_t vp = (uint32_t)__builtin_amdgcn_readlane(v_lo, l) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(v_hi, l) << 32;
-      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)kp, (short)0, rows * kr, kBufferWord3);
-      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)vp, (short)0, rows * vr, kBufferWord3);
-      int ka[2] = {kat[0], kat[1]}, va[2] = {vat[0], vat[1]};
-      if (i >= t_hi || i < t_lo) {  // it may hold keys that no row sees
-        const int key0 = (real ? first_key(i) : 0) + kRows * wave + fresh_lane_id() / kBlk;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int key = key0 + kLoadRows * r;
-          const bool load = key < span.end && !(key >= span.skip_lo && key < span.skip_hi);
-          ka[r] = load ? ka[r] : INT32_MAX;
-          va[r] = load ? va[r] : INT32_MAX;
-        }
-      }
-      char* const dst = lds + i % kBuf * kTileBytes + kRows * wave * kRowBytes;
+    const int c = it.c_begin + i;
+    return kKeys * (c < span.sinks ? c : c - span.sinks + span.first);
+  };
+  // Chunks of the part before lo and from hi on hold keys that not all rows
+  // at positions [p0, p1] see (those before lo may also be seen by all).
+  auto unmasked = [&](int p0, int p1, int& lo, int& hi) {
+    // the chunks of the window start at stream place span.sinks; the last key
+    // of the one at place c is first_key + kKeys - 1
+    hi = span.sinks + (p0 + 1) / kKeys - span.first - it.c_begin;
+    lo = 0;
+    if (a.window > 0 && p1 >= a.window) lo = span.sinks + (p1 - a.window) / kKeys + 1 - span.first - it.c_begin;
+  };
+  // Lane l keeps the addresses of this wave's rows of K and of V of chunk 64 b +
+  // l of the current batch b, and whether they are fetched at all.
+  int batch_first = 0, k_lo = 0, k_hi = 0, v_lo = 0, v_hi = 0, fetched = 0;
+  bool bad_page = false;
+  auto load_pages = [&](int i) {
+    batch_first = i;
+    const int key0 = first_key(min(i + fresh_lane_id(), nc - 1)) + kRows * wave;
+    // (the last chunk may reach beyond the block table's last page)
+    int page = bt[min(key0 >> a.page_shift, a.max_pages - 1)];
+    // rows that some row of the tile sees
+    const bool seen = key0 < span.end && !(key0 >= span.skip_lo && key0 + kRows <= span.skip_hi);
+    const bool in = (uint32_t)page < (uint32_t)a.n_pages;
+    bad_page |= __any(seen && !in);
+    fetched = seen && in ? kRows : 0;
+    page = in ? page : 0;
+    const int64_t off = key0 & ((1 << a.page_shift) - 1);
+    const uint64_t kp = kbase + 2 * (uint64_t)(page * a.kc_sp + off * a.kc_st), vp = vbase + 2 * (uint64_t)(page * a.vc_sp + off * a.vc_st);
+    k_lo = (int)(uint32_t)kp, k_hi = (int)(uint32_t)(kp >> 32);
+    v_lo = (int)(uint32_t)vp, v_hi = (int)(uint32_t)(vp >> 32);
+  };
+  // Chunk i into its buffer, i mod kBuf; past the end: zeros.
+  auto fetch = [&](int i) {
+    const bool real = i < nc;
+    if (real && i >= batch_first + 64) load_pages(i);
+    const int l = real ? i - batch_first : 0;
+    const int rows = real ? __builtin_amdgcn_readlane(fetched, l) : 0;
+    const uint64_t kp = (uint32_t)__builtin_amdgcn_readlane(k_lo, l) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(k_hi, l) << 32;
+    const uint64_t vp = (uint32_t)__builtin_amdgcn_readlane(v_lo, l) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(v_hi, l) << 32;
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)kp, (short)0, rows * kr, kBufferWord3);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)vp, (short)0, rows * vr, kBufferWord3);
+    int ka[2] = {kat[0], kat[1]}, va[2] = {vat[0], vat[1]};
+    if (i >= t_hi || i < t_lo) {  // it may hold keys that no row sees
+      const int key0 = (real ? first_key(i) : 0) + kRows * wave + fresh_lane_id() / kBlk;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)(dst + 1024 * r), 16, ka[r], 0, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(dst + kVBase + 1024 * r), 16, va[r], 0, 0, 0);
+        const int key = key0 + kLoadRows * r;
+        const bool load = key < span.end && !(key >= span.skip_lo && key < span.skip_hi);
+        ka[r] = load ? ka[r] : INT32_MAX;
+        va[r] = load ? va[r] : INT32_MAX;
       }
-    };
-    constexpr int kLoadsPerChunk = 4;
+    }
+    char* const dst = lds + i % kBuf * kTileBytes + kRows * wave * kRowBytes;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)(dst + 1024 * r), 16, ka[r], 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(dst + kVBase + 1024 * r), 16, va[r], 0, 0, 0);
+    }
+  };
+  constexpr int kLoadsPerChunk = 4;
 
-    // 0 times an infinity or NaN is NaN: a key that only some of the rows see
-    // must not reach the others.  Where the rows differ in what they see of chunk
-    // i, such values among the V rows that this wave fetched (landed by now)
-    // become zeros; after the loop the rows that see them get them.
-    auto clean = [&](int i) {
-      if (i >= nc || (i >= t_lo && i < t_hi)) return;
-      const int lane = fresh_lane_id(), at = kVBase + i % kBuf * kTileBytes + kRows * wave * kRowBytes + lane * 16;
-      i32x4* const v = (i32x4*)(lds + at);
-      KFrag vr[2] = {read_b128<0>(lds_base + at), read_b128<1024>(lds_base + at)};
-      wait_b128<1>(vr[0]);
-      wait_b128<0>(vr[1]);
-      bool odd = false;
+  // 0 times an infinity or NaN is NaN: a key that only some of the rows see
+  // must not reach the others.  Where the rows differ in what they see of chunk
+  // i, such values among the V rows that this wave fetched (landed by now)
+  // become zeros; after the loop the rows that see them get them.
+  auto clean = [&](int i) {
+    if (i >= nc || (i >= t_lo && i < t_hi)) return;
+    const int lane = fresh_lane_id(), at = kVBase + i % kBuf * kTileBytes + kRows * wave * kRowBytes + lane * 16;
+    i32x4* const v = (i32x4*)(lds + at);
+    KFrag vr[2] = {read_b128<0>(lds_base + at), read_b128<1024>(lds_base + at)};
+    wait_b128<1>(vr[0]);
+    wait_b128<0>(vr[1]);
+    bool odd = false;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        i32x4 x = __builtin_bit_cast(i32x4, vr[r]);
+    for (int r = 0; r < 2; ++r) {
+      i32x4 x = __builtin_bit_cast(i32x4, vr[r]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool hi = (x[e] & 0x7f800000) == 0x7f800000, lo = (x[e] & 0x7f80) == 0x7f80;
-          odd |= hi | lo;
-          x[e] &= (hi ? 0 : (int)0xffff0000) | (lo ? 0 : 0xffff);
-        }
-        if (odd) v[64 * r] = x;
+      for (int e = 0; e < 4; ++e) {
+        const bool hi = (x[e] & 0x7f800000) == 0x7f800000, lo = (x[e] & 0x7f80) == 0x7f80;
+        odd |= hi | lo;
+        x[e] &= (hi ? 0 : (int)0xffff0000) | (lo ? 0 : 0xffff);
       }
-      if (__ballot(odd) && lane == 0) *(volatile int32_t*)&odd_s = 1;
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    };
-    auto mask_sub = [&](f32x16& s, int key0) {
-      // bounds of the register's place, 8 (i / 4) + i % 4 (constants to compare
-      // with, where the keys themselves would be 16 values to hold)
-      const int k0 = key0 + 4 * fresh_half(), hi = pos - k0;
-      const int lo = a.window == 0 || pos < a.window ? INT32_MIN : pos - a.window - k0, first = a.sinks - k0;
+      if (odd) v[64 * r] = x;
+    }
+    if (__ballot(odd) && lane == 0) *(volatile int32_t*)&odd_s = 1;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+  auto mask_sub = [&](f32x16& s, int key0) {
+    // bounds of the register's place, 8 (i / 4) + i % 4 (constants to compare
+    // with, where the keys themselves would be 16 values to hold)
+    const int k0 = key0 + 4 * fresh_half(), hi = pos - k0;
+    const int lo = a.window == 0 || pos < a.window ? INT32_MIN : pos - a.window - k0, first = a.sinks - k0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int at = 8 * (i >> 2) + (i & 3);
-        s[i] = (at <= hi) & ((at > lo) | (at < first)) ? s[i] : -INFINITY;
-      }
-    };
+    for (int i = 0; i < 16; ++i) {
+      const int at = 8 * (i >> 2) + (i & 3);
+      s[i] = (at <= hi) & ((at > lo) | (at < first)) ? s[i] : -INFINITY;
+    }
+  };
 
   // Takes the run's next item and asks for its Q, its pages and its first chunks.
   auto begin = [&] {
