@@ -1495,3 +1495,63 @@ def test_scores_near_the_largest_that_are_exact(gpu, many, kind, hq, hkv, d, sig
     # the weights of a row are equal, to half a step of bf16 where the two lane halves or pieces differ in their factor
     half = HALF[kind]
     assert bool(((out - mean).abs() <= (2 * half if kind == "bf16" else 2.0 ** -18) * size + half * mean.abs() * 1.01).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("many,kind,hq,hkv,d", [(False, "bf16", 8, 2, 128), (False, "bf16", 4, 2, 256), (False, "f32", 4, 2, 128), (True, "bf16", 8, 2, 128),
+                                                (True, "bf16", 4, 2, 256)])
+def test_infinities_of_v_in_caches_of_other_strides(gpu, many, kind, hq, hkv, d):
+    """Head-major caches, out inside a larger buffer, in place of q, infinities of the first and the last KV head."""
+    import torch
+    for window, sinks in ((0, 0), (70, 5)):
+        kw = dict(window=window, sinks=sinks) if window else {}
+        extra = dict(window=window) if many else {}
+        p = (_Many if many else _Paged)(gpu, [600, 20], [100, 1], hq, hkv, d, kind, 32, seed=7, head_major=True, **extra)
+        clean = p.run(**kw)
+        rows, g = torch.arange(600, 700, device=gpu), hq // hkv
+        for j, head in ((3, 0), (590, hkv - 1), (640, 0), (698, hkv - 1)):
+            page, off = int(p.table[0, j // 32]), j % 32
+            held = p.v[page, off, head, d - 1].clone()
+            p.v[page, off, head, d - 1] = -math.inf
+            out = torch.full((p.t, 2 * hq, d), 5.0, dtype=p.q.dtype, device=gpu)[:, ::2]
+            p.run(out=out, **kw)
+            q = p.q.clone()
+            assert torch.equal(p.run(out=p.q, **kw)[:100], out[:100])
+            p.q = q
+            p.v[page, off, head, d - 1] = held
+            sees = (j <= rows) & ((window == 0) | (j > rows - window) | (j < sinks))
+            assert bool((out[:100][sees][:, head * g: (head + 1) * g, d - 1] == -math.inf).all())
+            got, want = out[:101].clone(), clean[:101].clone()
+            got[:100][sees, head * g: (head + 1) * g, d - 1] = 0
+            want[:100][sees, head * g: (head + 1) * g, d - 1] = 0
+            assert bool(got.isfinite().all()) and (kind == "f32" or torch.equal(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("requests,room", [(20, 1500), (300, 6000)])
+def test_tables_of_many_workgroups_in_a_graph(gpu, requests, room):
+    """One captured step in place, replayed while requests grow, end and come back,
+    with eager steps and other work between the replays."""
+    import torch
+    rng = random.Random(requests)
+    s = _Tables(gpu, [rng.randint(0, 60) for _ in range(requests)], 16, 30, requests * 20, seed=3, max_tokens=room)
+    new = s.t([0] * requests)
+
+    def step():
+        cev_hip.paged_tables(s.lengths, new, s.table, 16, s.cu, s.pos, s.slots, free=s.free, ring=s.ring)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for k in range(8):
+        add = [rng.choice([-1, 0, 1, 20]) for _ in range(requests)]
+        want = s.expect(add)
+        new.copy_(s.t(add))
+        if k % 3 == 2:
+            step()
+        else:
+            graph.replay()
+        torch.randn(1000, 1000, device=gpu).sum()
+        torch.cuda.synchronize()
+        s.check(want, k)
