@@ -23,15 +23,15 @@
 // ones, so that a row's weights add up to one.
 //
 // What bounds it, alone on the card, us:
-//   bf16 d = 128  64 requests of one token, 64 to 8192 keys, 8 KV heads: 186, for
-//                 1077 MB 5.8 TB/s: HBM
-//   bf16 d = 128  one token after 300 keys: 8.8, a chain of trips: the list's item,
+//   bf16 d = 128  64 requests of one token, 64 to 8192 keys, 8 KV heads: 186 to
+//                 189, for 1077 MB 5.7 TB/s: HBM
+//   bf16 d = 128  one token after 300 keys: 9.0, a chain of trips: the list's item,
 //                 page ids, K, scores, V, the pieces' join; a launch is 3.5
-//   bf16 d = 256  28 requests of 1 to 8 rows and 4 of 64, 100 to 4096 keys: 91, for
-//                 560 MB 6.1 TB/s of HBM and MALL.  276 MB would do: the tiles of
+//   bf16 d = 256  28 requests of 1 to 8 rows and 4 of 64, 100 to 4096 keys: 92 to
+//                 104, for 560 MB 6.1 to 5.4 TB/s of HBM and MALL.  276 MB would do: the tiles of
 //                 one request read its keys each for themselves.  Of a round's 7000
 //                 cycles 4000 are spent handing out loads that wait for room
-//   f32           12 chunks of 17 to 41 rows, 256 to 2048 keys: 58, of which a
+//   f32           12 chunks of 17 to 41 rows, 256 to 2048 keys: 59, of which a
 //                 quarter are the items' starts and joins; a round of 9100 cycles has 3000
 //                 of MFMAs, the rest makes bf16 parts of K and V beside them and
 //                 hands over the loads

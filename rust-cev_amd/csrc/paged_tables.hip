@@ -101,10 +101,10 @@ struct TablesArgs {
 //
 // Of an ended request only the entries that are pages go back (its holder enters
 // another value for what the request does not hold), so every workgroup counts
-// them first, in steps that end one: 2.6 us for 50 that end among 512.
+// them first, in steps that end one: 1.8 us for 50 that end among 512.
 //
 // Bound by the launch and a chain of three trips to memory, four where requests
-// end: 3.4 us for 64 requests of one token, 9.8 for 20000 tokens of 512 requests
+// end: 3.5 us for 64 requests of one token, 9.0 for 20000 tokens of 512 requests
 // (10 workgroups).
 template <int W, int PER>
 __global__ __launch_bounds__(64 * W) void paged_tables_kernel(TablesArgs a) {
