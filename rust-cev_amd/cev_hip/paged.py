@@ -119,8 +119,9 @@ def rope(q_in, k_in, pos, rot: RotaryAngles, interleaved: bool = False, transpos
     interleaved.  With slots (t) int32, k and v go to those slots of k_out and
     v_out, (pages, page_size, hkv, d) caches; a slot outside them stores
     nothing, and no two tokens may have the same one.  transposed: the gradient
-    of q_in and k_in from that of q_out and k_out.  Outputs may be their
-    inputs.  Returns (q_out, k_out), with v_in also v_out."""
+    of q_in and k_in from that of q_out and k_out (the call itself records
+    nothing for autograd).  Outputs may be their inputs.  Returns (q_out,
+    k_out), with v_in also v_out."""
     if slots is not None and (k_out is None or (v_in is not None and v_out is None)):
         raise CevError(-1, "rope: slots need caches to store into")
     if stream is not None:  # (outputs that the call makes come from the current stream's pool)
