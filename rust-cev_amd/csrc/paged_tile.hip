@@ -23,11 +23,11 @@
 //
 // Bound by the matrix cores and the softmax beside them: a chunk of 64 keys takes
 // 4100 cycles of a workgroup (2048 of MFMAs a SIMD).  4 chunks of 450 rows after 12000
-// to 32000 keys (32 over 8 heads) 556 to 576 us by box, 990 to 950 TFLOP/s; 7600 rows that see 1024
+// to 32000 keys (32 over 8 heads) 556 to 576 us by card, 990 to 950 TFLOP/s; 7600 rows that see 1024
 // keys and the first four 185 to 191 us, 710 to 690 TFLOP/s: a tile of 19 chunks has 15000 cycles of its
 // own (first scores and their maximum 5000, a chunk's masks, the rows' stores).
 // Without the fetch the chunks' call took 478 of 569 us, without the exponentials 536.
-// d = 256: 64 requests of 256 rows in 2048 keys (16 over 4 heads) 592 to 670 us by box,
+// d = 256: 64 requests of 256 rows in 2048 keys (16 over 4 heads) 592 to 670 us by card,
 // 870 to 770 TFLOP/s; 32 slots a workgroup took 2800.  What lies in scratch counts by
 // how it is used: two values that a chunk reloads are in this form (592 us); with
 // parts of Q reloaded it took 790 where this one took 623, with K reads three units
