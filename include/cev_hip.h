@@ -477,7 +477,7 @@ int32_t cev_rope(const cev_rope_desc* d, const void* q_in, const void* k_in, con
  * sinks).  lengths include the new tokens, whose k and v are in the cache
  * already.  Rows of no request are left as they were.  Pages that no row
  * sees (behind a window) are not read and may have been given back; requests
- * may share pages.  Infinities and NaN of v reach the rows that see them and no
+ * may share pages that none of them adds to.  Infinities and NaN of v reach the rows that see them and no
  * others: their column is the sum of all of them, whatever their weights.
  * Scores, sums and maxima are f32.  bf16: the probabilities are rounded to
  * bf16 for the product with v, and a row is divided by the sum of the rounded

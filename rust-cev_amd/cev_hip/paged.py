@@ -60,7 +60,8 @@ def paged_tables(lengths, new_len, block_table, page_size: int, cu, pos, slots, 
     A page has one holder: the ring takes back every page that an ended
     request's row names.  Entries outside [0, n_pages) are passed over, so enter
     -1 where a page is another request's (a shared prefix) or was given back
-    before (behind a window) and then end the request.
+    before (behind a window) and then end the request.  New tokens go to the
+    last page that is not full: share whole pages.
 
     All tensors are int32 on the GPU: lengths, new_len (requests), block_table
     (requests, pages), pos and slots (the most rows of a step), free (n_pages)
