@@ -534,6 +534,69 @@ int32_t cev_paged_attention(const cev_paged_desc* d, const void* q, const void* 
                             void* out, void* work, size_t work_bytes, cev_stream stream);
 
 /* ------------------------------------------------------------------ */
+/* Projections in 8-bit floating point.
+ *
+ * Values are e4m3 (4 significant bits, largest 448, no infinity), 128 of them
+ * under one scale.  Rows of activations (t, k): q (t, kp) bytes, kp = k up to
+ * a multiple of 128, zeros behind k, and a scale for 128 columns of a row, (t,
+ * kp / 128) bytes e8m0 (2^(byte - 127)).  A scale made here is the least power
+ * of two 2^e, e >= -127, with 448 * 2^e not below the block's largest finite
+ * magnitude; q is x / 2^e, which is exact in f32, rounded to nearest even.  A
+ * value that is not finite becomes NaN and counts for no scale.  Weights (n,
+ * k): a scale for 128 x 128 values, from cev_fp8_blocks or brought along.
+ * Nothing here has a gradient. */
+enum { CEV_E4M3 = 2 };                                   /* beside CEV_F32 and CEV_BF16, where a call says so */
+enum { CEV_FP8_SCALES_E8M0 = 0, CEV_FP8_SCALES_F32 = 1 }; /* a weight's scales: bytes 2^(byte - 127), or any f32 */
+
+/* x (t, k) rows of f32 or bf16 into e4m3: before a projection whose rows no
+ * other call makes (the attention output before o_proj, qwen3.rs:219).  x is
+ * 16-byte aligned with x_stride a multiple of 8 (bf16) or 4 (f32) elements;
+ * q 16-byte aligned. */
+int32_t cev_fp8_rows(int32_t dtype, int64_t t, int64_t k, const void* x, int64_t x_stride, void* q, void* scales, cev_stream stream);
+
+/* The RMS norm before a projection (qwen3.rs:254-255), with the residual add
+ * where h is given (qwen3.rs:261): x_out = dtype(x + h) is written (x_out may
+ * be x), and x_out / sqrt(mean x_out^2 + eps) * w, f32 throughout, goes into
+ * e4m3 with that one rounding.  Alignment as above, for w too. */
+int32_t cev_fp8_rms_norm(int32_t dtype, int64_t rows, int64_t k, const void* x, int64_t x_stride, const void* h, int64_t h_stride,
+                         void* x_out, int64_t x_out_stride, const void* w, float eps, int32_t weight_plus_one, void* q, void* scales,
+                         cev_stream stream);
+
+/* A weight w (n, k) of f32 or bf16 into e4m3: q (n, k), and a scale for each
+ * 128 x 128 block, (ceil(n / 128), ceil(k / 128)) bytes e8m0. */
+int32_t cev_fp8_blocks(int32_t dtype, int64_t n, int64_t k, const void* w, int64_t ldw, void* q, void* scales, cev_stream stream);
+
+/* A weight in the order in which the products read it, made once.  q (n, k)
+ * e4m3 with row stride ldq, scales (ceil(n / 128), ceil(k / 128)) of
+ * scale_kind with row stride lds (in scales).  up_q given: a gate (q) and an
+ * up projection of the same n, for cev_fp8_product with gate_up.
+ * weight: cev_fp8_weight_size bytes, 256-byte aligned. */
+int32_t cev_fp8_weight_size(int64_t n, int64_t k, int32_t gate_up, size_t* bytes);
+int32_t cev_fp8_weight_pack(int64_t n, int64_t k, int32_t scale_kind, const void* q, int64_t ldq, const void* scales, int64_t lds,
+                            const void* up_q, int64_t up_ldq, const void* up_scales, int64_t up_lds, void* weight, size_t weight_bytes,
+                            cev_stream stream);
+
+/* Linear::forward without bias (qwen3.rs:175-178, :229-233) with such a
+ * weight: out (t, n) = rows . w^T, sums in f32, one rounding.  Rows of f32 or
+ * bf16 go into e4m3 first, as cev_fp8_rows does.  gate_up: Mlp::forward's silu(rows . gate^T) *
+ * (rows . up^T) (qwen3.rs:230-233) in f32, into e4m3 rows of n columns for the
+ * down projection.  A row of e4m3 with a NaN has NaN in every column. */
+typedef struct {
+  int32_t x_dtype;   /* CEV_F32, CEV_BF16, or CEV_E4M3: dense rows as cev_fp8_rows writes them */
+  int32_t out_dtype; /* CEV_F32 or CEV_BF16; with gate_up CEV_E4M3, dense rows too */
+  int32_t scales;    /* CEV_FP8_SCALES_*: the kind that the weight was packed with */
+  int32_t gate_up;
+  int64_t t, n, k;
+  int64_t x_stride;   /* elements; not for CEV_E4M3 */
+  int64_t out_stride; /* elements; not with gate_up */
+} cev_fp8_desc;
+/* Bytes of the workspace (256-byte aligned; needs no values).  Calls that
+ * overlap must not share one. */
+int32_t cev_fp8_work_size(const cev_fp8_desc* d, size_t* bytes);
+int32_t cev_fp8_product(const cev_fp8_desc* d, const void* x, const void* x_scales, const void* weight, size_t weight_bytes, void* out,
+                        void* out_scales, void* work, size_t work_bytes, cev_stream stream);
+
+/* ------------------------------------------------------------------ */
 /* Table builders (host only). */
 
 /* The packed pass of engine.rs:365-442.  Plans p = 0..n_plans-1 in plan

@@ -25,6 +25,7 @@ __all__ = [
     "CEV_BF16", "CEV_F32", "CevError", "Block", "Span", "BlockTable", "AttnPlan", "PackedAttention",
     "packed_attention", "qknorm_rope", "rope_table", "Rotary", "device_info", "synth",
     "paged_tables", "free_ring", "RotaryAngles", "rope", "PagedAttention",
+    "Fp8Rows", "Fp8Weight", "fp8_rows", "fp8_blocks", "rms_norm_fp8", "linear_fp8", "gate_up_fp8",
     "Blas", "linear", "gather_rows", "D3Readout", "PrefixStore", "qknorm_rope_kv",
 ]
 
@@ -683,3 +684,8 @@ class GatedDeltaNet:
 # Paged caches
 
 from .paged import PagedAttention, RotaryAngles, free_ring, paged_tables, rope  # noqa: E402
+
+# ---------------------------------------------------------------------------
+# Projections in 8-bit floating point
+
+from .fp8 import Fp8Rows, Fp8Weight, fp8_blocks, fp8_rows, gate_up_fp8, linear_fp8, rms_norm_fp8  # noqa: E402

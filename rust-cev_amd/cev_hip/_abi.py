@@ -20,6 +20,8 @@ CEV_ERR_SPACE = -4
 CEV_F32 = 0
 CEV_BF16 = 1
 CEV_MAX_SPANS = 4
+CEV_E4M3 = 2
+CEV_FP8_SCALES_E8M0, CEV_FP8_SCALES_F32 = 0, 1
 CEV_ROPE_PLAIN, CEV_ROPE_LINEAR, CEV_ROPE_YARN, CEV_ROPE_WAVELENGTH = range(4)
 CEV_ATTN_SCRATCH_BYTES = 64 << 20
 CEV_LINEAR_WORKSPACE_BYTES = 32 << 20
@@ -118,6 +120,13 @@ class PagedDesc(C.Structure):
     ]
 
 
+class Fp8Desc(C.Structure):
+    _fields_ = [
+        ("x_dtype", i32), ("out_dtype", i32), ("scales", i32), ("gate_up", i32),
+        ("t", i64), ("n", i64), ("k", i64), ("x_stride", i64), ("out_stride", i64),
+    ]
+
+
 P = C.c_void_p
 Pi32 = C.POINTER(i32)
 PBlock = C.POINTER(Block)
@@ -155,6 +164,13 @@ SIGNATURES = {
     "cev_paged_work_size": (i32, [C.POINTER(PagedDesc), C.POINTER(C.c_size_t)]),
     "cev_paged_plan": (i32, [C.POINTER(PagedDesc), P, P, P, C.c_size_t, P]),
     "cev_paged_attention": (i32, [C.POINTER(PagedDesc), P, P, P, P, P, P, C.c_size_t, P]),
+    "cev_fp8_rows": (i32, [i32, i64, i64, P, i64, P, P, P]),
+    "cev_fp8_rms_norm": (i32, [i32, i64, i64, P, i64, P, i64, P, i64, P, C.c_float, i32, P, P, P]),
+    "cev_fp8_blocks": (i32, [i32, i64, i64, P, i64, P, P, P]),
+    "cev_fp8_weight_size": (i32, [i64, i64, i32, C.POINTER(C.c_size_t)]),
+    "cev_fp8_weight_pack": (i32, [i64, i64, i32, P, i64, P, i64, P, i64, P, i64, P, C.c_size_t, P]),
+    "cev_fp8_work_size": (i32, [C.POINTER(Fp8Desc), C.POINTER(C.c_size_t)]),
+    "cev_fp8_product": (i32, [C.POINTER(Fp8Desc), P, P, P, C.c_size_t, P, P, P, C.c_size_t, P]),
     "cev_table_from_plans": (i32, [i32, Pi32, Pi32, Pi32, i32, Pi32, Pi32, PBlock, i32, Pi32, Pi32, i32, Pi32, Pi32]),
     "cev_table_from_rows": (i32, [i32, i32, i32, i32, Pi32, PBlock, i32]),
     "cev_table_from_slots": (i32, [i32, Pi32, Pi32, Pi32, i32, Pi32, Pi32, Pi32, i32, PBlock, i32, Pi32, Pi32, Pi32, i32, Pi32, Pi32]),

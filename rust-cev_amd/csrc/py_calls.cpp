@@ -14,6 +14,7 @@
 #include <Python.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPCachingAllocator.h>
@@ -43,6 +44,13 @@ struct Api {
   decltype(&cev_rope) rope;
   decltype(&cev_paged_plan) paged_plan;
   decltype(&cev_paged_attention) paged_attention;
+  decltype(&cev_fp8_rows) fp8_rows;
+  decltype(&cev_fp8_rms_norm) fp8_rms_norm;
+  decltype(&cev_fp8_blocks) fp8_blocks;
+  decltype(&cev_fp8_weight_size) fp8_weight_size;
+  decltype(&cev_fp8_weight_pack) fp8_weight_pack;
+  decltype(&cev_fp8_work_size) fp8_work_size;
+  decltype(&cev_fp8_product) fp8_product;
   decltype(&cev_last_error) last_error;
 } api;
 PyObject* cev_error = nullptr;  // cev_hip.CevError
@@ -583,6 +591,200 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// Returns made(): guarded() for calls that have a result.
+template <typename Fn>
+PyObject* guarded_result(Fn&& fn) {
+  PyObject* result = nullptr;
+  PyObject* const done = guarded([&] { result = fn(); });
+  if (!done) {
+    Py_XDECREF(result);
+    return nullptr;
+  }
+  Py_DECREF(done);
+  return result;
+}
+
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+// The rows in e4m3 and their scales that a call writes: the caller's, or
+// new ones (from the current stream's pool).
+struct Fp8Out {
+  at::Tensor q, s;
+  Fp8Out(const char* call, PyObject* oq, PyObject* os, const at::Tensor& on, int64_t t, int64_t k) {
+    const int64_t kb = blocks_of(k);
+    want((oq == Py_None) == (os == Py_None), call, "out's values and scales go together");
+    if (oq == Py_None) {
+      q = at::empty({t, kb * 128}, on.options().dtype(at::kFloat8_e4m3fn));
+      s = at::empty({t, kb}, on.options().dtype(at::kFloat8_e8m0fnu));
+      return;
+    }
+    q = tensor(oq, "out.q"), s = tensor(os, "out.s");
+    want(q.scalar_type() == at::kFloat8_e4m3fn && q.dim() == 2 && q.is_contiguous() && q.size(0) == t && q.size(1) == kb * 128 &&
+             s.scalar_type() == at::kFloat8_e8m0fnu && s.dim() == 2 && s.is_contiguous() && s.size(0) == t && s.size(1) == kb,
+         call, "out must be Fp8Rows of " + std::to_string(t) + " rows and " + std::to_string(k) + " columns");
+  }
+  PyObject* pair() const { return Py_BuildValue("(NN)", THPVariable_Wrap(q), THPVariable_Wrap(s)); }
+};
+
+// fp8_rows(x, q, s, stream) -> (q, s)
+PyObject* py_fp8_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded_result([&] {
+    need_args(n, 4);
+    const char* const me = "fp8_rows";
+    const at::Tensor& x = tensor(a[0], "x");
+    want(x.dim() == 2 && x.size(1) >= 1, me, "x must be (t, k)");
+    const int dt = dtype_code(x);
+    if (x.size(1) > 1) rows_contiguous(x);
+    const OnDevice dev(me, {{"x", &x}});
+    const Fp8Out out(me, a[1], a[2], x, x.size(0), x.size(1));
+    const OnDevice all(me, {{"x", &x}, {"out.q", &out.q}, {"out.s", &out.s}});
+    void* const s = dev.stream(a[3]);
+    call([&] { return api.fp8_rows(dt, x.size(0), x.size(1), ptr(x), x.stride(0), ptr(out.q), ptr(out.s), s); });
+    return out.pair();
+  });
+}
+
+// fp8_rms_norm(x, w, eps, h, x_out, plus_one, q, s, stream) -> (q, s)
+PyObject* py_fp8_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded_result([&] {
+    need_args(n, 9);
+    const char* const me = "rms_norm_fp8";
+    const at::Tensor &x = tensor(a[0], "x"), &w = tensor(a[1], "w");
+    const at::Tensor *const h = tensor_or_none(a[3], "h"), *const x_out = tensor_or_none(a[4], "x_out");
+    want(x.dim() == 2 && x.size(1) >= 1, me, "x must be (rows, hidden)");
+    const int dt = dtype_code(x);
+    want(!x_out || h, me, "x_out goes with h");
+    want(w.dim() == 1 && w.size(0) == x.size(1), me, "w must have a value for each column");
+    for (const at::Tensor* t : {&x, &w, h, x_out}) {
+      if (!t) continue;
+      if (t->scalar_type() != x.scalar_type() || (x.size(1) > 1 && t->stride(-1) != 1))
+        raise_cev(CEV_ERR_UNSUPPORTED, "rms_norm_fp8: tensors must share the dtype and have a contiguous last dim");
+      want(t == &w || t->sizes().equals(x.sizes()), me, "h and x_out must have x's shape");
+    }
+    const float eps = (float)as_double(a[2]);
+    const int32_t plus = as_bool(a[5]) ? 1 : 0;
+    const OnDevice dev(me, {{"x", &x}, {"w", &w}, {"h", h}, {"x_out", x_out}});
+    const Fp8Out out(me, a[6], a[7], x, x.size(0), x.size(1));
+    const OnDevice all(me, {{"x", &x}, {"out.q", &out.q}, {"out.s", &out.s}});
+    void* const s = dev.stream(a[8]);
+    call([&] {
+      return api.fp8_rms_norm(dt, x.size(0), x.size(1), ptr(x), x.stride(0), ptr(h), h ? h->stride(0) : 0, ptr(x_out), x_out ? x_out->stride(0) : 0,
+                              ptr(w), eps, plus, ptr(out.q), ptr(out.s), s);
+    });
+    return out.pair();
+  });
+}
+
+// fp8_blocks(w, stream) -> (q, scales)
+PyObject* py_fp8_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded_result([&] {
+    need_args(n, 2);
+    const char* const me = "fp8_blocks";
+    const at::Tensor& w = tensor(a[0], "w");
+    want(w.dim() == 2 && w.size(0) >= 1 && w.size(1) >= 1, me, "w must be (n, k)");
+    const int dt = dtype_code(w);
+    if (w.size(1) > 1) rows_contiguous(w);
+    const OnDevice dev(me, {{"w", &w}});
+    const at::Tensor q = at::empty({w.size(0), w.size(1)}, w.options().dtype(at::kFloat8_e4m3fn)),
+                     s = at::empty({blocks_of(w.size(0)), blocks_of(w.size(1))}, w.options().dtype(at::kFloat8_e8m0fnu));
+    void* const st = dev.stream(a[1]);
+    call([&] { return api.fp8_blocks(dt, w.size(0), w.size(1), ptr(w), w.stride(0), ptr(q), ptr(s), st); });
+    return Py_BuildValue("(NN)", THPVariable_Wrap(q), THPVariable_Wrap(s));
+  });
+}
+
+// fp8_pack(q, scales, up_q, up_scales, stream) -> the packed weight
+PyObject* py_fp8_pack(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded_result([&] {
+    need_args(n, 5);
+    const char* const me = "Fp8Weight";
+    const at::Tensor &q = tensor(a[0], "q"), &sc = tensor(a[1], "scales");
+    const at::Tensor *const up = tensor_or_none(a[2], "up q"), *const up_s = tensor_or_none(a[3], "up scales");
+    want((up == nullptr) == (up_s == nullptr), me, "values and scales go together");
+    want(q.dim() == 2 && q.size(0) >= 1 && q.size(1) >= 1, me, "a weight must be (n, k)");
+    for (const at::Tensor* t : {&q, up}) {
+      if (!t) continue;
+      if (t->scalar_type() != at::kFloat8_e4m3fn)
+        raise_cev(CEV_ERR_UNSUPPORTED, std::string("dtype torch.") + c10::toString(t->scalar_type()) + " not supported (float8_e4m3fn)");
+      want(t->sizes().equals(q.sizes()), me, "gate and up must have one shape");
+      if (t->size(1) > 1) rows_contiguous(*t);
+    }
+    for (const at::Tensor* t : {&sc, up_s}) {
+      if (!t) continue;
+      if (t->scalar_type() != at::kFloat && t->scalar_type() != at::kFloat8_e8m0fnu)
+        raise_cev(CEV_ERR_UNSUPPORTED, std::string("scales of torch.") + c10::toString(t->scalar_type()) + " not supported (float32, float8_e8m0fnu)");
+      want(t->scalar_type() == sc.scalar_type(), me, "gate and up must have scales of one type");
+      want(t->dim() == 2 && t->size(0) == blocks_of(q.size(0)) && t->size(1) == blocks_of(q.size(1)), me,
+           "scales must be (" + std::to_string(blocks_of(q.size(0))) + ", " + std::to_string(blocks_of(q.size(1))) + "), one for 128 x 128 values");
+      if (t->size(1) > 1) rows_contiguous(*t);
+    }
+    const OnDevice dev(me, {{"q", &q}, {"scales", &sc}, {"up q", up}, {"up scales", up_s}});
+    size_t bytes = 0;
+    check(api.fp8_weight_size(q.size(0), q.size(1), up != nullptr, &bytes));
+    const at::Tensor w = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    void* const s = dev.stream(a[4]);
+    const int32_t kind = sc.scalar_type() == at::kFloat ? CEV_FP8_SCALES_F32 : CEV_FP8_SCALES_E8M0;
+    call([&] {
+      return api.fp8_weight_pack(q.size(0), q.size(1), kind, ptr(q), q.stride(0), ptr(sc), sc.stride(0), ptr(up), up ? up->stride(0) : 0, ptr(up_s),
+                                 up_s ? up_s->stride(0) : 0, ptr(w), bytes, s);
+    });
+    return THPVariable_Wrap(w);
+  });
+}
+
+// fp8_product(x, x_scales, x_k, weight, n, k, scales, gate_up, out, out_scales, out_dtype, stream) -> out, with gate_up (q, s).  x_k: the
+// columns of rows in e4m3; out_dtype: of an output that the call makes
+PyObject* py_fp8_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded_result([&] {
+    need_args(n, 12);
+    const at::Tensor &x = tensor(a[0], "x"), &w = tensor(a[3], "weight");
+    const at::Tensor* const xs = tensor_or_none(a[1], "x's scales");
+    cev_fp8_desc d{};
+    d.n = as_int(a[4]), d.k = as_int(a[5]);
+    d.scales = (int32_t)as_int(a[6]);
+    d.gate_up = as_bool(a[7]) ? 1 : 0;
+    const char* const me = d.gate_up ? "gate_up_fp8" : "linear_fp8";
+    want(x.dim() == 2, me, "x must be (t, k)");
+    d.t = x.size(0);
+    const int64_t kb = blocks_of(d.k), x_k = xs ? as_int(a[2]) : x.size(1);
+    want(x_k == d.k, me, "rows of " + std::to_string(x_k) + " columns for a weight of " + std::to_string(d.k));
+    if (xs) {
+      want(x.scalar_type() == at::kFloat8_e4m3fn && x.is_contiguous() && x.size(1) == kb * 128 && xs->scalar_type() == at::kFloat8_e8m0fnu &&
+               xs->dim() == 2 && xs->is_contiguous() && xs->size(0) == d.t && xs->size(1) == kb,
+           me, "x is not what fp8_rows makes");
+      d.x_dtype = CEV_E4M3;
+    } else {
+      d.x_dtype = dtype_code(x);
+      if (d.k > 1) rows_contiguous(x);
+      d.x_stride = x.stride(0);
+    }
+    const OnDevice dev(me, {{"weight", &w}, {"x", &x}, {"x's scales", xs}});
+    void* const s = dev.stream(a[11]);
+    auto run = [&](const at::Tensor& out, const at::Tensor* out_s) {
+      const OnDevice all(me, {{"weight", &w}, {"out", &out}, {"out's scales", out_s}});
+      size_t bytes = 0;
+      check(api.fp8_work_size(&d, &bytes));
+      const CallBuffer work(x, bytes, s);
+      call([&] { return api.fp8_product(&d, ptr(x), ptr(xs), ptr(w), w.nbytes(), ptr(out), ptr(out_s), work.p, work.p ? bytes : 0, s); });
+    };
+    if (d.gate_up) {
+      const Fp8Out out(me, a[8], a[9], x, d.t, d.n);
+      d.out_dtype = CEV_E4M3;
+      run(out.q, &out.s);
+      return out.pair();
+    }
+    at::Tensor made;
+    if (a[8] == Py_None) made = at::empty({d.t, d.n}, x.options().dtype(as_int(a[10]) == CEV_F32 ? at::kFloat : at::kBFloat16));
+    const at::Tensor& out = a[8] == Py_None ? made : tensor(a[8], "out");
+    want(out.dim() == 2 && out.size(0) == d.t && out.size(1) == d.n, me, "out must be (" + std::to_string(d.t) + ", " + std::to_string(d.n) + ")");
+    if (d.n > 1) rows_contiguous(out);
+    d.out_dtype = dtype_code(out);
+    d.out_stride = out.stride(0);
+    run(out, nullptr);
+    return a[8] == Py_None ? THPVariable_Wrap(made) : Py_NewRef(a[8]);
+  });
+}
+
 // bind(error_class, {symbol: address})
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&] {
@@ -609,6 +811,13 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     get("cev_rope", api.rope);
     get("cev_paged_plan", api.paged_plan);
     get("cev_paged_attention", api.paged_attention);
+    get("cev_fp8_rows", api.fp8_rows);
+    get("cev_fp8_rms_norm", api.fp8_rms_norm);
+    get("cev_fp8_blocks", api.fp8_blocks);
+    get("cev_fp8_weight_size", api.fp8_weight_size);
+    get("cev_fp8_weight_pack", api.fp8_weight_pack);
+    get("cev_fp8_work_size", api.fp8_work_size);
+    get("cev_fp8_product", api.fp8_product);
     get("cev_last_error", api.last_error);
     Py_INCREF(a[0]);
     cev_error = a[0];
@@ -618,7 +827,8 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define CEV_METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {CEV_METHOD(bind),   CEV_METHOD(qknorm_rope), CEV_METHOD(attention),   CEV_METHOD(rms_norm), CEV_METHOD(swiglu),
                          CEV_METHOD(linear), CEV_METHOD(gather_rows), CEV_METHOD(gdn), CEV_METHOD(paged_tables), CEV_METHOD(rope),
-                         CEV_METHOD(paged_plan), CEV_METHOD(paged_attention), {nullptr, nullptr, 0, nullptr}};
+                         CEV_METHOD(paged_plan), CEV_METHOD(paged_attention), CEV_METHOD(fp8_rows), CEV_METHOD(fp8_rms_norm),
+                         CEV_METHOD(fp8_blocks), CEV_METHOD(fp8_pack), CEV_METHOD(fp8_product), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_cev_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
