@@ -15,162 +15,142 @@
 //   f32         v_mfma_f32_32x32x16_bf16 on the same values in bf16, which holds
 //               them exactly: products and sums in f32, at half the rate.
 #include <algorithm>
+#include <cmath>
 
-#include "cev_internal.h"
-#include "fp8_device.h"
+#include "fp8.h"
 
 namespace {
 
-constexpr int kWaves = 8;  // waves of a workgroup of the small-row kernel, each with its share of the column blocks
+constexpr int kWaves = 16;  // waves of a workgroup of the kernel for few rows, each with its share of the column blocks
 
-struct ProductArgs {
-  const void* x;          // rows
-  const uint8_t* xs;      // their scales (e4m3 rows)
-  const uint8_t* w;       // packed weight
-  const uint32_t* ws;     // its scales
-  void* out;
-  float* part;            // sums over parts of the columns
-  int64_t t, x_st, out_st, n;
-  int32_t k, kb;          // columns, blocks of them
-  int32_t groups;         // groups of 32 weight rows
-  int32_t parts, blocks_part;
-};
-
-__device__ __forceinline__ f32x16 mfma(const i32x8& a, const i32x8& b, const f32x16& c, int sa, int sb) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
-}
-
-// The two operands' 64 columns in bf16 (8 columns of each half of the lanes at
-// a time; any order of columns that both share will do).
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ bf16x8 widen(int lo, int hi) {
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, 1.0f, true);
-  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, 1.0f, true);
-  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-__device__ __forceinline__ f32x16 mfma_exact(const i32x8& a, const i32x8& b, f32x16 c) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen(a[2 * i], a[2 * i + 1]), widen(b[2 * i], b[2 * i + 1]), c, 0, 0, 0);
-  return c;
-}
-
-// 2^(code - 127); 2^-127 is subnormal.
-__device__ __forceinline__ float e8m0_value(uint32_t code) {
-  return __uint_as_float(code == 0 ? 0x400000u : code == 255 ? 0x7fc00000u : code << 23);
-}
-
-__device__ __forceinline__ i32x8 join8(const u32x4_t& a, const u32x4_t& b) {
-  return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
-}
-
-// The lane's share of block kb of its row: bytes 32 (lane / 32) .. + 31 of
-// each half of the block, as two operands; sc the row's scale.  Rows in the
-// model's type are brought into e4m3 on the way (the two lanes of a row hold
-// the whole block).
+// The lane's share of block kb of its row (columns 32 quad .. + 31), and the
+// row's scale.  Rows in the model's type are brought into e4m3 on the way: the
+// four lanes of a row hold the whole block.
 template <typename T>
-__device__ __forceinline__ void load_x(const ProductArgs& a, int64_t row, int kb, i32x8* o, int& sc) {
-  const int up = (threadIdx.x >> 5) & 1;
+__device__ __forceinline__ void load_x(const Fp8Args& a, int64_t row, int kb, int quad, i32x8& o, int& sc) {
   if constexpr (sizeof(T) == 1) {
-    const uint8_t* const p = (const uint8_t*)a.x + (row * a.kb + kb) * kFp8Block + up * 32;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) o[s] = join8(*(const u32x4_t*)(p + s * 64), *(const u32x4_t*)(p + s * 64 + 16));
+    const uint8_t* const p = (const uint8_t*)a.x + (row * a.kb + kb) * kFp8Block + quad * 32;
+    o = fp8_join(*(const u32x4_t*)p, *(const u32x4_t*)(p + 16));
     sc = a.xs[row * a.kb + kb];
   } else {
-    float v[8][8];
+    float v[4][8];
     uint32_t top = 0;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const int col = kb * kFp8Block + (c >> 2) * 64 + up * 32 + (c & 3) * 8;
+    for (int c = 0; c < 4; ++c) {
+      const int col = kb * kFp8Block + quad * 32 + c * 8;
       load8((const T*)a.x + row * a.x_st + (col < a.k ? col : 0), a.k - col, v[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = max(top, fp8_size(v[c][j]));
-    }
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
     top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
     const uint32_t code = fp8_code(top);
     const float f = fp8_inverse(code);
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      o[c >> 2][(c & 3) * 2] = (int)fp8_pack4(v[c][0] * f, v[c][1] * f, v[c][2] * f, v[c][3] * f);
-      o[c >> 2][(c & 3) * 2 + 1] = (int)fp8_pack4(v[c][4] * f, v[c][5] * f, v[c][6] * f, v[c][7] * f);
+    for (int c = 0; c < 4; ++c) {
+      o[2 * c] = (int)fp8_pack4(v[c][0] * f, v[c][1] * f, v[c][2] * f, v[c][3] * f);
+      o[2 * c + 1] = (int)fp8_pack4(v[c][4] * f, v[c][5] * f, v[c][6] * f, v[c][7] * f);
     }
     sc = (int)code;
   }
 }
 
-// Four neighbouring columns of a row of the output; the row's last ones and
-// rows that are not aligned to four go one by one.
-template <typename O>
-__device__ __forceinline__ void store4(O* row, int64_t n, int64_t col, const f32x4& v) {
-  O* const p = row + col;
-  if (col + 4 <= n && ((uintptr_t)p & (4 * sizeof(O) - 1)) == 0) {
-    if constexpr (sizeof(O) == 2)
-      *(u32x2_t*)p = u32x2_t{(uint32_t)bf16_bits(v[0]) | (uint32_t)bf16_bits(v[1]) << 16, (uint32_t)bf16_bits(v[2]) | (uint32_t)bf16_bits(v[3]) << 16};
-    else
-      *(f32x4*)p = v;
-  } else {
+// 16 MT rows times 16 weight rows (GATE_UP: times 16 of gate and of up).  The
+// weight streams through once, so what counts is how much of it is on the way:
+// a workgroup holds few weight rows and its 16 waves share the column blocks,
+// each with DEEP of them under way; their sums are joined in LDS, in the waves'
+// order.  (Parts of the columns in other workgroups would cost a second launch.)
+template <typename T, typename O, bool E8M0, bool GATE_UP, int MT>
+__global__ __launch_bounds__(kWaves * 64) void fp8_small_kernel(Fp8Args a, unsigned col_tiles) {
+  constexpr int NH = GATE_UP ? 2 : 1, DEEP = sizeof(T) == 1 ? (MT == 1 ? 4 : 2) : GATE_UP ? 1 : 2;
+  constexpr bool EXACT = sizeof(O) == 4 && !GATE_UP;
+  constexpr int QUAD = 80;  // floats of a quad's 16 rows x 4 columns, and 16 more: the sums' reads fall on different banks
+  __shared__ __align__(16) float sums[kWaves][NH * MT][4 * QUAD];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4, l16 = lane & 15;
+  const unsigned row_tile = blockIdx.x / col_tiles, c16 = blockIdx.x - row_tile * col_tiles;  // 16 MT rows, 16 columns
+  const int64_t tile = row_tile;
+  int64_t row[MT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (col + i < n) p[i] = (O)v[i];
-  }
-}
-
-// 32 rows times a group of 32 weight rows, the column blocks dealt to the
-// workgroup's waves, their sums joined in LDS in the waves' order.
-template <typename T, typename O, bool E8M0>
-__global__ __launch_bounds__(kWaves * 64) void fp8_small_kernel(ProductArgs a) {
-  __shared__ f32x4 sums[kWaves][4][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int group = (int)(blockIdx.x % a.groups);
-  const int64_t tile = blockIdx.x / a.groups / a.parts;
-  const int part = (int)(blockIdx.x / a.groups % a.parts);
-  const int64_t row = min(tile * 32 + (lane & 31), a.t - 1);
-  const int end = min(a.kb, (part + 1) * a.blocks_part);
-  f32x16 acc = {};
-  for (int kb = part * a.blocks_part + wave; kb < end; kb += kWaves) {
-    const uint8_t* const wp = a.w + ((int64_t)group * a.kb + kb) * kFp8GroupBytes + lane * 16;
-    i32x8 w[2], x[2];
+  for (int i = 0; i < MT; ++i) row[i] = min((tile * MT + i) * 16 + l16, a.t - 1);
+  // the group of 32 weight rows (gate's; up's follows), and the lane's place in its half
+  const int64_t group = (int64_t)(c16 >> 1) * NH;
+  const uint8_t* const wp = a.w + group * a.kb * kFp8GroupBytes + (quad >> 1) * 2048 + (quad & 1) * 512 + (c16 & 1) * 256 + l16 * 16;
+  f32x4 acc[NH][MT];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) w[s] = join8(*(const u32x4_t*)(wp + s * 2048), *(const u32x4_t*)(wp + s * 2048 + 1024));
-    const uint32_t sw = a.ws[(int64_t)group * a.kb + kb];
-    int sx;
-    load_x<T>(a, row, kb, x, sx);
-    if constexpr (sizeof(O) == 4) {
-      f32x16 b = {};
-      b = mfma_exact(w[0], x[0], b);
-      b = mfma_exact(w[1], x[1], b);
-      const float f = (E8M0 ? e8m0_value(sw) : __uint_as_float(sw)) * e8m0_value(sx);
+  for (int h = 0; h < NH; ++h)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[i] = __builtin_fmaf(b[i], f, acc[i]);
-    } else if constexpr (E8M0) {
-      acc = mfma(w[0], x[0], acc, (int)sw, sx);
-      acc = mfma(w[1], x[1], acc, (int)sw, sx);
-    } else {
-      f32x16 b = {};
-      b = mfma(w[0], x[0], b, 127, sx);
-      b = mfma(w[1], x[1], b, 127, sx);
-      const float f = __uint_as_float(sw);
+    for (int i = 0; i < MT; ++i) acc[h][i] = f32x4{};
+  for (int kb0 = wave; kb0 < a.kb; kb0 += kWaves * DEEP) {
+    u32x4_t w[DEEP][NH][2];
+    uint32_t sw[DEEP][NH];
+    i32x8 x[DEEP][MT];
+    int sx[DEEP][MT];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[i] = __builtin_fmaf(b[i], f, acc[i]);
+    for (int d = 0; d < DEEP; ++d) {
+      const int kb = kb0 + d * kWaves;
+      if (kb >= a.kb) break;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const uint8_t* const p = wp + ((int64_t)h * a.kb + kb) * kFp8GroupBytes;
+        w[d][h][0] = *(const u32x4_t*)p;
+        w[d][h][1] = *(const u32x4_t*)(p + 1024);
+        const int64_t at = (group + h) * a.ws_pitch + kb;
+        sw[d][h] = E8M0 ? a.ws[at] : ((const uint32_t*)a.ws)[at];
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) load_x<T>(a, row[i], kb, quad, x[d][i], sx[d][i]);
+    }
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d) {
+      if (kb0 + d * kWaves >= a.kb) break;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const i32x8 wv = fp8_join(w[d][h][0], w[d][h][1]);
+        const float f = E8M0 ? fp8_scale_value(sw[d][h]) : __uint_as_float(sw[d][h]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          if constexpr (EXACT) {
+            f32x4 p = {};
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(wv[2 * c], wv[2 * c + 1]), fp8_widen(x[d][i][2 * c], x[d][i][2 * c + 1]), p, 0, 0, 0);
+            const float s = f * fp8_scale_value((uint32_t)sx[d][i]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[h][i][r] = __builtin_fmaf(p[r], s, acc[h][i][r]);
+          } else if constexpr (E8M0) {
+            acc[h][i] = fp8_mfma(wv, x[d][i], acc[h][i], (int)sw[d][h], sx[d][i]);
+          } else {
+            const f32x4 p = fp8_mfma(wv, x[d][i], f32x4{}, 127, sx[d][i]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[h][i][r] = __builtin_fmaf(p[r], f, acc[h][i][r]);
+          }
+        }
+      }
     }
   }
-  // lane l holds row l % 32, columns 8 i + 4 (l / 32) .. + 3 of the group in registers 4 i .. 4 i + 3
+  // lane l holds row l % 16, columns 4 (l / 16) .. + 3
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sums[wave][i][lane] = f32x4{acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]};
+  for (int h = 0; h < NH; ++h)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) *(f32x4*)&sums[wave][h * MT + i][quad * QUAD + l16 * 4] = acc[h][i];
   __syncthreads();
-  if (threadIdx.x < 256) {
-    const int i = threadIdx.x >> 6;
-    f32x4 v = sums[0][i][lane];
+  for (int e = threadIdx.x; e < MT * 256; e += kWaves * 64) {
+    const int i = e >> 8, r = (e >> 4) & 15, n = e & 15, at = (n >> 2) * QUAD + r * 4 + (n & 3);
+    float v[NH];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) v += sums[w][i][lane];
-    const int64_t out_row = tile * 32 + (lane & 31);
-    const int64_t col = (int64_t)group * kFp8Group + 8 * i + 4 * (lane >> 5);
-    if (out_row < a.t) {
-      if (a.part)
-        *(f32x4*)(a.part + ((int64_t)part * a.t + out_row) * ((int64_t)a.groups * kFp8Group) + col) = v;
-      else
-        store4((O*)a.out + out_row * a.out_st, a.n, col, v);
+    for (int h = 0; h < NH; ++h) {
+      v[h] = sums[0][h * MT + i][at];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) v[h] += sums[w][h * MT + i][at];
     }
+    const int64_t out_row = (tile * MT + i) * 16 + r, col = (int64_t)c16 * 16 + n;
+    if (out_row >= a.t || col >= a.n) continue;
+    if constexpr (GATE_UP)
+      a.part[out_row * a.out_st + col] = fp8_swiglu(v[0], v[1]);
+    else
+      ((O*)a.out)[out_row * a.out_st + col] = (O)v[0];
   }
 }
 
@@ -192,13 +172,7 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(JoinArgs a) {
   const float* p = a.part + row * a.width + col;
   f32x4 v = *(const f32x4*)p;
   for (int s = 1; s < a.parts; ++s) v += *(const f32x4*)(p + (int64_t)s * a.t * a.width);
-  store4((O*)a.out + row * a.out_st, a.n, col, v);
-}
-
-// silu(g) u in f32 (the hardware's exp2 and reciprocal, within 2^-20 of the
-// value: e4m3 keeps 4 bits of it).
-__device__ __forceinline__ float swiglu(float g, float u) {
-  return g * __builtin_amdgcn_rcpf(1.0f + fast_exp2(-1.44269504f * g)) * u;
+  fp8_store4((O*)a.out + row * a.out_st, a.n, col, v);
 }
 
 // Sums of gate and up (groups of 32 columns in turn) into rows in e4m3: 8
@@ -218,7 +192,7 @@ __global__ __launch_bounds__(256) void fp8_join_gate_up_kernel(JoinArgs a) {
     }
   float v[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = col + j < a.n ? swiglu(g[j >> 2][j & 3], u[j >> 2][j & 3]) : 0.0f;
+  for (int j = 0; j < 8; ++j) v[j] = col + j < a.n ? fp8_swiglu(g[j >> 2][j & 3], u[j >> 2][j & 3]) : 0.0f;
   uint32_t code;
   const u32x2_t q = fp8_block16(v, code);
   *(u32x2_t*)((uint8_t*)a.out + (row * a.quads + col / 8) * 8) = q;
@@ -230,8 +204,11 @@ int32_t launched(const char* what) {
   return e == hipSuccess ? CEV_OK : cev_fail(CEV_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
 }
 
+constexpr int kTileBlocks = 32768;  // column blocks that the offsets of the kernel for many rows reach
+
 // How a product runs.
 struct Form {
+  int32_t tt;   // the kernel for many rows, 16 tt of them a workgroup; 0: the one for few
   bool pack_x;  // rows of the model's type go into e4m3 in a launch of their own
   int32_t groups, kb, parts, blocks_part;
   size_t rows_bytes, scales_bytes, part_bytes;
@@ -239,19 +216,72 @@ struct Form {
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// Times of the kernel for many rows in us, measured at 64 to 4096 rows, 2048
+// to 12288 weight rows, 2048 to 12288 columns: a launch, and a block of columns
+// with one workgroup a CU and with two (tt = 16: one, alone on the card and
+// with all CUs busy).
+struct TileTimes {
+  float fixed, one, two;
+};
+constexpr TileTimes kE8m0Times[] = {{4.0f, 0.45f, 0.95f}, {5.6f, 0.57f, 1.5f}, {4.0f, 0.9f, 1.36f}};
+constexpr TileTimes kF32Times[] = {{4.3f, 0.54f, 1.1f}, {5.5f, 0.88f, 1.85f}};
+constexpr TileTimes kExactTimes[] = {{4.3f, 0.9f, 1.5f}};
+
+// Fewer, larger tiles read less and compute at a higher rate; more of them,
+// and parts of the columns, fill the card.  A part's sums cost a round trip
+// through memory (7 TB/s, most of it in the card's cache) and another launch.
+void plan_tiles(const cev_fp8_desc& d, Form& f) {
+  const bool exact = !d.gate_up && d.out_dtype == CEV_F32, e8m0 = d.scales == CEV_FP8_SCALES_E8M0;
+  const TileTimes* const times = exact ? kExactTimes : e8m0 ? kE8m0Times : kF32Times;
+  const int kinds = exact ? 1 : e8m0 ? 3 : 2;
+  const double sums = (double)d.t * f.groups * kFp8Group * 4;  // bytes of one part's
+  double best = 1e300;
+  for (int i = 0; i < kinds; ++i) {
+    const int tt = 4 << i;
+    const double tiles = (double)((d.t + 16 * tt - 1) / (16 * tt)) * (f.groups / kFp8TileGroups);
+    for (int p = 1; p <= 16; p *= 2) {
+      const int blocks = ((f.kb + p - 1) / p + 3) & ~3, parts = (f.kb + blocks - 1) / blocks;
+      if (p > 1 && blocks < 8) break;
+      const double wgs = tiles * parts, room = tt == 16 ? 256 : 512;  // workgroups that run together
+      // up to a full card the others' reads slow a block down by and by; beyond, CUs take turns
+      double block = times[i].one;
+      if (wgs > room)
+        block = times[i].two * std::ceil(wgs / 256) * 256 / room;
+      else if (tt == 16 || wgs > 256)
+        block += (times[i].two - times[i].one) * wgs / room;
+      // (a tile's start and end: under the other workgroup's blocks, where a CU has one)
+      const double turns = std::ceil(wgs / room);
+      const double starts = tt == 16 ? (d.gate_up ? 9.0 : 5.5) * turns : times[i].fixed * (0.5 * turns - 0.5);
+      const double us = times[i].fixed + starts + blocks * block + (parts > 1 ? 3.0 + 2 * parts * sums / 7e6 : 0.0);
+      if (us < best) {
+        best = us;
+        f.tt = tt, f.parts = parts, f.blocks_part = blocks;
+      }
+    }
+  }
+}
+
 Form form_of(const cev_fp8_desc& d) {
   Form f{};
   f.kb = (int32_t)((d.k + 127) / 128);
   f.groups = (int32_t)(d.gate_up ? (d.n + 127) / 128 * 8 : (d.n + 255) / 256 * 8);
-  const int64_t tiles = (d.t + 31) / 32;
-  f.pack_x = d.x_dtype != CEV_E4M3 && tiles > 1;
+  f.parts = 1;
+  f.blocks_part = f.kb;
+  // Up to 16 rows the kernel for few streams the weight faster (8 rows x 4096
+  // x 4096: 6.6 us against 12), up to 32 in one launch where the columns are
+  // few enough that the rows' own reads do not count (32 x 4096 x 2048: 7.4 us
+  // against 9.2; x 12288: 19.8 against 15.3; gate and up, two launches here
+  // too, 32 x 6144 x 2048: 18.3 against 11.7).
+  if ((d.t > 32 || (d.t > 16 && (f.kb > 32 || d.gate_up))) && f.kb <= kTileBlocks) plan_tiles(d, f);
+  f.pack_x = d.x_dtype != CEV_E4M3 && (d.t > 16 || f.tt > 0);
   if (f.pack_x) {
     f.rows_bytes = up256((size_t)d.t * f.kb * kFp8Block);
     f.scales_bytes = up256((size_t)d.t * f.kb);
   }
-  f.parts = 1;
-  f.blocks_part = f.kb;
-  if (d.gate_up) f.part_bytes = (size_t)f.parts * d.t * f.groups * kFp8Group * 4;
+  if (f.parts > 1)
+    f.part_bytes = (size_t)f.parts * d.t * f.groups * kFp8Group * 4;
+  else if (d.gate_up && f.tt == 0)
+    f.part_bytes = (size_t)d.t * ((d.n + 127) / 128) * 128 * 4;
   return f;
 }
 
@@ -268,22 +298,23 @@ int32_t check_desc(const char* what, const cev_fp8_desc* d) {
   return CEV_OK;
 }
 
-template <typename T, typename O>
-int32_t launch_small(const ProductArgs& a, bool e8m0, hipStream_t s) {
-  const int64_t grid = (a.t + 31) / 32 * a.parts * a.groups;
+template <typename T, typename O, bool GATE_UP, int MT>
+int32_t launch_small(const Fp8Args& a, bool e8m0, hipStream_t s) {
+  const int64_t col_tiles = (a.n + 15) / 16, grid = (a.t + 16 * MT - 1) / (16 * MT) * col_tiles;
   if (grid > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_product: grid too large");
   if (e8m0)
-    hipLaunchKernelGGL((fp8_small_kernel<T, O, true>), dim3((unsigned)grid), dim3(kWaves * 64), 0, s, a);
+    hipLaunchKernelGGL((fp8_small_kernel<T, O, true, GATE_UP, MT>), dim3((unsigned)grid), dim3(kWaves * 64), 0, s, a, (unsigned)col_tiles);
   else
-    hipLaunchKernelGGL((fp8_small_kernel<T, O, false>), dim3((unsigned)grid), dim3(kWaves * 64), 0, s, a);
+    hipLaunchKernelGGL((fp8_small_kernel<T, O, false, GATE_UP, MT>), dim3((unsigned)grid), dim3(kWaves * 64), 0, s, a, (unsigned)col_tiles);
   return launched("cev_fp8_product");
 }
 
-template <typename O>
-int32_t launch_small(const ProductArgs& a, int x_dtype, bool e8m0, hipStream_t s) {
-  if (x_dtype == CEV_E4M3) return launch_small<uint8_t, O>(a, e8m0, s);
-  if (x_dtype == CEV_BF16) return launch_small<__bf16, O>(a, e8m0, s);
-  return launch_small<float, O>(a, e8m0, s);
+template <typename O, bool GATE_UP>
+int32_t launch_small(const Fp8Args& a, int x_dtype, bool e8m0, hipStream_t s) {
+  if (x_dtype == CEV_BF16) return launch_small<__bf16, O, GATE_UP, 1>(a, e8m0, s);
+  if (x_dtype == CEV_F32) return launch_small<float, O, GATE_UP, 1>(a, e8m0, s);
+  if (a.t <= 16) return launch_small<uint8_t, O, GATE_UP, 1>(a, e8m0, s);
+  return launch_small<uint8_t, O, GATE_UP, 2>(a, e8m0, s);
 }
 
 }  // namespace
@@ -293,6 +324,15 @@ extern "C" int32_t cev_fp8_work_size(const cev_fp8_desc* d, size_t* bytes) {
   CEV_CHECK_ARG(bytes != nullptr, "cev_fp8_work_size: null output");
   const Form f = form_of(*d);
   *bytes = f.rows_bytes + f.scales_bytes + f.part_bytes;
+  return CEV_OK;
+}
+
+extern "C" int32_t cev_fp8_form(const cev_fp8_desc* d, int32_t* rows, int32_t* parts) {
+  if (const int32_t rc = check_desc("cev_fp8_form", d)) return rc;
+  CEV_CHECK_ARG(rows && parts, "cev_fp8_form: null output");
+  const Form f = form_of(*d);
+  *rows = 16 * f.tt;
+  *parts = f.parts;
   return CEV_OK;
 }
 
@@ -325,7 +365,7 @@ extern "C" int32_t cev_fp8_product(const cev_fp8_desc* d, const void* x, const v
   const hipStream_t s = (hipStream_t)stream;
   uint8_t* const space = (uint8_t*)work;
   int x_dtype = d->x_dtype;
-  ProductArgs a{};
+  Fp8Args a{};
   a.x = x, a.xs = (const uint8_t*)x_scales;
   a.x_st = d->t > 1 ? d->x_stride : 0;
   if (f.pack_x) {
@@ -334,12 +374,20 @@ extern "C" int32_t cev_fp8_product(const cev_fp8_desc* d, const void* x, const v
     x_dtype = CEV_E4M3;
   }
   a.w = (const uint8_t*)weight;
-  a.ws = (const uint32_t*)(a.w + (int64_t)f.groups * f.kb * kFp8GroupBytes);
+  a.ws = a.w + (int64_t)f.groups * f.kb * kFp8GroupBytes;
+  a.ws_pitch = d->scales == CEV_FP8_SCALES_E8M0 ? (f.kb + 3) & ~3 : f.kb;
   a.out = out, a.out_st = d->t > 1 ? d->out_stride : 0;
   a.t = d->t, a.n = d->n, a.k = (int32_t)d->k, a.kb = f.kb, a.groups = f.groups, a.parts = f.parts, a.blocks_part = f.blocks_part;
   if (f.part_bytes) a.part = (float*)(space + f.rows_bytes + f.scales_bytes);
   const bool e8m0 = d->scales == CEV_FP8_SCALES_E8M0;
-  const int32_t rc = d->out_dtype == CEV_F32 ? launch_small<float>(a, x_dtype, e8m0, s) : launch_small<__bf16>(a, x_dtype, e8m0, s);
+  a.out_s = (uint8_t*)out_scales;
+  if (d->gate_up && f.tt == 0) {
+    a.out_st = (d->n + 127) / 128 * 128;
+    if (const int32_t rc = launch_small<float, true>(a, x_dtype, e8m0, s)) return rc;
+    return cev_fp8_rows(CEV_F32, d->t, d->n, a.part, a.out_st, out, out_scales, stream);
+  }
+  const int32_t rc = f.tt > 0 ? fp8_launch_tile(a, f.tt, !d->gate_up && d->out_dtype == CEV_F32, e8m0, d->gate_up != 0, s)
+                     : d->out_dtype == CEV_F32 ? launch_small<float, false>(a, x_dtype, e8m0, s) : launch_small<__bf16, false>(a, x_dtype, e8m0, s);
   if (rc || !a.part) return rc;
   JoinArgs j{a.part, out, (uint8_t*)out_scales, d->t, d->n, a.out_st, (int64_t)f.groups * kFp8Group, f.parts, 0};
   j.quads = (int32_t)(d->gate_up ? (d->n + 127) / 128 * 16 : (d->n + 3) / 4);

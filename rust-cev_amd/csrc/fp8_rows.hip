@@ -251,7 +251,10 @@ __global__ __launch_bounds__(kThreads) void fp8_pack_kernel(PackArgs a) {
       const int64_t at = (row0 / kFp8Block) * a.lds[which] + kb;
       s = a.f32_scales ? ((const uint32_t*)a.s[which])[at] : ((const uint8_t*)a.s[which])[at];
     }
-    a.out_s[group * a.kb + kb] = s;
+    if (a.f32_scales)
+      a.out_s[group * a.kb + kb] = s;
+    else  // bytes, a group's blocks up to a multiple of 4
+      ((uint8_t*)a.out_s)[group * ((a.kb + 3) & ~3) + kb] = (uint8_t)s;
   }
 }
 

@@ -273,6 +273,32 @@ def test_norm_of_rows_that_are_zero_or_not_finite(gpu):
 # ---------------------------------------------------------------------------
 # Products
 
+
+def form_of(t, n, k, kind, out=torch.bfloat16, gate_up=False):
+    """(rows of a tile, parts of the columns) of the kernel that runs it; 0 rows: the kernel for few."""
+    import ctypes as C
+    from cev_hip import _abi
+    d = _abi.Fp8Desc(x_dtype=2, out_dtype=2 if gate_up else 0 if out == torch.float32 else 1, scales=0 if kind == "e8m0" else 1, gate_up=gate_up,
+                     t=t, n=n, k=k, x_stride=k, out_stride=n)
+    rows, parts = C.c_int32(), C.c_int32()
+    _abi.check(_abi.lib().cev_fp8_form(C.byref(d), C.byref(rows), C.byref(parts)))
+    return rows.value, parts.value
+
+
+def test_every_kernel_is_among_the_tested_products(cev):
+    forms = {(kind,) + form_of(t, n, k, kind) for kind in ("e8m0", "f32") for t, n, k in PRODUCTS + LARGE}
+    rows = {f[:2] for f in forms}
+    assert rows >= {("e8m0", 0), ("e8m0", 64), ("e8m0", 128), ("e8m0", 256), ("f32", 0), ("f32", 64), ("f32", 128)}, forms
+    assert {f[2] for f in forms} >= {1, 2} and max(f[2] for f in forms) > 2, forms
+    exact = {(kind,) + form_of(t, n, k, kind, torch.float32) for kind in ("e8m0", "f32") for t, n, k in PRODUCTS}
+    assert {f[1] for f in exact} == {0, 64} and max(f[2] for f in exact) > 2, exact
+    gate = {(kind,) + form_of(t, n, k, kind, gate_up=True) for kind in ("e8m0", "f32") for t, n, k in GATE_UPS + [LARGE_GATE_UP]}
+    assert {f[:2] for f in gate} >= {("e8m0", 0), ("e8m0", 64), ("e8m0", 128), ("e8m0", 256), ("f32", 0), ("f32", 64), ("f32", 128)}, gate
+    assert max(f[2] for f in gate) > 1, gate
+
+
+LARGE = [(2048, 4096, 2048), (1030, 8320, 264), (4096, 4000, 4104), (400, 4096, 6144)]
+LARGE_GATE_UP = (2048, 12288, 4096)
 PRODUCTS = [(1, 1, 1), (1, 40, 128), (2, 256, 136), (7, 129, 1000), (16, 300, 520), (31, 64, 2048), (32, 1000, 264), (33, 257, 384), (64, 512, 1280),
             (100, 136, 4104), (129, 520, 640), (257, 1000, 392), (400, 384, 1152), (1, 2048, 6144), (300, 2048, 256)]
 
@@ -296,7 +322,21 @@ def test_linear(gpu, t, n, k, given, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("t,n,k", [(1, 128, 128), (5, 200, 300), (40, 96, 512), (200, 384, 640), (600, 520, 1032), (1000, 1300, 520)])
+@pytest.mark.parametrize("kind", ["e8m0", "f32"])
+@pytest.mark.parametrize("t,n,k", LARGE)
+def test_linear_large(gpu, t, n, k, kind):
+    """Several tiles in each direction, last ones in part: rows and columns drawn from all of them."""
+    x, w = activations(t, k, torch.bfloat16, 7), weight_of(n, k, kind, 8)
+    q, e = oracle_rows(x)
+    at_t = torch.cat([torch.randint(0, t, (60,), generator=gen(1)), torch.tensor([0, t - 1])])
+    at_n = torch.cat([torch.randint(0, n, (60,), generator=gen(2)), torch.tensor([0, n - 1])])
+    y = cev_hip.linear_fp8(x.to(gpu), packed(w, gpu)).cpu()[at_t][:, at_n]
+    xv = (q * torch.exp2(e).repeat_interleave(128, 1))[:, :k]
+    check_product(y, xv[at_t], weight_values(*w)[at_n], torch.bfloat16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,n,k", [(1, 128, 128), (5, 200, 300), (40, 96, 512), (200, 384, 640), (600, 520, 1032), (1000, 1300, 520), (2048, 4096, 260), (1100, 4096, 520), (64, 256, 4096)])
 def test_linear_of_integers_is_exact(gpu, t, n, k):
     g = gen(9)
     x = torch.randint(-8, 9, (t, k), generator=g).float()
@@ -310,11 +350,13 @@ def test_linear_of_integers_is_exact(gpu, t, n, k):
         for operand in (rows, x.to(gpu) if k % 4 == 0 else rows):
             y = cev_hip.linear_fp8(operand, w, out_dtype=torch.float32)
             assert torch.equal(y.double().cpu(), want)
+            # (products of at most 64 within 2^13 of each other: nothing is cut)
+            assert torch.equal(cev_hip.linear_fp8(operand, w, out_dtype=torch.bfloat16).cpu(), want.float().bfloat16())
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["e8m0", "f32"])
-@pytest.mark.parametrize("t", [1, 20, 70, 300, 700])
+@pytest.mark.parametrize("t", [1, 20, 70, 300, 700, 5000])
 def test_linear_nan_and_infinity_stay_in_their_rows(gpu, t, kind):
     x, w = activations(t, 520, torch.bfloat16, 10), weight_of(300, 520, kind, 11)
     clean = cev_hip.linear_fp8(x.to(gpu), packed(w, gpu)).cpu()
@@ -371,11 +413,14 @@ def test_no_rows(gpu):
 # Gate and up
 
 
+GATE_UPS = [(1, 1, 8), (1, 256, 128), (3, 130, 264), (16, 1000, 512), (20, 136, 4104), (33, 128, 1032), (65, 300, 640), (130, 520, 384), (300, 384, 256), (513, 640, 520),
+            (260, 5130, 264), (1030, 4100, 200)]
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["e8m0", "f32"])
 @pytest.mark.parametrize("given", ["rows", torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("t,n,k", [(1, 1, 8), (1, 256, 128), (3, 130, 264), (16, 1000, 512), (33, 128, 1032), (65, 300, 640), (130, 520, 384), (300, 384, 256),
-                                   (513, 640, 520)])
+@pytest.mark.parametrize("t,n,k", GATE_UPS)
 def test_gate_up(gpu, t, n, k, given, kind):
     x = activations(t, k, torch.float32 if given == "rows" else given, 15)
     x *= 1.5 / math.sqrt(k)
@@ -405,6 +450,30 @@ def test_gate_up(gpu, t, n, k, given, kind):
     # the bound is wide where sums are long: nearly all values are the nearest of the exact ones.  On data like these the
     # cut leaves each product within 2^-13 of itself, so of values 2^-4 of themselves apart at least 2 * 2 * 2^-13 / 2^-4 may fall to the other side
     assert float((q[:, :n] != round_e4m3(v[:, :n].clamp(-448, 448))).double().mean()) <= 2.0 ** -7 + 2 / q.numel()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["e8m0", "f32"])
+def test_gate_up_of_many_tiles(gpu, kind):
+    """Rows and blocks of columns drawn from all tiles of a wide layer."""
+    t, n, k = LARGE_GATE_UP
+    g = torch.Generator(device=gpu).manual_seed(36)
+    x = torch.randn(t, k, generator=g, device=gpu) * 0.03
+    weights = [((torch.randn(n, k, generator=g, device=gpu) * 100).clamp(-448, 448).to(E4M3), weight_of(n, k, kind, 37 + i)[1].to(gpu)) for i in range(2)]
+    rows = cev_hip.fp8_rows(x)
+    got = cev_hip.gate_up_fp8(rows, Fp8Weight.gate_up(*weights))
+    at = torch.tensor([0, 1, 127, 128, 255, 256, 300, 1000, 1023, 1024, 2000, 2047])
+    blocks = [0, 1, 31, 64, 95]
+    xv = values(rows.q[at.to(gpu)].cpu(), rows.s[at.to(gpu)].cpu())
+    for b in blocks:
+        cols = slice(128 * b, 128 * b + 128)
+        wv = [q[cols].cpu().double() * s[b].cpu().double().repeat_interleave(128) for q, s in weights]
+        gv, uv = xv @ wv[0].t(), xv @ wv[1].t()
+        want = gv * torch.sigmoid(gv) * uv
+        have = (got.q[:, cols].cpu()[at].double() * got.s[:, b].cpu()[at].double()[:, None])
+        # half a step of e4m3 (2^-4 of the value, 2^-10 of the scale), and the sums' 2^-13 of a typical size
+        tol = want.abs() * 2.0 ** -4 + want.abs().amax(1, keepdim=True) * (2.0 ** -17 + 2.0 ** -11)
+        assert bool(((have - want).abs() <= tol).all()), b
 
 
 @pytest.mark.gpu
