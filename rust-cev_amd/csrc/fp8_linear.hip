@@ -4,15 +4,15 @@
 //
 // Two kinds of matrix product, by the output's type:
 //
-//   bf16, e4m3  v_mfma_scale_f32_32x32x64_f8f6f4, which takes 2^e as an operand
+//   bf16, e4m3  v_mfma_scale_f32_16x16x128_f8f6f4, which takes 2^e as an operand
 //               (and s where it is a power of two; an f32 s multiplies the
-//               block's 32 x 32 results).  It adds eight neighbouring columns'
+//               block's 16 x 16 results).  It adds eight neighbouring columns'
 //               products after cutting each towards zero to a multiple of
 //               2^(E - 13), 2^E the largest one's power of two (measured bit by
 //               bit); what follows is f32.  A sum is therefore up to 7 * 2^-13
 //               of its largest products off; on normal data it is 4.5e-5 of
 //               the result, a fortieth of bf16's rounding.
-//   f32         v_mfma_f32_32x32x16_bf16 on the same values in bf16, which holds
+//   f32         v_mfma_f32_16x16x32_bf16 on the same values in bf16, which holds
 //               them exactly: products and sums in f32, at half the rate.
 #include <algorithm>
 #include <cmath>
@@ -21,59 +21,45 @@
 
 namespace {
 
-constexpr int kWaves = 16;  // waves of a workgroup of the kernel for few rows, each with its share of the column blocks
+constexpr int kWaves = 8;  // waves of a workgroup of the kernel for few rows, each with its share of the column blocks
 
-// The lane's share of block kb of its row (columns 32 quad .. + 31), and the
-// row's scale.  Rows in the model's type are brought into e4m3 on the way: the
-// four lanes of a row hold the whole block.
-template <typename T>
-__device__ __forceinline__ void load_x(const Fp8Args& a, int64_t row, int kb, int quad, i32x8& o, int& sc) {
-  if constexpr (sizeof(T) == 1) {
-    const uint8_t* const p = (const uint8_t*)a.x + (row * a.kb + kb) * kFp8Block + quad * 32;
-    o = fp8_join(*(const u32x4_t*)p, *(const u32x4_t*)(p + 16));
-    sc = a.xs[row * a.kb + kb];
-  } else {
-    float v[4][8];
-    uint32_t top = 0;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int col = kb * kFp8Block + quad * 32 + c * 8;
-      load8((const T*)a.x + row * a.x_st + (col < a.k ? col : 0), a.k - col, v[c]);
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, fp8_size(v[c][j]));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-    const uint32_t code = fp8_code(top);
-    const float f = fp8_inverse(code);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      o[2 * c] = (int)fp8_pack4(v[c][0] * f, v[c][1] * f, v[c][2] * f, v[c][3] * f);
-      o[2 * c + 1] = (int)fp8_pack4(v[c][4] * f, v[c][5] * f, v[c][6] * f, v[c][7] * f);
-    }
-    sc = (int)code;
-  }
-}
+// Where 16 bytes of a staged block of 16 rows x 128 columns stand: rows of 128
+// bytes, their pieces in an order of their own, so that neither a store nor an
+// operand's read meets a bank twice.
+__device__ __forceinline__ int staged(int r, int piece) { return r * 128 + ((piece ^ ((r >> 1) + 2)) & 7) * 16; }
 
 // 16 MT rows times 16 weight rows (GATE_UP: times 16 of gate and of up).  The
 // weight streams through once, so what counts is how much of it is on the way:
-// a workgroup holds few weight rows and its 16 waves share the column blocks,
-// each with DEEP of them under way; their sums are joined in LDS, in the waves'
+// a workgroup holds few weight rows and its waves share the column blocks, each
+// with DEEP of them under way; their sums are joined in LDS, in the waves'
 // order.  (Parts of the columns in other workgroups would cost a second launch.)
+// An operand's lanes hold 16 rows, and a load by that pattern costs the L1 16
+// lines; so a wave loads its rows in memory's order and turns them in LDS (16
+// rows x 12288 x 4096 12.3 us before, 10.0 after, 5.1 TB/s; 64 x 4096 x 4096 14.2
+// and 8.1).  Rows in the model's type go into e4m3 on the way.  Eight waves, as
+// with sixteen a CU holds one workgroup and waits for its slowest wave (14.1 us
+// instead of 12.3).
 template <typename T, typename O, bool E8M0, bool GATE_UP, int MT>
-__global__ __launch_bounds__(kWaves * 64) void fp8_small_kernel(Fp8Args a, unsigned col_tiles) {
-  constexpr int NH = GATE_UP ? 2 : 1, DEEP = sizeof(T) == 1 ? (MT == 1 ? 4 : 2) : GATE_UP ? 1 : 2;
+__global__ __launch_bounds__(kWaves * 64, 4) void fp8_small_kernel(Fp8Args a, unsigned col_tiles) {
+  constexpr bool PACK = sizeof(T) > 1;
+  constexpr int NH = GATE_UP ? 2 : 1, DEEP = (PACK ? 2 : 4 / MT) / NH;
   constexpr bool EXACT = sizeof(O) == 4 && !GATE_UP;
   constexpr int QUAD = 80;  // floats of a quad's 16 rows x 4 columns, and 16 more: the sums' reads fall on different banks
-  __shared__ __align__(16) float sums[kWaves][NH * MT][4 * QUAD];
+  constexpr int STAGE = DEEP * MT * 2048, SUMS = NH * MT * 4 * QUAD * 4;
+  __shared__ __align__(16) uint8_t space[kWaves][STAGE > SUMS ? STAGE : SUMS];  // a wave's rows, then its sums
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4, l16 = lane & 15;
   const unsigned row_tile = blockIdx.x / col_tiles, c16 = blockIdx.x - row_tile * col_tiles;  // 16 MT rows, 16 columns
-  const int64_t tile = row_tile;
-  int64_t row[MT];
+  const int64_t row0 = (int64_t)row_tile * (16 * MT);
+  uint8_t* const own = space[wave];
+  // what the lane loads: PACK, 8 values of rows 4 j + lane / 16, else 16 bytes of rows 8 j + lane / 8
+  constexpr int LOADS = PACK ? 4 : 2 * MT, LANES = PACK ? 16 : 8;
+  const uint8_t* xp[LOADS];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) row[i] = min((tile * MT + i) * 16 + l16, a.t - 1);
+  for (int j = 0; j < LOADS; ++j) {
+    const int64_t row = min(row0 + j * (64 / LANES) + lane / LANES, a.t - 1);
+    xp[j] = (const uint8_t*)a.x + (PACK ? row * a.x_st * (int64_t)sizeof(T) : row * a.kb * kFp8Block);
+  }
+  const uint8_t* const sp = PACK ? nullptr : a.xs + min(row0 + lane / DEEP, a.t - 1) * a.kb;
   // the group of 32 weight rows (gate's; up's follows), and the lane's place in its half
   const int64_t group = (int64_t)(c16 >> 1) * NH;
   const uint8_t* const wp = a.w + group * a.kb * kFp8GroupBytes + (quad >> 1) * 2048 + (quad & 1) * 512 + (c16 & 1) * 256 + l16 * 16;
@@ -82,15 +68,27 @@ __global__ __launch_bounds__(kWaves * 64) void fp8_small_kernel(Fp8Args a, unsig
   for (int h = 0; h < NH; ++h)
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[h][i] = f32x4{};
-  for (int kb0 = wave; kb0 < a.kb; kb0 += kWaves * DEEP) {
+  const int share = (a.kb + kWaves - 1) / kWaves, end = min(a.kb, (wave + 1) * share);
+  for (int kb0 = wave * share; kb0 < end; kb0 += DEEP) {
     u32x4_t w[DEEP][NH][2];
     uint32_t sw[DEEP][NH];
-    i32x8 x[DEEP][MT];
-    int sx[DEEP][MT];
+    u32x4_t x[DEEP][LOADS];
+    float v[DEEP][LOADS][8];
+    int codes = 127;
+    if constexpr (!PACK) codes = sp[min(kb0 + lane % DEEP, a.kb - 1)];
 #pragma unroll
     for (int d = 0; d < DEEP; ++d) {
-      const int kb = kb0 + d * kWaves;
-      if (kb >= a.kb) break;
+      const int kb = kb0 + d;
+      if (kb >= end) break;
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        if constexpr (PACK) {
+          const int col = kb * kFp8Block + l16 * 8;
+          load8((const T*)xp[j] + (col < a.k ? col : 0), a.k - col, v[d][j]);
+        } else {
+          x[d][j] = *(const u32x4_t*)(xp[j] + (int64_t)kb * kFp8Block + lane % LANES * 16);
+        }
+      }
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
         const uint8_t* const p = wp + ((int64_t)h * a.kb + kb) * kFp8GroupBytes;
@@ -99,12 +97,39 @@ __global__ __launch_bounds__(kWaves * 64) void fp8_small_kernel(Fp8Args a, unsig
         const int64_t at = (group + h) * a.ws_pitch + kb;
         sw[d][h] = E8M0 ? a.ws[at] : ((const uint32_t*)a.ws)[at];
       }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) load_x<T>(a, row[i], kb, quad, x[d][i], sx[d][i]);
     }
+    int sx[DEEP][MT];
 #pragma unroll
     for (int d = 0; d < DEEP; ++d) {
-      if (kb0 + d * kWaves >= a.kb) break;
+      if (kb0 + d >= end) break;
+      uint8_t* const at = own + d * MT * 2048;
+      if constexpr (PACK) {
+        uint32_t code[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * j + quad;
+          *(u32x2_t*)(at + staged(r, l16 >> 1) + (l16 & 1) * 8) = fp8_block16(v[d][j], code[j]);
+        }
+        // row r's scale is in the lanes 16 (r % 4) .. + 15, as their code[r / 4]
+        const uint32_t c = (l16 & 2) ? (l16 & 1) ? code[3] : code[2] : (l16 & 1) ? code[1] : code[0];
+        sx[d][0] = __shfl((int)c, (l16 & 3) * 16 + (l16 >> 2), 64);
+      } else {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) *(u32x4_t*)(at + (j >> 1) * 2048 + staged((j & 1) * 8 + (lane >> 3), lane & 7)) = x[d][j];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sx[d][i] = __shfl(codes, (i * 16 + l16) * DEEP + d, 64);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the wave's own stores: LDS takes them in order)
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d) {
+      if (kb0 + d >= end) break;
+      i32x8 xv[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const uint8_t* const at = own + (d * MT + i) * 2048;
+        xv[i] = fp8_join(*(const u32x4_t*)(at + staged(l16, 2 * quad)), *(const u32x4_t*)(at + staged(l16, 2 * quad + 1)));
+      }
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
         const i32x8 wv = fp8_join(w[d][h][0], w[d][h][1]);
@@ -115,37 +140,38 @@ __global__ __launch_bounds__(kWaves * 64) void fp8_small_kernel(Fp8Args a, unsig
             f32x4 p = {};
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(wv[2 * c], wv[2 * c + 1]), fp8_widen(x[d][i][2 * c], x[d][i][2 * c + 1]), p, 0, 0, 0);
+              p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(wv[2 * c], wv[2 * c + 1]), fp8_widen(xv[i][2 * c], xv[i][2 * c + 1]), p, 0, 0, 0);
             const float s = f * fp8_scale_value((uint32_t)sx[d][i]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[h][i][r] = __builtin_fmaf(p[r], s, acc[h][i][r]);
           } else if constexpr (E8M0) {
-            acc[h][i] = fp8_mfma(wv, x[d][i], acc[h][i], (int)sw[d][h], sx[d][i]);
+            acc[h][i] = fp8_mfma(wv, xv[i], acc[h][i], (int)sw[d][h], sx[d][i]);
           } else {
-            const f32x4 p = fp8_mfma(wv, x[d][i], f32x4{}, 127, sx[d][i]);
+            const f32x4 p = fp8_mfma(wv, xv[i], f32x4{}, 127, sx[d][i]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[h][i][r] = __builtin_fmaf(p[r], f, acc[h][i][r]);
           }
         }
       }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
   // lane l holds row l % 16, columns 4 (l / 16) .. + 3
 #pragma unroll
   for (int h = 0; h < NH; ++h)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) *(f32x4*)&sums[wave][h * MT + i][quad * QUAD + l16 * 4] = acc[h][i];
+    for (int i = 0; i < MT; ++i) *(f32x4*)((float*)own + (h * MT + i) * 4 * QUAD + quad * QUAD + l16 * 4) = acc[h][i];
   __syncthreads();
   for (int e = threadIdx.x; e < MT * 256; e += kWaves * 64) {
-    const int i = e >> 8, r = (e >> 4) & 15, n = e & 15, at = (n >> 2) * QUAD + r * 4 + (n & 3);
+    const int i = e >> 8, r = (e >> 4) & 15, n = e & 15, at = i * 4 * QUAD + (n >> 2) * QUAD + r * 4 + (n & 3);
     float v[NH];
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
-      v[h] = sums[0][h * MT + i][at];
+      v[h] = ((const float*)space[0])[h * MT * 4 * QUAD + at];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) v[h] += sums[w][h * MT + i][at];
+      for (int w = 1; w < kWaves; ++w) v[h] += ((const float*)space[w])[h * MT * 4 * QUAD + at];
     }
-    const int64_t out_row = (tile * MT + i) * 16 + r, col = (int64_t)c16 * 16 + n;
+    const int64_t out_row = row0 + i * 16 + r, col = (int64_t)c16 * 16 + n;
     if (out_row >= a.t || col >= a.n) continue;
     if constexpr (GATE_UP)
       a.part[out_row * a.out_st + col] = fp8_swiglu(v[0], v[1]);
@@ -225,17 +251,29 @@ struct TileTimes {
 };
 constexpr TileTimes kE8m0Times[] = {{4.0f, 0.45f, 0.95f}, {5.6f, 0.57f, 1.5f}, {4.0f, 0.9f, 1.36f}};
 constexpr TileTimes kF32Times[] = {{4.3f, 0.54f, 1.1f}, {5.5f, 0.88f, 1.85f}};
-constexpr TileTimes kExactTimes[] = {{4.3f, 0.9f, 1.5f}};
+constexpr TileTimes kExactTimes[] = {{4.3f, 1.28f, 2.0f}};
 
-// Fewer, larger tiles read less and compute at a higher rate; more of them,
-// and parts of the columns, fill the card.  A part's sums cost a round trip
-// through memory (7 TB/s, most of it in the card's cache) and another launch.
-void plan_tiles(const cev_fp8_desc& d, Form& f) {
+// 32 rows x 16 weight rows x a block of columns of the kernel for few rows,
+// which reads its rows again for every 16 weight rows.
+double units_of(const cev_fp8_desc& d, int32_t kb) { return (double)((d.t + 31) / 32) * ((d.n + 15) / 16) * kb; }
+
+// Which kernel, with which tile, by the time that each would take.  The one for
+// few rows streams the weight at the card's rate (16 rows x 12288 x 4096: 10 us
+// against 14), and is ahead as long as its repeated reads of the rows cost less
+// than the other's slow start (12288 x 4096: 32 rows 10.6 us against 15.4, 64
+// rows 17.6 against 17.3, 256 rows 58.6 against 20.2; 4096 x 4096: 128 rows 12.1
+// against 15.4).  Of the other's tiles, fewer and larger ones read less and
+// compute at a higher rate; more of them, and parts of the columns, fill the
+// card.  A part's sums cost a round trip through memory (7 TB/s, most of it in
+// the card's cache) and another launch.
+void plan(const cev_fp8_desc& d, Form& f) {
   const bool exact = !d.gate_up && d.out_dtype == CEV_F32, e8m0 = d.scales == CEV_FP8_SCALES_E8M0;
+  double best = 1e-3 * units_of(d, f.kb) * (d.gate_up ? 0.57 : exact ? 0.33 : 0.30) + (d.gate_up ? 6.8 : exact ? 3.0 : 2.6);
   const TileTimes* const times = exact ? kExactTimes : e8m0 ? kE8m0Times : kF32Times;
-  const int kinds = exact ? 1 : e8m0 ? 3 : 2;
+  // (it reads the rows' scales four at a time, so that there have to be four;
+  // up to 16 rows it is never the faster one by more than the model's error)
+  const int kinds = d.t <= 16 || f.kb > kTileBlocks ? 0 : exact ? 1 : e8m0 ? 3 : 2;
   const double sums = (double)d.t * f.groups * kFp8Group * 4;  // bytes of one part's
-  double best = 1e300;
   for (int i = 0; i < kinds; ++i) {
     const int tt = 4 << i;
     const double tiles = (double)((d.t + 16 * tt - 1) / (16 * tt)) * (f.groups / kFp8TileGroups);
@@ -267,13 +305,11 @@ Form form_of(const cev_fp8_desc& d) {
   f.groups = (int32_t)(d.gate_up ? (d.n + 127) / 128 * 8 : (d.n + 255) / 256 * 8);
   f.parts = 1;
   f.blocks_part = f.kb;
-  // Up to 16 rows the kernel for few streams the weight faster (8 rows x 4096
-  // x 4096: 6.6 us against 12), up to 32 in one launch where the columns are
-  // few enough that the rows' own reads do not count (32 x 4096 x 2048: 7.4 us
-  // against 9.2; x 12288: 19.8 against 15.3; gate and up, two launches here
-  // too, 32 x 6144 x 2048: 18.3 against 11.7).
-  if ((d.t > 32 || (d.t > 16 && (f.kb > 32 || d.gate_up))) && f.kb <= kTileBlocks) plan_tiles(d, f);
-  f.pack_x = d.x_dtype != CEV_E4M3 && (d.t > 16 || f.tt > 0);
+  // The kernel for few rows can bring its 16 rows into e4m3 by itself, over and
+  // over in each workgroup: for small weights that costs less than a launch (16
+  // rows x 4096 x 2048: 5.9 us against 6.9; x 12288 x 4096: 22 against 14).
+  f.pack_x = d.x_dtype != CEV_E4M3 && (d.t > 16 || units_of(d, f.kb) > 4096);
+  if (d.x_dtype == CEV_E4M3 || f.pack_x) plan(d, f);
   if (f.pack_x) {
     f.rows_bytes = up256((size_t)d.t * f.kb * kFp8Block);
     f.scales_bytes = up256((size_t)d.t * f.kb);

@@ -15,7 +15,6 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRowChunks = 4;  // chunks of 8 columns of a thread
 
 struct RowsArgs {
   const void* x;
@@ -26,32 +25,21 @@ struct RowsArgs {
   int32_t rows_wg;    // rows of a workgroup (1: a part of a wide row)
 };
 
+// 8 columns a thread (8192 x 4096 bf16: 18.0 us, 5.6 TB/s; 32 columns a thread
+// take 20.4 there and 3.5 instead of 2.4 for one row).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void fp8_rows_kernel(RowsArgs a, int parts) {
-  const int64_t r0 = (int64_t)(blockIdx.x / parts) * a.rows_wg;
-  const int c0 = (int)(blockIdx.x % parts) * (kThreads * kRowChunks);
-  float v[kRowChunks][8];
-  int64_t row[kRowChunks];
-  int col[kRowChunks];
-#pragma unroll
-  for (int b = 0; b < kRowChunks; ++b) {
-    const int i = c0 + b * kThreads + (int)threadIdx.x;
-    const int rr = a.rows_wg > 1 ? i / a.chunks : 0;
-    row[b] = r0 + rr;
-    col[b] = i - rr * a.chunks;
-    const bool on = rr < a.rows_wg && col[b] < a.chunks && row[b] < a.t;
-    if (!on) row[b] = -1;
-    load8((const T*)a.x + (on ? row[b] * a.x_st + (int64_t)col[b] * 8 : 0), on ? a.k - col[b] * 8 : 0, v[b]);
-  }
-#pragma unroll
-  for (int b = 0; b < kRowChunks; ++b) {
-    uint32_t code;
-    const u32x2_t q = fp8_block16(v[b], code);
-    if (row[b] >= 0) {
-      *(u32x2_t*)(a.q + (row[b] * a.chunks + col[b]) * 8) = q;
-      if ((col[b] & 15) == 0) a.s[row[b] * (a.chunks >> 4) + (col[b] >> 4)] = (uint8_t)code;
-    }
-  }
+  const int i = (int)(blockIdx.x % parts) * kThreads + (int)threadIdx.x;
+  const int rr = a.rows_wg > 1 ? i / a.chunks : 0, col = i - rr * a.chunks;
+  const int64_t row = (int64_t)(blockIdx.x / parts) * a.rows_wg + rr;
+  const bool on = rr < a.rows_wg && col < a.chunks && row < a.t;  // (16 lanes of a block alike)
+  float v[8];
+  load8((const T*)a.x + (on ? row * a.x_st + (int64_t)col * 8 : 0), on ? a.k - col * 8 : 0, v);
+  uint32_t code;
+  const u32x2_t q = fp8_block16(v, code);
+  if (!on) return;
+  *(u32x2_t*)(a.q + (row * a.chunks + col) * 8) = q;
+  if ((col & 15) == 0) a.s[row * (a.chunks >> 4) + (col >> 4)] = (uint8_t)code;
 }
 
 struct NormArgs {
@@ -88,9 +76,9 @@ __device__ __forceinline__ void store8(T* p, int have, const float* v) {
 // One row for WAVES waves, NCH chunks of 8 columns a lane in registers; a
 // row wider than that reads its residual a second time.
 template <typename T, int WAVES, int NCH, bool RES>
-__global__ __launch_bounds__(kThreads) void fp8_norm_kernel(NormArgs a) {
-  constexpr int LANES = WAVES * 64, ROWS = kThreads / LANES;
-  __shared__ float part[kThreads / 64];
+__global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : kThreads) void fp8_norm_kernel(NormArgs a) {
+  constexpr int LANES = WAVES * 64, ROWS = WAVES > 4 ? 1 : kThreads / LANES;
+  __shared__ float part[ROWS * WAVES];
   const int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
   const int lane = threadIdx.x % LANES;
   const bool live = r < a.rows;
@@ -132,7 +120,7 @@ __global__ __launch_bounds__(kThreads) void fp8_norm_kernel(NormArgs a) {
     __syncthreads();
     sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) sum += part[w];
+    for (int w = 0; w < WAVES; ++w) sum += part[threadIdx.x / LANES * WAVES + w];
   }
   const float inv = 1.0f / sqrtf(sum / (float)a.k + a.eps);
   auto give = [&](int c, float* o) {  // the row's chunk c, normalised, into e4m3
@@ -284,15 +272,11 @@ extern "C" int32_t cev_fp8_rows(int32_t dtype, int64_t t, int64_t k, const void*
   if (const int32_t rc = check_rows("cev_fp8_rows", dtype, t, k, "x", x, x_stride)) return rc;
   CEV_CHECK_ARG(q && scales && aligned(q, 16), "cev_fp8_rows: null or misaligned output");
   RowsArgs a{x, (uint8_t*)q, (uint8_t*)scales, t, x_stride, (int32_t)k, (int32_t)((k + 127) / 128 * 16), 1};
-  const int most = kThreads * kRowChunks;
-  a.rows_wg = a.chunks >= most ? 1 : most / a.chunks;
-  const int parts = a.chunks > most ? (a.chunks + most - 1) / most : 1;
+  a.rows_wg = a.chunks >= kThreads ? 1 : kThreads / a.chunks;
+  const int parts = a.chunks > kThreads ? (a.chunks + kThreads - 1) / kThreads : 1;
   const int64_t grid = (t + a.rows_wg - 1) / a.rows_wg * parts;
   if (grid > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_rows: too many rows");
-  if (dtype == CEV_BF16)
-    hipLaunchKernelGGL(fp8_rows_kernel<__bf16>, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, a, parts);
-  else
-    hipLaunchKernelGGL(fp8_rows_kernel<float>, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, a, parts);
+  hipLaunchKernelGGL(dtype == CEV_BF16 ? fp8_rows_kernel<__bf16> : fp8_rows_kernel<float>, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, a, parts);
   return launched("cev_fp8_rows");
 }
 
@@ -300,21 +284,29 @@ namespace {
 
 template <typename T, int WAVES, int NCH>
 int32_t launch_norm(const NormArgs& a, hipStream_t s) {
-  const int64_t grid = (a.rows + 4 / WAVES - 1) / (4 / WAVES);
+  constexpr int ROWS = WAVES > 4 ? 1 : 4 / WAVES;
+  const int64_t grid = (a.rows + ROWS - 1) / ROWS;
   if (grid > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_rms_norm: too many rows");
   if (a.h)
-    hipLaunchKernelGGL((fp8_norm_kernel<T, WAVES, NCH, true>), dim3((unsigned)grid), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((fp8_norm_kernel<T, WAVES, NCH, true>), dim3((unsigned)grid), dim3(ROWS * WAVES * 64), 0, s, a);
   else
-    hipLaunchKernelGGL((fp8_norm_kernel<T, WAVES, NCH, false>), dim3((unsigned)grid), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((fp8_norm_kernel<T, WAVES, NCH, false>), dim3((unsigned)grid), dim3(ROWS * WAVES * 64), 0, s, a);
   return launched("cev_fp8_rms_norm");
 }
 
 template <typename T>
 int32_t launch_norm(const NormArgs& a, hipStream_t s) {
+  // A row's chunks of 8 columns go to one lane each; where there are more rows
+  // than fill the card, to as few waves as hold them in registers (us, bf16 with
+  // the residual: 64 x 4096 with 8 waves 3.6, with 4 4.1; 8192 x 4096 42.8
+  // and 41.4; 64 x 12288 with 16 waves 4.9, with 8 5.8; 4096 x 1024 with 4
+  // waves 10.0, with 2 7.7).
   if (a.chunks <= 64) return launch_norm<T, 1, 1>(a, s);
+  const bool few = a.rows <= 512;
+  if (a.chunks <= 128 && !few) return launch_norm<T, 2, 1>(a, s);
   if (a.chunks <= 256) return launch_norm<T, 4, 1>(a, s);
-  if (a.chunks <= 512) return launch_norm<T, 4, 2>(a, s);
-  return launch_norm<T, 4, 4>(a, s);
+  if (a.chunks <= 512) return few ? launch_norm<T, 8, 1>(a, s) : launch_norm<T, 4, 2>(a, s);
+  return few ? launch_norm<T, 16, 1>(a, s) : launch_norm<T, 8, 2>(a, s);
 }
 
 }  // namespace

@@ -258,6 +258,20 @@ def test_norm(gpu, t, k, add, plus_one, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("add", [False, True])
+@pytest.mark.parametrize("t,k", [(515, 512), (514, 1000), (513, 2056), (600, 4096), (513, 4104), (514, 8200), (513, 17000)])
+def test_norm_of_many_rows(gpu, t, k, add, dtype):
+    x, h = activations(t, k, dtype, 3), activations(t, k, dtype, 4)
+    w = (1 + 0.1 * torch.randn(k, generator=gen(5))).to(dtype)
+    xg = x.to(gpu)
+    got = cev_hip.rms_norm_fp8(xg, w.to(gpu), 1e-6, h=h.to(gpu) if add else None)
+    xo, want = oracle_norm(x, w, 1e-6, h if add else None, False)
+    assert torch.equal(xg.double().cpu(), xo)
+    check_rows_near(got, want, (k / 128 + 16) * 2.0 ** -24 + 8 * 2.0 ** -24)  # as above
+
+
+@pytest.mark.gpu
 def test_norm_of_rows_that_are_zero_or_not_finite(gpu):
     x = activations(5, 200, torch.float32, 6)
     x[1] = 0
@@ -292,15 +306,16 @@ def test_every_kernel_is_among_the_tested_products(cev):
     assert {f[2] for f in forms} >= {1, 2} and max(f[2] for f in forms) > 2, forms
     exact = {(kind,) + form_of(t, n, k, kind, torch.float32) for kind in ("e8m0", "f32") for t, n, k in PRODUCTS}
     assert {f[1] for f in exact} == {0, 64} and max(f[2] for f in exact) > 2, exact
-    gate = {(kind,) + form_of(t, n, k, kind, gate_up=True) for kind in ("e8m0", "f32") for t, n, k in GATE_UPS + [LARGE_GATE_UP]}
+    gate = {(kind,) + form_of(t, n, k, kind, gate_up=True) for kind in ("e8m0", "f32") for t, n, k in GATE_UPS + LARGE_GATE_UPS}
     assert {f[:2] for f in gate} >= {("e8m0", 0), ("e8m0", 64), ("e8m0", 128), ("e8m0", 256), ("f32", 0), ("f32", 64), ("f32", 128)}, gate
     assert max(f[2] for f in gate) > 1, gate
 
 
 LARGE = [(2048, 4096, 2048), (1030, 8320, 264), (4096, 4000, 4104), (400, 4096, 6144)]
-LARGE_GATE_UP = (2048, 12288, 4096)
+LARGE_GATE_UPS = [(2048, 12288, 4096), (2048, 12288, 6144)]
 PRODUCTS = [(1, 1, 1), (1, 40, 128), (2, 256, 136), (7, 129, 1000), (16, 300, 520), (31, 64, 2048), (32, 1000, 264), (33, 257, 384), (64, 512, 1280),
-            (100, 136, 4104), (129, 520, 640), (257, 1000, 392), (400, 384, 1152), (1, 2048, 6144), (300, 2048, 256)]
+            (100, 136, 4104), (129, 520, 640), (257, 1000, 392), (400, 384, 1152), (1, 2048, 6144), (300, 2048, 256), (9, 40, 4104),
+            (300, 2000, 6152), (333, 4100, 4104)]
 
 
 @pytest.mark.gpu
@@ -333,6 +348,19 @@ def test_linear_large(gpu, t, n, k, kind):
     y = cev_hip.linear_fp8(x.to(gpu), packed(w, gpu)).cpu()[at_t][:, at_n]
     xv = (q * torch.exp2(e).repeat_interleave(128, 1))[:, :k]
     check_product(y, xv[at_t], weight_values(*w)[at_n], torch.bfloat16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["e8m0", "f32"])
+@pytest.mark.parametrize("t,n,k", [(700, 4100, 2056), (1021, 2056, 4104), (3000, 4100, 1032)])
+def test_linear_large_f32(gpu, t, n, k, kind):
+    x, w = activations(t, k, torch.float32, 7), weight_of(n, k, kind, 8)
+    q, e = oracle_rows(x)
+    at_t = torch.cat([torch.randint(0, t, (60,), generator=gen(1)), torch.tensor([0, t - 1])])
+    at_n = torch.cat([torch.randint(0, n, (60,), generator=gen(2)), torch.tensor([0, n - 1])])
+    y = cev_hip.linear_fp8(x.to(gpu), packed(w, gpu)).cpu()[at_t][:, at_n]
+    xv = (q * torch.exp2(e).repeat_interleave(128, 1))[:, :k]
+    check_product(y, xv[at_t], weight_values(*w)[at_n], torch.float32)
 
 
 @pytest.mark.gpu
@@ -414,7 +442,7 @@ def test_no_rows(gpu):
 
 
 GATE_UPS = [(1, 1, 8), (1, 256, 128), (3, 130, 264), (16, 1000, 512), (20, 136, 4104), (33, 128, 1032), (65, 300, 640), (130, 520, 384), (300, 384, 256), (513, 640, 520),
-            (260, 5130, 264), (1030, 4100, 200)]
+            (260, 5130, 264), (1030, 4100, 200), (11, 136, 4104), (132, 2217, 2104)]
 
 
 @pytest.mark.gpu
@@ -454,9 +482,9 @@ def test_gate_up(gpu, t, n, k, given, kind):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["e8m0", "f32"])
-def test_gate_up_of_many_tiles(gpu, kind):
+@pytest.mark.parametrize("t,n,k", LARGE_GATE_UPS)
+def test_gate_up_of_many_tiles(gpu, t, n, k, kind):
     """Rows and blocks of columns drawn from all tiles of a wide layer."""
-    t, n, k = LARGE_GATE_UP
     g = torch.Generator(device=gpu).manual_seed(36)
     x = torch.randn(t, k, generator=g, device=gpu) * 0.03
     weights = [((torch.randn(n, k, generator=g, device=gpu) * 100).clamp(-448, 448).to(E4M3), weight_of(n, k, kind, 37 + i)[1].to(gpu)) for i in range(2)]
