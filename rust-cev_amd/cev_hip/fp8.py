@@ -17,6 +17,15 @@ from ._abi import CEV_BF16, CEV_F32, CEV_FP8_SCALES_E8M0, CEV_FP8_SCALES_F32, Ce
 from .paged import _on
 
 
+def _call(name: str, stream, *args):
+    """The native call, its allocations for work on `stream`."""
+    f = getattr(calls(), name)
+    if stream is None:
+        return f(*args, None)
+    with _on(stream):
+        return f(*args, stream)
+
+
 class Fp8Rows:
     """Rows of k columns in e4m3: q (t, k up to a multiple of 128), with zeros
     behind column k, and s (t, q's columns / 128), the scales as
@@ -42,7 +51,7 @@ class Fp8Weight:
     def __init__(self, q, scales, stream=None, _up=(None, None)):
         import torch
         wide = lambda s: s.float() if s is not None and s.dtype == torch.bfloat16 else s  # noqa: E731
-        with _on(stream):
+        with _on(stream):  # (the wide scales too)
             self.data = calls().fp8_pack(q, wide(scales), _up[0], wide(_up[1]), stream)
         self.n, self.k = q.shape
         self.is_gate_up = _up[0] is not None
@@ -58,15 +67,13 @@ def fp8_rows(x, out=None, stream=None):
     """x (t, k) in e4m3 (cev_fp8_rows), for several projections of the same
     rows.  Returns Fp8Rows."""
     q, s = (None, None) if out is None else (out.q, out.s)
-    with _on(stream):
-        return Fp8Rows(*calls().fp8_rows(x, q, s, stream), x.shape[1])
+    return Fp8Rows(*_call("fp8_rows", stream, x, q, s), x.shape[1])
 
 
 def fp8_blocks(w, stream=None):
     """A weight (n, k) in e4m3 with a scale for 128 x 128 values
     (cev_fp8_blocks): (q, scales) for Fp8Weight."""
-    with _on(stream):
-        return calls().fp8_blocks(w, stream)
+    return _call("fp8_blocks", stream, w)
 
 
 def rms_norm_fp8(x, w, eps: float, h=None, x_out=None, out=None, plus_one: bool = False, stream=None):
@@ -76,8 +83,7 @@ def rms_norm_fp8(x, w, eps: float, h=None, x_out=None, out=None, plus_one: bool 
     if h is not None and x_out is None:
         x_out = x
     q, s = (None, None) if out is None else (out.q, out.s)
-    with _on(stream):
-        return Fp8Rows(*calls().fp8_rms_norm(x, w, eps, h, x_out, plus_one, q, s, stream), x.shape[1])
+    return Fp8Rows(*_call("fp8_rms_norm", stream, x, w, eps, h, x_out, plus_one, q, s), x.shape[1])
 
 
 def _operand(x):
@@ -97,8 +103,7 @@ def linear_fp8(x, w: Fp8Weight, out=None, out_dtype=None, stream=None):
     if out_dtype not in (None, torch.float32, torch.bfloat16):
         raise CevError(-2, f"dtype {out_dtype} not supported (float32, bfloat16)")
     code = CEV_F32 if out_dtype == torch.float32 else CEV_BF16
-    with _on(stream):
-        return calls().fp8_product(*_operand(x), w.data, w.n, w.k, w.scale_kind, False, out, None, code, stream)
+    return _call("fp8_product", stream, *_operand(x), w.data, w.n, w.k, w.scale_kind, False, out, None, code)
 
 
 def gate_up_fp8(x, w: Fp8Weight, out=None, stream=None):
@@ -108,5 +113,4 @@ def gate_up_fp8(x, w: Fp8Weight, out=None, stream=None):
     if not w.is_gate_up:
         raise CevError(-1, "gate_up_fp8: the weight is no Fp8Weight.gate_up")
     q, s = (None, None) if out is None else (out.q, out.s)
-    with _on(stream):
-        return Fp8Rows(*calls().fp8_product(*_operand(x), w.data, w.n, w.k, w.scale_kind, True, q, s, CEV_BF16, stream), w.n)
+    return Fp8Rows(*_call("fp8_product", stream, *_operand(x), w.data, w.n, w.k, w.scale_kind, True, q, s, CEV_BF16), w.n)

@@ -613,15 +613,23 @@ struct Fp8Out {
   Fp8Out(const char* call, PyObject* oq, PyObject* os, const at::Tensor& on, int64_t t, int64_t k) {
     const int64_t kb = blocks_of(k);
     want((oq == Py_None) == (os == Py_None), call, "out's values and scales go together");
-    if (oq == Py_None) {
-      q = at::empty({t, kb * 128}, on.options().dtype(at::kFloat8_e4m3fn));
-      s = at::empty({t, kb}, on.options().dtype(at::kFloat8_e8m0fnu));
+    if (oq == Py_None) {  // one allocation, and no more dispatch than that: small calls wait for the host
+      const at::Tensor both = at::empty({t * kb * 129}, on.options().dtype(at::kByte));
+      auto part = [&](at::ScalarType type, int64_t columns, int64_t offset) {
+        at::Tensor r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(both.storage()), both.key_set(), caffe2::TypeMeta::fromScalarType(type));
+        r.unsafeGetTensorImpl()->set_sizes_contiguous({t, columns});
+        r.unsafeGetTensorImpl()->set_storage_offset(offset);
+        return r;
+      };
+      q = part(at::kFloat8_e4m3fn, kb * 128, 0);
+      s = part(at::kFloat8_e8m0fnu, kb, t * kb * 128);
       return;
     }
     q = tensor(oq, "out.q"), s = tensor(os, "out.s");
     want(q.scalar_type() == at::kFloat8_e4m3fn && q.dim() == 2 && q.is_contiguous() && q.size(0) == t && q.size(1) == kb * 128 &&
              s.scalar_type() == at::kFloat8_e8m0fnu && s.dim() == 2 && s.is_contiguous() && s.size(0) == t && s.size(1) == kb,
          call, "out must be Fp8Rows of " + std::to_string(t) + " rows and " + std::to_string(k) + " columns");
+    want(q.device() == on.device() && s.device() == on.device(), call, "out and x are on different devices");
   }
   PyObject* pair() const { return Py_BuildValue("(NN)", THPVariable_Wrap(q), THPVariable_Wrap(s)); }
 };
@@ -637,7 +645,6 @@ PyObject* py_fp8_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (x.size(1) > 1) rows_contiguous(x);
     const OnDevice dev(me, {{"x", &x}});
     const Fp8Out out(me, a[1], a[2], x, x.size(0), x.size(1));
-    const OnDevice all(me, {{"x", &x}, {"out.q", &out.q}, {"out.s", &out.s}});
     void* const s = dev.stream(a[3]);
     call([&] { return api.fp8_rows(dt, x.size(0), x.size(1), ptr(x), x.stride(0), ptr(out.q), ptr(out.s), s); });
     return out.pair();
@@ -665,7 +672,6 @@ PyObject* py_fp8_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int32_t plus = as_bool(a[5]) ? 1 : 0;
     const OnDevice dev(me, {{"x", &x}, {"w", &w}, {"h", h}, {"x_out", x_out}});
     const Fp8Out out(me, a[6], a[7], x, x.size(0), x.size(1));
-    const OnDevice all(me, {{"x", &x}, {"out.q", &out.q}, {"out.s", &out.s}});
     void* const s = dev.stream(a[8]);
     call([&] {
       return api.fp8_rms_norm(dt, x.size(0), x.size(1), ptr(x), x.stride(0), ptr(h), h ? h->stride(0) : 0, ptr(x_out), x_out ? x_out->stride(0) : 0,
@@ -761,7 +767,7 @@ PyObject* py_fp8_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const OnDevice dev(me, {{"weight", &w}, {"x", &x}, {"x's scales", xs}});
     void* const s = dev.stream(a[11]);
     auto run = [&](const at::Tensor& out, const at::Tensor* out_s) {
-      const OnDevice all(me, {{"weight", &w}, {"out", &out}, {"out's scales", out_s}});
+      want(out.device() == dev.device, me, "out and x are on different devices");
       size_t bytes = 0;
       check(api.fp8_work_size(&d, &bytes));
       const CallBuffer work(x, bytes, s);
