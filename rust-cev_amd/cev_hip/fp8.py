@@ -35,6 +35,14 @@ class Fp8Rows:
     def __init__(self, q, s, k: int):
         self.q, self.s, self.k = q, s, k
 
+    @classmethod
+    def empty(cls, t: int, k: int, device):
+        """Room for t rows of k columns, to be a call's `out`."""
+        import torch
+        kb = -(-k // 128)
+        return cls(torch.empty((t, kb * 128), dtype=torch.float8_e4m3fn, device=device),
+                   torch.empty((t, kb), dtype=torch.float8_e8m0fnu, device=device), k)
+
     def float(self):
         """The values that the rows stand for (t, k), as f32."""
         return (self.q.float() * self.s.float().repeat_interleave(128, 1))[:, : self.k]

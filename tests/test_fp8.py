@@ -445,22 +445,12 @@ GATE_UPS = [(1, 1, 8), (1, 256, 128), (3, 130, 264), (16, 1000, 512), (20, 136, 
             (260, 5130, 264), (1030, 4100, 200), (11, 136, 4104), (132, 2217, 2104)]
 
 
-@pytest.mark.gpu
-@pytest.mark.parametrize("kind", ["e8m0", "f32"])
-@pytest.mark.parametrize("given", ["rows", torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("t,n,k", GATE_UPS)
-def test_gate_up(gpu, t, n, k, given, kind):
-    x = activations(t, k, torch.float32 if given == "rows" else given, 15)
-    x *= 1.5 / math.sqrt(k)
-    gate, up = weight_of(n, k, kind, 16), weight_of(n, k, kind, 17)
-    rows = oracle_rows(x)
-    xv = (rows[0] * torch.exp2(rows[1]).repeat_interleave(128, 1))[:, :k]
-    g, u = (xv @ weight_values(*w).t() for w in (gate, up))
-    size = [xv.abs() @ weight_values(*w).abs().t() for w in (gate, up)]
+def check_gate_up(got, xv, gate, up):
+    """got against silu(x . gate^T) * (x . up^T) in 64 bits, x (t, k), gate and up (n, k)."""
+    t, k, n = xv.shape[0], xv.shape[1], gate.shape[0]
+    g, u = (xv @ w.t() for w in (gate, up))
+    size = [xv.abs() @ w.abs().t() for w in (gate, up)]
     want = g * torch.sigmoid(g) * u
-    xg = cev_hip.fp8_rows(x.to(gpu)) if given == "rows" else x.to(gpu)
-    w = Fp8Weight.gate_up(tuple(y.to(gpu) for y in gate), tuple(y.to(gpu) for y in up))
-    got = cev_hip.gate_up_fp8(xg, w)
     # each product within c = (K + K / 64 + 16) 2^-23 of its sum of magnitudes; silu's slope is at most 1.1; the exponential of
     # -g within 2^-22 (1 + |g|) of itself, and the rest a few f32 roundings
     c = (k + k / 64 + 16) * 2.0 ** -23 + CUT
@@ -478,6 +468,22 @@ def test_gate_up(gpu, t, n, k, given, kind):
     # the bound is wide where sums are long: nearly all values are the nearest of the exact ones.  On data like these the
     # cut leaves each product within 2^-13 of itself, so of values 2^-4 of themselves apart at least 2 * 2 * 2^-13 / 2^-4 may fall to the other side
     assert float((q[:, :n] != round_e4m3(v[:, :n].clamp(-448, 448))).double().mean()) <= 2.0 ** -7 + 2 / q.numel()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["e8m0", "f32"])
+@pytest.mark.parametrize("given", ["rows", torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t,n,k", GATE_UPS)
+def test_gate_up(gpu, t, n, k, given, kind):
+    x = activations(t, k, torch.float32 if given == "rows" else given, 15)
+    x *= 1.5 / math.sqrt(k)
+    gate, up = weight_of(n, k, kind, 16), weight_of(n, k, kind, 17)
+    rows = oracle_rows(x)
+    xv = (rows[0] * torch.exp2(rows[1]).repeat_interleave(128, 1))[:, :k]
+    xg = cev_hip.fp8_rows(x.to(gpu)) if given == "rows" else x.to(gpu)
+    w = Fp8Weight.gate_up(tuple(y.to(gpu) for y in gate), tuple(y.to(gpu) for y in up))
+    got = cev_hip.gate_up_fp8(xg, w)
+    check_gate_up(got, xv, weight_values(*gate), weight_values(*up))
 
 
 @pytest.mark.gpu
