@@ -170,7 +170,7 @@ SIGNATURES = {
     "cev_fp8_weight_size": (i32, [i64, i64, i32, C.POINTER(C.c_size_t)]),
     "cev_fp8_weight_pack": (i32, [i64, i64, i32, P, i64, P, i64, P, i64, P, i64, P, C.c_size_t, P]),
     "cev_fp8_work_size": (i32, [C.POINTER(Fp8Desc), C.POINTER(C.c_size_t)]),
-    "cev_fp8_form": (i32, [C.POINTER(Fp8Desc), Pi32, Pi32]),
+    "cev_fp8_form": (i32, [C.POINTER(Fp8Desc), Pi32, Pi32, Pi32]),
     "cev_fp8_product": (i32, [C.POINTER(Fp8Desc), P, P, P, C.c_size_t, P, P, P, C.c_size_t, P]),
     "cev_table_from_plans": (i32, [i32, Pi32, Pi32, Pi32, i32, Pi32, Pi32, PBlock, i32, Pi32, Pi32, i32, Pi32, Pi32]),
     "cev_table_from_rows": (i32, [i32, i32, i32, i32, Pi32, PBlock, i32]),

@@ -20,8 +20,9 @@ struct Fp8Args {
 };
 
 // The kernel for many rows, 16 tt of them a workgroup (tt 4 or 8, with scales
-// in e8m0 also 16; exact, for f32 outputs: 4).
-int32_t fp8_launch_tile(const Fp8Args& a, int tt, bool exact, bool e8m0, bool gate_up, hipStream_t s);
+// in e8m0 also 16; exact, for f32 outputs: 4) of one team of waves or two (tt
+// 4, with f32 scales also 8).
+int32_t fp8_launch_tile(const Fp8Args& a, int tt, int teams, bool exact, bool e8m0, bool gate_up, hipStream_t s);
 
 __device__ __forceinline__ f32x4 fp8_mfma(const i32x8& a, const i32x8& b, const f32x4& c, int sa, int sb) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);

@@ -197,6 +197,7 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(JoinArgs a) {
   const int64_t col = (i - row * a.quads) * 4;
   const float* p = a.part + row * a.width + col;
   f32x4 v = *(const f32x4*)p;
+#pragma unroll 4
   for (int s = 1; s < a.parts; ++s) v += *(const f32x4*)(p + (int64_t)s * a.t * a.width);
   fp8_store4((O*)a.out + row * a.out_st, a.n, col, v);
 }
@@ -210,6 +211,7 @@ __global__ __launch_bounds__(256) void fp8_join_gate_up_kernel(JoinArgs a) {
   const int col = (int)(i - row * a.quads) * 8;
   const float* p = a.part + row * a.width + col / kFp8Group * 2 * kFp8Group + col % kFp8Group;
   f32x4 g[2] = {}, u[2] = {};
+#pragma unroll 4
   for (int s = 0; s < a.parts; ++s, p += a.t * a.width)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -236,6 +238,7 @@ constexpr int kTileBlocks = 32768;  // column blocks that the offsets of the ker
 struct Form {
   int32_t tt;   // the kernel for many rows, 16 tt of them a workgroup; 0: the one for few
   bool pack_x;  // rows of the model's type go into e4m3 in a launch of their own
+  int32_t teams;  // of the kernel for many rows
   int32_t groups, kb, parts, blocks_part;
   size_t rows_bytes, scales_bytes, part_bytes;
 };
@@ -244,14 +247,17 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Times of the kernel for many rows in us, measured at 64 to 4096 rows, 2048
 // to 12288 weight rows, 2048 to 12288 columns: a launch, and a block of columns
-// with one workgroup a CU and with two (tt = 16: one, alone on the card and
-// with all CUs busy).
+// (with two teams: two blocks) alone on the card, with a workgroup on every CU,
+// and with two.
 struct TileTimes {
-  float fixed, one, two;
+  float fixed, one, all, two;
 };
-constexpr TileTimes kE8m0Times[] = {{4.0f, 0.45f, 0.95f}, {5.6f, 0.57f, 1.5f}, {4.0f, 0.9f, 1.36f}};
-constexpr TileTimes kF32Times[] = {{4.3f, 0.54f, 1.1f}, {5.5f, 0.88f, 1.85f}};
-constexpr TileTimes kExactTimes[] = {{4.3f, 1.28f, 2.0f}};
+constexpr TileTimes kE8m0Times[] = {{4.2f, 0.455f, 0.54f, 0.95f}, {5.6f, 0.57f, 0.745f, 1.5f}, {4.0f, 0.9f, 1.36f, 0.0f}};
+constexpr TileTimes kF32Times[] = {{4.8f, 0.545f, 0.665f, 1.1f}, {5.8f, 0.87f, 1.02f, 1.85f}};
+constexpr TileTimes kExactTimes[] = {{4.7f, 1.3f, 1.33f, 1.9f}};
+constexpr TileTimes kE8m0Teams[] = {{6.0f, 0.77f, 0.95f, 0.0f}};
+constexpr TileTimes kF32Teams[] = {{5.6f, 0.87f, 1.1f, 0.0f}, {8.0f, 1.3f, 1.8f, 0.0f}};
+constexpr TileTimes kExactTeams[] = {{7.7f, 1.7f, 1.92f, 0.0f}};
 
 // 32 rows x 16 weight rows x a block of columns of the kernel for few rows,
 // which reads its rows again for every 16 weight rows.
@@ -265,13 +271,17 @@ double units_of(const cev_fp8_desc& d, int32_t kb) { return (double)((d.t + 31) 
 // against 15.4).  Of the other's tiles, fewer and larger ones read less and
 // compute at a higher rate; more of them, and parts of the columns, fill the
 // card.  A part's sums cost a round trip through memory (7 TB/s, most of it in
-// the card's cache) and another launch.
+// the card's cache) and another launch.  Two teams go where a CU has one
+// workgroup; with e8m0 scales and 128 rows they gain nothing (1536 x 4096 x 4096:
+// 27.6 us against 26.9).
 void plan(const cev_fp8_desc& d, Form& f) {
   const bool exact = !d.gate_up && d.out_dtype == CEV_F32, e8m0 = d.scales == CEV_FP8_SCALES_E8M0;
   double best = 1e-3 * units_of(d, f.kb) * (d.gate_up ? 0.57 : exact ? 0.33 : 0.30) + (d.gate_up ? 6.8 : exact ? 3.0 : 2.6);
   const TileTimes* const times = exact ? kExactTimes : e8m0 ? kE8m0Times : kF32Times;
   // (it reads the rows' scales four at a time, so that there have to be four;
   // up to 16 rows it is never the faster one by more than the model's error)
+  const TileTimes* const teams = exact ? kExactTeams : e8m0 ? kE8m0Teams : kF32Teams;
+  const int teamed = exact || e8m0 ? 1 : 2;  // kinds with two teams
   const int kinds = d.t <= 16 || f.kb > kTileBlocks ? 0 : exact ? 1 : e8m0 ? 3 : 2;
   const double sums = (double)d.t * f.groups * kFp8Group * 4;  // bytes of one part's
   for (int i = 0; i < kinds; ++i) {
@@ -281,20 +291,24 @@ void plan(const cev_fp8_desc& d, Form& f) {
       const int blocks = ((f.kb + p - 1) / p + 3) & ~3, parts = (f.kb + blocks - 1) / blocks;
       if (p > 1 && blocks < 8) break;
       const double wgs = tiles * parts, room = tt == 16 ? 256 : 512;  // workgroups that run together
+      const double join = parts > 1 ? 3.0 + 2 * parts * sums / 7e6 : 0.0;
+      auto take = [&](int teams_n, double us) {
+        if (us >= best) return;
+        best = us;
+        f.tt = tt, f.teams = teams_n, f.parts = parts, f.blocks_part = blocks;
+      };
       // up to a full card the others' reads slow a block down by and by; beyond, CUs take turns
-      double block = times[i].one;
+      double block = times[i].one + (times[i].all - times[i].one) * wgs / 256;
       if (wgs > room)
-        block = times[i].two * std::ceil(wgs / 256) * 256 / room;
-      else if (tt == 16 || wgs > 256)
-        block += (times[i].two - times[i].one) * wgs / room;
+        block = (tt == 16 ? times[i].all : times[i].two) * std::ceil(wgs / 256) * 256 / room;
+      else if (wgs > 256)
+        block = times[i].one + (times[i].two - times[i].one) * wgs / 512;
       // (a tile's start and end: under the other workgroup's blocks, where a CU has one)
       const double turns = std::ceil(wgs / room);
       const double starts = tt == 16 ? (d.gate_up ? 9.0 : 5.5) * turns : times[i].fixed * (0.5 * turns - 0.5);
-      const double us = times[i].fixed + starts + blocks * block + (parts > 1 ? 3.0 + 2 * parts * sums / 7e6 : 0.0);
-      if (us < best) {
-        best = us;
-        f.tt = tt, f.parts = parts, f.blocks_part = blocks;
-      }
+      take(1, times[i].fixed + starts + blocks * block + join);
+      if (i < teamed && wgs <= 256 && blocks >= 8)
+        take(2, teams[i].fixed + (blocks + 7) / 8 * 4 * (teams[i].one + (teams[i].all - teams[i].one) * wgs / 256) + join);
     }
   }
 }
@@ -303,7 +317,7 @@ Form form_of(const cev_fp8_desc& d) {
   Form f{};
   f.kb = (int32_t)((d.k + 127) / 128);
   f.groups = (int32_t)(d.gate_up ? (d.n + 127) / 128 * 8 : (d.n + 255) / 256 * 8);
-  f.parts = 1;
+  f.teams = f.parts = 1;
   f.blocks_part = f.kb;
   // The kernel for few rows can bring its 16 rows into e4m3 by itself, over and
   // over in each workgroup: for small weights that costs less than a launch (16
@@ -363,12 +377,13 @@ extern "C" int32_t cev_fp8_work_size(const cev_fp8_desc* d, size_t* bytes) {
   return CEV_OK;
 }
 
-extern "C" int32_t cev_fp8_form(const cev_fp8_desc* d, int32_t* rows, int32_t* parts) {
+extern "C" int32_t cev_fp8_form(const cev_fp8_desc* d, int32_t* rows, int32_t* parts, int32_t* teams) {
   if (const int32_t rc = check_desc("cev_fp8_form", d)) return rc;
-  CEV_CHECK_ARG(rows && parts, "cev_fp8_form: null output");
+  CEV_CHECK_ARG(rows && parts && teams, "cev_fp8_form: null output");
   const Form f = form_of(*d);
   *rows = 16 * f.tt;
   *parts = f.parts;
+  *teams = f.teams;
   return CEV_OK;
 }
 
@@ -422,7 +437,7 @@ extern "C" int32_t cev_fp8_product(const cev_fp8_desc* d, const void* x, const v
     if (const int32_t rc = launch_small<float, true>(a, x_dtype, e8m0, s)) return rc;
     return cev_fp8_rows(CEV_F32, d->t, d->n, a.part, a.out_st, out, out_scales, stream);
   }
-  const int32_t rc = f.tt > 0 ? fp8_launch_tile(a, f.tt, !d->gate_up && d->out_dtype == CEV_F32, e8m0, d->gate_up != 0, s)
+  const int32_t rc = f.tt > 0 ? fp8_launch_tile(a, f.tt, f.teams, !d->gate_up && d->out_dtype == CEV_F32, e8m0, d->gate_up != 0, s)
                      : d->out_dtype == CEV_F32 ? launch_small<float, false>(a, x_dtype, e8m0, s) : launch_small<__bf16, false>(a, x_dtype, e8m0, s);
   if (rc || !a.part) return rc;
   JoinArgs j{a.part, out, (uint8_t*)out_scales, d->t, d->n, a.out_st, (int64_t)f.groups * kFp8Group, f.parts, 0};

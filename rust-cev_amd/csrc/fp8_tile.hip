@@ -5,7 +5,11 @@
 // instruction, and 8 % more of them under the card's power limit than of the
 // 32 x 32 x 64 form (4.35 against 4.03 PFLOP/s with nothing else to do).  Up
 // to 128 rows two workgroups a CU: they share no barrier, so one's reads,
-// scalings and waits lie under the other's matrix products.  Column blocks:
+// scalings and waits lie under the other's matrix products.  Where there are
+// no more workgroups than CUs, two teams of 4 waves stand in for the second one:
+// each takes half of the column blocks, in LDS of its own, and their sums meet
+// there at the end (1021 x 4096 x 12288, 256 workgroups: 52.3 us against 56.1,
+// with f32 scales 58.1 against 68.4).  Column blocks:
 //   rows     into LDS straight from memory (buffer_load ... lds), four blocks
 //            deep, the 16-byte pieces c of row r at place c ^ (r / 2 + 2 & 7):
 //            the lanes that LDS serves together (0-3, 12-15 and 20-27 of 32,
@@ -62,7 +66,7 @@ __device__ __forceinline__ void wait_unit(Unit& u) {
   asm volatile("s_waitcnt lgkmcnt(%3)" : "+v"(u.v[0]), "+v"(u.v[1]), "+v"(u.s) : "i"(N));
 }
 
-template <bool E8M0, bool GATE_UP, bool EXACT, int TT>
+template <bool E8M0, bool GATE_UP, bool EXACT, int TT, int TEAMS>
 __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_tiles) {
   constexpr int ROWS = 16 * TT;
     constexpr int STAGE = ROWS * kFp8Block;
@@ -71,8 +75,10 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
   constexpr int OUT = GATE_UP ? ROWS * (PITCH + 16) : 4 * ROWS * PITCH;
   constexpr int SCALES = kStages * STAGE;  // of the rows, four blocks each: of three groups of four blocks
   constexpr int LDS = SCALES + 3 * ROWS * 4 > OUT ? SCALES + 3 * ROWS * 4 : OUT;
-  __shared__ __align__(1024) char lds[LDS];
-  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4, l16 = lane & 15;
+  __shared__ __align__(1024) char all_lds[TEAMS * LDS];
+  const int team = TEAMS > 1 ? uniform(threadIdx.x >> 8) : 0, tid = threadIdx.x & 255;
+  const int wave = uniform(tid >> 6), lane = tid & 63, quad = lane >> 4, l16 = lane & 15;
+  char* const lds = all_lds + team * LDS;
 
   // which tile: XCD b % 8 gets a run of tiles, in panels of kPanel row tiles
   int64_t row0;
@@ -86,7 +92,10 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
     col_tile = r / high;
     row0 = (int64_t)(panel * kPanel + r - col_tile * high) * ROWS;
   }
-  const int kb0 = part * a.blocks_part, kb1 = min(a.kb, kb0 + a.blocks_part);
+  // the team's column blocks, whole groups of four in the first team
+  const int part0 = part * a.blocks_part, part1 = min(a.kb, part0 + a.blocks_part);
+  const int share = TEAMS > 1 ? (part1 - part0 + 7) / 8 * 4 : part1 - part0;
+  const int kb0 = part0 + team * share, kb1 = min(part1, kb0 + share);
   const int pitch = a.kb * kFp8Block;  // bytes of a row
   const int group0 = col_tile * 8 + wave * 2;
   const int rows_left = (int)min<int64_t>(ROWS, a.t - row0);
@@ -98,7 +107,7 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
   for (int q = 0; q < XQ; ++q)
     xat[q] = min((wave * XQ + q) * 8 + (lane >> 3), rows_left - 1) * pitch + (((lane & 7) ^ (((wave * XQ + q) * 4 + quad + 2) & 7)) << 4);
   auto fetch_x = [&](int q, int kb, int stage) {
-    const int at = min(kb, kb1 - 1) * kFp8Block;
+    const int at = min(kb, part1 - 1) * kFp8Block;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (__attribute__((address_space(3))) void*)(lds + stage + (wave * XQ + q) * 1024), 16, xat[q], at, 0, 0);
   };
 
@@ -115,7 +124,7 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
   asm volatile("" : "+v"(nil));
   auto fetch_w = [&](auto b_c, auto p_c, int kb) {  // an eighth of them
     constexpr int B = decltype(b_c)::value, P = decltype(p_c)::value, J = P / 2, H = P % 2;
-    const int at = min(kb, kb1 - 1);
+    const int at = min(kb, part1 - 1);
     w[B][J][H] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
                                                  rw, wat, at * kFp8GroupBytes + (J >> 1) * group_bytes + (J & 1) * 256 + H * 1024, 0));
     if constexpr (!E8M0 && P < 2) sw[B][P] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rws, nil, (P * a.ws_pitch + at) * 4, 0);
@@ -132,14 +141,14 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
   const int64_t s_bytes = (a.t - row0) * a.kb + early;
   const __amdgpu_buffer_rsrc_t rs = buffer(a.xs + row0 * a.kb - early, s_bytes);
   const int s_last = ((uint32_t)(s_bytes >> 31) ? INT32_MAX : (int)s_bytes) - 4;
-  const int sat = min((int)threadIdx.x, rows_left - 1) * a.kb + early;
+  const int sat = min(tid, rows_left - 1) * a.kb + early;
   auto fetch_xs = [&](int kb) {
-    const int from = sat + min(kb, kb1 - 1), at = min(from, s_last), n = kb1 - kb;
+    const int from = sat + min(kb, part1 - 1), at = min(from, s_last), n = kb1 - kb;
     const uint32_t v = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0) >> (8 * (from - at) & 31);
     return v & (n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << 8 * n) - 1);
   };
   auto put_xs = [&](uint32_t v, int slot) {
-    if (ROWS == 256 || threadIdx.x < ROWS) *(uint32_t*)(lds + SCALES + (slot * ROWS + (int)threadIdx.x) * 4) = v;
+    if (ROWS == 256 || tid < ROWS) *(uint32_t*)(lds + SCALES + (slot * ROWS + tid) * 4) = v;
   };
 
   // Reads of the rows, AHEAD tiles of 16 ahead of the one that is computed.
@@ -280,7 +289,25 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
     if constexpr (E8M0) sw4[0] = sw4_next[0], sw4[1] = sw4_next[1];
     slot = slot_next;
   }
+  if constexpr (TEAMS > 1)  // a barrier a block, also for blocks that the second team has not got
+    for (int kb = 2 * ((max(kb1 - kb0, 0) + 1) / 2); kb < 2 * ((share + 1) / 2); ++kb) asm volatile("s_barrier" ::: "memory");
   asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  if constexpr (TEAMS > 1) {  // the teams' sums
+    f32x4* const sums = (f32x4*)all_lds + tid;
+    if (team == 1) {
+#pragma unroll
+      for (int i = 0; i < TT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sums[(i * 4 + j) * 256] = acc[i][j];
+    }
+    __syncthreads();
+    if (team == 1) return;
+#pragma unroll
+    for (int i = 0; i < TT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] += sums[(i * 4 + j) * 256];
+    __syncthreads();
+  }
 
   // Results.  Lane l holds row l % 16 of each row tile, columns 16 j + 4 (l /
   // 16) .. + 3 of the wave's 64.
@@ -371,38 +398,46 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < TT / 2; ++i) {
-      const int r = i * 32 + (threadIdx.x >> 3);
-      const u32x4_t v = *(const u32x4_t*)(lds + r * PITCH + (threadIdx.x & 7) * 16);
-      if (row0 + r < a.t) *(u32x4_t*)((uint8_t*)a.out + ((row0 + r) * blocks + col_tile) * 128 + (threadIdx.x & 7) * 16) = v;
+      const int r = i * 32 + (tid >> 3);
+      const u32x4_t v = *(const u32x4_t*)(lds + r * PITCH + (tid & 7) * 16);
+      if (row0 + r < a.t) *(u32x4_t*)((uint8_t*)a.out + ((row0 + r) * blocks + col_tile) * 128 + (tid & 7) * 16) = v;
     }
   }
 }
 
-template <bool E8M0, bool GATE_UP, bool EXACT, int TT>
-__global__ __launch_bounds__(256, TT > 8 ? 1 : 2) void fp8_tile_kernel(Fp8Args a, int row_tiles, int col_tiles) {
-  tile<E8M0, GATE_UP, EXACT, TT>(a, row_tiles, col_tiles);
+template <bool E8M0, bool GATE_UP, bool EXACT, int TT, int TEAMS>
+__global__ __launch_bounds__(256 * TEAMS, TT > 8 ? 1 : 2) void fp8_tile_kernel(Fp8Args a, int row_tiles, int col_tiles) {
+  tile<E8M0, GATE_UP, EXACT, TT, TEAMS>(a, row_tiles, col_tiles);
 }
 
-template <bool E8M0, bool GATE_UP, bool EXACT, int TT>
+template <bool E8M0, bool GATE_UP, bool EXACT, int TT, int TEAMS>
 int32_t launch(const Fp8Args& a, hipStream_t s) {
   const int64_t row_tiles = (a.t + 16 * TT - 1) / (16 * TT), col_tiles = a.groups / kFp8TileGroups, grid = row_tiles * col_tiles * a.parts;
   if (grid > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_product: grid too large");
-  hipLaunchKernelGGL((fp8_tile_kernel<E8M0, GATE_UP, EXACT, TT>), dim3((unsigned)grid), dim3(256), 0, s, a, (int)row_tiles, (int)col_tiles);
+  hipLaunchKernelGGL((fp8_tile_kernel<E8M0, GATE_UP, EXACT, TT, TEAMS>), dim3((unsigned)grid), dim3(256 * TEAMS), 0, s, a, (int)row_tiles, (int)col_tiles);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? CEV_OK : cev_fail(CEV_ERR_HIP, "cev_fp8_product launch: %s", hipGetErrorString(e));
 }
 
-template <int TT>
-int32_t launch(const Fp8Args& a, bool e8m0, bool gate_up, hipStream_t s) {
-  if (gate_up) return e8m0 ? launch<true, true, false, TT>(a, s) : launch<false, true, false, TT>(a, s);
-  return e8m0 ? launch<true, false, false, TT>(a, s) : launch<false, false, false, TT>(a, s);
+template <bool E8M0, bool EXACT, int TT, int TEAMS>
+int32_t launch(const Fp8Args& a, bool gate_up, hipStream_t s) {
+  if constexpr (!EXACT)
+    if (gate_up) return launch<E8M0, true, false, TT, TEAMS>(a, s);
+  return launch<E8M0, false, EXACT, TT, TEAMS>(a, s);
+}
+
+template <bool EXACT, int TEAMS>
+int32_t launch4(const Fp8Args& a, bool e8m0, bool gate_up, hipStream_t s) {
+  return e8m0 ? launch<true, EXACT, 4, TEAMS>(a, gate_up, s) : launch<false, EXACT, 4, TEAMS>(a, gate_up, s);
 }
 
 }  // namespace
 
-int32_t fp8_launch_tile(const Fp8Args& a, int tt, bool exact, bool e8m0, bool gate_up, hipStream_t s) {
+int32_t fp8_launch_tile(const Fp8Args& a, int tt, int teams, bool exact, bool e8m0, bool gate_up, hipStream_t s) {
   if (a.part) gate_up = false;  // (sums of parts are joined elsewhere)
-  if (exact) return e8m0 ? launch<true, false, true, 4>(a, s) : launch<false, false, true, 4>(a, s);
-  if (tt == 16 && e8m0) return gate_up ? launch<true, true, false, 16>(a, s) : launch<true, false, false, 16>(a, s);
-  return tt >= 8 ? launch<8>(a, e8m0, gate_up, s) : launch<4>(a, e8m0, gate_up, s);
+  if (exact) return teams > 1 ? launch4<true, 2>(a, e8m0, false, s) : launch4<true, 1>(a, e8m0, false, s);
+  if (tt == 4) return teams > 1 ? launch4<false, 2>(a, e8m0, gate_up, s) : launch4<false, 1>(a, e8m0, gate_up, s);
+  if (tt == 16) return launch<true, false, 16, 1>(a, gate_up, s);
+  if (e8m0) return launch<true, false, 8, 1>(a, gate_up, s);
+  return teams > 1 ? launch<false, false, 8, 2>(a, gate_up, s) : launch<false, false, 8, 1>(a, gate_up, s);
 }

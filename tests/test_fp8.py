@@ -289,14 +289,14 @@ def test_norm_of_rows_that_are_zero_or_not_finite(gpu):
 
 
 def form_of(t, n, k, kind, out=torch.bfloat16, gate_up=False):
-    """(rows of a tile, parts of the columns) of the kernel that runs it; 0 rows: the kernel for few."""
+    """(rows of a tile, parts of the columns, teams that share a part) of the kernel that runs it; 0 rows: the kernel for few."""
     import ctypes as C
     from cev_hip import _abi
     d = _abi.Fp8Desc(x_dtype=2, out_dtype=2 if gate_up else 0 if out == torch.float32 else 1, scales=0 if kind == "e8m0" else 1, gate_up=gate_up,
                      t=t, n=n, k=k, x_stride=k, out_stride=n)
-    rows, parts = C.c_int32(), C.c_int32()
-    _abi.check(_abi.lib().cev_fp8_form(C.byref(d), C.byref(rows), C.byref(parts)))
-    return rows.value, parts.value
+    rows, parts, teams = C.c_int32(), C.c_int32(), C.c_int32()
+    _abi.check(_abi.lib().cev_fp8_form(C.byref(d), C.byref(rows), C.byref(parts), C.byref(teams)))
+    return rows.value, parts.value, teams.value
 
 
 def test_every_kernel_is_among_the_tested_products(cev):
@@ -304,15 +304,20 @@ def test_every_kernel_is_among_the_tested_products(cev):
     rows = {f[:2] for f in forms}
     assert rows >= {("e8m0", 0), ("e8m0", 64), ("e8m0", 128), ("e8m0", 256), ("f32", 0), ("f32", 64), ("f32", 128)}, forms
     assert {f[2] for f in forms} >= {1, 2} and max(f[2] for f in forms) > 2, forms
-    exact = {(kind,) + form_of(t, n, k, kind, torch.float32) for kind in ("e8m0", "f32") for t, n, k in PRODUCTS}
+    # two teams: the last one with fewer blocks, and with as many
+    assert {f[:2] + f[3:] for f in forms} >= {("e8m0", 64, 1), ("e8m0", 64, 2), ("f32", 64, 1), ("f32", 64, 2), ("f32", 128, 1), ("f32", 128, 2)}, forms
+    exact = {(kind,) + form_of(t, n, k, kind, torch.float32) for kind in ("e8m0", "f32") for t, n, k in PRODUCTS + LARGE_F32}
+    assert {(f[0], f[3]) for f in exact if f[1]} == {(kind, teams) for kind in ("e8m0", "f32") for teams in (1, 2)}, exact
     assert {f[1] for f in exact} == {0, 64} and max(f[2] for f in exact) > 2, exact
     gate = {(kind,) + form_of(t, n, k, kind, gate_up=True) for kind in ("e8m0", "f32") for t, n, k in GATE_UPS + LARGE_GATE_UPS}
     assert {f[:2] for f in gate} >= {("e8m0", 0), ("e8m0", 64), ("e8m0", 128), ("e8m0", 256), ("f32", 0), ("f32", 64), ("f32", 128)}, gate
     assert max(f[2] for f in gate) > 1, gate
+    assert {f[:2] for f in gate if f[3] == 2 and f[2] == 1} >= {("e8m0", 64), ("f32", 64), ("f32", 128)}, gate
 
 
-LARGE = [(2048, 4096, 2048), (1030, 8320, 264), (4096, 4000, 4104), (400, 4096, 6144)]
-LARGE_GATE_UPS = [(2048, 12288, 4096), (2048, 12288, 6144)]
+LARGE = [(2048, 4096, 2048), (1030, 8320, 264), (4096, 4000, 4104), (400, 4096, 6144), (900, 4000, 8200), (1536, 4000, 8328)]
+LARGE_F32 = [(700, 4100, 2056), (1021, 2056, 4104), (3000, 4100, 1032), (900, 4000, 8200)]
+LARGE_GATE_UPS = [(2048, 12288, 4096), (2048, 12288, 6144), (400, 4096, 6080), (900, 4000, 8200), (1000, 1030, 4360)]
 PRODUCTS = [(1, 1, 1), (1, 40, 128), (2, 256, 136), (7, 129, 1000), (16, 300, 520), (31, 64, 2048), (32, 1000, 264), (33, 257, 384), (64, 512, 1280),
             (100, 136, 4104), (129, 520, 640), (257, 1000, 392), (400, 384, 1152), (1, 2048, 6144), (300, 2048, 256), (9, 40, 4104),
             (300, 2000, 6152), (333, 4100, 4104)]
@@ -352,7 +357,7 @@ def test_linear_large(gpu, t, n, k, kind):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["e8m0", "f32"])
-@pytest.mark.parametrize("t,n,k", [(700, 4100, 2056), (1021, 2056, 4104), (3000, 4100, 1032)])
+@pytest.mark.parametrize("t,n,k", LARGE_F32)
 def test_linear_large_f32(gpu, t, n, k, kind):
     x, w = activations(t, k, torch.float32, 7), weight_of(n, k, kind, 8)
     q, e = oracle_rows(x)
@@ -496,12 +501,12 @@ def test_gate_up_of_many_tiles(gpu, t, n, k, kind):
     weights = [((torch.randn(n, k, generator=g, device=gpu) * 100).clamp(-448, 448).to(E4M3), weight_of(n, k, kind, 37 + i)[1].to(gpu)) for i in range(2)]
     rows = cev_hip.fp8_rows(x)
     got = cev_hip.gate_up_fp8(rows, Fp8Weight.gate_up(*weights))
-    at = torch.tensor([0, 1, 127, 128, 255, 256, 300, 1000, 1023, 1024, 2000, 2047])
-    blocks = [0, 1, 31, 64, 95]
-    xv = values(rows.q[at.to(gpu)].cpu(), rows.s[at.to(gpu)].cpu())
+    at = torch.tensor([r for r in (0, 1, 127, 128, 255, 256, 300, 1000, 1023, 1024, 2000) if r < t] + [t - 1])
+    blocks = [b for b in (0, 1, 31, 64, 95) if b < up128(n) // 128]
+    xv = values(rows.q[at.to(gpu)].cpu(), rows.s[at.to(gpu)].cpu())[:, :k]
     for b in blocks:
-        cols = slice(128 * b, 128 * b + 128)
-        wv = [q[cols].cpu().double() * s[b].cpu().double().repeat_interleave(128) for q, s in weights]
+        cols = slice(128 * b, min(128 * b + 128, n))
+        wv = [q[cols].cpu().double() * s[b].cpu().double().repeat_interleave(128)[:k] for q, s in weights]
         gv, uv = xv @ wv[0].t(), xv @ wv[1].t()
         want = gv * torch.sigmoid(gv) * uv
         have = (got.q[:, cols].cpu()[at].double() * got.s[:, b].cpu()[at].double()[:, None])
