@@ -2,18 +2,24 @@
 //
 //   y[t, n] = sum over blocks b of 128 columns:  2^e[t, b] s[n / 128, b] (q[t, b] . w[n, b])
 //
-// Two kinds of matrix product, by the output's type:
+// Two kinds of matrix product:
 //
-//   bf16, e4m3  v_mfma_scale_f32_16x16x128_f8f6f4, which takes 2^e as an operand
-//               (and s where it is a power of two; an f32 s multiplies the
-//               block's 16 x 16 results).  It adds eight neighbouring columns'
-//               products after cutting each towards zero to a multiple of
-//               2^(E - 13), 2^E the largest one's power of two (measured bit by
-//               bit); what follows is f32.  A sum is therefore up to 7 * 2^-13
-//               of its largest products off; on normal data it is 4.5e-5 of
-//               the result, a fortieth of bf16's rounding.
-//   f32         v_mfma_f32_16x16x32_bf16 on the same values in bf16, which holds
-//               them exactly: products and sums in f32, at half the rate.
+//   bf16 outputs, and gate and up of many rows
+//       v_mfma_scale_f32_16x16x128_f8f6f4, which takes 2^e as an operand (and s
+//       where it is a power of two; an f32 s multiplies the block's 16 x 16
+//       results).  It adds eight neighbouring columns' products after cutting
+//       each towards zero to a multiple of 2^(E - 13), 2^E the largest one's
+//       power of two (measured bit by bit); what follows is f32.  A sum is
+//       therefore up to 7 * 2^-13 of its largest products off; on normal data
+//       it is 4.5e-5 of the result, a fortieth of bf16's rounding.  Of gate and
+//       up's e4m3 values, whose steps are 2^-3 to 2^-4 apart, one in a thousand
+//       becomes the nearest but one.  (In bf16 the same product takes twice as
+//       long: 4096 x 12288 x 4096 1331 instead of 2600 TFLOP/s at best.)
+//   f32 outputs, and gate and up of few rows
+//       v_mfma_f32_16x16x32_bf16 on the same values in bf16, which holds them
+//       exactly: products and sums in f32, at half the rate.  Where the weight's
+//       bytes are what counts that is nearly free (gate and up of 16 x 6144 x
+//       2048: 9.2 us against 8.8).
 #include <algorithm>
 #include <cmath>
 
@@ -43,7 +49,7 @@ template <typename T, typename O, bool E8M0, bool GATE_UP, int MT>
 __global__ __launch_bounds__(kWaves * 64, 4) void fp8_small_kernel(Fp8Args a, unsigned col_tiles) {
   constexpr bool PACK = sizeof(T) > 1;
   constexpr int NH = GATE_UP ? 2 : 1, DEEP = (PACK ? 2 : 4 / MT) / NH;
-  constexpr bool EXACT = sizeof(O) == 4 && !GATE_UP;
+  constexpr bool EXACT = sizeof(O) == 4;
   constexpr int QUAD = 80;  // floats of a quad's 16 rows x 4 columns, and 16 more: the sums' reads fall on different banks
   constexpr int STAGE = DEEP * MT * 2048, SUMS = NH * MT * 4 * QUAD * 4;
   __shared__ __align__(16) uint8_t space[kWaves][STAGE > SUMS ? STAGE : SUMS];  // a wave's rows, then its sums
