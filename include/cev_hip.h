@@ -599,7 +599,8 @@ typedef struct {
  * overlap must not share one. */
 int32_t cev_fp8_work_size(const cev_fp8_desc* d, size_t* bytes);
 /* Which kernel a product runs: the one for few rows (*rows = 0), or tiles of
- * *rows rows over *parts parts of the columns (host only). */
+ * *rows rows over *parts parts of the columns, each shared by *teams teams of
+ * waves (host only). */
 int32_t cev_fp8_form(const cev_fp8_desc* d, int32_t* rows, int32_t* parts, int32_t* teams);
 int32_t cev_fp8_product(const cev_fp8_desc* d, const void* x, const void* x_scales, const void* weight, size_t weight_bytes, void* out,
                         void* out_scales, void* work, size_t work_bytes, cev_stream stream);
