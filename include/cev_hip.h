@@ -544,6 +544,7 @@ int32_t cev_paged_attention(const cev_paged_desc* d, const void* q, const void* 
  * magnitude; q is x / 2^e, which is exact in f32, rounded to nearest even.  A
  * value that is not finite becomes NaN and counts for no scale.  Weights (n,
  * k): a scale for 128 x 128 values, from cev_fp8_blocks or brought along.
+ * Outputs and workspaces overlap no input but where a call says so.
  * Nothing here has a gradient. */
 enum { CEV_E4M3 = 2 };                                   /* beside CEV_F32 and CEV_BF16, where a call says so */
 enum { CEV_FP8_SCALES_E8M0 = 0, CEV_FP8_SCALES_F32 = 1 }; /* a weight's scales: bytes 2^(byte - 127), or any f32 */

@@ -147,9 +147,10 @@ __global__ __launch_bounds__(kWaves * 64, 4) void fp8_small_kernel(Fp8Args a, un
 #pragma unroll
             for (int c = 0; c < 4; ++c)
               p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(wv[2 * c], wv[2 * c + 1]), fp8_widen(xv[i][2 * c], xv[i][2 * c + 1]), p, 0, 0, 0);
-            const float s = f * fp8_scale_value((uint32_t)sx[d][i]);
+            // (one scale after the other: their product may leave f32's range where the result does not)
+            const float s = fp8_scale_value((uint32_t)sx[d][i]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[h][i][r] = __builtin_fmaf(p[r], s, acc[h][i][r]);
+            for (int r = 0; r < 4; ++r) acc[h][i][r] = __builtin_fmaf(p[r] * s, f, acc[h][i][r]);
           } else if constexpr (E8M0) {
             acc[h][i] = fp8_mfma(wv, xv[i], acc[h][i], (int)sw[d][h], sx[d][i]);
           } else {
@@ -415,6 +416,8 @@ extern "C" int32_t cev_fp8_product(const cev_fp8_desc* d, const void* x, const v
   } else {
     CEV_CHECK_ARG(((uintptr_t)out & 15) == 0, "%s: rows in e4m3 must be 16-byte aligned", me);
   }
+  for (const void* p : {x, x_scales, weight})
+    CEV_CHECK_ARG(out != p && (!out_scales || (out_scales != p && out_scales != out)), "%s: the output must have memory of its own", me);
   const Form f = form_of(*d);
   need = f.rows_bytes + f.scales_bytes + f.part_bytes;
   if (work_bytes < need) return cev_fail(CEV_ERR_SPACE, "%s: a workspace of %zu bytes, %zu needed", me, work_bytes, need);

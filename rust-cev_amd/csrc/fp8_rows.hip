@@ -281,6 +281,7 @@ extern "C" int32_t cev_fp8_rows(int32_t dtype, int64_t t, int64_t k, const void*
   const int parts = a.chunks > kThreads ? (a.chunks + kThreads - 1) / kThreads : 1;
   const int64_t grid = (t + a.rows_wg - 1) / a.rows_wg * parts;
   if (grid > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_rows: too many rows");
+  CEV_CHECK_ARG(q != x && scales != x && q != scales, "cev_fp8_rows: the outputs must have memory of their own");
   hipLaunchKernelGGL(dtype == CEV_BF16 ? fp8_rows_kernel<__bf16> : fp8_rows_kernel<float>, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, a, parts);
   return launched("cev_fp8_rows");
 }
@@ -331,6 +332,8 @@ extern "C" int32_t cev_fp8_rms_norm(int32_t dtype, int64_t rows, int64_t k, cons
     if (const int32_t rc = check_rows("cev_fp8_rms_norm", dtype, rows, k, "x_out", x_out, x_out_stride)) return rc;
   }
   CEV_CHECK_ARG(q && scales && aligned(q, 16), "cev_fp8_rms_norm: null or misaligned output");
+  for (const void* p : {x, h, (const void*)x_out, w})
+    CEV_CHECK_ARG(q != p && scales != p && q != scales, "cev_fp8_rms_norm: the rows in e4m3 must have memory of their own");
   const NormArgs a{x, h, x_out, w, (uint8_t*)q, (uint8_t*)scales, rows, x_stride, h_stride, x_out_stride, (int32_t)k, (int32_t)((k + 127) / 128 * 16),
                    weight_plus_one, eps};
   return dtype == CEV_BF16 ? launch_norm<__bf16>(a, (hipStream_t)stream) : launch_norm<float>(a, (hipStream_t)stream);
@@ -341,6 +344,7 @@ extern "C" int32_t cev_fp8_blocks(int32_t dtype, int64_t n, int64_t k, const voi
   CEV_CHECK_ARG(n >= 1 && n <= INT32_MAX - 256 && k >= 1 && k <= INT32_MAX - 128, "cev_fp8_blocks: a weight of %lld x %lld", (long long)n, (long long)k);
   if (const int32_t rc = check_rows("cev_fp8_blocks", dtype, n, k, "w", w, ldw)) return rc;
   CEV_CHECK_ARG(q && scales && aligned(q, 16), "cev_fp8_blocks: null or misaligned output");
+  CEV_CHECK_ARG(q != w && scales != w && q != scales, "cev_fp8_blocks: the outputs must have memory of their own");
   const BlocksArgs a{w, (uint8_t*)q, (uint8_t*)scales, n, ldw, (int32_t)k, (int32_t)((k + 127) / 128)};
   const int64_t grid = (n + 127) / 128 * a.kb;
   if (grid > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_blocks: weight too large");

@@ -236,9 +236,10 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
           f32x4 q = {};
 #pragma unroll
           for (int c = 0; c < 4; ++c) q = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(wv[2 * c], wv[2 * c + 1]), wide[c], q, 0, 0, 0);
-          const float f = (E8M0 ? fp8_scale_value(s2[J >> 1] & 255) : __uint_as_float(sw[B][J >> 1])) * fx;
+          // (one scale after the other: their product may leave f32's range where the result does not)
+          const float f = E8M0 ? fp8_scale_value(s2[J >> 1] & 255) : __uint_as_float(sw[B][J >> 1]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[U][J][r] = __builtin_fmaf(q[r], f, acc[U][J][r]);
+          for (int r = 0; r < 4; ++r) acc[U][J][r] = __builtin_fmaf(q[r] * fx, f, acc[U][J][r]);
         } else if constexpr (E8M0) {
           acc[U][J] = fp8_mfma(wv, x, acc[U][J], (int)s2[J >> 1], sx);
         } else {
@@ -301,7 +302,7 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
         for (int j = 0; j < 4; ++j) sums[(i * 4 + j) * 256] = acc[i][j];
     }
     __syncthreads();
-    if (team == 1) return;
+    if (team == 1) return;  // (later barriers do not wait for waves that have ended)
 #pragma unroll
     for (int i = 0; i < TT; ++i)
 #pragma unroll

@@ -628,6 +628,37 @@ def test_calls_on_two_streams(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t,n,k", [(2, 40, 128), (20, 40, 1032), (3000, 4100, 1032), (900, 4000, 8200)])
+@pytest.mark.parametrize("x_exp,w_exp", [(-110, -40), (-40, -110), (10, 112), (-118, 120)])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+def test_scales_far_apart(gpu, t, n, k, x_exp, w_exp, out_dtype):
+    """Products of a row's and a weight's scale that leave f32's range, where the result stays within it."""
+    m = 2.0 ** -9 if x_exp + w_exp > 100 else 448.0
+    x = torch.full((t, k), m * 2.0 ** x_exp, dtype=torch.float32, device=gpu)
+    x[:, ::128] = 448 * 2.0 ** x_exp  # each block's scale
+    q = torch.full((n, k), m).to(E4M3)
+    q[:, ::128] = 0
+    w = Fp8Weight(q.to(gpu), torch.full((up128(n) // 128, up128(k) // 128), 2.0 ** w_exp, device=gpu))
+    want = m * m * 2.0 ** (x_exp + w_exp) * (k - len(range(0, k, 128)))
+    y = cev_hip.linear_fp8(x, w, out_dtype=out_dtype).double().cpu()
+    # equal products: nothing is cut, and sums of fewer than 2^24 of them are exact
+    assert 2.0 ** -126 < want < 2.0 ** 127 and bool(((y - want).abs() <= half_ulp(out_dtype) * want).all()), (want, y.min(), y.max())
+
+
+@pytest.mark.gpu
+def test_no_rows(gpu):
+    w = packed(weight_of(40, 300, "f32", 35), gpu)
+    gu = Fp8Weight.gate_up(*[tuple(y.to(gpu) for y in weight_of(40, 300, "e8m0", 35))] * 2)
+    x = torch.zeros(0, 300, device=gpu)
+    rows = cev_hip.fp8_rows(x)
+    assert rows.q.shape == (0, 384) and rows.s.shape == (0, 3) and rows.float().shape == (0, 300)
+    assert cev_hip.rms_norm_fp8(x, torch.ones(300, device=gpu), 1e-6, h=torch.zeros_like(x)).q.shape == (0, 384)
+    for given in (x, rows):
+        assert cev_hip.linear_fp8(given, w).shape == (0, 40)
+        assert cev_hip.gate_up_fp8(given, gu).s.shape == (0, 1)
+
+
+@pytest.mark.gpu
 def test_given_outputs(gpu):
     x = activations(20, 300, torch.float32, 34).to(gpu)
     rows = cev_hip.fp8_rows(x)
@@ -635,6 +666,15 @@ def test_given_outputs(gpu):
     got = cev_hip.fp8_rows(x, out=other)
     assert got.q.data_ptr() == other.q.data_ptr() and torch.equal(got.q.view(torch.uint8), rows.q.view(torch.uint8))
     assert torch.equal(got.s.view(torch.uint8), rows.s.view(torch.uint8))
+    dense = torch.zeros(20, 128, device=gpu)
+    with pytest.raises(CevError, match="of their own"):
+        cev_hip.fp8_rows(dense, out=Fp8Rows(dense.view(E4M3)[:, :128].as_strided((20, 128), (128, 1)), torch.empty(20, 1, dtype=E8M0, device=gpu), 128))
+    square = Fp8Weight.gate_up(*[tuple(y.to(gpu) for y in weight_of(128, 128, "f32", 35))] * 2)
+    rows_128 = cev_hip.fp8_rows(dense)
+    with pytest.raises(CevError, match="of its own"):
+        cev_hip.gate_up_fp8(rows_128, square, out=rows_128)
+    with pytest.raises(CevError, match="of its own"):
+        cev_hip.linear_fp8(dense, packed(weight_of(128, 128, "f32", 35), gpu), out=dense)
     with pytest.raises(CevError, match="Fp8Rows of 20 rows"):
         cev_hip.fp8_rows(x, out=Fp8Rows(rows.q[:10], rows.s[:10], 300))
     with pytest.raises(CevError, match="contiguous"):
@@ -732,7 +772,7 @@ def test_abi_refusals(cev):
     refused(L.cev_fp8_weight_pack(128, 128, 1, p, 128, p, 1, None, 0, None, 0, p, 100, None), -4, "needed")
     refused(L.cev_fp8_weight_pack(128, 128, 1, p, 128, p, 1, p, 128, None, 0, p, 1 << 20, None), -1, "null")
 
-    def product(d, x=p, xs=None, w=p, wb=1 << 40, out=p, outs=None, work=p, wk=1 << 40):
+    def product(d, x=p, xs=None, w=p, wb=1 << 40, out=C.c_void_p(8192), outs=None, work=p, wk=1 << 40):
         return L.cev_fp8_product(C.byref(d), x, xs, w, wb, out, outs, work, wk, None)
 
     good = dict(x_dtype=1, out_dtype=1, scales=1, gate_up=0, t=4, n=256, k=128, x_stride=128, out_stride=256)
@@ -753,6 +793,9 @@ def test_abi_refusals(cev):
     refused(product(desc(**dict(good, out_stride=255))), -1, "stride of out")
     refused(product(desc(**good), out=C.c_void_p(4097)), -1, "misaligned")
     refused(product(desc(**good), x=C.c_void_p(4104)), -1, "aligned")
+    refused(L.cev_fp8_rows(0, 2, 8, p, 8, p, C.c_void_p(8192), None), -1, "of their own")
+    refused(L.cev_fp8_rms_norm(1, 2, 8, p, 8, None, 0, None, 0, C.c_void_p(8192), 1e-6, 0, p, C.c_void_p(16384), None), -1, "of their own")
+    refused(product(desc(**good), out=p), -1, "of its own")
     big = desc(**dict(good, t=4000))
     assert L.cev_fp8_work_size(C.byref(big), C.byref(size)) == 0 and size.value >= 4000 * 129
     refused(product(big, wk=size.value - 1), -4, "workspace")
