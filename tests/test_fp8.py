@@ -432,6 +432,20 @@ def test_linear_writes_its_rows_only(gpu, t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t,n,k", [(530000, 40, 4096), (40, 530000, 4096)])
+def test_offsets_past_31_bits(gpu, t, n, k):
+    """Rows, or a weight, of more than 2^31 bytes: the last ones as by themselves.  Small integers, whose sums are exact in any order."""
+    g = torch.Generator(device=gpu).manual_seed(60)
+    x = torch.randint(-2, 3, (t, k), generator=g, device=gpu, dtype=torch.int8).bfloat16()
+    q = torch.randint(-2, 3, (n, k), generator=g, device=gpu, dtype=torch.int8).to(E4M3)
+    s = torch.ones(up128(n) // 128, up128(k) // 128, device=gpu)
+    y = cev_hip.linear_fp8(x, Fp8Weight(q, s))
+    rows, cols = min(t, 200), min(n, 128 + n % 128)
+    want = (x[-rows:].double() @ q[-cols:].double().t()).to(torch.bfloat16)
+    assert torch.equal(y[-rows:, -cols:], want)
+
+
+@pytest.mark.gpu
 def test_no_rows(gpu):
     w = packed(weight_of(40, 72, "e8m0", 14), gpu)
     x = torch.zeros(0, 72, dtype=torch.bfloat16, device=gpu)
