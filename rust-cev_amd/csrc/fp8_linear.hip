@@ -34,7 +34,8 @@ constexpr int kWaves = 8;  // waves of a workgroup of the kernel for few rows, e
 // operand's read meets a bank twice.
 __device__ __forceinline__ int staged(int r, int piece) { return r * 128 + ((piece ^ ((r >> 1) + 2)) & 7) * 16; }
 
-// 16 MT rows times 16 weight rows (GATE_UP: times 16 of gate and of up).  The
+// 16 MT rows times 16 weight rows (GATE_UP: times 16 of gate and of up; MT = 4:
+// times 32, so that the rows are read half as often).  The
 // weight streams through once, so what counts is how much of it is on the way:
 // a workgroup holds few weight rows and its waves share the column blocks, each
 // with DEEP of them under way; their sums are joined in LDS, in the waves'
@@ -48,7 +49,8 @@ __device__ __forceinline__ int staged(int r, int piece) { return r * 128 + ((pie
 template <typename T, typename O, bool E8M0, bool GATE_UP, int MT>
 __global__ __launch_bounds__(kWaves * 64, 4) void fp8_small_kernel(Fp8Args a, unsigned col_tiles) {
   constexpr bool PACK = sizeof(T) > 1;
-  constexpr int NH = GATE_UP ? 2 : 1, DEEP = (PACK ? 2 : 4 / MT) / NH;
+  constexpr bool WIDE = MT == 4;  // both halves of a group of 32 weight rows
+  constexpr int NH = GATE_UP || WIDE ? 2 : 1, DEEP = WIDE ? 1 : (PACK ? 2 : 4 / MT) / NH;
   constexpr bool EXACT = sizeof(O) == 4;
   constexpr int QUAD = 80;  // floats of a quad's 16 rows x 4 columns, and 16 more: the sums' reads fall on different banks
   constexpr int STAGE = DEEP * MT * 2048, SUMS = NH * MT * 4 * QUAD * 4;
@@ -67,8 +69,8 @@ __global__ __launch_bounds__(kWaves * 64, 4) void fp8_small_kernel(Fp8Args a, un
   }
   const uint8_t* const sp = PACK ? nullptr : a.xs + min(row0 + lane / DEEP, a.t - 1) * a.kb;
   // the group of 32 weight rows (gate's; up's follows), and the lane's place in its half
-  const int64_t group = (int64_t)(c16 >> 1) * NH;
-  const uint8_t* const wp = a.w + group * a.kb * kFp8GroupBytes + (quad >> 1) * 2048 + (quad & 1) * 512 + (c16 & 1) * 256 + l16 * 16;
+  const int64_t group = WIDE ? c16 : (int64_t)(c16 >> 1) * NH;
+  const uint8_t* const wp = a.w + group * a.kb * kFp8GroupBytes + (quad >> 1) * 2048 + (quad & 1) * 512 + (WIDE ? 0 : (c16 & 1) * 256) + l16 * 16;
   f32x4 acc[NH][MT];
 #pragma unroll
   for (int h = 0; h < NH; ++h)
@@ -97,10 +99,10 @@ __global__ __launch_bounds__(kWaves * 64, 4) void fp8_small_kernel(Fp8Args a, un
       }
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
-        const uint8_t* const p = wp + ((int64_t)h * a.kb + kb) * kFp8GroupBytes;
+        const uint8_t* const p = wp + (WIDE ? (int64_t)kb * kFp8GroupBytes + h * 256 : ((int64_t)h * a.kb + kb) * kFp8GroupBytes);
         w[d][h][0] = *(const u32x4_t*)p;
         w[d][h][1] = *(const u32x4_t*)(p + 1024);
-        const int64_t at = (group + h) * a.ws_pitch + kb;
+        const int64_t at = (group + (WIDE ? 0 : h)) * a.ws_pitch + kb;
         sw[d][h] = E8M0 ? a.ws[at] : ((const uint32_t*)a.ws)[at];
       }
     }
@@ -178,12 +180,15 @@ __global__ __launch_bounds__(kWaves * 64, 4) void fp8_small_kernel(Fp8Args a, un
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) v[h] += ((const float*)space[w])[h * MT * 4 * QUAD + at];
     }
-    const int64_t out_row = row0 + i * 16 + r, col = (int64_t)c16 * 16 + n;
-    if (out_row >= a.t || col >= a.n) continue;
-    if constexpr (GATE_UP)
-      a.part[out_row * a.out_st + col] = fp8_swiglu(v[0], v[1]);
-    else
-      ((O*)a.out)[out_row * a.out_st + col] = (O)v[0];
+    const int64_t out_row = row0 + i * 16 + r, col = (int64_t)c16 * (WIDE ? 32 : 16) + n;
+    if (out_row >= a.t) continue;
+    if constexpr (GATE_UP) {
+      if (col < a.n) a.part[out_row * a.out_st + col] = fp8_swiglu(v[0], v[1]);
+    } else {
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+        if (col + h * 16 < a.n) ((O*)a.out)[out_row * a.out_st + col + h * 16] = (O)v[h];
+    }
   }
 }
 
@@ -245,6 +250,7 @@ constexpr int kTileBlocks = 32768;  // column blocks that the offsets of the ker
 struct Form {
   int32_t tt;   // the kernel for many rows, 16 tt of them a workgroup; 0: the one for few
   bool pack_x;  // rows of the model's type go into e4m3 in a launch of their own
+  int32_t mt;     // of the kernel for few, 16 mt of them a workgroup
   int32_t teams;  // of the kernel for many rows
   int32_t groups, kb, parts, blocks_part;
   size_t rows_bytes, scales_bytes, part_bytes;
@@ -266,16 +272,18 @@ constexpr TileTimes kE8m0Teams[] = {{6.0f, 0.77f, 0.95f, 0.0f}};
 constexpr TileTimes kF32Teams[] = {{5.6f, 0.87f, 1.1f, 0.0f}, {8.0f, 1.3f, 1.8f, 0.0f}};
 constexpr TileTimes kExactTeams[] = {{7.7f, 1.7f, 1.92f, 0.0f}};
 
-// 32 rows x 16 weight rows x a block of columns of the kernel for few rows,
-// which reads its rows again for every 16 weight rows.
-double units_of(const cev_fp8_desc& d, int32_t kb) { return (double)((d.t + 31) / 32) * ((d.n + 15) / 16) * kb; }
+// Blocks of columns that all workgroups of the kernel for few rows go through,
+// where each holds `rows` rows and `columns` weight rows.
+double units_of(const cev_fp8_desc& d, int32_t kb, int rows, int columns) {
+  return (double)((d.t + rows - 1) / rows) * ((d.n + columns - 1) / columns) * kb;
+}
 
 // Which kernel, with which tile, by the time that each would take.  The one for
 // few rows streams the weight at the card's rate (16 rows x 12288 x 4096: 10 us
 // against 14), and is ahead as long as its repeated reads of the rows cost less
 // than the other's slow start (12288 x 4096: 32 rows 10.6 us against 15.4, 64
-// rows 17.6 against 17.3, 256 rows 58.6 against 20.2; 4096 x 4096: 128 rows 12.1
-// against 15.4).  Of the other's tiles, fewer and larger ones read less and
+// rows 14.7 against 17.1, 128 rows 21.2 against 18.7; 4096 x 4096: 128 rows 8.7
+// against 15.3).  Of the other's tiles, fewer and larger ones read less and
 // compute at a higher rate; more of them, and parts of the columns, fill the
 // card.  A part's sums cost a round trip through memory (7 TB/s, most of it in
 // the card's cache) and another launch.  Two teams go where a CU has one
@@ -283,7 +291,15 @@ double units_of(const cev_fp8_desc& d, int32_t kb) { return (double)((d.t + 31) 
 // 27.6 us against 26.9).
 void plan(const cev_fp8_desc& d, Form& f) {
   const bool exact = !d.gate_up && d.out_dtype == CEV_F32, e8m0 = d.scales == CEV_FP8_SCALES_E8M0;
-  double best = 1e-3 * units_of(d, f.kb) * (d.gate_up ? 0.57 : exact ? 0.33 : 0.30) + (d.gate_up ? 6.8 : exact ? 3.0 : 2.6);
+  double best = 1e-3 * units_of(d, f.kb, 32, 16) * (d.gate_up ? 0.57 : exact ? 0.33 : 0.30) + (d.gate_up ? 6.8 : exact ? 3.0 : 2.6);
+  if (!exact && !d.gate_up && d.t > 32) {
+    // 64 rows and 32 weight rows a workgroup, whose waves take at least 1.3 us
+    // for a block (128 rows x 4096 x 4096: 8.7 us against 12.3, 64 rows 8.5 against
+    // 7.9, 64 rows x 12288 x 4096 14.7 against 17.6).  In f32 sums the registers
+    // do not hold it.
+    const double wide = 3.5 + std::max(0.74e-3 * units_of(d, f.kb, 64, 32), 1.3 / kWaves * f.kb);
+    if (wide < best) best = wide, f.mt = 4;
+  }
   const TileTimes* const times = exact ? kExactTimes : e8m0 ? kE8m0Times : kF32Times;
   // (it reads the rows' scales four at a time, so that there have to be four;
   // up to 16 rows it is never the faster one by more than the model's error)
@@ -294,7 +310,7 @@ void plan(const cev_fp8_desc& d, Form& f) {
   for (int i = 0; i < kinds; ++i) {
     const int tt = 4 << i;
     const double tiles = (double)((d.t + 16 * tt - 1) / (16 * tt)) * (f.groups / kFp8TileGroups);
-    for (int p = 1; p <= 16; p *= 2) {
+    for (int p = 1; p <= 8; p *= 2) {  // (16 parts cost more to join than they save)
       const int blocks = ((f.kb + p - 1) / p + 3) & ~3, parts = (f.kb + blocks - 1) / blocks;
       if (p > 1 && blocks < 8) break;
       const double wgs = tiles * parts, room = tt == 16 ? 256 : 512;  // workgroups that run together
@@ -325,11 +341,12 @@ Form form_of(const cev_fp8_desc& d) {
   f.kb = (int32_t)((d.k + 127) / 128);
   f.groups = (int32_t)(d.gate_up ? (d.n + 127) / 128 * 8 : (d.n + 255) / 256 * 8);
   f.teams = f.parts = 1;
+  f.mt = d.t <= 16 ? 1 : 2;
   f.blocks_part = f.kb;
   // The kernel for few rows can bring its 16 rows into e4m3 by itself, over and
   // over in each workgroup: for small weights that costs less than a launch (16
   // rows x 4096 x 2048: 5.9 us against 6.9; x 12288 x 4096: 22 against 14).
-  f.pack_x = d.x_dtype != CEV_E4M3 && (d.t > 16 || units_of(d, f.kb) > 4096);
+  f.pack_x = d.x_dtype != CEV_E4M3 && (d.t > 16 || units_of(d, f.kb, 16, 16) > 4096);
   if (d.x_dtype == CEV_E4M3 || f.pack_x) plan(d, f);
   if (f.pack_x) {
     f.rows_bytes = up256((size_t)d.t * f.kb * kFp8Block);
@@ -357,7 +374,8 @@ int32_t check_desc(const char* what, const cev_fp8_desc* d) {
 
 template <typename T, typename O, bool GATE_UP, int MT>
 int32_t launch_small(const Fp8Args& a, bool e8m0, hipStream_t s) {
-  const int64_t col_tiles = (a.n + 15) / 16, grid = (a.t + 16 * MT - 1) / (16 * MT) * col_tiles;
+  const int columns = MT == 4 ? 32 : 16;
+  const int64_t col_tiles = (a.n + columns - 1) / columns, grid = (a.t + 16 * MT - 1) / (16 * MT) * col_tiles;
   if (grid > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_product: grid too large");
   if (e8m0)
     hipLaunchKernelGGL((fp8_small_kernel<T, O, true, GATE_UP, MT>), dim3((unsigned)grid), dim3(kWaves * 64), 0, s, a, (unsigned)col_tiles);
@@ -367,11 +385,12 @@ int32_t launch_small(const Fp8Args& a, bool e8m0, hipStream_t s) {
 }
 
 template <typename O, bool GATE_UP>
-int32_t launch_small(const Fp8Args& a, int x_dtype, bool e8m0, hipStream_t s) {
+int32_t launch_small(const Fp8Args& a, int x_dtype, int mt, bool e8m0, hipStream_t s) {
   if (x_dtype == CEV_BF16) return launch_small<__bf16, O, GATE_UP, 1>(a, e8m0, s);
   if (x_dtype == CEV_F32) return launch_small<float, O, GATE_UP, 1>(a, e8m0, s);
-  if (a.t <= 16) return launch_small<uint8_t, O, GATE_UP, 1>(a, e8m0, s);
-  return launch_small<uint8_t, O, GATE_UP, 2>(a, e8m0, s);
+  if constexpr (sizeof(O) == 2)
+    if (mt == 4) return launch_small<uint8_t, O, GATE_UP, 4>(a, e8m0, s);
+  return mt == 1 ? launch_small<uint8_t, O, GATE_UP, 1>(a, e8m0, s) : launch_small<uint8_t, O, GATE_UP, 2>(a, e8m0, s);
 }
 
 }  // namespace
@@ -388,9 +407,9 @@ extern "C" int32_t cev_fp8_form(const cev_fp8_desc* d, int32_t* rows, int32_t* p
   if (const int32_t rc = check_desc("cev_fp8_form", d)) return rc;
   CEV_CHECK_ARG(rows && parts && teams, "cev_fp8_form: null output");
   const Form f = form_of(*d);
-  *rows = 16 * f.tt;
+  *rows = 16 * (f.tt ? f.tt : f.mt);
   *parts = f.parts;
-  *teams = f.teams;
+  *teams = f.tt ? f.teams : 0;
   return CEV_OK;
 }
 
@@ -443,11 +462,12 @@ extern "C" int32_t cev_fp8_product(const cev_fp8_desc* d, const void* x, const v
   a.out_s = (uint8_t*)out_scales;
   if (d->gate_up && f.tt == 0) {
     a.out_st = (d->n + 127) / 128 * 128;
-    if (const int32_t rc = launch_small<float, true>(a, x_dtype, e8m0, s)) return rc;
+    if (const int32_t rc = launch_small<float, true>(a, x_dtype, f.mt, e8m0, s)) return rc;
     return cev_fp8_rows(CEV_F32, d->t, d->n, a.part, a.out_st, out, out_scales, stream);
   }
   const int32_t rc = f.tt > 0 ? fp8_launch_tile(a, f.tt, f.teams, !d->gate_up && d->out_dtype == CEV_F32, e8m0, d->gate_up != 0, s)
-                     : d->out_dtype == CEV_F32 ? launch_small<float, false>(a, x_dtype, e8m0, s) : launch_small<__bf16, false>(a, x_dtype, e8m0, s);
+                     : d->out_dtype == CEV_F32 ? launch_small<float, false>(a, x_dtype, f.mt, e8m0, s)
+                                               : launch_small<__bf16, false>(a, x_dtype, f.mt, e8m0, s);
   if (rc || !a.part) return rc;
   JoinArgs j{a.part, out, (uint8_t*)out_scales, d->t, d->n, a.out_st, (int64_t)f.groups * kFp8Group, f.parts, 0};
   j.quads = (int32_t)(d->gate_up ? (d->n + 127) / 128 * 16 : (d->n + 3) / 4);

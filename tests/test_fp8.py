@@ -289,38 +289,42 @@ def test_norm_of_rows_that_are_zero_or_not_finite(gpu):
 
 
 def form_of(t, n, k, kind, out=torch.bfloat16, gate_up=False):
-    """(rows of a tile, parts of the columns, teams that share a part) of the kernel that runs it; 0 rows: the kernel for few."""
+    """(rows of a tile, parts of the columns, teams that share a part) of the kernel that runs it; of the one for few rows (0,
+    rows of a workgroup, 0)."""
     import ctypes as C
     from cev_hip import _abi
     d = _abi.Fp8Desc(x_dtype=2, out_dtype=2 if gate_up else 0 if out == torch.float32 else 1, scales=0 if kind == "e8m0" else 1, gate_up=gate_up,
                      t=t, n=n, k=k, x_stride=k, out_stride=n)
     rows, parts, teams = C.c_int32(), C.c_int32(), C.c_int32()
     _abi.check(_abi.lib().cev_fp8_form(C.byref(d), C.byref(rows), C.byref(parts), C.byref(teams)))
-    return rows.value, parts.value, teams.value
+    return (rows.value, parts.value, teams.value) if teams.value else (0, rows.value, 0)
 
 
 def test_every_kernel_is_among_the_tested_products(cev):
-    forms = {(kind,) + form_of(t, n, k, kind) for kind in ("e8m0", "f32") for t, n, k in PRODUCTS + LARGE}
-    rows = {f[:2] for f in forms}
-    assert rows >= {("e8m0", 0), ("e8m0", 64), ("e8m0", 128), ("e8m0", 256), ("f32", 0), ("f32", 64), ("f32", 128)}, forms
-    assert {f[2] for f in forms} >= {1, 2} and max(f[2] for f in forms) > 2, forms
-    # two teams: the last one with fewer blocks, and with as many
-    assert {f[:2] + f[3:] for f in forms} >= {("e8m0", 64, 1), ("e8m0", 64, 2), ("f32", 64, 1), ("f32", 64, 2), ("f32", 128, 1), ("f32", 128, 2)}, forms
-    exact = {(kind,) + form_of(t, n, k, kind, torch.float32) for kind in ("e8m0", "f32") for t, n, k in PRODUCTS + LARGE_F32}
-    assert {(f[0], f[3]) for f in exact if f[1]} == {(kind, teams) for kind in ("e8m0", "f32") for teams in (1, 2)}, exact
-    assert {f[1] for f in exact} == {0, 64} and max(f[2] for f in exact) > 2, exact
-    gate = {(kind,) + form_of(t, n, k, kind, gate_up=True) for kind in ("e8m0", "f32") for t, n, k in GATE_UPS + LARGE_GATE_UPS}
-    assert {f[:2] for f in gate} >= {("e8m0", 0), ("e8m0", 64), ("e8m0", 128), ("e8m0", 256), ("f32", 0), ("f32", 64), ("f32", 128)}, gate
-    assert max(f[2] for f in gate) > 1, gate
-    assert {f[:2] for f in gate if f[3] == 2 and f[2] == 1} >= {("e8m0", 64), ("f32", 64), ("f32", 128)}, gate
+    def forms_of(products, **kw):
+        f = {(kind,) + form_of(t, n, k, kind, **kw) for kind in ("e8m0", "f32") for t, n, k in products}
+        few = {(kind, rows) for kind, tile, rows, _ in f if not tile}
+        return few, {(kind, tile, teams) for kind, tile, _, teams in f if tile}, {parts for _, tile, parts, _ in f if tile}
+
+    few, tiles, parts = forms_of(PRODUCTS + LARGE)
+    assert few == {(kind, rows) for kind in ("e8m0", "f32") for rows in (16, 32, 64)}, few
+    assert tiles == {("e8m0", 64, 1), ("e8m0", 64, 2), ("e8m0", 128, 1), ("e8m0", 256, 1), ("f32", 64, 1), ("f32", 64, 2), ("f32", 128, 1), ("f32", 128, 2)}, tiles
+    assert parts >= {1, 2} and max(parts) > 2, parts
+    few, tiles, parts = forms_of(PRODUCTS + LARGE_F32, out=torch.float32)
+    assert few == {(kind, rows) for kind in ("e8m0", "f32") for rows in (16, 32)}, few
+    assert tiles == {(kind, 64, teams) for kind in ("e8m0", "f32") for teams in (1, 2)} and max(parts) > 2, (tiles, parts)
+    few, tiles, parts = forms_of(GATE_UPS + LARGE_GATE_UPS, gate_up=True)
+    assert few == {(kind, rows) for kind in ("e8m0", "f32") for rows in (16, 32)}, few
+    assert tiles == {("e8m0", 64, 1), ("e8m0", 64, 2), ("e8m0", 128, 1), ("e8m0", 256, 1), ("f32", 64, 1), ("f32", 64, 2), ("f32", 128, 1), ("f32", 128, 2)}, tiles
+    assert max(parts) > 1, parts
 
 
-LARGE = [(2048, 4096, 2048), (1030, 8320, 264), (4096, 4000, 4104), (400, 4096, 6144), (900, 4000, 8200), (1536, 4000, 8328)]
+LARGE = [(2048, 4096, 2048), (1030, 8320, 264), (4096, 4000, 4104), (400, 4096, 6144), (900, 4000, 8200), (1536, 4000, 8328), (130, 5000, 8200), (260, 2056, 12296)]
 LARGE_F32 = [(700, 4100, 2056), (1021, 2056, 4104), (3000, 4100, 1032), (900, 4000, 8200)]
 LARGE_GATE_UPS = [(2048, 12288, 4096), (2048, 12288, 6144), (400, 4096, 6080), (900, 4000, 8200), (1000, 1030, 4360)]
 PRODUCTS = [(1, 1, 1), (1, 40, 128), (2, 256, 136), (7, 129, 1000), (16, 300, 520), (31, 64, 2048), (32, 1000, 264), (33, 257, 384), (64, 512, 1280),
             (100, 136, 4104), (129, 520, 640), (257, 1000, 392), (400, 384, 1152), (1, 2048, 6144), (300, 2048, 256), (9, 40, 4104),
-            (300, 2000, 6152), (333, 4100, 4104)]
+            (300, 2000, 6152), (333, 4100, 4104), (190, 4100, 1032), (40, 7000, 1160)]
 
 
 @pytest.mark.gpu
