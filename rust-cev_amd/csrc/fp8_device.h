@@ -17,6 +17,9 @@ constexpr int kFp8Group = 32;     // weight rows of one matrix-core operand
 constexpr int kFp8GroupBytes = kFp8Group * kFp8Block;
 constexpr int kFp8TileGroups = 8;  // weight rows are padded to 8 groups
 
+// A launch counts its threads in 32 bits.
+inline bool fp8_grid_fits(int64_t grid, int threads) { return grid <= (int64_t)(UINT32_MAX / (uint32_t)threads); }
+
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));

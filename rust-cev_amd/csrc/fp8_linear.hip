@@ -376,7 +376,7 @@ template <typename T, typename O, bool GATE_UP, int MT>
 int32_t launch_small(const Fp8Args& a, bool e8m0, hipStream_t s) {
   const int columns = MT == 4 ? 32 : 16;
   const int64_t col_tiles = (a.n + columns - 1) / columns, grid = (a.t + 16 * MT - 1) / (16 * MT) * col_tiles;
-  if (grid > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_product: grid too large");
+  if (!fp8_grid_fits(grid, kWaves * 64)) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_product: grid too large");
   if (e8m0)
     hipLaunchKernelGGL((fp8_small_kernel<T, O, true, GATE_UP, MT>), dim3((unsigned)grid), dim3(kWaves * 64), 0, s, a, (unsigned)col_tiles);
   else
@@ -472,7 +472,7 @@ extern "C" int32_t cev_fp8_product(const cev_fp8_desc* d, const void* x, const v
   JoinArgs j{a.part, out, (uint8_t*)out_scales, d->t, d->n, a.out_st, (int64_t)f.groups * kFp8Group, f.parts, 0};
   j.quads = (int32_t)(d->gate_up ? (d->n + 127) / 128 * 16 : (d->n + 3) / 4);
   const int64_t grid = (d->t * j.quads + 255) / 256;
-  if (grid > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "%s: too many rows", me);
+  if (!fp8_grid_fits(grid, 256)) return cev_fail(CEV_ERR_UNSUPPORTED, "%s: too many rows", me);
   if (d->gate_up)
     hipLaunchKernelGGL(fp8_join_gate_up_kernel, dim3((unsigned)grid), dim3(256), 0, s, j);
   else if (d->out_dtype == CEV_BF16)

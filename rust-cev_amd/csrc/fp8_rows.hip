@@ -280,7 +280,7 @@ extern "C" int32_t cev_fp8_rows(int32_t dtype, int64_t t, int64_t k, const void*
   a.rows_wg = a.chunks >= kThreads ? 1 : kThreads / a.chunks;
   const int parts = a.chunks > kThreads ? (a.chunks + kThreads - 1) / kThreads : 1;
   const int64_t grid = (t + a.rows_wg - 1) / a.rows_wg * parts;
-  if (grid > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_rows: too many rows");
+  if (!fp8_grid_fits(grid, kThreads)) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_rows: too many rows");
   CEV_CHECK_ARG(q != x && scales != x && q != scales, "cev_fp8_rows: the outputs must have memory of their own");
   hipLaunchKernelGGL(dtype == CEV_BF16 ? fp8_rows_kernel<__bf16> : fp8_rows_kernel<float>, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, a, parts);
   return launched("cev_fp8_rows");
@@ -292,7 +292,7 @@ template <typename T, int WAVES, int NCH>
 int32_t launch_norm(const NormArgs& a, hipStream_t s) {
   constexpr int ROWS = WAVES > 4 ? 1 : 4 / WAVES;
   const int64_t grid = (a.rows + ROWS - 1) / ROWS;
-  if (grid > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_rms_norm: too many rows");
+  if (!fp8_grid_fits(grid, ROWS * WAVES * 64)) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_rms_norm: too many rows");
   if (a.h)
     hipLaunchKernelGGL((fp8_norm_kernel<T, WAVES, NCH, true>), dim3((unsigned)grid), dim3(ROWS * WAVES * 64), 0, s, a);
   else
@@ -347,7 +347,7 @@ extern "C" int32_t cev_fp8_blocks(int32_t dtype, int64_t n, int64_t k, const voi
   CEV_CHECK_ARG(q != w && scales != w && q != scales, "cev_fp8_blocks: the outputs must have memory of their own");
   const BlocksArgs a{w, (uint8_t*)q, (uint8_t*)scales, n, ldw, (int32_t)k, (int32_t)((k + 127) / 128)};
   const int64_t grid = (n + 127) / 128 * a.kb;
-  if (grid > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_blocks: weight too large");
+  if (!fp8_grid_fits(grid, kBlockThreads)) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_blocks: weight too large");
   if (dtype == CEV_BF16)
     hipLaunchKernelGGL(fp8_blocks_kernel<__bf16>, dim3((unsigned)grid), dim3(kBlockThreads), 0, (hipStream_t)stream, a);
   else
@@ -392,7 +392,7 @@ extern "C" int32_t cev_fp8_weight_pack(int64_t n, int64_t k, int32_t scale_kind,
   a.out_s = (uint32_t*)(a.out + a.groups * kb * kFp8GroupBytes);
   a.gate_up = gate_up, a.f32_scales = scale_kind == CEV_FP8_SCALES_F32;
   const int64_t grid = a.groups * kb;
-  if (grid > INT32_MAX) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_weight_pack: weight too large");
+  if (!fp8_grid_fits(grid, kThreads)) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_weight_pack: weight too large");
   hipLaunchKernelGGL(fp8_pack_kernel, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, a);
   return launched("cev_fp8_weight_pack");
 }

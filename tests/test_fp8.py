@@ -776,6 +776,7 @@ def test_abi_refusals(cev):
     refused(L.cev_fp8_rows(0, 2, 8, C.c_void_p(4100), 8, p, p, None), -1, "aligned")
     refused(L.cev_fp8_rows(0, 2, 8, p, 8, None, p, None), -1, "output")
     refused(L.cev_fp8_rows(0, 1 << 28, 1 << 30, p, 1 << 30, p, p, None), -2, "too many")
+    refused(L.cev_fp8_rows(0, 1 << 25, 1 << 11, p, 1 << 11, C.c_void_p(8192), C.c_void_p(16384), None), -2, "too many")  # 2^33 threads
     assert L.cev_fp8_rows(0, 0, 8, None, 8, None, None, None) == 0
     refused(L.cev_fp8_rms_norm(1, 2, 8, p, 8, None, 0, None, 0, None, 1e-6, 0, p, p, None), -1, "null w")
     refused(L.cev_fp8_rms_norm(1, 2, 8, p, 8, p, 8, None, 0, p, 1e-6, 0, p, p, None), -1, "null x_out")
