@@ -557,8 +557,9 @@ int32_t cev_fp8_rows(int32_t dtype, int64_t t, int64_t k, const void* x, int64_t
 
 /* The RMS norm before a projection (qwen3.rs:254-255), with the residual add
  * where h is given (qwen3.rs:261): x_out = dtype(x + h) is written (x_out may
- * be x), and x_out / sqrt(mean x_out^2 + eps) * w, f32 throughout, goes into
- * e4m3 with that one rounding.  Alignment as above, for w too. */
+ * be x), and x_out / sqrt(mean x_out^2 + eps) * w goes into e4m3 with one
+ * rounding, that of the exact value (with weight_plus_one 1 + w is f32).
+ * Alignment as above, for w too. */
 int32_t cev_fp8_rms_norm(int32_t dtype, int64_t rows, int64_t k, const void* x, int64_t x_stride, const void* h, int64_t h_stride,
                          void* x_out, int64_t x_out_stride, const void* w, float eps, int32_t weight_plus_one, void* q, void* scales,
                          cev_stream stream);

@@ -86,8 +86,8 @@ def fp8_blocks(w, stream=None):
 
 def rms_norm_fp8(x, w, eps: float, h=None, x_out=None, out=None, plus_one: bool = False, stream=None):
     """rms_norm into e4m3 (cev_fp8_rms_norm): with h the residual add first,
-    x_out = x + h in x's type (x_out defaults to x), then the norm in f32, its
-    only rounding the one into e4m3.  Returns Fp8Rows."""
+    x_out = x + h in x's type (x_out defaults to x), then the norm, its only
+    rounding the one into e4m3.  Returns Fp8Rows."""
     if h is not None and x_out is None:
         x_out = x
     q, s = (None, None) if out is None else (out.q, out.s)

@@ -84,7 +84,12 @@ __device__ __forceinline__ void load8(const T* p, int have, float* v) {
 __device__ __forceinline__ u32x2_t fp8_block16(const float* v, uint32_t& code) {
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, fp8_size(v[i]));
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  if (top >= 0x7f800000u) {  // (what is not finite does not count)
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, fp8_size(v[i]));
+  }
   code = fp8_code(max_of_16(top));
   const float f = fp8_inverse(code);
   return u32x2_t{fp8_pack4(v[0] * f, v[1] * f, v[2] * f, v[3] * f), fp8_pack4(v[4] * f, v[5] * f, v[6] * f, v[7] * f)};

@@ -56,7 +56,11 @@ __global__ __launch_bounds__(kWaves * 64, 4) void fp8_small_kernel(Fp8Args a, un
   constexpr int STAGE = DEEP * MT * 2048, SUMS = NH * MT * 4 * QUAD * 4;
   __shared__ __align__(16) uint8_t space[kWaves][STAGE > SUMS ? STAGE : SUMS];  // a wave's rows, then its sums
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, quad = lane >> 4, l16 = lane & 15;
-  const unsigned row_tile = blockIdx.x / col_tiles, c16 = blockIdx.x - row_tile * col_tiles;  // 16 MT rows, 16 columns
+  // 16 MT rows, 16 columns.  Workgroups b and b + 8 run on one XCD: those of the
+  // same columns follow each other there, so that its L2 serves all but the
+  // first (192 x 1000 x 2056: 4.9 us, 6.3 with all columns of a row tile first).
+  const unsigned row_tile = blockIdx.x / 8, c16 = blockIdx.y * 8 + blockIdx.x % 8;
+  if (c16 >= col_tiles) return;
   const int64_t row0 = (int64_t)row_tile * (16 * MT);
   uint8_t* const own = space[wave];
   // what the lane loads: PACK, 8 values of rows 4 j + lane / 16, else 16 bytes of rows 8 j + lane / 8
@@ -375,12 +379,12 @@ int32_t check_desc(const char* what, const cev_fp8_desc* d) {
 template <typename T, typename O, bool GATE_UP, int MT>
 int32_t launch_small(const Fp8Args& a, bool e8m0, hipStream_t s) {
   const int columns = MT == 4 ? 32 : 16;
-  const int64_t col_tiles = (a.n + columns - 1) / columns, grid = (a.t + 16 * MT - 1) / (16 * MT) * col_tiles;
-  if (!fp8_grid_fits(grid, kWaves * 64)) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_product: grid too large");
+  const int64_t col_tiles = (a.n + columns - 1) / columns, row_tiles = (a.t + 16 * MT - 1) / (16 * MT), grid = row_tiles * ((col_tiles + 7) / 8 * 8);
+  if (!fp8_grid_fits(grid, kWaves * 64) || col_tiles > 8 * 65535) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_product: grid too large");
   if (e8m0)
-    hipLaunchKernelGGL((fp8_small_kernel<T, O, true, GATE_UP, MT>), dim3((unsigned)grid), dim3(kWaves * 64), 0, s, a, (unsigned)col_tiles);
+    hipLaunchKernelGGL((fp8_small_kernel<T, O, true, GATE_UP, MT>), dim3((unsigned)row_tiles * 8, (unsigned)((col_tiles + 7) / 8)), dim3(kWaves * 64), 0, s, a, (unsigned)col_tiles);
   else
-    hipLaunchKernelGGL((fp8_small_kernel<T, O, false, GATE_UP, MT>), dim3((unsigned)grid), dim3(kWaves * 64), 0, s, a, (unsigned)col_tiles);
+    hipLaunchKernelGGL((fp8_small_kernel<T, O, false, GATE_UP, MT>), dim3((unsigned)row_tiles * 8, (unsigned)((col_tiles + 7) / 8)), dim3(kWaves * 64), 0, s, a, (unsigned)col_tiles);
   return launched("cev_fp8_product");
 }
 

@@ -2,8 +2,9 @@
 // 128 values, and weights laid out for the products of fp8_linear.hip.
 //
 //   rows    q = e4m3(x / 2^e), a scale for 128 columns of a row
-//   norm    the same of the RMS norm of x (+ h): f32 from the rounded
-//           residual to the one rounding into e4m3
+//   norm    the same of the RMS norm of x (+ h): from the rounded residual on
+//           as good as exact (the sum in f64, products in f32 where no border
+//           of e4m3 is near) up to the one rounding
 //   blocks  the same of a weight, a scale for 128 x 128 values
 //   pack    an e4m3 weight in the order in which the matrix cores read it
 //
@@ -52,6 +53,7 @@ struct NormArgs {
   int64_t rows, x_st, h_st, xo_st;
   int32_t k, chunks, plus_one;
   float eps;
+  double inv_k;
 };
 
 template <typename T>
@@ -73,12 +75,23 @@ __device__ __forceinline__ void store8(T* p, int have, const float* v) {
   }
 }
 
+// v * (high + low) * w, the product of the first two to 2^-46, in f32 rounded
+// to odd: what is rounded to fewer bits after it comes out as the exact
+// product's own rounding would.
+__device__ __forceinline__ float scaled_odd(float v, float high, float low, float w) {
+  const float a = v * high, a_rest = __builtin_fmaf(v, low, __builtin_fmaf(v, high, -a));
+  const float p = a * w, rest = __builtin_fmaf(a_rest, w, __builtin_fmaf(a, w, -p));
+  const uint32_t u = __float_as_uint(p);
+  const uint32_t down = (u ^ __float_as_uint(rest)) >> 31;  // p is the larger one
+  return __builtin_fabsf(rest) > 0.0f ? __uint_as_float((u - down) | 1u) : p;
+}
+
 // One row for WAVES waves, NCH chunks of 8 columns a lane in registers; a
 // row wider than that reads its residual a second time.
 template <typename T, int WAVES, int NCH, bool RES>
 __global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : kThreads) void fp8_norm_kernel(NormArgs a) {
   constexpr int LANES = WAVES * 64, ROWS = WAVES > 4 ? 1 : kThreads / LANES;
-  __shared__ float part[ROWS * WAVES];
+  __shared__ double part[ROWS * WAVES];
   const int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
   const int lane = threadIdx.x % LANES;
   const bool live = r < a.rows;
@@ -86,7 +99,7 @@ __global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : kThreads) void fp8_norm_ke
   const T* const h = RES ? (const T*)a.h + (live ? r : 0) * a.h_st : nullptr;
   T* const xo = RES ? (T*)a.x_out + (live ? r : 0) * a.xo_st : nullptr;
   float v[NCH][8];
-  float sum = 0.0f;
+  double sum = 0.0;
   auto take = [&](int c, float* o) {  // chunk c of the row, the residual added and rounded
     const int have = live ? a.k - c * 8 : 0;
     load8(x + (have > 0 ? c * 8 : 0), have, o);
@@ -106,29 +119,52 @@ __global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : kThreads) void fp8_norm_ke
 #pragma unroll
   for (int b = 0; b < NCH; ++b)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(v[b][j], v[b][j], sum);
+    for (int j = 0; j < 8; ++j) sum = __builtin_fma((double)v[b][j], (double)v[b][j], sum);
   for (int c = lane + NCH * LANES; c < a.chunks; c += LANES) {
     float o[8];
     take(c, o);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(o[j], o[j], sum);
+    for (int j = 0; j < 8; ++j) sum = __builtin_fma((double)o[j], (double)o[j], sum);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
   if constexpr (WAVES > 1) {
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
     __syncthreads();
-    sum = 0.0f;
+    sum = 0.0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) sum += part[threadIdx.x / LANES * WAVES + w];
   }
-  const float inv = 1.0f / sqrtf(sum / (float)a.k + a.eps);
+  // 1 / root to 2^-43: the f32 one and a step of Newton's, where f32 holds the mean
+  const double mean = __builtin_fma(sum, a.inv_k, (double)a.eps);
+  double inv;
+  if (mean > 1e-30 && mean < 1e30) {
+    const double y = rsqrtf((float)mean);
+    inv = __builtin_fma(0.5 * y, __builtin_fma(-mean * y, y, 1.0), y);
+  } else {
+    inv = 1.0 / sqrt(mean);
+  }
+  const float inv_high = (float)inv, inv_low = (float)(inv - (double)inv_high);
   auto give = [&](int c, float* o) {  // the row's chunk c, normalised, into e4m3
     float w[8];
     const int have = a.k - c * 8;
     load8((const T*)a.w + (have > 0 ? c * 8 : 0), have, w);
+    // The f32 products are within 1.5 * 2^-24 of the exact ones, 2 units of their
+    // last place.  e4m3's borders (between two of its values, and of its scale)
+    // are multiples of 2^19 units: next to one, the exact product decides.
+    uint32_t near = ~0u;
+    float p[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = j < have ? o[j] * inv * (a.plus_one ? w[j] + 1.0f : w[j]) : 0.0f;
+    for (int j = 0; j < 8; ++j) {
+      if (a.plus_one) w[j] += 1.0f;
+      p[j] = o[j] * inv_high * w[j];
+      near = min(near, (__float_as_uint(p[j]) + 4) & 0x7ffffu);
+    }
+    if (near < 8)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = scaled_odd(o[j], inv_high, inv_low, w[j]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = j < have ? p[j] : 0.0f;
     uint32_t code;
     const u32x2_t q = fp8_block16(o, code);
     if (live && c < a.chunks) {
@@ -304,8 +340,8 @@ template <typename T>
 int32_t launch_norm(const NormArgs& a, hipStream_t s) {
   // A row's chunks of 8 columns go to one lane each; where there are more rows
   // than fill the card, to as few waves as hold them in registers (us, bf16 with
-  // the residual: 64 x 4096 with 8 waves 3.6, with 4 4.1; 8192 x 4096 42.8
-  // and 41.4; 64 x 12288 with 16 waves 4.9, with 8 5.8; 4096 x 1024 with 4
+  // the residual: 64 x 4096 with 8 waves 3.7, with 4 4.1; 8192 x 4096 42.8
+  // and 41.7, 5.6 TB/s; 64 x 12288 with 16 waves 4.9, with 8 5.8; 4096 x 1024 with 4
   // waves 10.0, with 2 7.7).
   if (a.chunks <= 64) return launch_norm<T, 1, 1>(a, s);
   const bool few = a.rows <= 512;
@@ -335,7 +371,7 @@ extern "C" int32_t cev_fp8_rms_norm(int32_t dtype, int64_t rows, int64_t k, cons
   for (const void* p : {x, h, (const void*)x_out, w})
     CEV_CHECK_ARG(q != p && scales != p && q != scales, "cev_fp8_rms_norm: the rows in e4m3 must have memory of their own");
   const NormArgs a{x, h, x_out, w, (uint8_t*)q, (uint8_t*)scales, rows, x_stride, h_stride, x_out_stride, (int32_t)k, (int32_t)((k + 127) / 128 * 16),
-                   weight_plus_one, eps};
+                   weight_plus_one, eps, 1.0 / (double)k};
   return dtype == CEV_BF16 ? launch_norm<__bf16>(a, (hipStream_t)stream) : launch_norm<float>(a, (hipStream_t)stream);
 }
 

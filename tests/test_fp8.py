@@ -272,6 +272,20 @@ def test_norm_of_many_rows(gpu, t, k, add, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1.0, 1e25, 1e-25])
+@pytest.mark.parametrize("t,k", [(64, 4096), (700, 2056), (5, 296)])
+def test_norm_is_the_nearest(gpu, t, k, size, dtype):
+    """The norm is f64 up to the rounding into e4m3: every value and scale is that of 64-bit arithmetic, also where f32 squares
+    leave its range.  (64-bit sums in another order differ by 2^-50 or so: of 10^6 values one is that near a border once in 10^8.)"""
+    x = activations(t, k, torch.float32, 61).mul(size).to(dtype)
+    w = (1 + 0.1 * torch.randn(k, generator=gen(62))).to(dtype)
+    got = cev_hip.rms_norm_fp8(x.to(gpu), w.to(gpu), 0.0)
+    q, e = oracle_rows(oracle_norm(x, w, 0.0, None, False)[1])
+    assert torch.equal(got.s.view(torch.uint8).cpu().double(), e + 127) and torch.equal(got.q.double().cpu(), q)
+
+
+@pytest.mark.gpu
 def test_norm_of_rows_that_are_zero_or_not_finite(gpu):
     x = activations(5, 200, torch.float32, 6)
     x[1] = 0
@@ -815,6 +829,7 @@ def test_abi_refusals(cev):
     refused(L.cev_fp8_rows(0, 2, 8, p, 8, p, C.c_void_p(8192), None), -1, "of their own")
     refused(L.cev_fp8_rms_norm(1, 2, 8, p, 8, None, 0, None, 0, C.c_void_p(8192), 1e-6, 0, p, C.c_void_p(16384), None), -1, "of their own")
     refused(product(desc(**good), out=p), -1, "of its own")
+    refused(product(desc(**dict(good, x_dtype=2, n=1 << 27, out_stride=1 << 27)), xs=C.c_void_p(16384)), -2, "grid too large")
     big = desc(**dict(good, t=4000))
     assert L.cev_fp8_work_size(C.byref(big), C.byref(size)) == 0 and size.value >= 4000 * 129
     refused(product(big, wk=size.value - 1), -4, "workspace")
