@@ -243,7 +243,11 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
         } else if constexpr (E8M0) {
           acc[U][J] = fp8_mfma(wv, x, acc[U][J], (int)s2[J >> 1], sx);
         } else {
+          // (ahead of the other wave's scalings, which fill its time: gate and up of
+          // 2048 x 12288 x 4096 192.1 us without, 188.4 with; e8m0 and f32 outputs the same)
+          __builtin_amdgcn_s_setprio(1);
           p[J % 2] = fp8_mfma(wv, x, f32x4{}, 127, sx);
+          __builtin_amdgcn_s_setprio(0);
         }
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (J < 3) {
