@@ -35,6 +35,18 @@ def _on(stream):
     return _HERE if stream is None else torch.cuda.stream(stream)
 
 
+def _stream(stream, device):
+    """A call's stream, torch's or another object with a cuda_stream, as a torch stream."""
+    import torch
+    return stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream.cuda_stream or 0, device=device)
+
+
+def _capturing(stream) -> bool:
+    import torch
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _like(x):
     """A contiguous tensor of x's shape and type, without values."""
     import torch
@@ -142,9 +154,11 @@ class PagedAttention:
     row sees that many last keys, itself among them, and the first `sinks`
     ones; 0: all.  plan() makes the step's work list from cu and lengths on the
     device; every call until the next plan() uses it.  out may be q.  The object
-    is made on the current stream, which other streams wait for as for a
-    tensor; its workspace (17 MB for decoding steps, 85 to 152 MB for bf16
-    steps with chunks) serves one step at a time."""
+    is made on the current stream.  A call's `stream` waits for that, and holds
+    the workspace (17 MB for decoding steps, 85 to 152 MB for bf16 steps with
+    chunks) until it is done; the workspace serves one step at a time, so a plan
+    and its calls on several streams are the caller's to order.  A read of `work`
+    on the current stream comes behind the plan."""
 
     def __init__(self, q, k_cache, block_table, max_new: Optional[int] = None, window: int = 0, sinks: int = 0, scale: Optional[float] = None):
         import torch
@@ -167,17 +181,47 @@ class PagedAttention:
         n = C.c_size_t()
         check(lib().cev_paged_work_size(C.byref(d), C.byref(n)))
         self.desc = d
-        self.work = torch.zeros(n.value, dtype=torch.uint8, device=q.device)
+        self._work = torch.zeros(n.value, dtype=torch.uint8, device=q.device)
+        self._made = self._planned = None  # the event behind the zeros; the stream of the last plan, where it was given
+        self._streams = set()  # handles of those that were joined
+        if self._work.is_cuda and not torch.cuda.is_current_stream_capturing():
+            self._made = torch.cuda.Event()
+            self._made.record(torch.cuda.current_stream(self._work.device))
+
+    def _join(self, stream):
+        """The first use on a stream of the caller's: behind the zeros, and the
+        memory goes back to the allocator behind it."""
+        import torch
+        if stream is None or stream.cuda_stream in self._streams or not self._work.is_cuda:
+            return
+        s = _stream(stream, self._work.device)
+        if self._made is not None and not _capturing(s):  # (what a captured step uses was made before the capture)
+            s.wait_event(self._made)
+        self._work.record_stream(s)
+        self._streams.add(stream.cuda_stream)
+
+    @property
+    def work(self):
+        """The plan and the partial results (uint8)."""
+        import torch
+        if self._planned is not None:
+            s, here = _stream(self._planned, self._work.device), torch.cuda.current_stream(self._work.device)
+            if s != here and not _capturing(s) and not _capturing(here):
+                here.wait_stream(s)
+        return self._work
 
     def plan(self, cu, lengths, stream=None):
         """The step's work list: cu (requests + 1) and lengths (requests, new
         tokens included) as paged_tables writes them."""
-        calls().paged_plan(self.desc, cu, lengths, self.work, stream)
+        self._join(stream)
+        calls().paged_plan(self.desc, cu, lengths, self._work, stream)
+        self._planned = stream
         return self
 
     def __call__(self, q, k_cache, v_cache, block_table, out=None, stream=None):
         if out is None:
             with _on(stream):
                 out = _like(q)
-        calls().paged_attention(self.desc, q, k_cache, v_cache, block_table, out, self.work, stream)
+        self._join(stream)
+        calls().paged_attention(self.desc, q, k_cache, v_cache, block_table, out, self._work, stream)
         return out
