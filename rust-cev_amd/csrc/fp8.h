@@ -36,9 +36,31 @@ __device__ __forceinline__ bf16x8 fp8_widen(int lo, int hi) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// 2^(code - 127); 2^-127 is subnormal, 255 is NaN.
-__device__ __forceinline__ float fp8_scale_value(uint32_t code) {
-  return __uint_as_float(code == 0 ? 0x400000u : code == 255 ? 0x7fc00000u : code << 23);
+// A weight's scale as 2^(code - 127) times the rest: 1 of an e8m0 byte, of an
+// f32 (whose exponent the matrix cores then apply) its significand, 1 to 2, so
+// that a product under the code alone leaves f32's range only where the result
+// does.  0 keeps code 0; infinities and NaN keep themselves as the rest.
+struct Fp8Scale {
+  int code;
+  float rest;
+};
+template <bool E8M0>
+__device__ __forceinline__ Fp8Scale fp8_scale(uint32_t s) {
+  if constexpr (E8M0) return {(int)s, s == 255 ? __builtin_nanf("") : 1.0f};
+  const int code = min((int)(s >> 23 & 255), 254);
+  return {code, __builtin_ldexpf(__uint_as_float(s), 127 - code)};
+}
+
+// The scales of a sum of unscaled products, which is 0 or between 2^-18 and
+// 2^25: (sum * first) * second, in range wherever the result is, and rounded
+// once, as `first` is a power of two (2^-100 to 2^100).
+struct Fp8Factors {
+  float first, second;
+};
+__device__ __forceinline__ Fp8Factors fp8_factors(int row_code, const Fp8Scale& w) {
+  const int e = row_code + w.code - 254, c = min(max(e, -100), 100);
+  const float first = __uint_as_float(row_code == 255 ? 0x7fc00000u : (uint32_t)(c + 127) << 23);
+  return {first, __builtin_ldexpf(w.rest, min(e - c, 126))};  // (2^126 and more: infinite, but for a sum of 0)
 }
 
 __device__ __forceinline__ i32x8 fp8_join(const u32x4_t& a, const u32x4_t& b) {

@@ -5,9 +5,9 @@
 // Two kinds of matrix product:
 //
 //   bf16 outputs, and gate and up of many rows
-//       v_mfma_scale_f32_16x16x128_f8f6f4, which takes 2^e as an operand (and s
-//       where it is a power of two; an f32 s multiplies the block's 16 x 16
-//       results).  It adds eight neighbouring columns' products after cutting
+//       v_mfma_scale_f32_16x16x128_f8f6f4, which takes 2^e as an operand, and s
+//       where it is a power of two (of an f32 s its power of two; the rest of it,
+//       1 to 2, multiplies the block's 16 x 16 results).  It adds eight neighbouring columns' products after cutting
 //       each towards zero to a multiple of 2^(E - 13), 2^E the largest one's
 //       power of two (measured bit by bit); what follows is f32.  A sum is
 //       therefore up to 7 * 2^-13 of its largest products off; on normal data
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(kWaves * 64, 4) void fp8_small_kernel(Fp8Args a, un
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
         const i32x8 wv = fp8_join(w[d][h][0], w[d][h][1]);
-        const float f = E8M0 ? fp8_scale_value(sw[d][h]) : __uint_as_float(sw[d][h]);
+        const Fp8Scale f = fp8_scale<E8M0>(sw[d][h]);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           if constexpr (EXACT) {
@@ -153,16 +153,15 @@ __global__ __launch_bounds__(kWaves * 64, 4) void fp8_small_kernel(Fp8Args a, un
 #pragma unroll
             for (int c = 0; c < 4; ++c)
               p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(wv[2 * c], wv[2 * c + 1]), fp8_widen(xv[i][2 * c], xv[i][2 * c + 1]), p, 0, 0, 0);
-            // (one scale after the other: their product may leave f32's range where the result does not)
-            const float s = fp8_scale_value((uint32_t)sx[d][i]);
+            const Fp8Factors by = fp8_factors(sx[d][i], f);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[h][i][r] = __builtin_fmaf(p[r] * s, f, acc[h][i][r]);
+            for (int r = 0; r < 4; ++r) acc[h][i][r] = __builtin_fmaf(p[r] * by.first, by.second, acc[h][i][r]);
           } else if constexpr (E8M0) {
             acc[h][i] = fp8_mfma(wv, xv[i], acc[h][i], (int)sw[d][h], sx[d][i]);
           } else {
-            const f32x4 p = fp8_mfma(wv, xv[i], f32x4{}, 127, sx[d][i]);
+            const f32x4 p = fp8_mfma(wv, xv[i], f32x4{}, f.code, sx[d][i]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[h][i][r] = __builtin_fmaf(p[r], f, acc[h][i][r]);
+            for (int r = 0; r < 4; ++r) acc[h][i][r] = __builtin_fmaf(p[r], f.rest, acc[h][i][r]);
           }
         }
       }

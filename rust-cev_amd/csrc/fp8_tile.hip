@@ -200,12 +200,15 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
     if constexpr (E8M0)
 #pragma unroll
       for (int j = 0; j < 2; ++j) s2[j] = sw4[j] >> (8 * b4);
+    Fp8Scale s[2];
+    if constexpr (!E8M0 || EXACT)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s[j] = fp8_scale<E8M0>(E8M0 ? s2[j] & 255 : sw[B][j]);
     f32x4 p[2];
     auto scale_in = [&](auto u_c, auto j_c) {
       constexpr int U = decltype(u_c)::value, J = decltype(j_c)::value;
-      const float f = __uint_as_float(sw[B][J >> 1]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[U][J][r] = __builtin_fmaf(p[J % 2][r], f, acc[U][J][r]);
+      for (int r = 0; r < 4; ++r) acc[U][J][r] = __builtin_fmaf(p[J % 2][r], s[J >> 1].rest, acc[U][J][r]);
     };
     static_for<TT>([&](auto u_c) {
       constexpr int U = decltype(u_c)::value;
@@ -221,11 +224,12 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
       const i32x8 x = fp8_join(xr[U % RING].v[0], xr[U % RING].v[1]);
       const int sx = xr[U % RING].s;
       bf16x8 wide[4];
-      float fx = 0.0f;
+      Fp8Factors by[2];
       if constexpr (EXACT) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) wide[c] = fp8_widen(x[2 * c], x[2 * c + 1]);
-        fx = fp8_scale_value((uint32_t)sx);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) by[j] = fp8_factors(sx, s[j]);
       }
       // Four matrix products, and between them what is read for later ones: a
       // product takes 32 cycles, in which seven other instructions can start.
@@ -236,17 +240,15 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
           f32x4 q = {};
 #pragma unroll
           for (int c = 0; c < 4; ++c) q = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(wv[2 * c], wv[2 * c + 1]), wide[c], q, 0, 0, 0);
-          // (one scale after the other: their product may leave f32's range where the result does not)
-          const float f = E8M0 ? fp8_scale_value(s2[J >> 1] & 255) : __uint_as_float(sw[B][J >> 1]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[U][J][r] = __builtin_fmaf(q[r] * fx, f, acc[U][J][r]);
+          for (int r = 0; r < 4; ++r) acc[U][J][r] = __builtin_fmaf(q[r] * by[J >> 1].first, by[J >> 1].second, acc[U][J][r]);
         } else if constexpr (E8M0) {
           acc[U][J] = fp8_mfma(wv, x, acc[U][J], (int)s2[J >> 1], sx);
         } else {
           // (ahead of the other wave's scalings, which fill its time: gate and up of
           // 2048 x 12288 x 4096 192.1 us without, 188.4 with; e8m0 and f32 outputs the same)
           __builtin_amdgcn_s_setprio(1);
-          p[J % 2] = fp8_mfma(wv, x, f32x4{}, 127, sx);
+          p[J % 2] = fp8_mfma(wv, x, f32x4{}, s[J >> 1].code, sx);
           __builtin_amdgcn_s_setprio(0);
         }
         __builtin_amdgcn_sched_barrier(0);
