@@ -544,7 +544,8 @@ int32_t cev_paged_attention(const cev_paged_desc* d, const void* q, const void* 
  * magnitude; q is x / 2^e, which is exact in f32, rounded to nearest even.  A
  * value that is not finite becomes NaN and counts for no scale.  Weights (n,
  * k): a scale for 128 x 128 values, from cev_fp8_blocks or brought along.
- * Outputs and workspaces overlap no input but where a call says so.
+ * A call whose outputs or workspace overlap each other or an input, but where
+ * it says so, is refused (columns side by side in one buffer do not overlap).
  * Nothing here has a gradient. */
 enum { CEV_E4M3 = 2 };                                   /* beside CEV_F32 and CEV_BF16, where a call says so */
 enum { CEV_FP8_SCALES_E8M0 = 0, CEV_FP8_SCALES_F32 = 1 }; /* a weight's scales: bytes 2^(byte - 127), or any f32 */
@@ -557,7 +558,7 @@ int32_t cev_fp8_rows(int32_t dtype, int64_t t, int64_t k, const void* x, int64_t
 
 /* The RMS norm before a projection (qwen3.rs:254-255), with the residual add
  * where h is given (qwen3.rs:261): x_out = dtype(x + h) is written (x_out may
- * be x), and x_out / sqrt(mean x_out^2 + eps) * w goes into e4m3 with one
+ * be x or h), and x_out / sqrt(mean x_out^2 + eps) * w goes into e4m3 with one
  * rounding, that of the exact value (with weight_plus_one 1 + w is f32).
  * Alignment as above, for w too. */
 int32_t cev_fp8_rms_norm(int32_t dtype, int64_t rows, int64_t k, const void* x, int64_t x_stride, const void* h, int64_t h_stride,

@@ -9,7 +9,8 @@ of them (of a row of activations 128 columns, of a weight 128 x 128).
 
 Scales that are made here are powers of two (cev_hip.h says which), so that
 they cost no significant bit.  Sums are f32; every result is rounded once.  The
-calls record nothing for autograd.
+calls record nothing for autograd.  An output has memory of its own: one that
+lies over a part of an input is refused.
 """
 from __future__ import annotations
 
@@ -86,7 +87,7 @@ def fp8_blocks(w, stream=None):
 
 def rms_norm_fp8(x, w, eps: float, h=None, x_out=None, out=None, plus_one: bool = False, stream=None):
     """rms_norm into e4m3 (cev_fp8_rms_norm): with h the residual add first,
-    x_out = x + h in x's type (x_out defaults to x), then the norm, its only
+    x_out = x + h in x's type (x_out defaults to x, and may be h), then the norm, its only
     rounding the one into e4m3.  Returns Fp8Rows."""
     if h is not None and x_out is None:
         x_out = x

@@ -129,6 +129,35 @@ extern "C" int32_t cev_rope_table(double theta, int32_t rot, int32_t n_pos, int3
 }
 
 // ---------------------------------------------------------------------
+// Overlapping rows
+
+extern "C" bool cev_overlap(const CevRows* x, const CevRows* y) {
+  if (x->rows <= 0 || y->rows <= 0 || x->bytes <= 0 || y->bytes <= 0) return false;
+  auto one = [](CevRows r) {
+    if (r.rows == 1) r.stride = r.bytes;
+    if (r.stride == r.bytes) r.bytes *= r.rows, r.stride = r.bytes, r.rows = 1;  // dense
+    return r;
+  };
+  CevRows a = one(*x), b = one(*y);
+  if (a.rows > b.rows) std::swap(a, b);
+  // Row j of b overlaps [at, at + bytes) where j * stride < at + bytes and j *
+  // stride + b.bytes > at: the last row of the first kind decides, as later rows
+  // end later.  `lo` is the first row there is.
+  auto hits = [&](int64_t at, int64_t lo) {
+    const int64_t end = at + a.bytes - 1, j = std::min(b.rows - 1, end >= 0 ? end / b.stride : -((-end + b.stride - 1) / b.stride));
+    return j >= lo && j * b.stride + b.bytes > at;
+  };
+  const int64_t at = (int64_t)((uintptr_t)a.p - (uintptr_t)b.p);
+  if (at >= (b.rows - 1) * b.stride + b.bytes || at + (a.rows - 1) * a.stride + a.bytes <= 0) return false;
+  if (a.rows == 1) return hits(at, 0);
+  // (one stride: row i of a meets row j of b where row 0 of a would meet row j - i)
+  if (a.stride == b.stride) return hits(at, -(a.rows - 1));
+  for (int64_t i = 0; i < a.rows; ++i)
+    if (hits(at + i * a.stride, 0)) return true;
+  return false;
+}
+
+// ---------------------------------------------------------------------
 // Table validation and planning
 
 namespace {

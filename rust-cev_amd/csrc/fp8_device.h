@@ -10,7 +10,10 @@
 // rounds to 0 in e4m3 either way), and the matrix cores take the scale as it
 // is stored: e + 127 in a byte (e8m0).
 #pragma once
+#include <initializer_list>
+
 #include "cev_device.h"
+#include "cev_internal.h"
 
 constexpr int kFp8Block = 128;    // values of a row under one scale
 constexpr int kFp8Group = 32;     // weight rows of one matrix-core operand
@@ -19,6 +22,17 @@ constexpr int kFp8TileGroups = 8;  // weight rows are padded to 8 groups
 
 // A launch counts its threads in 32 bits.
 inline bool fp8_grid_fits(int64_t grid, int threads) { return grid <= (int64_t)(UINT32_MAX / (uint32_t)threads); }
+
+// Whether a call's outputs overlap neither each other nor an input.
+inline bool fp8_apart(std::initializer_list<CevRows> outs, std::initializer_list<CevRows> ins) {
+  for (const CevRows& o : outs) {
+    for (const CevRows& other : outs)
+      if (&o < &other && cev_overlap(&o, &other)) return false;
+    for (const CevRows& in : ins)
+      if (cev_overlap(&o, &in)) return false;
+  }
+  return true;
+}
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));

@@ -362,6 +362,19 @@ Form form_of(const cev_fp8_desc& d) {
   return f;
 }
 
+// Whether a form's launches count their threads in 32 bits.
+bool grids_fit(const cev_fp8_desc& d, const Form& f) {
+  if (f.tt == 0) {
+    const int columns = f.mt == 4 ? 32 : 16;
+    const int64_t col_tiles = (d.n + columns - 1) / columns, row_tiles = (d.t + 16 * f.mt - 1) / (16 * f.mt);
+    return col_tiles <= 8 * 65535 && fp8_grid_fits(row_tiles * ((col_tiles + 7) / 8 * 8), kWaves * 64);
+  }
+  const int64_t row_tiles = (d.t + 16 * f.tt - 1) / (16 * f.tt);
+  if (!fp8_grid_fits(row_tiles * (f.groups / kFp8TileGroups) * f.parts, 256 * f.teams)) return false;
+  const int64_t quads = d.gate_up ? (d.n + 127) / 128 * 16 : (d.n + 3) / 4;
+  return f.parts == 1 || fp8_grid_fits((d.t * quads + 255) / 256, 256);
+}
+
 int32_t check_desc(const char* what, const cev_fp8_desc* d) {
   CEV_CHECK_ARG(d != nullptr, "%s: null descriptor", what);
   if (d->x_dtype != CEV_F32 && d->x_dtype != CEV_BF16 && d->x_dtype != CEV_E4M3) return cev_fail(CEV_ERR_UNSUPPORTED, "%s: x dtype %d", what, d->x_dtype);
@@ -378,8 +391,7 @@ int32_t check_desc(const char* what, const cev_fp8_desc* d) {
 template <typename T, typename O, bool GATE_UP, int MT>
 int32_t launch_small(const Fp8Args& a, bool e8m0, hipStream_t s) {
   const int columns = MT == 4 ? 32 : 16;
-  const int64_t col_tiles = (a.n + columns - 1) / columns, row_tiles = (a.t + 16 * MT - 1) / (16 * MT), grid = row_tiles * ((col_tiles + 7) / 8 * 8);
-  if (!fp8_grid_fits(grid, kWaves * 64) || col_tiles > 8 * 65535) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_product: grid too large");
+  const int64_t col_tiles = (a.n + columns - 1) / columns, row_tiles = (a.t + 16 * MT - 1) / (16 * MT);
   if (e8m0)
     hipLaunchKernelGGL((fp8_small_kernel<T, O, true, GATE_UP, MT>), dim3((unsigned)row_tiles * 8, (unsigned)((col_tiles + 7) / 8)), dim3(kWaves * 64), 0, s, a, (unsigned)col_tiles);
   else
@@ -438,12 +450,19 @@ extern "C" int32_t cev_fp8_product(const cev_fp8_desc* d, const void* x, const v
   } else {
     CEV_CHECK_ARG(((uintptr_t)out & 15) == 0, "%s: rows in e4m3 must be 16-byte aligned", me);
   }
-  for (const void* p : {x, x_scales, weight})
-    CEV_CHECK_ARG(out != p && (!out_scales || (out_scales != p && out_scales != out)), "%s: the output must have memory of its own", me);
   const Form f = form_of(*d);
-  need = f.rows_bytes + f.scales_bytes + f.part_bytes;
-  if (work_bytes < need) return cev_fail(CEV_ERR_SPACE, "%s: a workspace of %zu bytes, %zu needed", me, work_bytes, need);
-  CEV_CHECK_ARG(need == 0 || (work && ((uintptr_t)work & 255) == 0), "%s: the workspace must be 256-byte aligned", me);
+  const size_t space_bytes = f.rows_bytes + f.scales_bytes + f.part_bytes;
+  if (work_bytes < space_bytes) return cev_fail(CEV_ERR_SPACE, "%s: a workspace of %zu bytes, %zu needed", me, work_bytes, space_bytes);
+  CEV_CHECK_ARG(space_bytes == 0 || (work && ((uintptr_t)work & 255) == 0), "%s: the workspace must be 256-byte aligned", me);
+  if (!grids_fit(*d, f)) return cev_fail(CEV_ERR_UNSUPPORTED, "%s: grid too large", me);
+  {
+    const int64_t e = d->x_dtype == CEV_E4M3 ? 1 : d->x_dtype == CEV_BF16 ? 2 : 4, kb = f.kb, nb = (d->n + 127) / 128;
+    const CevRows o = d->gate_up ? CevRows{out, 1, 0, d->t * nb * 128} : cev_rows(out, d->t, d->out_stride, d->n, d->out_dtype == CEV_BF16 ? 2 : 4);
+    CEV_CHECK_ARG(fp8_apart({o, cev_rows(out_scales, 1, 0, d->t * nb, 1), cev_rows(space_bytes ? work : nullptr, 1, 0, (int64_t)space_bytes, 1)},
+                            {d->x_dtype == CEV_E4M3 ? CevRows{x, 1, 0, d->t * kb * 128} : cev_rows(x, d->t, d->x_stride, d->k, e),
+                             cev_rows(x_scales, 1, 0, d->t * kb, 1), cev_rows(weight, 1, 0, (int64_t)need, 1)}),
+                  "%s: the output, and the workspace, must have memory of its own", me);
+  }
   const hipStream_t s = (hipStream_t)stream;
   uint8_t* const space = (uint8_t*)work;
   int x_dtype = d->x_dtype;
@@ -475,7 +494,6 @@ extern "C" int32_t cev_fp8_product(const cev_fp8_desc* d, const void* x, const v
   JoinArgs j{a.part, out, (uint8_t*)out_scales, d->t, d->n, a.out_st, (int64_t)f.groups * kFp8Group, f.parts, 0};
   j.quads = (int32_t)(d->gate_up ? (d->n + 127) / 128 * 16 : (d->n + 3) / 4);
   const int64_t grid = (d->t * j.quads + 255) / 256;
-  if (!fp8_grid_fits(grid, 256)) return cev_fail(CEV_ERR_UNSUPPORTED, "%s: too many rows", me);
   if (d->gate_up)
     hipLaunchKernelGGL(fp8_join_gate_up_kernel, dim3((unsigned)grid), dim3(256), 0, s, j);
   else if (d->out_dtype == CEV_BF16)

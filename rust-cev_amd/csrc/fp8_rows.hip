@@ -294,6 +294,8 @@ int32_t launched(const char* what) {
   return e == hipSuccess ? CEV_OK : cev_fail(CEV_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
 }
 
+int64_t size_of(int32_t dtype) { return dtype == CEV_BF16 ? 2 : 4; }
+
 // The checks of a call's rows in the model's type.
 int32_t check_rows(const char* what, int32_t dtype, int64_t t, int64_t k, const char* name, const void* p, int64_t stride) {
   const int vec = dtype == CEV_BF16 ? 8 : 4;
@@ -317,7 +319,8 @@ extern "C" int32_t cev_fp8_rows(int32_t dtype, int64_t t, int64_t k, const void*
   const int parts = a.chunks > kThreads ? (a.chunks + kThreads - 1) / kThreads : 1;
   const int64_t grid = (t + a.rows_wg - 1) / a.rows_wg * parts;
   if (!fp8_grid_fits(grid, kThreads)) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_rows: too many rows");
-  CEV_CHECK_ARG(q != x && scales != x && q != scales, "cev_fp8_rows: the outputs must have memory of their own");
+  CEV_CHECK_ARG(fp8_apart({{q, 1, 0, t * a.chunks * 8}, {scales, 1, 0, t * (a.chunks / 16)}}, {cev_rows(x, t, x_stride, k, size_of(dtype))}),
+                "cev_fp8_rows: the outputs must have memory of their own");
   hipLaunchKernelGGL(dtype == CEV_BF16 ? fp8_rows_kernel<__bf16> : fp8_rows_kernel<float>, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, a, parts);
   return launched("cev_fp8_rows");
 }
@@ -368,8 +371,13 @@ extern "C" int32_t cev_fp8_rms_norm(int32_t dtype, int64_t rows, int64_t k, cons
     if (const int32_t rc = check_rows("cev_fp8_rms_norm", dtype, rows, k, "x_out", x_out, x_out_stride)) return rc;
   }
   CEV_CHECK_ARG(q && scales && aligned(q, 16), "cev_fp8_rms_norm: null or misaligned output");
-  for (const void* p : {x, h, (const void*)x_out, w})
-    CEV_CHECK_ARG(q != p && scales != p && q != scales, "cev_fp8_rms_norm: the rows in e4m3 must have memory of their own");
+  const int64_t e = size_of(dtype), kb = (k + 127) / 128;
+  const CevRows rx = cev_rows(x, rows, x_stride, k, e), rh = cev_rows(h, rows, h_stride, k, e), ro = cev_rows(h ? x_out : nullptr, rows, x_out_stride, k, e),
+                rw = cev_rows(w, 1, 0, k, e);
+  CEV_CHECK_ARG(fp8_apart({{q, 1, 0, rows * kb * 128}, {scales, 1, 0, rows * kb}}, {rx, rh, ro, rw}),
+                "cev_fp8_rms_norm: the rows in e4m3 must have memory of their own");
+  CEV_CHECK_ARG((cev_same(ro, rx) || !cev_overlap(&ro, &rx)) && (cev_same(ro, rh) || !cev_overlap(&ro, &rh)) && !cev_overlap(&ro, &rw),
+                "cev_fp8_rms_norm: x_out must be x or h, or have memory of its own");
   const NormArgs a{x, h, x_out, w, (uint8_t*)q, (uint8_t*)scales, rows, x_stride, h_stride, x_out_stride, (int32_t)k, (int32_t)((k + 127) / 128 * 16),
                    weight_plus_one, eps, 1.0 / (double)k};
   return dtype == CEV_BF16 ? launch_norm<__bf16>(a, (hipStream_t)stream) : launch_norm<float>(a, (hipStream_t)stream);
@@ -380,10 +388,11 @@ extern "C" int32_t cev_fp8_blocks(int32_t dtype, int64_t n, int64_t k, const voi
   CEV_CHECK_ARG(n >= 1 && n <= INT32_MAX - 256 && k >= 1 && k <= INT32_MAX - 128, "cev_fp8_blocks: a weight of %lld x %lld", (long long)n, (long long)k);
   if (const int32_t rc = check_rows("cev_fp8_blocks", dtype, n, k, "w", w, ldw)) return rc;
   CEV_CHECK_ARG(q && scales && aligned(q, 16), "cev_fp8_blocks: null or misaligned output");
-  CEV_CHECK_ARG(q != w && scales != w && q != scales, "cev_fp8_blocks: the outputs must have memory of their own");
   const BlocksArgs a{w, (uint8_t*)q, (uint8_t*)scales, n, ldw, (int32_t)k, (int32_t)((k + 127) / 128)};
   const int64_t grid = (n + 127) / 128 * a.kb;
   if (!fp8_grid_fits(grid, kBlockThreads)) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_blocks: weight too large");
+  CEV_CHECK_ARG(fp8_apart({{q, 1, 0, n * k}, {scales, 1, 0, grid}}, {cev_rows(w, n, ldw, k, size_of(dtype))}),
+                "cev_fp8_blocks: the outputs must have memory of their own");
   if (dtype == CEV_BF16)
     hipLaunchKernelGGL(fp8_blocks_kernel<__bf16>, dim3((unsigned)grid), dim3(kBlockThreads), 0, (hipStream_t)stream, a);
   else
@@ -429,6 +438,10 @@ extern "C" int32_t cev_fp8_weight_pack(int64_t n, int64_t k, int32_t scale_kind,
   a.gate_up = gate_up, a.f32_scales = scale_kind == CEV_FP8_SCALES_F32;
   const int64_t grid = a.groups * kb;
   if (!fp8_grid_fits(grid, kThreads)) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_weight_pack: weight too large");
+  const int64_t e = a.f32_scales ? 4 : 1;
+  CEV_CHECK_ARG(fp8_apart({{weight, 1, 0, (int64_t)need}},
+                          {cev_rows(q, n, ldq, k, 1), cev_rows(scales, nb, lds, kb, e), cev_rows(up_q, n, up_ldq, k, 1), cev_rows(up_scales, nb, up_lds, kb, e)}),
+                "cev_fp8_weight_pack: the weight must have memory of its own");
   hipLaunchKernelGGL(fp8_pack_kernel, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, a);
   return launched("cev_fp8_weight_pack");
 }

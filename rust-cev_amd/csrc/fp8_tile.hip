@@ -420,7 +420,6 @@ __global__ __launch_bounds__(256 * TEAMS, TT > 8 ? 1 : 2) void fp8_tile_kernel(F
 template <bool E8M0, bool GATE_UP, bool EXACT, int TT, int TEAMS>
 int32_t launch(const Fp8Args& a, hipStream_t s) {
   const int64_t row_tiles = (a.t + 16 * TT - 1) / (16 * TT), col_tiles = a.groups / kFp8TileGroups, grid = row_tiles * col_tiles * a.parts;
-  if (!fp8_grid_fits(grid, 256 * TEAMS)) return cev_fail(CEV_ERR_UNSUPPORTED, "cev_fp8_product: grid too large");
   hipLaunchKernelGGL((fp8_tile_kernel<E8M0, GATE_UP, EXACT, TT, TEAMS>), dim3((unsigned)grid), dim3(256 * TEAMS), 0, s, a, (int)row_tiles, (int)col_tiles);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? CEV_OK : cev_fail(CEV_ERR_HIP, "cev_fp8_product launch: %s", hipGetErrorString(e));

@@ -73,3 +73,125 @@ def test_scales_of_zero_infinity_and_nan(gpu, t, n, k, out_dtype):
         at = up128(n) - 128
         assert torch.equal(y[:, :at], want[:, :at])
         assert bool((y[:, at:] == bad).all() if bad == bad else torch.isnan(y[:, at:]).all())
+
+
+# ---------------------------------------------------------------------------
+# Overlapping memory
+
+
+def test_overlapping_rows_by_every_byte(cev):
+    """cev_overlap against the sets of bytes, for all small strides, lengths and distances."""
+    import ctypes as C
+    import itertools
+
+    class Rows(C.Structure):
+        _fields_ = [("p", C.c_void_p), ("rows", C.c_int64), ("stride", C.c_int64), ("bytes", C.c_int64)]
+
+    f = cev._abi.lib().cev_overlap
+    f.restype, f.argtypes = C.c_bool, [C.POINTER(Rows), C.POINTER(Rows)]
+    of = lambda p, rows, stride, n: {p + i * stride + j for i in range(rows) for j in range(n)}  # noqa: E731
+    shapes = [(r, s, n) for r in (0, 1, 2, 4) for n in (0, 1, 3) for s in (n, n + 1, n + 4) if r > 1 or s == n] + [(3, 7, 2), (1, -5, 2), (1, 0, 4)]
+    n = 0
+    for a, b in itertools.product(shapes, repeat=2):
+        for at in range(-24, 25):
+            want = bool(of(100, *a) & of(100 + at, *b))
+            assert f(C.byref(Rows(100, *a)), C.byref(Rows(100 + at, *b))) == want, (a, b, at)
+            n += want
+    assert n > 1000
+    big = 1 << 31
+    assert not f(C.byref(Rows(1 << 20, big, 256, 128)), C.byref(Rows((1 << 20) + 128, big, 256, 128)))
+    assert f(C.byref(Rows(1 << 20, big, 256, 129)), C.byref(Rows((1 << 20) + 128, big, 256, 128)))
+
+
+def test_shifted_outputs_are_refused(cev):
+    """An output that lies over a part of an input or of another output: refused before the GPU is looked at."""
+    import ctypes as C
+    L = cev._abi.lib()
+    at = lambda x: C.c_void_p((1 << 20) + x)  # noqa: E731
+
+    def refused(rc):
+        assert rc == -1 and " own" in L.cev_last_error().decode(), (rc, L.cev_last_error())
+
+    far = 1 << 24
+    # rows: x (4, 128) f32 with rows 256 elements apart, (4 * 256 - 128) * 4 bytes
+    rows = lambda q, s: L.cev_fp8_rows(0, 4, 128, at(0), 256, at(q), at(s), None)  # noqa: E731
+    refused(rows(16, far))
+    refused(rows(-16, far))
+    refused(rows(3 * 1024 + 496, far))
+    refused(rows(far, 511))
+    refused(rows(512 - 16, far))
+    refused(rows(far, far + 511))
+    refused(rows(far, far - 3))
+    # the norm: x, h (4, 64) bf16, x_out shifted against them, or over w
+    norm = lambda xo=0, so=64, h=far, w=2 * far, q=3 * far, s=4 * far: L.cev_fp8_rms_norm(1, 4, 64, at(0), 64, at(h), 64, at(xo), so, at(w), 1e-6, 0, at(q), at(s), None)  # noqa: E731
+    refused(norm(xo=128))
+    refused(norm(xo=-384))
+    refused(norm(xo=0, so=72))
+    refused(norm(xo=far + 16))
+    refused(norm(xo=2 * far - 16))
+    refused(norm(q=16))
+    refused(norm(q=far - 256))
+    refused(norm(xo=far, s=far + 511))
+    refused(norm(q=2 * far + 112))
+    refused(norm(s=2 * far + 127))
+    refused(norm(q=3 * far, s=3 * far + 511))
+    # blocks: w (130, 136) f32
+    blocks = lambda q, s: L.cev_fp8_blocks(0, 130, 136, at(0), 136, at(q), at(s), None)  # noqa: E731
+    refused(blocks(130 * 136 * 4 - 16, far))
+    refused(blocks(far, 130 * 136 * 4 - 1))
+    refused(blocks(far, far + 130 * 136 - 1))
+    # pack: q (130, 136), f32 scales (2, 2), 256-byte aligned weight of 2 * 8 * 2 pieces
+    pack = lambda w, up=None, ups=None: L.cev_fp8_weight_pack(130, 136, 1, at(0), 136, at(far), 2, up, 136 if up else 0, ups, 2 if up else 0, at(w), 1 << 22, None)  # noqa: E731
+    refused(pack(17408))
+    refused(pack(-256))
+    refused(pack(far))
+    refused(pack(2 * far, at(2 * far + 512), at(3 * far)))
+    refused(pack(2 * far, at(3 * far), at(2 * far + 512)))
+    # products: x (40, 128) bf16 with rows 256 apart, a weight of 8 pieces, out (40, 200)
+    desc = cev._abi.Fp8Desc
+    size = C.c_size_t()
+
+    def product(x=0, xs=None, w=far, out=2 * far, outs=None, work=4 * far, **kw):
+        d = desc(**{**dict(x_dtype=1, out_dtype=1, scales=1, gate_up=0, t=40, n=200, k=128, x_stride=256, out_stride=200), **kw})
+        assert L.cev_fp8_work_size(C.byref(d), C.byref(size)) == 0
+        return L.cev_fp8_product(C.byref(d), at(x), xs, at(w), 1 << 22, at(out), outs, at(work), size.value, None)
+
+    refused(product(out=16))
+    refused(product(out=-40 * 400 + 2))
+    refused(product(out=far + 8 * 4100 - 2))
+    refused(product(work=512))
+    refused(product(work=2 * far + 256))
+    refused(product(work=far))
+    refused(product(x=16, out=0, out_stride=256))
+    refused(product(x_dtype=2, xs=at(3 * far), out=40 * 128 - 2))
+    refused(product(x_dtype=2, xs=at(3 * far), out=3 * far + 38))
+    gate = dict(x_dtype=2, xs=at(3 * far), gate_up=1, out_dtype=2, n=128)
+    refused(product(outs=at(2 * far + 39), **gate))
+    refused(product(outs=at(40 * 128 - 1), **gate))
+    refused(product(out=16, outs=at(5 * far), **gate))
+    refused(product(work=5 * far, outs=at(5 * far + 100), **gate))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_outputs_beside_their_inputs_in_one_buffer(gpu, dtype):
+    """Columns of one wide buffer as x and out, the sum of a norm in place of x or of h, and x_out beside both."""
+    t, k, n = 40, 256, 200
+    g = torch.Generator().manual_seed(1)
+    room = torch.randn(t, 1024, generator=g).to(dtype).to(gpu)
+    x, h, out, xo = room[:, :k], room[:, 256: 512], room[:, 512: 512 + n], room[:, 768:]
+    w = Fp8Weight(*cev_hip.fp8_blocks(torch.randn(n, k, generator=g).to(dtype).to(gpu)))
+    gamma = torch.ones(k, dtype=dtype, device=gpu)
+    want = cev_hip.linear_fp8(x.contiguous(), w)
+    assert torch.equal(cev_hip.linear_fp8(x, w, out=out), want) and torch.equal(out, want)
+    total = x + h
+    rows = cev_hip.rms_norm_fp8(x.contiguous(), gamma, 1e-6, h=h)
+    for place in (xo, h, x):  # (h and x last: they are overwritten)
+        a, b = x.clone(), h.clone()
+        got = cev_hip.rms_norm_fp8(x, gamma, 1e-6, h=h, x_out=place)
+        assert torch.equal(place, total) and torch.equal(got.q.view(torch.uint8), rows.q.view(torch.uint8))
+        x.copy_(a), h.copy_(b)
+    with pytest.raises(cev_hip.CevError, match="of its own"):
+        cev_hip.rms_norm_fp8(room[:, 8: 8 + k], gamma, 1e-6, h=h.clone(), x_out=x)
+    with pytest.raises(cev_hip.CevError, match="of its own"):
+        cev_hip.linear_fp8(x, w, out=room[:, k - 8: k - 8 + n])
