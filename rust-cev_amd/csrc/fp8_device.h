@@ -93,9 +93,8 @@ __device__ __forceinline__ void load8(const T* p, int have, float* v) {
   }
 }
 
-// 16 adjacent lanes' 8 values each, one block: the lane's 8 bytes, and the
-// block's scale.
-__device__ __forceinline__ u32x2_t fp8_block16(const float* v, uint32_t& code) {
+// 16 adjacent lanes' 8 values each, one block: its largest size.
+__device__ __forceinline__ uint32_t fp8_top16(const float* v) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
@@ -104,7 +103,17 @@ __device__ __forceinline__ u32x2_t fp8_block16(const float* v, uint32_t& code) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, fp8_size(v[i]));
   }
-  code = fp8_code(max_of_16(top));
+  return max_of_16(top);
+}
+
+// The lane's 8 bytes under the block's scale.
+__device__ __forceinline__ u32x2_t fp8_pack8(const float* v, uint32_t code) {
   const float f = fp8_inverse(code);
   return u32x2_t{fp8_pack4(v[0] * f, v[1] * f, v[2] * f, v[3] * f), fp8_pack4(v[4] * f, v[5] * f, v[6] * f, v[7] * f)};
+}
+
+// Both.
+__device__ __forceinline__ u32x2_t fp8_block16(const float* v, uint32_t& code) {
+  code = fp8_code(fp8_top16(v));
+  return fp8_pack8(v, code);
 }

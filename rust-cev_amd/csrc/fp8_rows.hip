@@ -3,8 +3,8 @@
 //
 //   rows    q = e4m3(x / 2^e), a scale for 128 columns of a row
 //   norm    the same of the RMS norm of x (+ h): from the rounded residual on
-//           as good as exact (the sum in f64, products in f32 where no border
-//           of e4m3 is near) up to the one rounding
+//           as good as exact (the sum in f64, products in f32 only where that
+//           rounds the same way) up to the one rounding
 //   blocks  the same of a weight, a scale for 128 x 128 values
 //   pack    an e4m3 weight in the order in which the matrix cores read it
 //
@@ -75,16 +75,23 @@ __device__ __forceinline__ void store8(T* p, int have, const float* v) {
   }
 }
 
-// v * (high + low) * w, the product of the first two to 2^-46, in f32 rounded
-// to odd: what is rounded to fewer bits after it comes out as the exact
-// product's own rounding would.
-__device__ __forceinline__ float scaled_odd(float v, float high, float low, float w) {
-  const float a = v * high, a_rest = __builtin_fmaf(v, low, __builtin_fmaf(v, high, -a));
-  const float p = a * w, rest = __builtin_fmaf(a_rest, w, __builtin_fmaf(a, w, -p));
-  const uint32_t u = __float_as_uint(p);
-  const uint32_t down = (u ^ __float_as_uint(rest)) >> 31;  // p is the larger one
-  return __builtin_fabsf(rest) > 0.0f ? __uint_as_float((u - down) | 1u) : p;
+// v * inv * w in f64, then in f32 rounded to odd: what is rounded to fewer bits
+// after it comes out as the f64 product's own rounding would.  (Beyond f32's
+// range it is infinite, far below it 2^-149.)
+__device__ __forceinline__ float scaled_odd(float v, double inv, float w) {
+  asm("" : "+v"(v));  // (or the f64 values of the sum of squares are kept for it, in the registers of three waves a SIMD)
+  const double exact = (double)v * inv * (double)w;
+  const float p = (float)exact;
+  if (__builtin_fabsf(p) < __builtin_inff() && (double)p != exact) {
+    const uint32_t u = __float_as_uint(p), sign = (uint32_t)(__double_as_longlong(exact) >> 32) & 0x80000000u;
+    const uint32_t size = u & 0x7fffffffu, down = __builtin_fabs((double)p) > __builtin_fabs(exact);  // p is the larger one
+    return __uint_as_float(sign | (size - down) | 1u);
+  }
+  return p;
 }
+
+// The scale of a block that holds kSmallTop is more than 2^-57, and what is less than 2^-10 of it becomes 0.
+constexpr float kLargeWeight = 0x1p56f, kSmallTop = 0x1p-48f;
 
 // One row for WAVES waves, NCH chunks of 8 columns a lane in registers; a
 // row wider than that reads its residual a second time.
@@ -144,29 +151,45 @@ __global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : kThreads) void fp8_norm_ke
   } else {
     inv = 1.0 / sqrt(mean);
   }
-  const float inv_high = (float)inv, inv_low = (float)(inv - (double)inv_high);
+  const float inv_high = (float)inv;
+  const bool odd_row = !(inv_high >= 0x1p-126f && inv_high <= 0x1p126f);
   auto give = [&](int c, float* o) {  // the row's chunk c, normalised, into e4m3
     float w[8];
     const int have = a.k - c * 8;
     load8((const T*)a.w + (have > 0 ? c * 8 : 0), have, w);
-    // The f32 products are within 1.5 * 2^-24 of the exact ones, 2 units of their
-    // last place.  e4m3's borders (between two of its values, and of its scale)
-    // are multiples of 2^19 units: next to one, the exact product decides.
+    // Of normal numbers the f32 products, three roundings with that of inv_high,
+    // are within 3 * 2^-24 of the exact ones, less than 3 units of their last
+    // place.  e4m3's borders (between two of its values, and of its scale) are
+    // multiples of 2^19 units: within 4 units of one the f64 product decides.
     uint32_t near = ~0u;
-    float p[8];
+    float p[8], w_top = 0.0f;
+    auto from_border = [](float f) { return (__float_as_uint(f) << 13) + (4u << 13); };  // less than 8 << 13: that near
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if (a.plus_one) w[j] += 1.0f;
       p[j] = o[j] * inv_high * w[j];
-      near = min(near, (__float_as_uint(p[j]) + 4) & 0x7ffffu);
+      near = min(near, from_border(p[j]));
+      w_top = fmaxf(w_top, __builtin_fabsf(w[j]));
     }
-    if (near < 8)
+    bool redo = odd_row || w_top >= kLargeWeight;
+    if (near < 8u << 13)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = scaled_odd(o[j], inv_high, inv_low, w[j]);
+      for (int j = 0; j < 8; ++j) redo |= p[j] != 0.0f && from_border(p[j]) < 8u << 13;  // (0 is no border)
+    auto in_f64 = [&] {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = j < have ? p[j] : 0.0f;
-    uint32_t code;
-    const u32x2_t q = fp8_block16(o, code);
+      for (int j = 0; j < 8; ++j) p[j] = j < have ? scaled_odd(o[j], inv, w[j]) : 0.0f;
+    };
+    if (redo) in_f64();
+    // Where x * inv or the product is no normal number, the product with a
+    // smaller weight is less than 2^-126 * kLargeWeight = 2^-70: 0 in a block that
+    // holds kSmallTop.
+    uint32_t top = fp8_top16(p);
+    if (top - 1 < __builtin_bit_cast(uint32_t, kSmallTop) - 1) {  // (16 lanes alike; not a block of zeros)
+      in_f64();
+      top = fp8_top16(p);
+    }
+    const uint32_t code = fp8_code(top);
+    const u32x2_t q = fp8_pack8(p, code);
     if (live && c < a.chunks) {
       *(u32x2_t*)(a.q + (r * a.chunks + c) * 8) = q;
       if ((c & 15) == 0) a.s[r * (a.chunks >> 4) + (c >> 4)] = (uint8_t)code;

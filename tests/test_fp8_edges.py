@@ -5,7 +5,7 @@ import torch
 
 import cev_hip
 from cev_hip import Fp8Weight
-from test_fp8 import E4M3, E8M0, half_ulp, up128
+from test_fp8 import E4M3, E8M0, half_ulp, oracle_norm, oracle_rows, up128
 
 
 # ---------------------------------------------------------------------------
@@ -195,3 +195,63 @@ def test_outputs_beside_their_inputs_in_one_buffer(gpu, dtype):
         cev_hip.rms_norm_fp8(room[:, 8: 8 + k], gamma, 1e-6, h=h.clone(), x_out=x)
     with pytest.raises(cev_hip.CevError, match="of its own"):
         cev_hip.linear_fp8(x, w, out=room[:, k - 8: k - 8 + n])
+
+
+# ---------------------------------------------------------------------------
+# The norm at the ends of f32's range
+
+
+def norm_rows(kind, t, k, dtype):
+    """(x, weight) whose normalised values, or what they are made from, are not normal f32 numbers."""
+    g = torch.Generator().manual_seed(70)
+    x, w = torch.randn(t, k, generator=g).double(), 1 + 0.1 * torch.randn(k, generator=g).double()
+    if kind == "subnormal x":  # 1 / root is beyond f32
+        x *= 2.0 ** -135
+    elif kind == "large x":  # 1 / root is a subnormal f32
+        x = (x * 2.0 ** 126).clamp(-2.0 ** 127, 2.0 ** 127)
+    elif kind == "one large x":  # all others over the root are subnormal, and normal times w
+        x *= 2.0 ** -78
+        x[:, 5] = 2.0 ** 60
+        w *= 2.0 ** 100
+        w[5] = 1.0
+    elif kind == "small blocks":  # the same of whole blocks, beside ordinary weights
+        x *= 2.0 ** 60
+        x[:, 128: 256] *= 2.0 ** -130
+        x[:, 5: 9] *= 2.0 ** -130
+    elif kind == "small w":  # the results are subnormal
+        w *= 2.0 ** -129
+    elif kind == "smallest w":
+        w *= 2.0 ** -136
+    elif kind == "zeros":  # whole chunks of 8, beside others that need f64
+        x *= 2.0 ** -135
+        x[:, : k // 2] = 0
+        x[0] *= torch.rand(k, generator=g) < 0.3
+    return x.float().to(dtype), w.float().to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["subnormal x", "large x", "one large x", "small blocks", "small w", "smallest w", "zeros"])
+@pytest.mark.parametrize("t,k", [(3, 264), (64, 4096), (600, 2056), (2, 20000)])
+def test_norm_is_the_nearest_at_the_ends_of_the_range(gpu, t, k, kind, dtype):
+    """Every value and scale is that of 64-bit arithmetic, as for ordinary rows."""
+    x, w = norm_rows(kind, t, k, dtype)
+    got = cev_hip.rms_norm_fp8(x.to(gpu), w.to(gpu), 0.0)
+    q, e = oracle_rows(oracle_norm(x, w, 0.0, None, False)[1])
+    assert torch.equal(got.s.view(torch.uint8).cpu().double(), e + 127) and torch.equal(got.q.double().cpu(), q)
+
+
+@pytest.mark.gpu
+def test_norm_of_values_beyond_f32(gpu):
+    """A normalised value that f32 does not hold is not finite: NaN, and it counts for no scale."""
+    x, w = torch.ones(2, 256), torch.full((256,), 2.0)
+    x[:, 7] = 64.0
+    w[7] = 2.0 ** 127
+    got = cev_hip.rms_norm_fp8(x.to(gpu), w.to(gpu), 1e-6)
+    want = oracle_norm(x, w, 1e-6, None, False)[1]
+    assert float(want[0, 7]) > 2.0 ** 128
+    want[:, 7] = float("inf")
+    q, e = oracle_rows(want)
+    g = got.q.double().cpu()
+    assert torch.equal(got.s.view(torch.uint8).cpu().double(), e + 127)
+    assert torch.equal(torch.isnan(g), torch.isnan(q)) and torch.equal(torch.nan_to_num(g), torch.nan_to_num(q))
