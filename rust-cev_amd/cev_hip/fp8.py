@@ -72,10 +72,19 @@ class Fp8Weight:
         return cls(*gate, stream=stream, _up=tuple(up))
 
 
+def _room(call: str, out, k: int):
+    """The values and scales of `out`, which a call fills with rows of k columns."""
+    if out is None:
+        return None, None
+    if out.k != k:
+        raise CevError(-1, f"{call}: out must be Fp8Rows of {k} columns, not of {out.k}")
+    return out.q, out.s
+
+
 def fp8_rows(x, out=None, stream=None):
     """x (t, k) in e4m3 (cev_fp8_rows), for several projections of the same
     rows.  Returns Fp8Rows."""
-    q, s = (None, None) if out is None else (out.q, out.s)
+    q, s = _room("fp8_rows", out, x.shape[-1])
     return Fp8Rows(*_call("fp8_rows", stream, x, q, s), x.shape[1])
 
 
@@ -91,7 +100,7 @@ def rms_norm_fp8(x, w, eps: float, h=None, x_out=None, out=None, plus_one: bool 
     rounding the one into e4m3.  Returns Fp8Rows."""
     if h is not None and x_out is None:
         x_out = x
-    q, s = (None, None) if out is None else (out.q, out.s)
+    q, s = _room("rms_norm_fp8", out, x.shape[-1])
     return Fp8Rows(*_call("fp8_rms_norm", stream, x, w, eps, h, x_out, plus_one, q, s), x.shape[1])
 
 
@@ -121,5 +130,5 @@ def gate_up_fp8(x, w: Fp8Weight, out=None, stream=None):
     Returns Fp8Rows."""
     if not w.is_gate_up:
         raise CevError(-1, "gate_up_fp8: the weight is no Fp8Weight.gate_up")
-    q, s = (None, None) if out is None else (out.q, out.s)
+    q, s = _room("gate_up_fp8", out, w.n)
     return Fp8Rows(*_call("fp8_product", stream, *_operand(x), w.data, w.n, w.k, w.scale_kind, True, q, s, CEV_BF16), w.n)

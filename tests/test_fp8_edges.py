@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import cev_hip
-from cev_hip import Fp8Weight
+from cev_hip import Fp8Rows, Fp8Weight
 from test_fp8 import E4M3, E8M0, half_ulp, oracle_norm, oracle_rows, up128
 
 
@@ -255,3 +255,19 @@ def test_norm_of_values_beyond_f32(gpu):
     g = got.q.double().cpu()
     assert torch.equal(got.s.view(torch.uint8).cpu().double(), e + 127)
     assert torch.equal(torch.isnan(g), torch.isnan(q)) and torch.equal(torch.nan_to_num(g), torch.nan_to_num(q))
+
+
+# ---------------------------------------------------------------------------
+# Rows that a call fills
+
+
+def test_out_of_other_columns_is_refused(cev):
+    """Rows of 300 and of 310 columns take the same room; an `out` that says 300 is not filled with 310."""
+    z = torch.zeros
+    out = Fp8Rows(z(2, 384).to(E4M3), z(2, 3).to(E8M0), 300)
+    gate_up = type("W", (), dict(is_gate_up=True, data=z(1 << 16, dtype=torch.uint8), n=310, k=128, scale_kind=0))
+    for call in (lambda: cev_hip.fp8_rows(z(2, 310), out=out), lambda: cev_hip.rms_norm_fp8(z(2, 310), z(310), 1e-6, out=out),
+                 lambda: cev_hip.gate_up_fp8(z(2, 128), gate_up, out=out)):
+        with pytest.raises(cev_hip.CevError, match="310 columns, not of 300") as err:
+            call()
+        assert err.value.code == -1
