@@ -5,7 +5,8 @@ import torch
 
 import cev_hip
 from cev_hip import Fp8Rows, Fp8Weight
-from test_fp8 import E4M3, E8M0, half_ulp, oracle_norm, oracle_rows, up128
+from test_fp8 import (E4M3, E8M0, GATE_UPS, activations, check_product, form_of, half_ulp, oracle_norm, oracle_rows, packed, round_e4m3, up128, values,
+                      weight_of, weight_values)
 
 
 # ---------------------------------------------------------------------------
@@ -271,3 +272,87 @@ def test_out_of_other_columns_is_refused(cev):
         with pytest.raises(cev_hip.CevError, match="310 columns, not of 300") as err:
             call()
         assert err.value.code == -1
+
+
+# ---------------------------------------------------------------------------
+# Zero rows, a checkpoint's bfloat16 scales, f32 sums
+
+
+@pytest.mark.gpu
+def test_no_rows_of_bfloat16(gpu):
+    w = packed(weight_of(40, 72, "e8m0", 14), gpu)
+    x = torch.zeros(0, 72, dtype=torch.bfloat16, device=gpu)
+    assert cev_hip.linear_fp8(x, w).shape == (0, 40) and cev_hip.fp8_rows(x).q.shape == (0, 128)
+    assert cev_hip.linear_fp8(cev_hip.fp8_rows(x), w).shape == (0, 40)
+    assert cev_hip.rms_norm_fp8(x, torch.ones(72, dtype=torch.bfloat16, device=gpu), 1e-6).s.shape == (0, 1)
+    gu = Fp8Weight.gate_up(*[tuple(y.to(gpu) for y in weight_of(40, 72, "e8m0", 14)) for _ in range(2)])
+    assert cev_hip.gate_up_fp8(x, gu).q.shape == (0, 128)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("side", [False, True])
+@pytest.mark.parametrize("t,n,k", [(3, 300, 520), (300, 136, 1032)])
+def test_bfloat16_scales(gpu, side, t, n, k):
+    """A weight with bfloat16 scales is the one with the same scales in f32; on a side stream its f32 copies are that stream's."""
+    x = activations(t, k, torch.bfloat16, 71).to(gpu)
+    pairs = [tuple(y.to(gpu) for y in weight_of(n, k, "bf16", 72 + i)) for i in range(2)]
+    wide = [(q, s.float()) for q, s in pairs]
+    want = cev_hip.linear_fp8(x, Fp8Weight(*wide[0])), cev_hip.gate_up_fp8(x, Fp8Weight.gate_up(*wide))
+    s = torch.cuda.Stream() if side else None
+    torch.cuda.synchronize()
+    for _ in range(5):
+        w, gu = Fp8Weight(*pairs[0], stream=s), Fp8Weight.gate_up(*pairs, stream=s)
+        got = cev_hip.linear_fp8(x, w, stream=s), cev_hip.gate_up_fp8(x, gu, stream=s)
+        if side:
+            s.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1].q.view(torch.uint8), want[1].q.view(torch.uint8))
+        assert torch.equal(got[1].s.view(torch.uint8), want[1].s.view(torch.uint8))
+        check_product(got[0], values(*[y.cpu() for y in (lambda r: (r.q, r.s))(cev_hip.fp8_rows(x))])[:, :k], weight_values(*[y.cpu() for y in wide[0]]), torch.bfloat16)
+
+
+def check_nearest(got, xv, gate, up):
+    """Rows of silu(g) u from sums in f32: the nearest e4m3 values of 64-bit ones, but for those next to a border."""
+    k, n = xv.shape[1], gate.shape[0]
+    g, u = (xv @ w.t() for w in (gate, up))
+    size = [xv.abs() @ w.abs().t() for w in (gate, up)]
+    want = g * torch.sigmoid(g) * u
+    # each sum within c of its magnitudes; silu's slope is at most 1.1; the exponential within 2^-22 (1 + |g|), the rest some f32 roundings
+    c = (k + k / 64 + 16) * 2.0 ** -23
+    tol = 1.1 * c * size[0] * (u.abs() + c * size[1]) + g.abs() * c * size[1] + want.abs() * (2.0 ** -22 * (1 + g.abs()) + 2.0 ** -21)
+    e = got.s.view(torch.uint8).cpu().double() - 127
+    v, slack, q = (torch.zeros(xv.shape[0], up128(n), dtype=torch.float64) for _ in range(3))
+    v[:, :n], slack[:, :n] = want, tol
+    by = torch.exp2(-e).repeat_interleave(128, 1)
+    v, slack, q = v * by, slack * by, got.q.double().cpu()
+    step = torch.exp2(torch.floor(torch.log2((v.abs() + slack).clamp(min=2.0 ** -6))) - 3)
+    assert bool(((q - v).abs() <= step / 2 + slack + 1e-30).all())
+    # Errors are 2^-19 of a value at the root mean square (an order above f32 sums of these lengths); borders are 2^-4 of a
+    # value apart or more, so that 2 * 2^-19 / 2^-4 of the values may fall to the other side of one.
+    other = q[:, :n] != round_e4m3(v[:, :n].clamp(-448, 448))
+    assert int(other.sum()) <= 2.0 ** -14 * other.numel() + 2, int(other.sum())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["e8m0", "f32"])
+@pytest.mark.parametrize("t,n,k", GATE_UPS + [(16, 6144, 2048), (16, 2048, 4104)])
+def test_gate_up_of_few_rows_has_f32_sums(gpu, t, n, k, kind):
+    if form_of(t, n, k, kind, gate_up=True)[0]:
+        pytest.skip("the kernel for many rows")
+    x = activations(t, k, torch.float32, 15) * (1.5 / k ** 0.5)
+    gate, up = weight_of(n, k, kind, 16), weight_of(n, k, kind, 17)
+    rows = cev_hip.fp8_rows(x.to(gpu))
+    got = cev_hip.gate_up_fp8(rows, Fp8Weight.gate_up(tuple(y.to(gpu) for y in gate), tuple(y.to(gpu) for y in up)))
+    check_nearest(got, values(rows.q.cpu(), rows.s.cpu())[:, :k], weight_values(*gate), weight_values(*up))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["e8m0", "f32"])
+@pytest.mark.parametrize("t,n,k", [(17, 1000, 520), (300, 384, 2056), (700, 1000, 1032)])
+def test_gate_up_of_many_rows_with_f32_sums(gpu, t, n, k, kind):
+    """What a caller runs instead of gate_up_fp8 for sums in f32 whatever the number of rows."""
+    x = activations(t, k, torch.bfloat16, 15) * (1.5 / k ** 0.5)
+    gate, up = weight_of(n, k, kind, 16), weight_of(n, k, kind, 17)
+    rows = cev_hip.fp8_rows(x.to(gpu))
+    g, u = (cev_hip.linear_fp8(rows, packed(w, gpu), out_dtype=torch.float32) for w in (gate, up))
+    got = cev_hip.fp8_rows(cev_hip.swiglu(g, u))
+    check_nearest(got, values(rows.q.cpu(), rows.s.cpu())[:, :k], weight_values(*gate), weight_values(*up))
