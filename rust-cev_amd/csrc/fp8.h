@@ -28,11 +28,12 @@ __device__ __forceinline__ f32x4 fp8_mfma(const i32x8& a, const i32x8& b, const 
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
 }
 
-// 32 values of a lane in bf16, which holds e4m3's exactly: 8 for each of four products.
+// 32 values of a lane in bf16, which holds e4m3's exactly, times `by`, a power of
+// two: 8 for each of four products.
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ bf16x8 fp8_widen(int lo, int hi) {
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, 1.0f, true);
-  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, 1.0f, true);
+__device__ __forceinline__ bf16x8 fp8_widen(int lo, int hi, float by = 1.0f) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, by, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, by, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, by, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, by, true);
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
@@ -51,16 +52,22 @@ __device__ __forceinline__ Fp8Scale fp8_scale(uint32_t s) {
   return {code, __builtin_ldexpf(__uint_as_float(s), 127 - code)};
 }
 
-// The scales of a sum of unscaled products, which is 0 or between 2^-18 and
-// 2^25: (sum * first) * second, in range wherever the result is, and rounded
-// once, as `first` is a power of two (2^-100 to 2^100).
-struct Fp8Factors {
-  float first, second;
+// A row's scale 2^e in two: `values` widens the row with, 2^-100 to 2^100, so
+// that bf16 holds them and f32 the sums of their products exactly, and 2^rest
+// goes to the weight's scale (code 255: NaN).
+struct Fp8RowScale {
+  float values;
+  int rest;
+  bool nan;
 };
-__device__ __forceinline__ Fp8Factors fp8_factors(int row_code, const Fp8Scale& w) {
-  const int e = row_code + w.code - 254, c = min(max(e, -100), 100);
-  const float first = __uint_as_float(row_code == 255 ? 0x7fc00000u : (uint32_t)(c + 127) << 23);
-  return {first, __builtin_ldexpf(w.rest, min(e - c, 126))};  // (2^126 and more: infinite, but for a sum of 0)
+__device__ __forceinline__ Fp8RowScale fp8_row_scale(int code) {
+  const int c = min(max(code, 27), 227);
+  return {__uint_as_float((uint32_t)c << 23), code - c, code == 255};
+}
+// What multiplies such a sum: in range wherever the result is.  (2^126 and more: infinite, but for a sum of 0.)
+__device__ __forceinline__ float fp8_factor(const Fp8RowScale& row, const Fp8Scale& w) {
+  const float f = __builtin_ldexpf(w.rest, min(w.code - 127 + row.rest, 126));
+  return row.nan ? __builtin_nanf("") : f;
 }
 
 __device__ __forceinline__ i32x8 fp8_join(const u32x4_t& a, const u32x4_t& b) {

@@ -149,13 +149,14 @@ __global__ __launch_bounds__(kWaves * 64, 4) void fp8_small_kernel(Fp8Args a, un
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           if constexpr (EXACT) {
+            const Fp8RowScale row = fp8_row_scale(sx[d][i]);
             f32x4 p = {};
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(wv[2 * c], wv[2 * c + 1]), fp8_widen(xv[i][2 * c], xv[i][2 * c + 1]), p, 0, 0, 0);
-            const Fp8Factors by = fp8_factors(sx[d][i], f);
+              p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(wv[2 * c], wv[2 * c + 1]), fp8_widen(xv[i][2 * c], xv[i][2 * c + 1], row.values), p, 0, 0, 0);
+            const float by = fp8_factor(row, f);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[h][i][r] = __builtin_fmaf(p[r] * by.first, by.second, acc[h][i][r]);
+            for (int r = 0; r < 4; ++r) acc[h][i][r] = __builtin_fmaf(p[r], by, acc[h][i][r]);
           } else if constexpr (E8M0) {
             acc[h][i] = fp8_mfma(wv, xv[i], acc[h][i], (int)sw[d][h], sx[d][i]);
           } else {

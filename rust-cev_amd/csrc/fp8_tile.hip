@@ -224,12 +224,13 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
       const i32x8 x = fp8_join(xr[U % RING].v[0], xr[U % RING].v[1]);
       const int sx = xr[U % RING].s;
       bf16x8 wide[4];
-      Fp8Factors by[2];
+      float by[2] = {};
       if constexpr (EXACT) {
+        const Fp8RowScale row = fp8_row_scale(sx);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) wide[c] = fp8_widen(x[2 * c], x[2 * c + 1]);
+        for (int c = 0; c < 4; ++c) wide[c] = fp8_widen(x[2 * c], x[2 * c + 1], row.values);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) by[j] = fp8_factors(sx, s[j]);
+        for (int j = 0; j < 2; ++j) by[j] = fp8_factor(row, s[j]);
       }
       // Four matrix products, and between them what is read for later ones: a
       // product takes 32 cycles, in which seven other instructions can start.
@@ -241,7 +242,7 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
 #pragma unroll
           for (int c = 0; c < 4; ++c) q = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(wv[2 * c], wv[2 * c + 1]), wide[c], q, 0, 0, 0);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[U][J][r] = __builtin_fmaf(q[r] * by[J >> 1].first, by[J >> 1].second, acc[U][J][r]);
+          for (int r = 0; r < 4; ++r) acc[U][J][r] = __builtin_fmaf(q[r], by[J >> 1], acc[U][J][r]);
         } else if constexpr (E8M0) {
           acc[U][J] = fp8_mfma(wv, x, acc[U][J], (int)s2[J >> 1], sx);
         } else {
