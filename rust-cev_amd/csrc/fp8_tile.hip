@@ -148,7 +148,11 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
     return v & (n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << 8 * n) - 1);
   };
   auto put_xs = [&](uint32_t v, int slot) {
-    if (ROWS == 256 || tid < ROWS) *(uint32_t*)(lds + SCALES + (slot * ROWS + tid) * 4) = v;
+    // (tid from the lane again: kept over the loop, it went to memory, and its reload waited for all loads in flight)
+    int from = 0;
+    asm volatile("" : "+s"(from));
+    const int t = wave * 64 + (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, (uint32_t)from));
+    if (ROWS == 256 || t < ROWS) *(uint32_t*)(lds + SCALES + (slot * ROWS + t) * 4) = v;
   };
 
   // Reads of the rows, AHEAD tiles of 16 ahead of the one that is computed.
@@ -203,7 +207,11 @@ __device__ __forceinline__ void tile(const Fp8Args& a, int row_tiles, int col_ti
     Fp8Scale s[2];
     if constexpr (!E8M0 || EXACT)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) s[j] = fp8_scale<E8M0>(E8M0 ? s2[j] & 255 : sw[B][j]);
+      for (int j = 0; j < 2; ++j) {
+        s[j] = fp8_scale<E8M0>(E8M0 ? s2[j] & 255 : (uint32_t)uniform((int)sw[B][j]));
+        // (in scalar registers: two vector ones more and the loop reloads one, behind all loads in flight)
+        if constexpr (!E8M0 && !EXACT) s[j].rest = __uint_as_float((uint32_t)uniform((int)__float_as_uint(s[j].rest)));
+      }
     f32x4 p[2];
     auto scale_in = [&](auto u_c, auto j_c) {
       constexpr int U = decltype(u_c)::value, J = decltype(j_c)::value;
