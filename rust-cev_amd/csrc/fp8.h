@@ -91,8 +91,9 @@ __device__ __forceinline__ void fp8_store4(O* row, int64_t n, int64_t col, const
   }
 }
 
-// silu(g) u in f32 (the hardware's exp2 and reciprocal, within 2^-20 of the
-// value: e4m3 keeps 4 bits of it).
+// silu(g) u in f32, by the hardware's exp2 and reciprocal: within 2^-20 of the
+// value, and below g = 0 within |g| 2^-23 more (the exponent's own rounding);
+// e4m3 keeps 4 bits of it.
 __device__ __forceinline__ float fp8_swiglu(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + fast_exp2(-1.44269504f * g)) * u;
 }

@@ -7,14 +7,15 @@
 //   bf16 outputs, and gate and up of many rows
 //       v_mfma_scale_f32_16x16x128_f8f6f4, which takes 2^e as an operand, and s
 //       where it is a power of two (of an f32 s its power of two; the rest of it,
-//       1 to 2, multiplies the block's 16 x 16 results).  It adds eight neighbouring columns' products after cutting
-//       each towards zero to a multiple of 2^(E - 13), 2^E the largest one's
-//       power of two (measured bit by bit); what follows is f32.  A sum is
-//       therefore up to 7 * 2^-13 of its largest products off; on normal data
-//       it is 4.5e-5 of the result, a fortieth of bf16's rounding.  Of gate and
-//       up's e4m3 values, whose steps are 2^-3 to 2^-4 apart, one in a thousand
-//       becomes the nearest but one.  (In bf16 the same product takes twice as
-//       long: 4096 x 12288 x 4096 1331 instead of 2600 TFLOP/s at best.)
+//       1 to 2, multiplies the block's 16 x 16 results).  It adds eight
+//       neighbouring columns' products after cutting each towards zero to a
+//       multiple of 2^(E - 13), 2^E the largest one's power of two (measured bit
+//       by bit); what follows is f32.  A sum is therefore up to 7 * 2^-13 of its
+//       largest products off; on normal data it is 4.5e-5 of the result, a
+//       fortieth of bf16's rounding.  Of gate and up's e4m3 values, whose steps
+//       are 2^-3 to 2^-4 apart, one in a thousand becomes the nearest but one:
+//       which ones depends on the form, and with it on how many rows a call has.
+//       (By f32 sums 8192 x 4096 x 12288 takes 745 us instead of 278.)
 //   f32 outputs, and gate and up of few rows
 //       v_mfma_f32_16x16x32_bf16 on the same values in bf16, which holds them
 //       exactly: products and sums in f32, at half the rate.  Where the weight's

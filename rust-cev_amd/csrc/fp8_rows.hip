@@ -366,9 +366,10 @@ template <typename T>
 int32_t launch_norm(const NormArgs& a, hipStream_t s) {
   // A row's chunks of 8 columns go to one lane each; where there are more rows
   // than fill the card, to as few waves as hold them in registers (us, bf16 with
-  // the residual: 64 x 4096 with 8 waves 3.7, with 4 4.1; 8192 x 4096 42.8
-  // and 41.7, 5.6 TB/s; 64 x 12288 with 16 waves 4.9, with 8 5.8; 4096 x 1024 with 4
-  // waves 10.0, with 2 7.7).
+  // the residual, launches over three inputs in turn: 64 x 4096 with 8 waves 3.7,
+  // with 4 4.1; 8192 x 4096 42.8 and 41.5; 64 x 12288 with 16 waves 5.0, with 8
+  // 5.8; 4096 x 1024 with 4 waves 10.0, with 2 8.0.  Over inputs that change with
+  // every call 8192 x 4096 takes 47.4, 5.0 TB/s).
   if (a.chunks <= 64) return launch_norm<T, 1, 1>(a, s);
   const bool few = a.rows <= 512;
   if (a.chunks <= 128 && !few) return launch_norm<T, 2, 1>(a, s);
