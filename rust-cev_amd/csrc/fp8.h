@@ -64,9 +64,10 @@ __device__ __forceinline__ Fp8RowScale fp8_row_scale(int code) {
   const int c = min(max(code, 27), 227);
   return {__uint_as_float((uint32_t)c << 23), code - c, code == 255};
 }
-// What multiplies such a sum: in range wherever the result is.  (2^126 and more: infinite, but for a sum of 0.)
+// What multiplies such a sum: in range wherever the result is.  (More than 127
+// comes with values of 2^100: infinite, but for a sum of 0.)
 __device__ __forceinline__ float fp8_factor(const Fp8RowScale& row, const Fp8Scale& w) {
-  const float f = __builtin_ldexpf(w.rest, min(w.code - 127 + row.rest, 126));
+  const float f = __builtin_ldexpf(w.rest, min(w.code - 127 + row.rest, 127));
   return row.nan ? __builtin_nanf("") : f;
 }
 

@@ -13,7 +13,7 @@ from test_fp8 import (E4M3, E8M0, GATE_UPS, activations, check_product, form_of,
 # Scales far apart
 
 SCALES_APART = [(112, -40, 448.0), (118, -100, 448.0), (112, 10, 2.0 ** -9), (-118, 120, 448.0), (-118, 120, 2.0 ** -9), (-120, 100, 2.0 ** -9),
-                (100, -126, 448.0), (119, -149, 448.0)]
+                (100, -126, 448.0), (119, -149, 448.0), (-100, 127, 448.0), (-60, 127, 2.0 ** -9)]
 
 
 def far_rows(t, k, m, x_exp, gpu):
@@ -74,6 +74,32 @@ def test_scales_of_zero_infinity_and_nan(gpu, t, n, k, out_dtype):
         at = up128(n) - 128
         assert torch.equal(y[:, :at], want[:, :at])
         assert bool((y[:, at:] == bad).all() if bad == bad else torch.isnan(y[:, at:]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,n,k", [(2, 40, 128), (20, 40, 1032), (40, 300, 640), (300, 2048, 256), (900, 4000, 1160)])
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+def test_scales_of_rows_that_are_nan_or_at_their_ends(gpu, t, n, k, kind, out_dtype):
+    """A NaN scale of a row, in its first, last or some block, makes that row NaN and no other; the largest and least ones are used."""
+    rows = cev_hip.fp8_rows(activations(t, k, torch.bfloat16, 80).to(gpu))
+    w = packed(weight_of(n, k, kind, 81), gpu)
+    clean = cev_hip.linear_fp8(rows, w, out_dtype=out_dtype)
+    kb = rows.s.shape[1]
+    for row, block in ((0, 0), (t - 1, kb - 1), (t // 2, kb // 2)):
+        s = rows.s.view(torch.uint8).clone()
+        s[row, block] = 255
+        y = cev_hip.linear_fp8(Fp8Rows(rows.q, s.view(E8M0), k), w, out_dtype=out_dtype)
+        others = torch.arange(t, device=gpu) != row
+        assert bool(torch.isnan(y[row]).all()) and torch.equal(y[others], clean[others])
+    # scales of 2^127 and 2^-127 in turn, beside weights of 2^-126 (sums up to 2^25) and 2^126
+    for code, w_exp in ((254, -126), (0, 126)):
+        q = torch.ones_like(rows.q.float()).to(E4M3)
+        q[:, k:] = 0
+        y = cev_hip.linear_fp8(Fp8Rows(q, torch.full_like(s, code).view(E8M0), k),
+                               Fp8Weight(torch.ones(n, k, device=gpu).to(E4M3), torch.full((up128(n) // 128, kb), 2.0 ** w_exp, device=gpu).to(torch.float32 if kind == "f32" else E8M0)),
+                               out_dtype=out_dtype)
+        assert bool((y.double() == torch.tensor(k * 2.0 ** (code - 127 + w_exp)).to(out_dtype).double().to(gpu)).all())
 
 
 # ---------------------------------------------------------------------------
