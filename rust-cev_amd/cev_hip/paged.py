@@ -195,9 +195,11 @@ class PagedAttention:
         if stream is None or stream.cuda_stream in self._streams or not self._work.is_cuda:
             return
         s = _stream(stream, self._work.device)
-        if self._made is not None and not _capturing(s):  # (what a captured step uses was made before the capture)
-            s.wait_event(self._made)
         self._work.record_stream(s)
+        if _capturing(s):  # (what a captured step uses was made before the capture)
+            return
+        if self._made is not None:
+            s.wait_event(self._made)
         self._streams.add(stream.cuda_stream)
 
     @property
@@ -209,6 +211,11 @@ class PagedAttention:
             if s != here and not _capturing(s) and not _capturing(here):
                 here.wait_stream(s)
         return self._work
+
+    @work.setter
+    def work(self, work):
+        """Another workspace of this size, which is the caller's to order."""
+        self._work, self._made, self._planned, self._streams = work, None, None, set()
 
     def plan(self, cu, lengths, stream=None):
         """The step's work list: cu (requests + 1) and lengths (requests, new

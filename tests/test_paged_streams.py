@@ -88,3 +88,22 @@ def test_a_captured_step_of_an_object_made_before(gpu):
         assert torch.equal(out, want)
         assert torch.equal(p.run(), want)
         torch.cuda.synchronize()
+
+
+def test_objects_that_share_a_workspace(gpu):
+    """Two objects of one shape take turns in one workspace, the second one's own given up."""
+    import torch
+    p = _Paged(gpu, [700, 40, 2000], [1, 33, 5], 8, 2, 128, "bf16", 16, seed=13, pad=3)
+    want, windowed = p.run(), p.run(window=30)
+    a, b = p.attention(), p.attention(window=30)
+    b.work = a.work
+    assert b.work.data_ptr() == a.work.data_ptr()
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for att, expected in ((a, want), (b, windowed), (a, want)):
+        out = torch.full_like(p.q, 5.0)
+        s.wait_stream(torch.cuda.current_stream())
+        att.plan(p.cu, p.lengths, stream=s)
+        att(p.q, p.k, p.v, p.table, out=out, stream=s)
+        s.synchronize()
+        assert torch.equal(out, expected)
